@@ -11,12 +11,15 @@
 #include "linear_attn.h"
 #include "delta_prep.h"
 #include "delta_scan.h"
+#include "delta_step.h"
+#include "logits.h"
 #include "moe.h"
 #include "moe_route.h"
 #include "sparse_attn.h"
 #include "sparse_teacher.h"
 #include "nsa_compress.h"
 #include "msar.h"
+#include "paged.h"
 #include "plugin_ops.h"
 #include "probe_sm100.h"
 #include "residual.h"
@@ -1246,6 +1249,257 @@ std::vector<int64_t> read_errors() {
           static_cast<int64_t>(ws)};
 }
 
+// ------------------------------------------------------------------ serving
+// A tensor of heads [B, t, heads, D]: its element strides of row, token and head.  `align` elements start a
+// 16-byte (or narrower) vector in the kernels.
+void head_strides(const Tensor& t, const char* name, int64_t align, int64_t (&s)[3]) {
+  TORCH_CHECK(t.dim() == 4, name, " must have 4 dimensions (row, token, head, channel)");
+  TORCH_CHECK(t.stride(3) == 1 || t.size(3) == 1, name, " must have contiguous channels");
+  for (int i = 0; i < 3; ++i) {
+    s[i] = t.stride(i);
+    TORCH_CHECK(t.size(i) <= 1 || s[i] % align == 0, name, ": rows and heads must start on aligned elements");
+  }
+  TORCH_CHECK(reinterpret_cast<uintptr_t>(t.data_ptr()) % (align * t.element_size()) == 0, name, " must be aligned");
+}
+void check_ints(const Tensor& t, const Tensor& like, const char* name, int64_t dim) {
+  TORCH_CHECK(t.device() == like.device() && t.scalar_type() == at::kInt && t.is_contiguous() && t.dim() == dim, name,
+              " must be a contiguous int32 tensor on the operands' device");
+}
+const int* row_ints(const OptT& t, const Tensor& like, int64_t rows, const char* name) {
+  if (!t.has_value() || !t->defined()) return nullptr;
+  check_ints(*t, like, name, 1);
+  TORCH_CHECK(t->size(0) == rows, name, " must have one entry for each row");
+  return t->data_ptr<int>();
+}
+PagedCacheArgs paged_cache(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& table) {
+  TORCH_CHECK(q.is_cuda() && k.device() == q.device() && v.device() == q.device(), "queries and pages must be on one CUDA device");
+  TORCH_CHECK(q.scalar_type() == at::kBFloat16 || q.scalar_type() == at::kHalf, "paged attention takes bf16 or fp16");
+  TORCH_CHECK(k.scalar_type() == q.scalar_type() && v.scalar_type() == q.scalar_type(), "pages must have the queries' type");
+  TORCH_CHECK(q.dim() == 4 && k.dim() == 4 && v.dim() == 4 && k.sizes() == v.sizes(),
+              "q [B, t, H, D] and pages [P, Hk, page, D] expected");
+  TORCH_CHECK(k.size(3) == q.size(3) && (k.size(3) == 64 || k.size(3) == 128), "head dimension must be 64 or 128");
+  TORCH_CHECK(k.size(1) > 0 && q.size(2) % k.size(1) == 0, "KV heads must divide query heads");
+  TORCH_CHECK(k.size(2) > 0 && k.size(2) % 16 == 0, "tokens per page must be a multiple of 16");
+  check_ints(table, q, "table", 2);
+  TORCH_CHECK(table.size(0) == q.size(0), "table must have one line for each row");
+  PagedCacheArgs c;
+  int64_t ks[3], vs[3];
+  head_strides(k, "k_pages", 8, ks);
+  head_strides(v, "v_pages", 8, vs);
+  c.k = k.data_ptr();
+  c.v = v.data_ptr();
+  c.page_stride_k = ks[0]; c.head_stride_k = ks[1]; c.slot_stride_k = ks[2];
+  c.page_stride_v = vs[0]; c.head_stride_v = vs[1]; c.slot_stride_v = vs[2];
+  c.table = table.data_ptr<int>();
+  c.columns = static_cast<int>(table.size(1));
+  c.pages = k.size(0);
+  c.page = static_cast<int>(k.size(2));
+  return c;
+}
+
+Tensor paged_append(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& k_pages, const Tensor& v_pages,
+                    const Tensor& table, const Tensor& start, const OptT& count, const Tensor& cos, const Tensor& sin,
+                    c10::optional<double> qk_scale, const OptT& ve, const OptT& ve_gate) {
+  PagedAppendArgs a;
+  a.cache = paged_cache(q, k_pages, v_pages, table);
+  a.B = static_cast<int>(q.size(0));
+  a.t = static_cast<int>(q.size(1));
+  a.H = static_cast<int>(q.size(2));
+  a.D = static_cast<int>(q.size(3));
+  a.Hk = static_cast<int>(k_pages.size(1));
+  for (auto* x : {&k, &v}) {
+    TORCH_CHECK(x->device() == q.device() && x->scalar_type() == q.scalar_type(), "q, k and v must agree in device and type");
+    TORCH_CHECK(x->dim() == 4 && x->size(0) == a.B && x->size(1) == a.t && x->size(2) == a.Hk && x->size(3) == a.D,
+                "k and v must be [B, t, Hk, D]");
+  }
+  head_strides(q, "q", 8, a.qs);
+  head_strides(k, "k", 8, a.ks);
+  head_strides(v, "v", 8, a.vs);
+  a.q = q.data_ptr(); a.kin = k.data_ptr(); a.vin = v.data_ptr();
+  for (auto* x : {&cos, &sin}) {
+    TORCH_CHECK(x->device() == q.device() && x->scalar_type() == q.scalar_type() && x->is_contiguous() && x->dim() == 2 &&
+                    x->size(1) == a.D / 2 && x->size(0) == cos.size(0),
+                "cos and sin must be contiguous [positions, D / 2] tables in the type of q");
+    TORCH_CHECK(reinterpret_cast<uintptr_t>(x->data_ptr()) % 16 == 0, "cos and sin must be 16-byte aligned");
+  }
+  a.cos = cos.data_ptr();
+  a.sin = sin.data_ptr();
+  a.rope_rows = static_cast<int>(cos.size(0));
+  TORCH_CHECK((ve.has_value() && ve->defined()) == (ve_gate.has_value() && ve_gate->defined()), "ve and ve_gate go together");
+  if (ve.has_value() && ve->defined()) {
+    TORCH_CHECK(ve->device() == q.device() && ve_gate->device() == q.device() && ve->scalar_type() == q.scalar_type() &&
+                    ve_gate->scalar_type() == q.scalar_type() && ve->sizes() == v.sizes(),
+                "ve must be like v, ve_gate in its type");
+    TORCH_CHECK(ve_gate->dim() == 3 && ve_gate->size(0) == a.B && ve_gate->size(1) == a.t && ve_gate->size(2) == a.Hk,
+                "ve_gate must be [B, t, Hk]");
+    head_strides(*ve, "ve", 8, a.es);
+    for (int i = 0; i < 3; ++i) a.gs[i] = ve_gate->stride(i);
+    a.ve = ve->data_ptr();
+    a.ve_gate = ve_gate->data_ptr();
+  }
+  a.start = row_ints(start, q, a.B, "start");
+  a.count = row_ints(count, q, a.B, "count");
+  a.norm = qk_scale.has_value();
+  a.scale = static_cast<float>(qk_scale.value_or(1.0));
+  a.fp16 = q.scalar_type() == at::kHalf;
+  const c10::cuda::CUDAGuard guard(q.device());
+  Tensor out = at::empty({a.B, a.t, a.H, a.D}, q.options());
+  a.q_out = out.data_ptr();
+  ok(nt_paged_append(a, stream()), "paged_append");
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  return out;
+}
+
+Tensor paged_attention(const Tensor& q, const Tensor& k_pages, const Tensor& v_pages, const Tensor& table,
+                       const Tensor& start, const OptT& count, int64_t window, c10::optional<double> scale) {
+  PagedAttnArgs a;
+  a.cache = paged_cache(q, k_pages, v_pages, table);
+  a.B = static_cast<int>(q.size(0));
+  a.t = static_cast<int>(q.size(1));
+  a.H = static_cast<int>(q.size(2));
+  a.D = static_cast<int>(q.size(3));
+  a.Hk = static_cast<int>(k_pages.size(1));
+  head_strides(q, "q", 8, a.qs);
+  a.q = q.data_ptr();
+  a.start = row_ints(start, q, a.B, "start");
+  a.count = row_ints(count, q, a.B, "count");
+  a.window = window < 0 || window > INT32_MAX / 2 ? -1 : static_cast<int>(window);
+  a.scale = static_cast<float>(scale.value_or(1.0 / std::sqrt(static_cast<double>(a.D))));
+  a.fp16 = q.scalar_type() == at::kHalf;
+  a.sms = num_sms(q);
+  const c10::cuda::CUDAGuard guard(q.device());
+  Tensor out = at::empty({a.B, a.t, a.H, a.D}, q.options());
+  if (out.numel() == 0) return out;
+  a.out = out.data_ptr();
+  Tensor ws;
+  if (const size_t bytes = nt_paged_attn_workspace(a)) {
+    ws = at::empty({static_cast<int64_t>(bytes / sizeof(float))}, q.options().dtype(at::kFloat));
+    a.workspace = ws.data_ptr<float>();
+  }
+  ok(nt_paged_attn(a, stream()), "paged_attention");
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  return out;
+}
+
+Tensor delta_step(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& state, const Tensor& beta, const OptT& g,
+                  double scale, bool l2norm, const OptT& slots, const OptT& count) {
+  check_cuda(q, "q");
+  const auto type = q.scalar_type();
+  TORCH_CHECK(type == at::kBFloat16 || type == at::kHalf || type == at::kFloat, "delta_recurrent takes bf16, fp16 or fp32");
+  TORCH_CHECK(q.dim() == 4 && k.sizes() == q.sizes() && v.sizes() == q.sizes() && k.scalar_type() == type &&
+                  v.scalar_type() == type && k.device() == q.device() && v.device() == q.device(),
+              "q, k and v must be [B, T, H, D] of one type and device");
+  DeltaStepArgs a;
+  a.B = static_cast<int>(q.size(0));
+  a.T = static_cast<int>(q.size(1));
+  a.H = static_cast<int>(q.size(2));
+  a.D = static_cast<int>(q.size(3));
+  TORCH_CHECK(a.D == 64 || a.D == 128, "head dimension must be 64 or 128");
+  head_strides(q, "q", a.D / 32, a.qs);
+  head_strides(k, "k", a.D / 32, a.ks);
+  head_strides(v, "v", 1, a.vs);
+  a.q = q.data_ptr(); a.k = k.data_ptr(); a.v = v.data_ptr();
+  TORCH_CHECK(beta.device() == q.device() && (beta.scalar_type() == type || beta.scalar_type() == at::kFloat) &&
+                  beta.dim() == 3 && beta.sizes() == q.sizes().slice(0, 3),
+              "beta must be [B, T, H] in the type of q or fp32");
+  a.beta = beta.data_ptr();
+  a.beta_f32 = beta.scalar_type() == at::kFloat;
+  for (int i = 0; i < 3; ++i) a.bs[i] = beta.stride(i);
+  if (g.has_value() && g->defined()) {
+    TORCH_CHECK(g->device() == q.device() && g->scalar_type() == at::kFloat &&
+                    (g->sizes() == q.sizes() || g->sizes() == q.sizes().slice(0, 3)),
+                "g must be an fp32 log decay, [B, T, H] or [B, T, H, D]");
+    a.g = g->data_ptr<float>();
+    a.gate = g->dim() == 4 ? 2 : 1;
+    if (a.gate == 2) head_strides(*g, "g", a.D / 32, a.gs);
+    else
+      for (int i = 0; i < 3; ++i) a.gs[i] = g->stride(i);
+  }
+  TORCH_CHECK(state.device() == q.device() && state.scalar_type() == at::kFloat && state.is_contiguous() && state.dim() == 4 &&
+                  state.size(1) == a.H && state.size(2) == a.D && state.size(3) == a.D,
+              "state must be contiguous fp32 [states, H, D, D]");
+  a.state = state.data_ptr<float>();
+  a.states = state.size(0);
+  a.slots = row_ints(slots, q, a.B, "slots");
+  a.count = row_ints(count, q, a.B, "count");
+  TORCH_CHECK(a.slots || a.states >= a.B, "state must have an entry for each row");
+  a.l2norm = l2norm;
+  a.scale = static_cast<float>(scale);
+  a.type = type == at::kBFloat16 ? DELTA_STEP_BF16 : type == at::kHalf ? DELTA_STEP_FP16 : DELTA_STEP_FP32;
+  const c10::cuda::CUDAGuard guard(q.device());
+  Tensor o = at::empty({a.B, a.T, a.H, a.D}, q.options());
+  a.o = o.data_ptr();
+  ok(nt_delta_step(a, stream()), "delta_recurrent");
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  return o;
+}
+
+const float* row_floats(const OptT& t, const Tensor& like, int64_t rows, const char* name) {
+  if (!t.has_value() || !t->defined()) return nullptr;
+  TORCH_CHECK(t->device() == like.device() && t->scalar_type() == at::kFloat && t->is_contiguous() && t->dim() == 1 &&
+                  t->size(0) == rows,
+              name, " must be fp32 with one entry for each row");
+  return t->data_ptr<float>();
+}
+
+Tensor adjust_logits(const Tensor& logits, const OptT& tokens, const OptT& length, const OptT& prompt,
+                     const OptT& repetition, const OptT& presence, const OptT& frequency, const OptT& bias_ids,
+                     const OptT& bias, const OptT& allowed) {
+  check_cuda(logits, "logits");
+  const auto type = logits.scalar_type();
+  TORCH_CHECK(type == at::kBFloat16 || type == at::kHalf || type == at::kFloat, "logits must be bf16, fp16 or fp32");
+  TORCH_CHECK(logits.dim() == 2 && (logits.stride(1) == 1 || logits.size(1) == 1), "logits must be [B, V] with contiguous rows");
+  LogitsArgs a;
+  const int64_t B = logits.size(0), V = logits.size(1);
+  TORCH_CHECK(V <= INT32_MAX / 2 && B <= 65535, "logits: too many rows or entries");
+  a.B = static_cast<int>(B);
+  a.V = static_cast<int>(V);
+  a.logits = logits.data_ptr();
+  a.row_stride = logits.stride(0);
+  a.type = type == at::kBFloat16 ? LOGITS_BF16 : type == at::kHalf ? LOGITS_FP16 : LOGITS_FP32;
+  a.sms = num_sms(logits);
+  if (tokens.has_value() && tokens->defined()) {
+    check_ints(*tokens, logits, "tokens", 2);
+    TORCH_CHECK(tokens->size(0) == B, "tokens must have one line for each row");
+    a.L = static_cast<int>(tokens->size(1));
+    if (a.L) a.tokens = tokens->data_ptr<int>();
+  }
+  a.length = row_ints(length, logits, B, "length");
+  a.prompt = row_ints(prompt, logits, B, "prompt");
+  a.repetition = row_floats(repetition, logits, B, "repetition");
+  a.presence = row_floats(presence, logits, B, "presence");
+  a.frequency = row_floats(frequency, logits, B, "frequency");
+  TORCH_CHECK((bias_ids.has_value() && bias_ids->defined()) == (bias.has_value() && bias->defined()), "bias_ids and bias go together");
+  if (bias.has_value() && bias->defined()) {
+    check_ints(*bias_ids, logits, "bias_ids", 2);
+    TORCH_CHECK(bias->device() == logits.device() && bias->scalar_type() == at::kFloat && bias->is_contiguous() &&
+                    bias->sizes() == bias_ids->sizes() && bias->size(0) == B,
+                "bias must be contiguous fp32 [B, K] like bias_ids");
+    a.K = static_cast<int>(bias->size(1));
+    a.bias_ids = bias_ids->data_ptr<int>();
+    a.bias = bias->data_ptr<float>();
+  }
+  if (allowed.has_value() && allowed->defined()) {
+    check_ints(*allowed, logits, "allowed", 2);
+    TORCH_CHECK(allowed->size(0) == B && allowed->size(1) >= (V + 31) / 32, "allowed must be [B, ceil(V / 32)]");
+    a.allowed = allowed->data_ptr<int>();
+    a.words = static_cast<int>(allowed->size(1));
+  }
+  const c10::cuda::CUDAGuard guard(logits.device());
+  Tensor out = at::empty({B, V}, logits.options().dtype(at::kFloat));
+  a.out = out.data_ptr<float>();
+  ok(nt_adjust_logits(a, stream()), "adjust_logits");
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  return out;
+}
+
+std::vector<int64_t> read_serving_errors() {
+  unsigned wp = 0, wd = 0;
+  const int p = nt_paged_read_error(&wp);
+  const int d = nt_delta_step_read_error(&wd);
+  return {p, static_cast<int64_t>(wp), d, static_cast<int64_t>(wd)};
+}
+
 }  // namespace
 
 // tcgen05 issue-rate probe (microbenchmark): out int64 [ctas, 3]
@@ -1324,6 +1578,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("xsa_bwd", &xsa_bwd);
   m.def("gated_rmsnorm_fwd", &gated_rmsnorm_fwd);
   m.def("gated_rmsnorm_bwd", &gated_rmsnorm_bwd);
+  m.def("paged_append", &paged_append, "rotated, normalised keys and values into a paged cache; returns the queries");
+  m.def("paged_attention", &paged_attention, "attention of new tokens over a paged cache");
+  m.def("delta_step", &delta_step, "recurrent gated delta rule with a carried fp32 state");
+  m.def("adjust_logits", &adjust_logits, "penalties, biases and grammar mask on logits");
+  m.def("read_serving_errors", &read_serving_errors);
   m.def("read_comm_errors", &read_comm_errors);
   m.def("gemm_ce_dgrad", &gemm_ce_dgrad);
   m.attr("EPI_BF16") = static_cast<int>(EPI_BF16);

@@ -38,3 +38,10 @@ def check_errors():
     if g or a or d or sp:
         raise RuntimeError(f"device pipeline wait expired: gemm code {g} at {gw:#x}, attention code {a} at {aw:#x}, "
                            f"delta scan code {d} at {dw:#x}, sparse attention code {sp} at {sw:#x}")
+    p, pw, ds, dsw = ext().read_serving_errors()
+    if p:
+        what = {1: "a position lies behind the row's page table", 2: "a page number lies outside the cache",
+                3: "a position lies behind the rotary table"}
+        raise RuntimeError(f"paged cache: {what.get(p, f'code {p}')} (row {pw})")
+    if ds:
+        raise RuntimeError(f"delta_recurrent: slot outside the states (row {dsw})")
