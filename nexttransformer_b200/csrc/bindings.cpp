@@ -1,10 +1,14 @@
 // Python bindings of the sm_100a kernels.  Only this file includes torch headers; the .cu
 // files export plain C++ launchers so that they compile quickly and stay independent of torch.
 #include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
 #include <atomic>
+#include <map>
+#include <mutex>
+#include <utility>
 
 #include "attention_sm100.h"
 #include "comm.h"
@@ -1339,6 +1343,7 @@ Tensor paged_append(const Tensor& q, const Tensor& k, const Tensor& v, const Ten
   }
   a.start = row_ints(start, q, a.B, "start");
   a.count = row_ints(count, q, a.B, "count");
+  a.sms = num_sms(q);
   a.norm = qk_scale.has_value();
   a.scale = static_cast<float>(qk_scale.value_or(1.0));
   a.fp16 = q.scalar_type() == at::kHalf;
@@ -1348,6 +1353,35 @@ Tensor paged_append(const Tensor& q, const Tensor& k, const Tensor& v, const Ten
   ok(nt_paged_append(a, stream()), "paged_append");
   C10_CUDA_KERNEL_LAUNCH_CHECK();
   return out;
+}
+
+// Zeroed counters that every call leaves at zero: one buffer for each device and stream, whose calls follow one
+// another.  A call under graph capture gets counters that no other call ever uses, since the graph may be replayed
+// beside any of them: a slice of a buffer that an earlier call has zeroed, or, when there is none, its own buffer,
+// which the graph then has to zero.
+Tensor stream_counters(const Tensor& like, int n) {
+  constexpr int64_t GRAPH_CALLS = 2048;
+  struct Kept {
+    std::mutex lock;
+    std::map<std::pair<int, cudaStream_t>, Tensor> streams;
+    std::map<int, std::pair<Tensor, int64_t>> graphs;  // buffer, slices given away
+  };
+  static auto* kept = new Kept();  // outlives the CUDA context's end
+  const auto options = like.options().dtype(at::kInt);
+  const int device = like.get_device();
+  const std::lock_guard<std::mutex> held(kept->lock);
+  if (c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None) {
+    auto it = kept->graphs.find(device);
+    if (it == kept->graphs.end() || it->second.second == GRAPH_CALLS) return at::zeros({n}, options);
+    return it->second.first.narrow(0, n * it->second.second++, n);
+  }
+  if (!kept->graphs.count(device)) {
+    kept->graphs[device] = {at::zeros({n * GRAPH_CALLS}, options), 0};
+    C10_CUDA_CHECK(cudaStreamSynchronize(stream()));  // once: graphs run on streams that know nothing of this one
+  }
+  Tensor& t = kept->streams[{device, stream()}];
+  if (!t.defined()) t = at::zeros({n}, options);
+  return t;
 }
 
 Tensor paged_attention(const Tensor& q, const Tensor& k_pages, const Tensor& v_pages, const Tensor& table,
@@ -1371,10 +1405,12 @@ Tensor paged_attention(const Tensor& q, const Tensor& k_pages, const Tensor& v_p
   Tensor out = at::empty({a.B, a.t, a.H, a.D}, q.options());
   if (out.numel() == 0) return out;
   a.out = out.data_ptr();
-  Tensor ws;
+  Tensor ws, counters;
   if (const size_t bytes = nt_paged_attn_workspace(a)) {
     ws = at::empty({static_cast<int64_t>(bytes / sizeof(float))}, q.options().dtype(at::kFloat));
     a.workspace = ws.data_ptr<float>();
+    counters = stream_counters(q, nt_paged_attn_counters(a.sms));
+    a.counters = reinterpret_cast<unsigned*>(counters.data_ptr<int>());
   }
   ok(nt_paged_attn(a, stream()), "paged_attention");
   C10_CUDA_KERNEL_LAUNCH_CHECK();

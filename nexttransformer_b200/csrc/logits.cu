@@ -5,10 +5,10 @@
 //   listed                     x <- x + bias (an id's entries are added in their order)
 //   not allowed                x <- -inf
 //
-// A CTA owns a piece of one row.  It asks for the piece's logits first, counts the row's tokens that fall
-// into the piece in shared memory while they travel (whole-number atomics: the order does not matter), and
-// writes fp32.  Reading and writing V (in + 4) bytes a row bounds it; the token list is read again by each
-// piece, from L2.
+// A CTA owns a piece of one row.  It streams the piece through first, masked but otherwise as it is, which waits
+// for nothing but its loads; meanwhile it counts the row's tokens that fall into the piece in shared memory
+// (whole-number atomics: their order does not matter) and then mends the few entries that tokens or biases
+// concern.  Reading and writing V (in + 4) bytes a row bounds it; the token list is read again by each piece, from L2.
 #include "logits.h"
 #include "common.cuh"
 
@@ -30,117 +30,139 @@ template <> struct In<__half> {
 template <> struct In<float> {
   static NT_DEVICE float f(float v) { return v; }
 };
-template <class T>
-struct alignas(4 * sizeof(T)) Four {
-  T x[4];
+template <class T, int N>
+struct alignas(N * sizeof(T)) Vec {
+  T x[N];
 };
-
-// PIECE logits a CTA, in vectors of VEC (4, or 1 where rows do not start on a vector).
+// PIECE logits a CTA, in vectors of VEC (4: a warp stores whole lines; or 1 where rows do not start on one).
 template <class T, int PIECE, int VEC>
 __global__ void __launch_bounds__(THREADS) adjust_kernel(const LogitsArgs a) {
-  constexpr int N = PIECE / THREADS / VEC;
-  extern __shared__ uint32_t smem[];
-  const int b = blockIdx.y, c0 = blockIdx.x * PIECE, tid = threadIdx.x;
+  constexpr int N = PIECE / THREADS / VEC, EARLY = 4;
+  __shared__ __align__(16) uint32_t counts[PIECE];
+  const int b = blockIdx.y, c0 = blockIdx.x * PIECE, tid = threadIdx.x, lane = tid & 31;
   const int width = min(PIECE, a.V - c0);
-  uint32_t* counts = smem;
-  float* bias = reinterpret_cast<float*>(smem + (a.tokens ? PIECE : 0));
-
   const T* in = static_cast<const T*>(a.logits) + b * a.row_stride + c0;
-  T x[N][VEC];
+  const int* allowed = a.allowed ? a.allowed + static_cast<int64_t>(b) * a.words : nullptr;
+  float* out = a.out + static_cast<int64_t>(b) * a.V + c0;
+
+  // the loads that depend on nothing are all asked for first
+  Vec<T, VEC> x[N];
+  uint32_t word[N];
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     const int at = (i * THREADS + tid) * VEC;
-    if (VEC == 4) {
-      if (at < width) *reinterpret_cast<Four<T>*>(x[i]) = *reinterpret_cast<const Four<T>*>(in + at);
-    } else if (at < width) {
-      x[i][0] = in[at];
+    word[i] = 0xffffffffu;
+    if (at < width) {
+      x[i] = *reinterpret_cast<const Vec<T, VEC>*>(in + at);
+      if (allowed) word[i] = static_cast<uint32_t>(allowed[(c0 + at) >> 5]) >> (at & 31);
     }
   }
-  if (a.tokens || a.K) {
-    if (a.tokens)
-      for (int i = tid; i < PIECE; i += THREADS) counts[i] = 0;
-    if (a.K)
-      for (int i = tid; i < PIECE; i += THREADS) bias[i] = 0.f;
-    __syncthreads();
-    if (a.tokens) {
-      const int n = a.length ? min(a.length[b], a.L) : a.L, prompt = a.prompt ? a.prompt[b] : 0;
-      const int* row = a.tokens + static_cast<int64_t>(b) * a.L;
-#pragma unroll 4
-      for (int i = tid; i < n; i += THREADS) {
-        const uint32_t at = static_cast<uint32_t>(row[i] - c0);
-        if (at < static_cast<uint32_t>(width)) {
-          if (i < prompt) atomicOr(counts + at, PROMPT);
-          else atomicAdd(counts + at, 1u);
-        }
-      }
-    }
-    if (a.K && tid < 32) {
-      for (int i = 0; i < a.K; i += 32) {
-        const bool live = i + tid < a.K;
-        const int64_t e = static_cast<int64_t>(b) * a.K + i + tid;
-        const uint32_t at = live ? static_cast<uint32_t>(a.bias_ids[e] - c0) : 0xffffffffu;
-        const float v = live ? a.bias[e] : 0.f;
-        const uint32_t same = __match_any_sync(0xffffffffu, at);
-        float sum = at < static_cast<uint32_t>(width) ? bias[at] : 0.f;
+  const int* row = a.tokens + static_cast<int64_t>(b) * a.L;
+  int early[EARLY];
 #pragma unroll
-        for (int l = 0; l < 32; ++l) {
-          const float w = __shfl_sync(0xffffffffu, v, l);
-          if ((same >> l) & 1u) sum += w;
-        }
-        if (at < static_cast<uint32_t>(width) && (same & ((1u << tid) - 1u)) == 0) bias[at] = sum;
-        __syncwarp();
-      }
-    }
-    __syncthreads();
-  }
+  for (int i = 0; i < EARLY; ++i) early[i] = i * THREADS + tid < a.L ? row[i * THREADS + tid] : -1;
+  const int n = a.length ? min(a.length[b], a.L) : a.L, prompt = a.prompt ? a.prompt[b] : 0;
   const float r = a.repetition ? a.repetition[b] : 1.f;
   const float presence = a.presence ? a.presence[b] : 0.f, frequency = a.frequency ? a.frequency[b] : 0.f;
-  const int* allowed = a.allowed ? a.allowed + static_cast<int64_t>(b) * a.words : nullptr;
-  float* out = a.out + static_cast<int64_t>(b) * a.V + c0;
+  const bool adds_bias = a.K && tid >= THREADS - 32;  // one warp: repeated ids are added in their order
+  const int64_t entry = static_cast<int64_t>(b) * a.K + lane;
+  int bias_id = adds_bias && lane < a.K ? a.bias_ids[entry] : -1;
+  float bias_value = adds_bias && lane < a.K ? a.bias[entry] : 0.f;
+
+  auto count = [&](int i, int token) {
+    const uint32_t at = static_cast<uint32_t>(token - c0);
+    if (i < n && at < static_cast<uint32_t>(width)) {
+      if (i < prompt) atomicOr(counts + at, PROMPT);
+      else atomicAdd(counts + at, 1u);
+    }
+  };
+  if (a.tokens) {
+    for (int i = tid; i < PIECE / 4; i += THREADS) reinterpret_cast<uint4*>(counts)[i] = make_uint4(0, 0, 0, 0);
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < EARLY; ++i) count(i * THREADS + tid, early[i]);
+#pragma unroll 4
+    for (int i = EARLY * THREADS + tid; i < n; i += THREADS) count(i, row[i]);
+  }
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     const int at = (i * THREADS + tid) * VEC;
     if (at >= width) continue;
-    const uint32_t word = allowed ? static_cast<uint32_t>(allowed[(c0 + at) >> 5]) >> (at & 31) : 0xffffffffu;
     float y[VEC];
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-      float v = In<T>::f(x[i][e]);
-      if (a.tokens) {
-        const uint32_t c = counts[at + e], n = c & ~PROMPT;
-        if (c) v = v > 0.f ? v / r : v * r;
-        if (n) v = v - frequency * static_cast<float>(n) - presence;
-      }
-      if (a.K) v += bias[at + e];
-      y[e] = (word >> e) & 1u ? v : -INFINITY;
+    for (int e = 0; e < VEC; ++e) y[e] = (word[i] >> e) & 1u ? In<T>::f(x[i].x[e]) : -INFINITY;
+    if (VEC >= 4) {
+#pragma unroll
+      for (int e = 0; e < VEC / 4; ++e)
+        reinterpret_cast<float4*>(out + at)[e] = make_float4(y[4 * e], y[4 * e + 1], y[4 * e + 2], y[4 * e + 3]);
+    } else {
+      out[at] = y[0];
     }
-    if (VEC == 4) *reinterpret_cast<float4*>(out + at) = make_float4(y[0], y[VEC > 1 ? 1 : 0], y[VEC > 2 ? 2 : 0], y[VEC > 3 ? 3 : 0]);
-    else out[at] = y[0];
+  }
+  if (!a.tokens && !a.K) return;
+  __syncthreads();
+
+  auto is_allowed = [&](uint32_t at) { return !allowed || (static_cast<uint32_t>(allowed[(c0 + at) >> 5]) >> ((c0 + at) & 31)) & 1u; };
+  auto mend = [&](int i, int token) {  // whoever takes an entry's count mends it
+    const uint32_t at = static_cast<uint32_t>(token - c0);
+    if (i >= n || at >= static_cast<uint32_t>(width)) return;
+    const uint32_t c = atomicExch(counts + at, 0u), times = c & ~PROMPT;
+    if (c == 0 || !is_allowed(at)) return;
+    float v = In<T>::f(in[at]);
+    v = v > 0.f ? v / r : v * r;
+    if (times) v = v - frequency * static_cast<float>(times) - presence;
+    out[at] = v;
+  };
+  if (a.tokens) {
+#pragma unroll 1
+    for (int i = 0; i < EARLY; ++i) {
+      int token = early[0];
+#pragma unroll
+      for (int e = 1; e < EARLY; ++e) token = i == e ? early[e] : token;
+      mend(i * THREADS + tid, token);
+    }
+    for (int i = EARLY * THREADS + tid; i < n; i += THREADS) mend(i, row[i]);
+    if (a.K) __syncthreads();
+  }
+  if (!adds_bias) return;
+  for (int i = 0; i < a.K; i += 32) {
+    const int id = bias_id;
+    const float v = bias_value;
+    const bool more = i + 32 + lane < a.K;
+    bias_id = more ? a.bias_ids[entry + i + 32] : -1;
+    bias_value = more ? a.bias[entry + i + 32] : 0.f;
+    const uint32_t at = static_cast<uint32_t>(id - c0);
+    const bool mine = id >= 0 && at < static_cast<uint32_t>(width);
+    if (!__any_sync(0xffffffffu, mine)) continue;
+    unsigned same = __match_any_sync(0xffffffffu, mine ? at : 0xffffffffu);
+    const bool first = (same & ((1u << lane) - 1u)) == 0;
+    if (!mine) same = 0;
+    float sum = mine ? out[at] : 0.f;
+    while (__any_sync(0xffffffffu, same)) {
+      const float w = __shfl_sync(0xffffffffu, v, same ? __ffs(same) - 1 : 0);
+      if (same) sum += w;
+      same &= same - (same ? 1u : 0u);
+    }
+    if (mine && first && is_allowed(at)) out[at] = sum;
+    __syncwarp();
   }
 }
 
 template <class T, int PIECE>
 static int launch(const LogitsArgs& a, cudaStream_t s) {
+  constexpr int VEC = 4;
   const dim3 grid((a.V + PIECE - 1) / PIECE, a.B);
-  const int smem = PIECE * 4 * ((a.tokens ? 1 : 0) + (a.K ? 1 : 0));
-  const bool vec = a.V % 4 == 0 && a.row_stride % 4 == 0 &&
-                   reinterpret_cast<uintptr_t>(a.logits) % (4 * sizeof(T)) == 0;
-  if (vec) {
-    static std::atomic<uint64_t> done{0};
-    if (smem_limit(done, adjust_kernel<T, PIECE, 4>, PIECE * 8) != cudaSuccess) return -1;
-    adjust_kernel<T, PIECE, 4><<<grid, THREADS, smem, s>>>(a);
-  } else {
-    static std::atomic<uint64_t> done{0};
-    if (smem_limit(done, adjust_kernel<T, PIECE, 1>, PIECE * 8) != cudaSuccess) return -1;
-    adjust_kernel<T, PIECE, 1><<<grid, THREADS, smem, s>>>(a);
-  }
+  if (a.V % VEC == 0 && a.row_stride % VEC == 0 && reinterpret_cast<uintptr_t>(a.logits) % (4 * sizeof(T)) == 0)
+    adjust_kernel<T, PIECE, VEC><<<grid, THREADS, 0, s>>>(a);
+  else
+    adjust_kernel<T, PIECE, 1><<<grid, THREADS, 0, s>>>(a);
   return 0;
 }
 template <class T>
 static int by_piece(const LogitsArgs& a, cudaStream_t s) {
   // large pieces read the token list less often, small ones reach more SMs
-  if (static_cast<int64_t>(a.B) * ((a.V + 4095) / 4096) >= 2 * a.sms) return launch<T, 4096>(a, s);
-  return launch<T, 1024>(a, s);
+  if (static_cast<int64_t>(a.B) * ((a.V + 8191) / 8192) >= 2 * a.sms) return launch<T, 8192>(a, s);
+  return launch<T, 2048>(a, s);
 }
 
 }  // namespace logits

@@ -41,100 +41,204 @@ template <> struct Num<__half> {
   }
 };
 
-template <class T>
-NT_DEVICE void unpack8(const uint4& u, float (&x)[8]) {
-  const float2 a = Num<T>::unpack(u.x), b = Num<T>::unpack(u.y), c = Num<T>::unpack(u.z), d = Num<T>::unpack(u.w);
-  x[0] = a.x; x[1] = a.y; x[2] = b.x; x[3] = b.y; x[4] = c.x; x[5] = c.y; x[6] = d.x; x[7] = d.y;
-}
-template <class T>
-NT_DEVICE uint4 pack8(const float (&x)[8]) {
-  return make_uint4(Num<T>::pack(x[0], x[1]), Num<T>::pack(x[2], x[3]), Num<T>::pack(x[4], x[5]), Num<T>::pack(x[6], x[7]));
-}
-
 // ------------------------------------------------------------------------------------ append
-// D / 8 lanes hold one head of one token, 16 bytes each; the two halves of a rotated pair are D / 16
-// lanes apart.  One pass: every input element is read once and every output element written once.
-template <class T, int D>
-__global__ void __launch_bounds__(256) append_kernel(const PagedAppendArgs a) {
-  constexpr int L = D / 8;
-  const int heads = a.H + 2 * a.Hk;
-  const int64_t unit = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) / L;
-  const int lane = threadIdx.x % L;
-  const int64_t units = static_cast<int64_t>(a.B) * a.t * heads;
-  const bool live = unit < units;  // whole warps stay for the shuffles
-  const int64_t tok = live ? unit / heads : 0;
-  const int h = live ? static_cast<int>(unit - tok * heads) : 0;
-  const int b = static_cast<int>(tok / a.t), i = static_cast<int>(tok - static_cast<int64_t>(b) * a.t);
-  const int kind = h < a.H ? 0 : h < a.H + a.Hk ? 1 : 2;  // q, k, v
-  const int hh = kind == 0 ? h : kind == 1 ? h - a.H : h - a.H - a.Hk;
-
-  const T* src = static_cast<const T*>(kind == 0 ? a.q : kind == 1 ? a.kin : a.vin);
-  const int64_t* st = kind == 0 ? a.qs : kind == 1 ? a.ks : a.vs;
-  const uint4 raw = live ? *reinterpret_cast<const uint4*>(src + b * st[0] + i * st[1] + hh * st[2] + lane * 8)
-                         : make_uint4(0, 0, 0, 0);
+// D / 8 lanes hold one head of one token; lane j has channels 4 j to 4 j + 3 of each half, so that it holds
+// both members of its rotated pairs.  They take PER heads of their token, whose loads are all in flight at once
+// and which share the token's angles and place in the cache.  Blocks with small y turn queries and keys, the
+// others mix values.  One pass: every input element is read once and every output element written once.
+template <class T>
+NT_DEVICE void load_halves(const T* p, int half, uint2& lo, uint2& hi) {
+  lo = __ldcs(reinterpret_cast<const uint2*>(p));
+  hi = __ldcs(reinterpret_cast<const uint2*>(p + half));
+}
+template <class T>
+NT_DEVICE void unpack4(uint2 u, float (&x)[4]) {
+  const float2 a = Num<T>::unpack(u.x), b = Num<T>::unpack(u.y);
+  x[0] = a.x; x[1] = a.y; x[2] = b.x; x[3] = b.y;
+}
+template <class T>
+NT_DEVICE uint2 pack4(const float (&x)[4]) {
+  return make_uint2(Num<T>::pack(x[0], x[1]), Num<T>::pack(x[2], x[3]));
+}
+// x / n for 0 <= x < 2^31 and 0 < n: the float quotient is at most a few units off
+NT_DEVICE int quotient(int x, int n) {
+  int q = static_cast<int>(__fdividef(static_cast<float>(x), static_cast<float>(n)));
+  int rest = x - q * n;
+  while (rest < 0) {
+    --q;
+    rest += n;
+  }
+  while (rest >= n) {
+    ++q;
+    rest -= n;
+  }
+  return q;
+}
+template <class T, int D, int PER>
+__global__ void __launch_bounds__(256, 5) append_kernel(const PagedAppendArgs a, const int turning) {
+  constexpr int L = D / 8, HALF = D / 2;
+  const int lane = threadIdx.x % L, tok = blockIdx.x * (256 / L) + threadIdx.x / L;
+  const bool live = tok < a.B * a.t;  // whole warps stay for the shuffles
+  const int b = live ? (a.t == 1 ? tok : quotient(tok, a.t)) : 0, i = live ? tok - b * a.t : 0;
   const int start = a.start[b], n = a.count ? a.count[b] : a.t;
-  const bool real = live && i < n && start >= 0;
-  const int64_t pos = static_cast<int64_t>(start) + i;
-
-  const bool turned = kind < 2;
-  const bool in = real && (!turned || pos < a.rope_rows);
-  if (real && !in && lane == 0) record_error(3, b);
-  float x[8], y[8], c[8], s[8];
-  unpack8<T>(raw, x);
-  uint4 cw = make_uint4(0, 0, 0, 0), sw = cw;
-  if (turned && in) {
-    const int64_t at = pos * (D / 2) + (lane % (L / 2)) * 8;
-    cw = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.cos) + at);
-    sw = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.sin) + at);
+  bool real = live && i < n && start >= 0;
+  if (real && start >= a.rope_rows - i) {
+    if (lane == 0) record_error(3, b);
+    real = false;
   }
-  unpack8<T>(cw, c);
-  unpack8<T>(sw, s);
-  const float sign = lane < L / 2 ? 1.f : -1.f;
-  float sum = 0.f;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const float other = __shfl_xor_sync(0xffffffffu, x[e], L / 2);
-    y[e] = fmaf(sign * other, s[e], x[e] * c[e]);
-    sum = fmaf(y[e], y[e], sum);
-  }
-#pragma unroll
-  for (int o = L / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  if (!live) return;
-  if (turned) {
-    const float r = a.norm ? a.scale * rsqrtf(sum * (1.f / D) + EPS) : 1.f;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = in ? y[e] * r : 0.f;
-  } else if (a.ve && real) {
-    float w[8];
-    unpack8<T>(*reinterpret_cast<const uint4*>(static_cast<const T*>(a.ve) + b * a.es[0] + i * a.es[1] + hh * a.es[2] +
-                                               lane * 8),
-               w);
-    const float gate = Num<T>::one(static_cast<const T*>(a.ve_gate)[b * a.gs[0] + i * a.gs[1] + hh * a.gs[2]]);
-    const float f = 3.f / (1.f + __expf(-gate));
-#pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = fmaf(f, w[e], x[e]);
-  }
-  const uint4 o = pack8<T>(x);
-  if (kind == 0) {  // tokens behind a row's count give zeros
-    *reinterpret_cast<uint4*>(static_cast<T*>(a.q_out) + (tok * a.H + hh) * D + lane * 8) = o;
-    return;
-  }
-  if (!in) return;
+  const int pos = real ? start + i : 0;
+  // the token's place in the cache
   const PagedCacheArgs& m = a.cache;
-  const int64_t column = pos / m.page;
-  if (column >= m.columns) {
-    if (lane == 0) record_error(1, b);
-    return;
-  }
-  const int64_t page = m.table[static_cast<int64_t>(b) * m.columns + column];
-  if (page < 0 || page >= m.pages) {
+  auto find_page = [&](int& slot) -> int64_t {
+    const int column = quotient(pos, m.page);
+    slot = pos - column * m.page;
+    if (column >= m.columns) {
+      if (lane == 0) record_error(1, b);
+      return -1;
+    }
+    const int page = m.table[static_cast<int64_t>(b) * m.columns + column];
+    if (page >= 0 && page < m.pages) return page;
     if (lane == 0) record_error(2, b);
+    return -1;
+  };
+
+  if (static_cast<int>(blockIdx.y) >= turning) {
+    // ---- values
+    if (!real) return;
+    const int h0 = (blockIdx.y - turning) * PER, heads = min(PER, a.Hk - h0);
+    uint2 lo[PER], hi[PER], elo[PER], ehi[PER];
+    T gate[PER];
+    const T* src = static_cast<const T*>(a.vin) + b * a.vs[0] + i * a.vs[1] + h0 * a.vs[2] + lane * 4;
+#pragma unroll
+    for (int e = 0; e < PER; ++e)
+      if (e < heads) {
+        load_halves(src, HALF, lo[e], hi[e]);
+        src += a.vs[2];
+      }
+    if (a.ve) {
+      const T* es = static_cast<const T*>(a.ve) + b * a.es[0] + i * a.es[1] + h0 * a.es[2] + lane * 4;
+      const T* gs = static_cast<const T*>(a.ve_gate) + b * a.gs[0] + i * a.gs[1] + h0 * a.gs[2];
+#pragma unroll
+      for (int e = 0; e < PER; ++e)
+        if (e < heads) {
+          load_halves(es, HALF, elo[e], ehi[e]);
+          gate[e] = *gs;
+          es += a.es[2];
+          gs += a.gs[2];
+        }
+    }
+    int slot;
+    const int64_t page = find_page(slot);
+    if (page < 0) return;
+    T* dst = static_cast<T*>(m.v) + page * m.page_stride_v + slot * m.slot_stride_v + h0 * m.head_stride_v + lane * 4;
+#pragma unroll
+    for (int e = 0; e < PER; ++e) {
+      if (e >= heads) break;
+      if (a.ve) {
+        float x[4], y[4], w[4];
+        const float f = 3.f / (1.f + __expf(-Num<T>::one(gate[e])));
+        unpack4<T>(lo[e], x); unpack4<T>(elo[e], w);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[j] = fmaf(f, w[j], x[j]);
+        unpack4<T>(hi[e], y); unpack4<T>(ehi[e], w);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) y[j] = fmaf(f, w[j], y[j]);
+        lo[e] = pack4<T>(x);
+        hi[e] = pack4<T>(y);
+      }
+      *reinterpret_cast<uint2*>(dst) = lo[e];
+      *reinterpret_cast<uint2*>(dst + HALF) = hi[e];
+      dst += m.head_stride_v;
+    }
     return;
   }
-  const int64_t slot = pos - column * m.page;
-  T* dst = kind == 1 ? static_cast<T*>(m.k) + page * m.page_stride_k + hh * m.head_stride_k + slot * m.slot_stride_k
-                     : static_cast<T*>(m.v) + page * m.page_stride_v + hh * m.head_stride_v + slot * m.slot_stride_v;
-  *reinterpret_cast<uint4*>(dst + lane * 8) = o;
+
+  // ---- queries and keys; h counts through both
+  const int h0 = blockIdx.y * PER, heads = min(PER, a.H + a.Hk - h0);
+  T* q_out = static_cast<T*>(a.q_out) + (static_cast<int64_t>(tok) * a.H + h0) * D + lane * 4;
+  uint2 lo[PER], hi[PER];
+#pragma unroll
+  for (int e = 0; e < PER; ++e) lo[e] = hi[e] = make_uint2(0, 0);
+  if (real) {
+    const T* src = h0 < a.H ? static_cast<const T*>(a.q) + b * a.qs[0] + i * a.qs[1] + h0 * a.qs[2] + lane * 4 : nullptr;
+    int64_t step = a.qs[2];
+#pragma unroll
+    for (int e = 0; e < PER; ++e)
+      if (e < heads) {
+        if (h0 + e == a.H || (e == 0 && h0 > a.H)) {
+          src = static_cast<const T*>(a.kin) + b * a.ks[0] + i * a.ks[1] + (h0 + e - a.H) * a.ks[2] + lane * 4;
+          step = a.ks[2];
+        }
+        load_halves(src, HALF, lo[e], hi[e]);
+        src += step;
+      }
+  }
+  T* k_out = nullptr;
+  float c[4] = {}, s[4] = {};
+  if (real) {
+    if (h0 + heads > a.H) {
+      int slot;
+      const int64_t page = find_page(slot);
+      if (page >= 0)
+        k_out = static_cast<T*>(m.k) + page * m.page_stride_k + slot * m.slot_stride_k + max(h0 - a.H, 0) * m.head_stride_k + lane * 4;
+    }
+    unpack4<T>(*reinterpret_cast<const uint2*>(static_cast<const T*>(a.cos) + static_cast<int64_t>(pos) * HALF + lane * 4), c);
+    unpack4<T>(*reinterpret_cast<const uint2*>(static_cast<const T*>(a.sin) + static_cast<int64_t>(pos) * HALF + lane * 4), s);
+  }
+#pragma unroll
+  for (int e = 0; e < PER; ++e) {
+    if (e >= heads) break;
+    float x[4], y[4], u[4], w[4], r = 1.f;
+    unpack4<T>(lo[e], x);
+    unpack4<T>(hi[e], y);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      u[j] = fmaf(y[j], s[j], x[j] * c[j]);
+      w[j] = fmaf(-x[j], s[j], y[j] * c[j]);
+    }
+    if (a.norm) {
+      float sum = 0.f;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) sum = fmaf(u[j], u[j], fmaf(w[j], w[j], sum));
+#pragma unroll
+      for (int o = L / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      r = a.scale * rsqrtf(sum * (1.f / D) + EPS);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        u[j] *= r;
+        w[j] *= r;
+      }
+    }
+    T* dst;
+    if (h0 + e < a.H) {  // tokens behind a row's count have zeros in, and give zeros
+      dst = live ? q_out : nullptr;
+      q_out += D;
+    } else {
+      dst = k_out;
+      if (k_out) k_out += m.head_stride_k;
+    }
+    if (dst) {
+      *reinterpret_cast<uint2*>(dst) = pack4<T>(u);
+      *reinterpret_cast<uint2*>(dst + HALF) = pack4<T>(w);
+    }
+  }
+}
+
+template <class T, int D, int PER>
+static int launch_append(const PagedAppendArgs& a, unsigned blocks, cudaStream_t s) {
+  const int turning = (a.H + a.Hk + PER - 1) / PER, mixing = (a.Hk + PER - 1) / PER;
+  if (turning + mixing > 65535) return -1;
+  append_kernel<T, D, PER><<<dim3(blocks, turning + mixing), 256, 0, s>>>(a, turning);
+  return 0;
+}
+template <class T, int D>
+static int launch_append(const PagedAppendArgs& a, cudaStream_t s) {
+  const int64_t tokens = static_cast<int64_t>(a.B) * a.t, per_block = 256 / (D / 8), blocks = (tokens + per_block - 1) / per_block;
+  if (tokens > INT32_MAX - per_block) return -1;
+  // four heads a thread keep enough bytes in flight and share a token's address work; with few tokens, one head
+  // a thread reaches more SMs
+  return blocks * ((a.H + 2 * a.Hk + 3) / 4) >= 2 * a.sms ? launch_append<T, D, 4>(a, static_cast<unsigned>(blocks), s)
+                                                          : launch_append<T, D, 1>(a, static_cast<unsigned>(blocks), s);
 }
 
 // --------------------------------------------------------------------------------- attention
@@ -150,9 +254,9 @@ __global__ void __launch_bounds__(256) append_kernel(const PagedAppendArgs a) {
 // Work: a row's keys (window cut off) are tiles of 16.  The tiles of all rows and KV heads form one line,
 // each CTA takes an equal piece of it and each warp an equal piece of that, so unequal rows load the SMs
 // equally and one long row uses all of them.  A warp that covers a whole (row, KV head) writes its result;
-// pieces are joined in the CTA through shared memory, and what crosses CTAs by join_kernel, both in the
-// order of the line, so results do not depend on timing.
-constexpr int WARPS = 8, TILE = 16, MIN_TILES = 1;
+// other pieces are joined in the CTA, and what crosses CTAs by the CTA that arrives last, up to 16 pieces at
+// a time.  Pieces are always joined in the order of the line, so results do not depend on timing.
+constexpr int WARPS = 8, TILE = 16, MIN_TILES = 4, FAN = 16;
 // Rows of the batch whose tiles a CTA lines up in shared memory; a larger batch has CTAs enough and gives
 // each (row, KV head) one.
 constexpr int MAX_ITEMS = 384;
@@ -160,53 +264,79 @@ constexpr int MAX_ITEMS = 384;
 template <int D, int NQ>
 struct Shape {
   static constexpr int NR = NQ * 8;
-  static constexpr int HALF = TILE * D * 2, STAGE = 2 * HALF;              // bytes of K, of K and V
-  static constexpr int STAGES = D == 128 ? (NQ == 1 ? 3 : 2) : (NQ == 1 ? 6 : 5);
-  static constexpr int RING = STAGES * STAGE;                              // of one warp
-  static constexpr int ROW = D + 4;                                        // floats: D sums, maximum, total, 2 unused
-  static constexpr int PART = NR * ROW * 4;
-  static constexpr int SMEM = WARPS * (RING + PART);
-  static_assert(PART <= RING, "a warp's last piece lies in its own ring");
-  static_assert(SMEM + 2048 <= 227 * 1024, "shared memory of an SM");
+  static constexpr int HALF = TILE * D * 2, STAGE = 2 * HALF;  // bytes of K, of K and V
+  static constexpr int STAGES = D == 128 ? 3 : 6;              // 24 KB a warp, 192 KB an SM
+  static constexpr int RING = STAGES * STAGE;
+  // Floats of a piece, in the order of the accumulators: NQ x D / 16 blocks of 32 lanes x 4 sums, then for each
+  // NQ and lane % 4 the maxima and totals of that lane's two queries
+  static constexpr int BLOCKS = NQ * (D / 16), PART = BLOCKS * 128 + NQ * 16;
+  static constexpr int SMEM = WARPS * RING;
+  static_assert(PART * 4 <= RING, "a warp's last piece lies in its own ring");
 };
+// Workspace: two pieces a CTA (1: a (row, KV head) that begins there, 0: one that began earlier), one piece
+// a warp (its first, where that is not its last), and three counters a CTA.
+static int64_t ws_floats(int64_t grid, int part) { return grid * (2 + WARPS) * part; }
+constexpr int COUNTERS = 3;
 
 struct Item {      // a row tile of one row of the batch
   int b, r0;       // row, first query row
   int start, n;    // tokens before the call, new tokens
   int first, end;  // keys [first, end) that one of the query rows sees
+  int all_from, all_to;  // keys [all_from, all_to) that all of them see
   int tiles;       // from first rounded down to 16; at least 1, so that rows without keys are written
 };
 
-NT_DEVICE Item get_item(const PagedAttnArgs& a, int id, int row_tiles, int NR, int group, int capacity) {
+// r / group with the rounded-up reciprocal of the group (exact while r group < 2^32; 0 stands for a group of 1)
+NT_DEVICE int token_of(int r, uint32_t inverse) { return inverse ? static_cast<int>(__umulhi(r, inverse)) : r; }
+
+struct Geometry {
+  int items, row_tiles, group, R, capacity;
+  uint32_t inverse;
+  bool direct;
+};
+
+// A row's tokens before the call, and its new ones.
+NT_DEVICE int2 span_of(const PagedAttnArgs& a, const Geometry& g, int id) {
+  const int b = g.row_tiles == 1 ? id : id / g.row_tiles, start = a.start[b], n = a.count ? min(a.count[b], a.t) : a.t;
+  return make_int2(start, start < 0 ? 0 : n);
+}
+template <int NR>
+NT_DEVICE Item get_item(const PagedAttnArgs& a, const Geometry& g, int id, int2 span) {
   Item it;
-  it.b = id / row_tiles;
-  it.r0 = (id - it.b * row_tiles) * NR;
-  it.start = a.start[it.b];
-  it.n = a.count ? min(a.count[it.b], a.t) : a.t;
-  if (it.start < 0) it.n = 0;
-  const int i0 = it.r0 / group, i1 = min((it.r0 + NR - 1) / group, it.n - 1);
-  it.first = it.end = 0;
+  it.b = g.row_tiles == 1 ? id : id / g.row_tiles;
+  it.r0 = (id - it.b * g.row_tiles) * NR;
+  it.start = span.x;
+  it.n = span.y;
+  const int i0 = token_of(it.r0, g.inverse), i1 = min(token_of(min(it.r0 + NR, g.R) - 1, g.inverse), it.n - 1);
+  it.first = it.end = it.all_from = it.all_to = 0;
   if (i0 <= i1) {
-    it.end = static_cast<int>(min(static_cast<int64_t>(it.start) + i1 + 1, static_cast<int64_t>(capacity)));
-    it.first = a.window >= 0 ? max(0, min(it.start + i0 - a.window, it.end)) : 0;
+    it.end = static_cast<int>(min(static_cast<int64_t>(it.start) + i1 + 1, static_cast<int64_t>(g.capacity)));
+    it.all_to = min(it.start + i0 + 1, it.end);
+    if (a.window >= 0) {
+      it.first = max(0, min(it.start + i0 - a.window, it.end));
+      it.all_from = max(0, it.start + i1 - a.window);
+    }
   }
   it.tiles = max(1, (it.end - (it.first & ~(TILE - 1)) + TILE - 1) / TILE);
   return it;
 }
 
-NT_DEVICE void cp_async16(uint32_t dst, const void* src, int bytes) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+NT_DEVICE void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+NT_DEVICE void cp_async16_or_zero(uint32_t dst, const void* src, bool valid) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
 }
 NT_DEVICE void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 NT_DEVICE void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 NT_DEVICE void ldsm4(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
 NT_DEVICE void ldsm4t(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
 NT_DEVICE uint32_t transpose8x8(uint32_t v) {
   uint32_t r;
@@ -222,13 +352,16 @@ NT_DEVICE float exp2_fast(float x) {
 NT_DEVICE float piece_weight(float m, float top) { return top == -INFINITY ? 0.f : exp2_fast(m - top); }
 // A row without keys gives zeros; a total of NaN stays NaN.
 NT_DEVICE float inverse_total(float l) { return l == 0.f ? 0.f : 1.f / l; }
+NT_DEVICE float weighted(float w, float x) { return w == 0.f ? 0.f : w * x; }
 
 // Where a warp's copies stand on the line.
 struct Cursor {
-  int id, hk, j;   // item, KV head, tile
+  int id, hk, j;       // item, KV head, tile
   Item it;
-  int column, slot;            // of the tile's first key
-  int seen, pages;             // lane l holds the page of column seen + l
+  int column, slot;    // of the tile's first key
+  int seen, pages;     // lane l holds the page of column seen + l
+  bool there;          // the page lies in the cache
+  const void *k, *v;   // this lane's first element of the tile
 };
 
 NT_DEVICE void load_pages(const PagedAttnArgs& a, Cursor& c, int lane) {
@@ -236,39 +369,131 @@ NT_DEVICE void load_pages(const PagedAttnArgs& a, Cursor& c, int lane) {
   const int col = c.column + lane;
   c.pages = col < a.cache.columns ? a.cache.table[static_cast<int64_t>(c.it.b) * a.cache.columns + col] : -1;
 }
-NT_DEVICE void enter(const PagedAttnArgs& a, Cursor& c, int row_tiles, int NR, int group, int capacity, int lane) {
-  c.it = get_item(a, c.id, row_tiles, NR, group, capacity);
+template <int NR>
+NT_DEVICE void enter(const PagedAttnArgs& a, const Geometry& g, Cursor& c, int2 span, int lane) {
+  c.it = get_item<NR>(a, g, c.id, span);
   const int key = (c.it.first & ~(TILE - 1)) + c.j * TILE;
-  c.column = key / a.cache.page;
+  c.column = quotient(key, a.cache.page);
   c.slot = key - c.column * a.cache.page;
   load_pages(a, c, lane);
+}
+// The tile's page is the next of the list (or the item's first).
+template <class T>
+NT_DEVICE void turn_page(const PagedAttnArgs& a, Cursor& c, const T* kc, const T* vc, int lane) {
+  if (c.column - c.seen >= 32) load_pages(a, c, lane);
+  const int page = __shfl_sync(0xffffffffu, c.pages, c.column - c.seen);
+  c.there = page >= 0 && page < a.cache.pages;
+  if (!c.there && c.it.first < c.it.end && lane == 0) record_error(2, c.it.b);
+  const int64_t p = c.there ? page : 0;
+  c.k = kc + p * a.cache.page_stride_k + c.hk * a.cache.head_stride_k + c.slot * a.cache.slot_stride_k;
+  c.v = vc + p * a.cache.page_stride_v + c.hk * a.cache.head_stride_v + c.slot * a.cache.slot_stride_v;
+}
+
+// Joins block blk of up to 16 pieces; piece(k) is the k-th, in the order of the line.  stat gets the maxima and
+// totals of the lane's two queries.
+template <int D, int NQ, bool L2, class Piece>
+NT_DEVICE float4 join_block(int n, int blk, int lane, Piece piece, float4& stat) {
+  using S = Shape<D, NQ>;
+  auto load = [](const float* p) {
+    return L2 ? __ldcg(reinterpret_cast<const float4*>(p)) : *reinterpret_cast<const float4*>(p);
+  };
+  const int stats = S::BLOCKS * 128 + (blk / (D / 16)) * 16 + (lane & 3) * 4, sums = blk * 128 + lane * 4;
+  float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+  stat = make_float4(-INFINITY, 0.f, -INFINITY, 0.f);
+#pragma unroll 1
+  for (int from = 0; from < n; from += 8) {
+    float4 t[8], v[8];  // eight pieces are asked for at once
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      t[k] = make_float4(-INFINITY, 0.f, -INFINITY, 0.f);
+      if (from + k < n) {
+        const float* p = piece(from + k);
+        t[k] = load(p + stats);
+        v[k] = load(p + sums);
+      }
+    }
+    float top0 = stat.x, top1 = stat.z;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      top0 = fmaxf(top0, t[k].x);
+      top1 = fmaxf(top1, t[k].z);
+    }
+    const float f0 = piece_weight(stat.x, top0), f1 = piece_weight(stat.z, top1);
+    stat = make_float4(top0, f0 * stat.y, top1, f1 * stat.w);
+    sum.x *= f0; sum.y *= f1; sum.z *= f0; sum.w *= f1;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const float w0 = piece_weight(t[k].x, top0), w1 = piece_weight(t[k].z, top1);
+      if (w0 != 0.f) {  // rows without keys count for nothing, whatever their sums are
+        stat.y = fmaf(w0, t[k].y, stat.y);
+        sum.x = fmaf(w0, v[k].x, sum.x);
+        sum.z = fmaf(w0, v[k].z, sum.z);
+      }
+      if (w1 != 0.f) {
+        stat.w = fmaf(w1, t[k].w, stat.w);
+        sum.y = fmaf(w1, v[k].y, sum.y);
+        sum.w = fmaf(w1, v[k].w, sum.w);
+      }
+    }
+  }
+  return sum;
+}
+template <int D, int NQ>
+NT_DEVICE void store_block(float* piece, int blk, int lane, const float4& sum, const float4& stat) {
+  using S = Shape<D, NQ>;
+  *reinterpret_cast<float4*>(piece + blk * 128 + lane * 4) = sum;
+  if (blk % (D / 16) == 0 && lane < 4)
+    *reinterpret_cast<float4*>(piece + S::BLOCKS * 128 + (blk / (D / 16)) * 16 + lane * 4) = stat;
+}
+// The output rows of a block of 8 queries: to the row of the query that a lane holds after the transpose.
+template <class T, int D>
+NT_DEVICE T* output_row(const PagedAttnArgs& a, const Geometry& g, int b, int r, int hk, int lane) {
+  r = min(r, g.R - 1);
+  const int i = token_of(r, g.inverse);
+  return static_cast<T*>(a.out) +
+         ((static_cast<int64_t>(b) * a.t + i) * a.H + hk * g.group + (r - i * g.group)) * D + (lane & 3) * 2;
+}
+template <class T>
+NT_DEVICE void write_block(T* row, bool live, int d, const float4& sum, float w0, float w1) {
+  const uint32_t u0 = transpose8x8(Num<T>::pack(weighted(w0, sum.x), weighted(w1, sum.y)));
+  const uint32_t u1 = transpose8x8(Num<T>::pack(weighted(w0, sum.z), weighted(w1, sum.w)));
+  if (live) {
+    *reinterpret_cast<uint32_t*>(row + d * 16) = u0;
+    *reinterpret_cast<uint32_t*>(row + d * 16 + 8) = u1;
+  }
 }
 
 template <class T, int D, int NQ>
 __global__ void __launch_bounds__(WARPS * 32, 1)
-    attn_kernel(const PagedAttnArgs a, const int items, const int row_tiles, const bool direct, float* ws_part, int4* ws_desc) {
+    attn_kernel(const PagedAttnArgs a, const Geometry g, float* ws, unsigned* counters) {
   using S = Shape<D, NQ>;
   constexpr int NR = S::NR, CHUNKS = D / 8;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ int pre[MAX_ITEMS + 1];
-  __shared__ int warp_sum_[WARPS];
+  __shared__ int2 spans[MAX_ITEMS];
+  __shared__ int warp_total[WARPS];
   __shared__ int part_id[2 * WARPS], part_flag[2 * WARPS];
+  __shared__ bool arrived_last;
+  float4* joined = reinterpret_cast<float4*>(smem);  // the rings are done with when CTAs' pieces are joined
+  float4* joined_stat = joined + S::BLOCKS * 32;
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int group = a.H / a.Hk, R = a.t * group, Hk = a.Hk;
-  const int capacity = static_cast<int>(min(static_cast<int64_t>(a.cache.columns) * a.cache.page, static_cast<int64_t>(INT32_MAX)));
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int Hk = a.Hk, me = blockIdx.x;
+  float* ws_warp = ws + (static_cast<int64_t>(gridDim.x) * 2 + static_cast<int64_t>(me) * WARPS) * S::PART;
 
-  // ---- this CTA's piece [lo, hi) of the line
-  int64_t lo, hi, W = 0;
-  int G = 1, base_id = 0, base_hk = 0;
-  if (direct) {
-    base_id = blockIdx.x / Hk;
-    base_hk = blockIdx.x - base_id * Hk;
-    lo = 0;
-    const Item it = get_item(a, base_id, row_tiles, NR, group, capacity);
+  // ---- this CTA's piece [lo, hi) of the line: each of G has `each` tiles, the first `more` one more
+  int lo = 0, hi, G = 1, each = 0, more = 0, base_id = 0, base_hk = 0;
+  if (g.direct) {
+    base_id = me / Hk;
+    base_hk = me - base_id * Hk;
+    const int2 span = span_of(a, g, base_id);
+    const Item it = get_item<NR>(a, g, base_id, span);
     hi = it.tiles;
-    if (tid == 0 && it.n > 0 && static_cast<int64_t>(it.start) + it.n > capacity) record_error(1, it.b);
+    if (tid == 0) {
+      spans[0] = span;
+      if (it.n > 0 && static_cast<int64_t>(it.start) + it.n > g.capacity) record_error(1, it.b);
+    }
+    __syncthreads();
   } else {
     constexpr int EACH = (MAX_ITEMS + WARPS * 32 - 1) / (WARPS * 32);
     int own[EACH], sum = 0;
@@ -276,10 +501,12 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
     for (int e = 0; e < EACH; ++e) {
       const int id = tid * EACH + e;
       own[e] = 0;
-      if (id < items) {
-        const Item it = get_item(a, id, row_tiles, NR, group, capacity);
+      if (id < g.items) {
+        const int2 span = span_of(a, g, id);
+        const Item it = get_item<NR>(a, g, id, span);
+        spans[id] = span;
         own[e] = it.tiles;
-        if (blockIdx.x == 0 && it.n > 0 && static_cast<int64_t>(it.start) + it.n > capacity) record_error(1, it.b);
+        if (me == 0 && it.n > 0 && static_cast<int64_t>(it.start) + it.n > g.capacity) record_error(1, it.b);
       }
       sum += own[e];
     }
@@ -289,100 +516,129 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
       const int v = __shfl_up_sync(0xffffffffu, scan, o);
       if (lane >= o) scan += v;
     }
-    if (lane == 31) warp_sum_[warp] = scan;
+    if (lane == 31) warp_total[warp] = scan;
     __syncthreads();
     int before = scan - sum;
-    for (int w = 0; w < warp; ++w) before += warp_sum_[w];
+    for (int w = 0; w < warp; ++w) before += warp_total[w];
 #pragma unroll
     for (int e = 0; e < EACH; ++e) {
       const int id = tid * EACH + e;
-      if (id < items) {
+      if (id < g.items) {
         pre[id] = before;
         before += own[e];
-        if (id == items - 1) pre[items] = before;
+        if (id == g.items - 1) pre[g.items] = before;
       }
     }
     __syncthreads();
-    W = static_cast<int64_t>(pre[items]) * Hk;
-    G = static_cast<int>(max(static_cast<int64_t>(1), min(static_cast<int64_t>(gridDim.x), W / (WARPS * MIN_TILES))));
-    if (static_cast<int>(blockIdx.x) >= G) {
-      if (tid == 0) ws_desc[blockIdx.x] = make_int4(-1, 0, 0, 0);
-      return;
-    }
-    lo = blockIdx.x * W / G;
-    hi = (blockIdx.x + 1) * W / G;
+    const int W = pre[g.items] * Hk;
+    G = max(1, min(static_cast<int>(gridDim.x), W / (WARPS * MIN_TILES)));
+    if (me >= G) return;
+    each = W / G;
+    more = W - each * G;
+    lo = me * each + min(me, more);
+    hi = lo + each + (me < more ? 1 : 0);
   }
-  const int64_t x0 = lo + warp * (hi - lo) / WARPS, x1 = lo + (warp + 1) * (hi - lo) / WARPS;
-  int fetch_left = static_cast<int>(x1 - x0), left = fetch_left;
+  auto cta_of = [&](int x) { return x < more * (each + 1) ? quotient(x, each + 1) : more + quotient(x - more * (each + 1), each); };
+  auto span_at = [&](int id) { return spans[g.direct ? 0 : id]; };
+  // a warp's piece of it; where there are fewer tiles than warps, the last warps have none
+  const int few = (hi - lo) / WARPS, rest_tiles = (hi - lo) % WARPS;
+  const int x0 = lo + warp * few + min(warp, rest_tiles), x1 = x0 + few + (warp < rest_tiles ? 1 : 0);
+  int fetch_left = x1 - x0, left = fetch_left;
   if (lane < 2) part_id[2 * warp + lane] = -1;
 
   if (left > 0) {
     Cursor f;
-    if (direct) {
-      f.id = base_id; f.hk = base_hk; f.j = static_cast<int>(x0);
+    if (g.direct) {
+      f.id = base_id; f.hk = base_hk; f.j = x0;
     } else {
-      int l = 0, r = items;  // the last item whose tiles begin at or before x0
+      int l = 0, r = g.items;  // the last item whose tiles begin at or before x0
       while (r - l > 1) {
         const int mid = (l + r) >> 1;
-        if (static_cast<int64_t>(pre[mid]) * Hk <= x0) l = mid; else r = mid;
+        if (pre[mid] * Hk <= x0) l = mid; else r = mid;
       }
-      const int64_t rest = x0 - static_cast<int64_t>(pre[l]) * Hk;
-      const int n = pre[l + 1] - pre[l];
+      const int rest = x0 - pre[l] * Hk, n = pre[l + 1] - pre[l];
       f.id = l;
-      f.hk = static_cast<int>(rest / n);
-      f.j = static_cast<int>(rest - static_cast<int64_t>(f.hk) * n);
+      f.hk = Hk == 1 ? 0 : quotient(rest, n);
+      f.j = rest - f.hk * n;
     }
-    enter(a, f, row_tiles, NR, group, capacity, lane);
+    enter<NR>(a, g, f, span_at(f.id), lane);
     Cursor c = f;  // where the products stand (its page fields are unused)
 
     uint8_t* ring = smem + warp * S::RING;
     const uint32_t ring_u = smem_u32(ring);
     const int lrow = lane / CHUNKS, lch = lane % CHUNKS;
-    constexpr int ROWS = 32 / CHUNKS;  // rows of one copy instruction of the warp
-    const T* kc = static_cast<const T*>(a.cache.k);
-    const T* vc = static_cast<const T*>(a.cache.v);
+    constexpr int ROWS = 32 / CHUNKS;       // rows of one copy instruction of the warp
+    constexpr int PERIOD = 8 / ROWS;        // copies after which the swizzle repeats
+    uint32_t to[PERIOD];
+#pragma unroll
+    for (int e = 0; e < PERIOD; ++e) to[e] = (e * ROWS + lrow) * (D * 2) + ((lch ^ ((e * ROWS + lrow) & 7)) << 4);
+    const T* kc = static_cast<const T*>(a.cache.k) + lrow * a.cache.slot_stride_k + lch * 8;
+    const T* vc = static_cast<const T*>(a.cache.v) + lrow * a.cache.slot_stride_v + lch * 8;
+    const int64_t kstep = ROWS * a.cache.slot_stride_k, vstep = ROWS * a.cache.slot_stride_v;
 
+    bool turn = true;
     auto fetch = [&](int stage) {
       if (fetch_left > 0) {
-        if (f.column - f.seen >= 32) load_pages(a, f, lane);
-        const int page = __shfl_sync(0xffffffffu, f.pages, f.column - f.seen);
+        if (turn) turn_page<T>(a, f, kc, vc, lane);
         const int key = (f.it.first & ~(TILE - 1)) + f.j * TILE;
-        const bool there = page >= 0 && page < a.cache.pages;
-        if (!there && f.it.first < f.it.end && lane == 0) record_error(2, f.it.b);
-        const int64_t p = there ? page : 0;
-        const T* ks = kc + p * a.cache.page_stride_k + f.hk * a.cache.head_stride_k + f.slot * a.cache.slot_stride_k + lch * 8;
-        const T* vs = vc + p * a.cache.page_stride_v + f.hk * a.cache.head_stride_v + f.slot * a.cache.slot_stride_v + lch * 8;
+        const T *ks = static_cast<const T*>(f.k), *vs = static_cast<const T*>(f.v);
         const uint32_t dst = ring_u + stage * S::STAGE;
+        if (f.there && key >= f.it.first && key + TILE <= f.it.end) {
 #pragma unroll
-        for (int e = 0; e < TILE / ROWS; ++e) {
+          for (int e = 0; e < TILE / ROWS; ++e) {
+            const uint32_t at = dst + to[e % PERIOD] + (e / PERIOD) * (8 * D * 2);
+            cp_async16(at, ks);
+            cp_async16(at + S::HALF, vs);
+            ks += kstep;
+            vs += vstep;
+          }
+        } else {
           // keys outside [first, end) become zeros: whatever their memory holds never meets a product
-          const int row = e * ROWS + lrow;
-          const bool valid = there && key + row >= f.it.first && key + row < f.it.end;
-          const uint32_t to = dst + row * (D * 2) + ((lch ^ (row & 7)) << 4);
-          cp_async16(to, ks + (valid ? row * a.cache.slot_stride_k : 0), valid ? 16 : 0);
-          cp_async16(to + S::HALF, vs + (valid ? row * a.cache.slot_stride_v : 0), valid ? 16 : 0);
+#pragma unroll 1
+          for (int e = 0; e < TILE / ROWS; ++e) {
+            const int row = e * ROWS + lrow;
+            const bool valid = f.there && key + row >= f.it.first && key + row < f.it.end;
+            const uint32_t at = dst + row * (D * 2) + ((lch ^ (row & 7)) << 4);
+            cp_async16_or_zero(at, valid ? ks : kc, valid);
+            cp_async16_or_zero(at + S::HALF, valid ? vs : vc, valid);
+            ks += kstep;
+            vs += vstep;
+          }
         }
         --fetch_left;
+        turn = false;
         if (++f.j == f.it.tiles) {
           f.j = 0;
           if (++f.hk == Hk) {
             f.hk = 0;
             ++f.id;
           }
-          if (fetch_left > 0) enter(a, f, row_tiles, NR, group, capacity, lane);
+          turn = true;
+          if (fetch_left > 0) enter<NR>(a, g, f, span_at(f.id), lane);
         } else if ((f.slot += TILE) == a.cache.page) {
           f.slot = 0;
           ++f.column;
+          turn = true;
+        } else {
+          f.k = static_cast<const T*>(f.k) + TILE * a.cache.slot_stride_k;
+          f.v = static_cast<const T*>(f.v) + TILE * a.cache.slot_stride_v;
         }
       }
       cp_commit();
     };
 
-#pragma unroll
+#pragma unroll 1
     for (int s = 0; s < S::STAGES - 1; ++s) fetch(s);
     int stage = 0;
     const float scale2 = a.scale * 1.4426950408889634f;
     const int qc = lane & 3, qr = lane >> 2;
+    uint32_t kat[4], vat[4];  // this lane's matrix rows in a stage, for channel blocks 0 to 3
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int krow = lane & 15, vrow = (lane & 7) + ((lane >> 4) << 3);
+      kat[e] = krow * (D * 2) + (((e * 2 + (lane >> 4)) ^ (krow & 7)) << 4);
+      vat[e] = S::HALF + vrow * (D * 2) + (((e * 2 + ((lane >> 3) & 1)) ^ (vrow & 7)) << 4);
+    }
 
     while (left > 0) {
       // ---- one piece: tiles [c.j, c.j + n) of (c.id, c.hk)
@@ -391,10 +647,10 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
       int last[NQ][2], oldest[NQ][2];  // newest and oldest key that this lane's two queries see
 #pragma unroll
       for (int nq = 0; nq < NQ; ++nq) {
-        const int r = c.it.r0 + nq * 8 + qr, i = r / group;
-        const bool live = r < R && i < c.it.n;
+        const int r = c.it.r0 + nq * 8 + qr, i = token_of(r, g.inverse);
+        const bool live = r < g.R && i < c.it.n;
         const T* qp = static_cast<const T*>(a.q) + c.it.b * a.qs[0] + (live ? i : 0) * a.qs[1] +
-                      (c.hk * group + (live ? r - i * group : 0)) * a.qs[2] + qc * 2;
+                      (c.hk * g.group + (live ? r - i * g.group : 0)) * a.qs[2] + qc * 2;
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) {
           qf[nq][kk][0] = live ? *reinterpret_cast<const uint32_t*>(qp + kk * 16) : 0u;
@@ -402,8 +658,8 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
         }
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const int rc = c.it.r0 + nq * 8 + qc * 2 + e, ic = rc / group;
-          const bool lc = rc < R && ic < c.it.n;
+          const int rc = c.it.r0 + nq * 8 + qc * 2 + e, ic = token_of(rc, g.inverse);
+          const bool lc = rc < g.R && ic < c.it.n;
           last[nq][e] = lc ? min(c.it.start + ic, c.it.end - 1) : -1;
           oldest[nq][e] = lc && a.window >= 0 ? c.it.start + ic - a.window : 0;
         }
@@ -428,34 +684,34 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
         int ahead = stage + S::STAGES - 1;
         if (ahead >= S::STAGES) ahead -= S::STAGES;
         fetch(ahead);
-        const uint32_t kbase = ring_u + stage * S::STAGE, vbase = kbase + S::HALF;
+        const uint32_t base = ring_u + stage * S::STAGE;
         if (++stage == S::STAGES) stage = 0;
 
-        float s[NQ][4];
+        float s[NQ][4], s2[NQ][4];  // two chains of products
 #pragma unroll
         for (int nq = 0; nq < NQ; ++nq)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) s[nq][e] = 0.f;
-        {
-          const int row = lane & 15;
+          for (int e = 0; e < 4; ++e) s[nq][e] = s2[nq][e] = 0.f;
 #pragma unroll
-          for (int kk = 0; kk < D / 16; ++kk) {
-            uint32_t kf[4];
-            ldsm4(kf, kbase + row * (D * 2) + (((kk * 2 + (lane >> 4)) ^ (row & 7)) << 4));
+        for (int kk = 0; kk < D / 16; ++kk) {
+          uint32_t kf[4];
+          ldsm4(kf, base + kat[kk & 3] + (kk >> 2) * 128);
 #pragma unroll
-            for (int nq = 0; nq < NQ; ++nq) Num<T>::mma(s[nq], kf, qf[nq][kk][0], qf[nq][kk][1]);
-          }
+          for (int nq = 0; nq < NQ; ++nq) Num<T>::mma(kk & 1 ? s2[nq] : s[nq], kf, qf[nq][kk][0], qf[nq][kk][1]);
         }
-        const int key = (c.it.first & ~(TILE - 1)) + (j0 + tile) * TILE + qr;
+        const int key0 = (c.it.first & ~(TILE - 1)) + (j0 + tile) * TILE, key = key0 + qr;
+        const bool edge = key0 < c.it.all_from || key0 < c.it.first || key0 + TILE > c.it.all_to;
         uint32_t pf[NQ][2];
 #pragma unroll
         for (int nq = 0; nq < NQ; ++nq) {
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const bool in0 = key <= last[nq][e] && key >= oldest[nq][e];
-            const bool in1 = key + 8 <= last[nq][e] && key + 8 >= oldest[nq][e];
-            s[nq][e] = in0 ? s[nq][e] * scale2 : -INFINITY;
-            s[nq][e + 2] = in1 ? s[nq][e + 2] * scale2 : -INFINITY;
+          for (int e = 0; e < 4; ++e) s[nq][e] = (s[nq][e] + s2[nq][e]) * scale2;
+          if (edge) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              if (key > last[nq][e] || key < oldest[nq][e]) s[nq][e] = -INFINITY;
+              if (key + 8 > last[nq][e] || key + 8 < oldest[nq][e]) s[nq][e + 2] = -INFINITY;
+            }
           }
           float top[2] = {fmaxf(s[nq][0], s[nq][2]), fmaxf(s[nq][1], s[nq][3])};
 #pragma unroll
@@ -463,74 +719,65 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
             top[0] = fmaxf(top[0], __shfl_xor_sync(0xffffffffu, top[0], d));
             top[1] = fmaxf(top[1], __shfl_xor_sync(0xffffffffu, top[1], d));
           }
-          float fix[2];
-          bool moved = false;
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const float mn = fmaxf(m[nq][e], top[e]);
-            moved |= mn != m[nq][e];
-            fix[e] = piece_weight(m[nq][e], mn);
-            m[nq][e] = mn;
-            const float ref = mn == -INFINITY ? 0.f : mn;
-            s[nq][e] = exp2_fast(s[nq][e] - ref);
-            s[nq][e + 2] = exp2_fast(s[nq][e + 2] - ref);
-            l[nq][e] = (mn == -INFINITY ? l[nq][e] : l[nq][e] * fix[e]) + s[nq][e] + s[nq][e + 2];
-          }
-          if (__any_sync(0xffffffffu, moved)) {
+          const float m0 = fmaxf(m[nq][0], top[0]), m1 = fmaxf(m[nq][1], top[1]);
+          if (__any_sync(0xffffffffu, m0 != m[nq][0] || m1 != m[nq][1])) {
+            const float f0 = piece_weight(m[nq][0], m0), f1 = piece_weight(m[nq][1], m1);
+            m[nq][0] = m0;
+            m[nq][1] = m1;
+            l[nq][0] *= f0;
+            l[nq][1] *= f1;
 #pragma unroll
             for (int d = 0; d < D / 16; ++d) {
-              o[nq][d][0] *= fix[0]; o[nq][d][1] *= fix[1];
-              o[nq][d][2] *= fix[0]; o[nq][d][3] *= fix[1];
+              o[nq][d][0] *= f0; o[nq][d][1] *= f1;
+              o[nq][d][2] *= f0; o[nq][d][3] *= f1;
             }
           }
+          const float r0 = m0 == -INFINITY ? 0.f : m0, r1 = m1 == -INFINITY ? 0.f : m1;
+          s[nq][0] = exp2_fast(s[nq][0] - r0); s[nq][1] = exp2_fast(s[nq][1] - r1);
+          s[nq][2] = exp2_fast(s[nq][2] - r0); s[nq][3] = exp2_fast(s[nq][3] - r1);
+          l[nq][0] += s[nq][0] + s[nq][2];
+          l[nq][1] += s[nq][1] + s[nq][3];
           // probabilities are at most 1; rounding them to the cache's type costs no more than the rounding of
           // V does (their sum stays in fp32)
           pf[nq][0] = transpose8x8(Num<T>::pack(s[nq][0], s[nq][1]));
           pf[nq][1] = transpose8x8(Num<T>::pack(s[nq][2], s[nq][3]));
         }
-        {
-          const int row = (lane & 7) + ((lane >> 4) << 3), ch = (lane >> 3) & 1;
 #pragma unroll
-          for (int d = 0; d < D / 16; ++d) {
-            uint32_t vf[4];
-            ldsm4t(vf, vbase + row * (D * 2) + (((d * 2 + ch) ^ (row & 7)) << 4));
+        for (int d = 0; d < D / 16; ++d) {
+          uint32_t vf[4];
+          ldsm4t(vf, base + vat[d & 3] + (d >> 2) * 128);
 #pragma unroll
-            for (int nq = 0; nq < NQ; ++nq) Num<T>::mma(o[nq][d], vf, pf[nq][0], pf[nq][1]);
-          }
+          for (int nq = 0; nq < NQ; ++nq) Num<T>::mma(o[nq][d], vf, pf[nq][0], pf[nq][1]);
         }
       }
 
-      // ---- the piece's end
+      // ---- the piece's end; rows that are no tokens have no keys
 #pragma unroll
       for (int nq = 0; nq < NQ; ++nq)
 #pragma unroll
-        for (int d = 4; d < 32; d <<= 1) {
-          l[nq][0] += __shfl_xor_sync(0xffffffffu, l[nq][0], d);
-          l[nq][1] += __shfl_xor_sync(0xffffffffu, l[nq][1], d);
+        for (int e = 0; e < 2; ++e) {
+#pragma unroll
+          for (int d = 4; d < 32; d <<= 1) l[nq][e] += __shfl_xor_sync(0xffffffffu, l[nq][e], d);
+          if (last[nq][e] < 0) {
+            l[nq][e] = 0.f;
+            m[nq][e] = -INFINITY;
+          }
         }
       const bool begins = j0 == 0, ends = j0 + n == c.it.tiles;
       left -= n;
       if (begins && ends) {
 #pragma unroll
         for (int nq = 0; nq < NQ; ++nq) {
+          const int r = c.it.r0 + nq * 8 + qr;
+          T* row = output_row<T, D>(a, g, c.it.b, r, c.hk, lane);
           const float w0 = inverse_total(l[nq][0]), w1 = inverse_total(l[nq][1]);
-          const int r = c.it.r0 + nq * 8 + qr, i = r / group;  // after the transpose this lane holds query qr
-          T* op = static_cast<T*>(a.out) +
-                  ((static_cast<int64_t>(c.it.b) * a.t + i) * a.H + c.hk * group + (r - i * group)) * D + qc * 2;
 #pragma unroll
-          for (int d = 0; d < D / 16; ++d) {
-            const uint32_t u0 = transpose8x8(Num<T>::pack(o[nq][d][0] * w0, o[nq][d][1] * w1));
-            const uint32_t u1 = transpose8x8(Num<T>::pack(o[nq][d][2] * w0, o[nq][d][3] * w1));
-            if (r < R) {
-              *reinterpret_cast<uint32_t*>(op + d * 16) = u0;
-              *reinterpret_cast<uint32_t*>(op + d * 16 + 8) = u1;
-            }
-          }
+          for (int d = 0; d < D / 16; ++d)
+            write_block<T>(row, r < g.R, d, make_float4(o[nq][d][0], o[nq][d][1], o[nq][d][2], o[nq][d][3]), w0, w1);
         }
       } else {
         const bool final_piece = left == 0;
-        const int slot = 2 * warp + (final_piece ? 1 : 0);
-        float* part = reinterpret_cast<float*>(final_piece ? ring : smem + WARPS * S::RING + warp * S::PART);
+        float* part = final_piece ? reinterpret_cast<float*>(ring) : ws_warp + warp * S::PART;
         if (final_piece) {
           cp_wait<0>();
           __syncwarp();
@@ -538,19 +785,11 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
 #pragma unroll
         for (int nq = 0; nq < NQ; ++nq)
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            float* row = part + (nq * 8 + qc * 2 + e) * S::ROW;
-#pragma unroll
-            for (int d = 0; d < D / 16; ++d) {
-              row[d * 16 + qr] = o[nq][d][e];
-              row[d * 16 + 8 + qr] = o[nq][d][e + 2];
-            }
-            if (qr == 0) {
-              row[D] = m[nq][e];
-              row[D + 1] = l[nq][e];
-            }
-          }
+          for (int d = 0; d < D / 16; ++d)
+            store_block<D, NQ>(part, nq * (D / 16) + d, lane, make_float4(o[nq][d][0], o[nq][d][1], o[nq][d][2], o[nq][d][3]),
+                               make_float4(m[nq][0], l[nq][0], m[nq][1], l[nq][1]));
         if (lane == 0) {
+          const int slot = 2 * warp + (final_piece ? 1 : 0);
           part_id[slot] = c.id * Hk + c.hk;
           part_flag[slot] = (begins ? 1 : 0) | (ends ? 2 : 0);
         }
@@ -561,7 +800,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
         if (++c.hk == Hk) {
           c.hk = 0;
           ++c.id;
-          if (left > 0) c.it = get_item(a, c.id, row_tiles, NR, group, capacity);
+          if (left > 0) c.it = get_item<NR>(a, g, c.id, span_at(c.id));
         }
       }
     }
@@ -569,137 +808,121 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
   }
   __syncthreads();
 
-  // ---- join the CTA's pieces in their order
-  if (!direct && tid == 0) ws_desc[blockIdx.x] = make_int4(-1, 0, 0, 0);
-  auto piece = [&](int s) {
-    return reinterpret_cast<const float*>((s & 1) ? smem + (s >> 1) * S::RING : smem + WARPS * S::RING + (s >> 1) * S::PART);
-  };
-  for (int s0 = 0; s0 < 2 * WARPS;) {
-    const int id = part_id[s0];
-    if (id < 0) {
-      ++s0;
-      continue;
+  // ---- join the CTA's pieces, a warp a block of 8 queries and 16 channels at a time
+  int open_id[2] = {-1, -1};  // what this CTA leaves open: 0 began in an earlier one, 1 begins here
+  {
+    // Slot 2 w is warp w's first piece where that is not its last, which is in slot 2 w + 1.  Places on the line
+    // only grow, so a piece that does not follow one of the same (row, KV head) leads.
+    const int part = lane & 15, id = part_id[part], flag = part_flag[part];
+    int before = part ? part_id[part - 1] : -1;
+#pragma unroll
+    for (int o = 1; o < 16; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, before, o, 16);
+      if (part >= o) before = max(before, v);
     }
-    int s1 = s0 + 1, tail = s0;
-    while (s1 < 2 * WARPS && (part_id[s1] == id || part_id[s1] < 0)) {
-      if (part_id[s1] == id) tail = s1;
-      ++s1;
-    }
-    const bool begins = part_flag[s0] & 1, ends = part_flag[tail] & 2;
-    const int item = id / Hk, hk = id - item * Hk;
-    const int b = item / row_tiles, r0 = (item - b * row_tiles) * NR;
-    for (int e = tid; e < NR * (D / 4); e += WARPS * 32) {
-      const int q = e / (D / 4), d = (e - q * (D / 4)) * 4, r = r0 + q;
-      if (r >= R) continue;
-      float top = -INFINITY;
-      for (int s = s0; s <= tail; ++s)
-        if (part_id[s] == id) top = fmaxf(top, piece(s)[q * S::ROW + D]);
-      float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-      float total = 0.f;
-      for (int s = s0; s <= tail; ++s) {
-        if (part_id[s] != id) continue;
-        const float* row = piece(s) + q * S::ROW;
-        const float w = piece_weight(row[D], top);
-        const float4 v = *reinterpret_cast<const float4*>(row + d);
-        sum.x = fmaf(w, v.x, sum.x); sum.y = fmaf(w, v.y, sum.y);
-        sum.z = fmaf(w, v.z, sum.z); sum.w = fmaf(w, v.w, sum.w);
-        total = fmaf(w, row[D + 1], total);
+    const unsigned valid = __ballot_sync(0xffffffffu, id >= 0) & 0xffffu;
+    unsigned leaders = __ballot_sync(0xffffffffu, id >= 0 && before < id) & 0xffffu;
+    int blk = warp;
+    while (leaders) {
+      const int leader = __ffs(leaders) - 1;
+      leaders &= leaders - 1;
+      const unsigned mask = valid & ~((1u << leader) - 1u) & (leaders ? (1u << (__ffs(leaders) - 1)) - 1u : 0xffffu);
+      const int end = 31 - __clz(mask), gid = __shfl_sync(0xffffffffu, id, leader);
+      const bool begins = __shfl_sync(0xffffffffu, flag, leader) & 1, ends = __shfl_sync(0xffffffffu, flag, end) & 2;
+      if (!(begins && ends)) open_id[begins ? 1 : 0] = gid;
+      // warps leader / 2 to end / 2 have one piece each
+      const int w0 = leader >> 1, n = (end >> 1) - w0 + 1;
+      for (; blk < S::BLOCKS; blk += WARPS) {
+        float4 stat;
+        const float4 sum = join_block<D, NQ, false>(n, blk, lane, [&](int k) {
+          return (mask >> (2 * (w0 + k))) & 1u ? ws_warp + (w0 + k) * S::PART : reinterpret_cast<const float*>(smem + (w0 + k) * S::RING);
+        }, stat);
+        if (!(begins && ends)) {
+          store_block<D, NQ>(ws + (static_cast<int64_t>(me) * 2 + (begins ? 1 : 0)) * S::PART, blk, lane, sum, stat);
+        } else {
+          const int item = quotient(gid, Hk), b = g.row_tiles == 1 ? item : item / g.row_tiles;
+          const int r = (item - b * g.row_tiles) * NR + (blk / (D / 16)) * 8 + (lane >> 2);
+          write_block<T>(output_row<T, D>(a, g, b, r, gid - item * Hk, lane), r < g.R, blk % (D / 16), sum, inverse_total(stat.y),
+                         inverse_total(stat.w));
+        }
       }
-      if (begins && ends) {
-        const float w = inverse_total(total);
-        const int i = r / group;
-        T* op = static_cast<T*>(a.out) + ((static_cast<int64_t>(b) * a.t + i) * a.H + hk * group + (r - i * group)) * D + d;
-        *reinterpret_cast<uint2*>(op) = make_uint2(Num<T>::pack(sum.x * w, sum.y * w), Num<T>::pack(sum.z * w, sum.w * w));
-      } else {
-        // slot 1: the (row, KV head) begins in this CTA; slot 0: it began in an earlier one
-        float* row = ws_part + ((static_cast<int64_t>(blockIdx.x) * 2 + (begins ? 1 : 0)) * NR + q) * S::ROW;
-        *reinterpret_cast<float4*>(row + d) = sum;
-        if (d == 0) *reinterpret_cast<float2*>(row + D) = make_float2(top, total);
-      }
+      blk -= S::BLOCKS;
     }
-    if (begins && !ends && tid == 0) {
-      // the (row, KV head) ends with the CTA that holds its last tile
-      const int64_t n = pre[item + 1] - pre[item];
-      const int64_t x = static_cast<int64_t>(pre[item]) * Hk + (hk + 1) * n - 1;
-      ws_desc[blockIdx.x] = make_int4(static_cast<int>(((x + 1) * G - 1) / W), b, r0, hk);
-    }
-    s0 = s1;
   }
-}
+  if (g.direct || (open_id[0] < 0 && open_id[1] < 0)) return;
 
-// Joins the pieces of a (row, KV head) that several CTAs hold: block (c, q) for query row q of the one that
-// begins in CTA c.  Eight (16 for heads of 64) groups of threads take every eighth piece, four channels a
-// thread, then the groups' sums are joined in their order.
-template <class T, int D, int NR>
-__global__ void __launch_bounds__(256) join_kernel(const PagedAttnArgs a, const float* ws_part, const int4* ws_desc) {
-  constexpr int LANES = D / 4, GROUPS = 256 / LANES, ROW = D + 4;
-  __shared__ float part[GROUPS][ROW];
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int c0 = blockIdx.x, q = blockIdx.y;
-  const int4 desc = ws_desc[c0];
-  if (desc.x < 0) return;
-  const int group = a.H / a.Hk, r = desc.z + q;
-  if (r >= a.t * group) return;
-  const int g = threadIdx.x / LANES, d = (threadIdx.x % LANES) * 4, n = desc.x - c0 + 1;
-  float top = -INFINITY, total = 0.f;
-  float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-  for (int p = g; p < n; p += GROUPS) {
-    const float* row = ws_part + ((static_cast<int64_t>(c0 + p) * 2 + (p == 0 ? 1 : 0)) * NR + q) * ROW;
-    const float4 v = *reinterpret_cast<const float4*>(row + d);
-    const float2 ml = *reinterpret_cast<const float2*>(row + D);
-    const float up = fmaxf(top, ml.x);
-    const float w0 = piece_weight(top, up), w1 = piece_weight(ml.x, up);
-    sum.x = sum.x * w0 + v.x * w1; sum.y = sum.y * w0 + v.y * w1;
-    sum.z = sum.z * w0 + v.z * w1; sum.w = sum.w * w0 + v.w * w1;
-    total = total * w0 + ml.y * w1;
-    top = up;
+  // ---- and what several CTAs hold: the last of up to 16 neighbours joins their pieces, the last of these the rest.
+  // The pieces were written by the whole CTA: the barrier orders them before the arriving thread's release, and its
+  // acquire before what the CTA reads behind the second barrier (past L1, which nothing invalidates).
+  auto arrive = [&](unsigned* counter, int n) {  // n arrivals bring the counter back to 0
+    unsigned before;
+    asm volatile("atom.acq_rel.gpu.global.inc.u32 %0, [%1], %2;" : "=r"(before) : "l"(counter), "r"(n - 1) : "memory");
+    return before == static_cast<unsigned>(n - 1);
+  };
+#pragma unroll 1
+  for (int side = 0; side < 2; ++side) {
+    const int gid = open_id[side];
+    if (gid < 0) continue;
+    const int item = quotient(gid, Hk), hk = gid - item * Hk, tiles = pre[item + 1] - pre[item], x = pre[item] * Hk + hk * tiles;
+    const int c0 = cta_of(x), c1 = cta_of(x + tiles - 1), lead = c0 + ((me - c0) & ~(FAN - 1)), groups = (c1 - c0) / FAN + 1;
+    const int b = g.row_tiles == 1 ? item : item / g.row_tiles, r0 = (item - b * g.row_tiles) * NR;
+    auto at = [&](int c) { return ws + (static_cast<int64_t>(c) * 2 + (c == c0 ? 1 : 0)) * S::PART; };
+    int first = lead, step = 1, n = min(FAN, c1 - lead + 1);
+    unsigned* counter = counters + lead * COUNTERS + (lead == c0 ? 1 : 0);
+#pragma unroll 1
+    for (int level = 0;; ++level) {
+      __syncthreads();
+      if (tid == 0) arrived_last = arrive(counter, n);
+      __syncthreads();
+      if (!arrived_last) break;
+      const bool done = level == 1 || groups == 1;
+      for (int blk = warp; blk < S::BLOCKS; blk += WARPS) {
+        float4 stat;
+        const float4 sum = join_block<D, NQ, true>(n, blk, lane, [&](int k) { return at(first + k * step); }, stat);
+        if (!done) {
+          // into the leader's piece: its sums are read by this warp alone, its maxima and totals by all
+          joined[blk * 32 + lane] = sum;
+          if (blk % (D / 16) == 0 && lane < 4) joined_stat[(blk / (D / 16)) * 4 + lane] = stat;
+        } else {
+          const int r = r0 + (blk / (D / 16)) * 8 + (lane >> 2);
+          write_block<T>(output_row<T, D>(a, g, b, r, hk, lane), r < g.R, blk % (D / 16), sum, inverse_total(stat.y), inverse_total(stat.w));
+        }
+      }
+      if (done) break;
+      __syncthreads();
+      for (int blk = warp; blk < S::BLOCKS; blk += WARPS)
+        store_block<D, NQ>(at(lead), blk, lane, joined[blk * 32 + lane], joined_stat[(blk / (D / 16)) * 4 + (lane & 3)]);
+      first = c0;
+      step = FAN;
+      n = groups;
+      counter = counters + c0 * COUNTERS + 2;
+    }
   }
-  *reinterpret_cast<float4*>(&part[g][d]) = sum;
-  if (d == 0) {
-    part[g][D] = top;
-    part[g][D + 1] = total;
-  }
-  __syncthreads();
-  if (g != 0) return;
-  top = -INFINITY;
-#pragma unroll
-  for (int p = 0; p < GROUPS; ++p) top = fmaxf(top, part[p][D]);
-  sum = make_float4(0.f, 0.f, 0.f, 0.f);
-  total = 0.f;
-#pragma unroll
-  for (int p = 0; p < GROUPS; ++p) {
-    const float w = piece_weight(part[p][D], top);
-    const float4 v = *reinterpret_cast<const float4*>(&part[p][d]);
-    sum.x = fmaf(w, v.x, sum.x); sum.y = fmaf(w, v.y, sum.y);
-    sum.z = fmaf(w, v.z, sum.z); sum.w = fmaf(w, v.w, sum.w);
-    total = fmaf(w, part[p][D + 1], total);
-  }
-  const float w = inverse_total(total);
-  const int i = r / group;
-  T* op = static_cast<T*>(a.out) +
-          ((static_cast<int64_t>(desc.y) * a.t + i) * a.H + desc.w * group + (r - i * group)) * D + d;
-  *reinterpret_cast<uint2*>(op) = make_uint2(Num<T>::pack(sum.x * w, sum.y * w), Num<T>::pack(sum.z * w, sum.w * w));
 }
 
 struct Plan {
-  int NR, row_tiles, grid;
-  int64_t items;
-  bool direct;
+  int NR, grid;
+  Geometry g;
 };
 static Plan make_plan(const PagedAttnArgs& a) {
   Plan p;
-  const int64_t R = static_cast<int64_t>(a.t) * (a.H / a.Hk);
+  Geometry& g = p.g;
+  const int64_t group = a.H / a.Hk, R = a.t * group;
+  g.group = static_cast<int>(group);
+  g.R = static_cast<int>(R);
+  g.inverse = group == 1 ? 0u : static_cast<uint32_t>(((int64_t{1} << 32) + group - 1) / group);
   p.NR = R <= 8 ? 8 : 16;
-  p.row_tiles = static_cast<int>((R + p.NR - 1) / p.NR);
-  p.items = static_cast<int64_t>(a.B) * p.row_tiles;
-  const int64_t capacity = static_cast<int64_t>(a.cache.columns) * a.cache.page;
-  p.direct = p.items > MAX_ITEMS || p.items * (capacity / TILE + 1) > INT32_MAX;  // the line's prefix sums are 32-bit
+  g.row_tiles = static_cast<int>((R + p.NR - 1) / p.NR);
+  const int64_t items = static_cast<int64_t>(a.B) * g.row_tiles;
+  const int64_t capacity = std::min<int64_t>(static_cast<int64_t>(a.cache.columns) * a.cache.page, INT32_MAX - TILE);
+  g.items = static_cast<int>(std::min<int64_t>(items, INT32_MAX));
+  g.capacity = static_cast<int>(capacity);
+  g.direct = items > MAX_ITEMS || items * (capacity / TILE + 1) * a.Hk > INT32_MAX;  // places on the line are 32-bit
   int64_t tiles = (capacity + TILE - 1) / TILE;
   if (a.window >= 0) tiles = std::min<int64_t>(tiles, (static_cast<int64_t>(a.window) + a.t) / TILE + 2);
-  tiles = std::max<int64_t>(tiles, 1) * p.items * a.Hk;
-  p.grid = static_cast<int>(p.direct ? p.items * a.Hk
-                                     : std::max<int64_t>(1, std::min<int64_t>(a.sms, tiles / (WARPS * MIN_TILES))));
+  tiles = std::max<int64_t>(tiles, 1) * items * a.Hk;
+  p.grid = static_cast<int>(g.direct ? std::min<int64_t>(items * a.Hk, INT32_MAX)
+                                     : std::max<int64_t>(1, std::min<int64_t>(std::min(a.sms, FAN * FAN), tiles / (WARPS * MIN_TILES))));
   return p;
 }
 
@@ -709,22 +932,8 @@ static int launch_attn(const PagedAttnArgs& a, const Plan& p, cudaStream_t s) {
   static std::atomic<uint64_t> done{0};
   auto kern = attn_kernel<T, D, NQ>;
   if (smem_limit(done, kern, S::SMEM) != cudaSuccess) return -1;
-  float* part = a.workspace;
-  int4* desc = reinterpret_cast<int4*>(part + static_cast<int64_t>(p.grid) * 2 * S::NR * S::ROW);
-  kern<<<p.grid, WARPS * 32, S::SMEM, s>>>(a, static_cast<int>(p.items), p.row_tiles, p.direct, part, desc);
-  if (p.direct || p.grid == 1) return 0;
-  // launched with the attention kernel still running: its blocks wait for the pieces on the device
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(p.grid - 1, static_cast<unsigned>(std::min<int64_t>(S::NR, static_cast<int64_t>(a.t) * (a.H / a.Hk))));
-  cfg.blockDim = dim3(256);
-  cfg.stream = s;
-  cudaLaunchAttribute attr = {};
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, join_kernel<T, D, S::NR>, a, static_cast<const float*>(part),
-                            static_cast<const int4*>(desc)) == cudaSuccess ? 0 : -1;
+  kern<<<p.grid, WARPS * 32, S::SMEM, s>>>(a, p.g, a.workspace, a.counters);
+  return 0;
 }
 
 }  // namespace paged
@@ -733,33 +942,26 @@ static int launch_attn(const PagedAttnArgs& a, const Plan& p, cudaStream_t s) {
 using namespace nt::paged;
 
 int nt_paged_append(const PagedAppendArgs& a, cudaStream_t s) {
-  const int64_t units = static_cast<int64_t>(a.B) * a.t * (a.H + 2 * a.Hk);
-  if (units == 0) return 0;
-  if (a.D != 64 && a.D != 128) return -1;
-  const int64_t blocks = (units * (a.D / 8) + 255) / 256;
-  if (blocks > INT32_MAX) return -1;
-  const unsigned g = static_cast<unsigned>(blocks);
-  if (a.fp16) {
-    if (a.D == 128) append_kernel<__half, 128><<<g, 256, 0, s>>>(a);
-    else append_kernel<__half, 64><<<g, 256, 0, s>>>(a);
-  } else {
-    if (a.D == 128) append_kernel<__nv_bfloat16, 128><<<g, 256, 0, s>>>(a);
-    else append_kernel<__nv_bfloat16, 64><<<g, 256, 0, s>>>(a);
-  }
-  return 0;
+  if (a.B == 0 || a.t == 0) return 0;
+  if (a.D == 128) return a.fp16 ? launch_append<__half, 128>(a, s) : launch_append<__nv_bfloat16, 128>(a, s);
+  if (a.D == 64) return a.fp16 ? launch_append<__half, 64>(a, s) : launch_append<__nv_bfloat16, 64>(a, s);
+  return -1;
 }
 
 size_t nt_paged_attn_workspace(const PagedAttnArgs& a) {
   const Plan p = make_plan(a);
-  if (p.direct) return 0;
-  return static_cast<size_t>(p.grid) * (2 * p.NR * (a.D + 4) * sizeof(float) + sizeof(int4));
+  return p.g.direct ? 0 : ws_floats(p.grid, p.NR * a.D + p.NR * 2) * sizeof(float);
 }
+int nt_paged_attn_counters(int sms) { return std::min(sms, FAN * FAN) * COUNTERS; }
 
 int nt_paged_attn(const PagedAttnArgs& a, cudaStream_t s) {
   if (a.B == 0 || a.t == 0) return 0;
   if (a.D != 64 && a.D != 128) return -1;
   const Plan p = make_plan(a);
-  if (p.items * a.Hk > INT32_MAX) return -1;
+  if (static_cast<int64_t>(p.g.items) * a.Hk >= INT32_MAX ||
+      static_cast<int64_t>(p.g.R) * p.g.group >= (int64_t{1} << 32) - 16 * p.g.group ||
+      static_cast<int64_t>(a.t) * p.g.group > INT32_MAX / 2)
+    return -1;
   if (a.fp16) {
     if (a.D == 128) return p.NR == 8 ? launch_attn<__half, 128, 1>(a, p, s) : launch_attn<__half, 128, 2>(a, p, s);
     return p.NR == 8 ? launch_attn<__half, 64, 1>(a, p, s) : launch_attn<__half, 64, 2>(a, p, s);

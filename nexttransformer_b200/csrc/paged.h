@@ -28,7 +28,7 @@ struct PagedAppendArgs {
   const int *start = nullptr, *count = nullptr;             // [B]; count null: t
   const void *cos = nullptr, *sin = nullptr;                // [rope_rows, D / 2]
   int rope_rows = 0;
-  int B = 0, t = 0, H = 0, Hk = 0, D = 0;
+  int B = 0, t = 0, H = 0, Hk = 0, D = 0, sms = 0;
   bool norm = false, fp16 = false;
   float scale = 1.f;
 };
@@ -44,9 +44,13 @@ struct PagedAttnArgs {
   bool fp16 = false;
   float scale = 1.f;
   float* workspace = nullptr;
+  unsigned* counters = nullptr;
 };
-// Bytes of scratch a call needs (0: none); the scratch holds nothing between calls.
+// Bytes of scratch a call needs (0: none; then no counters either); it holds nothing between calls.
 size_t nt_paged_attn_workspace(const PagedAttnArgs& a);
+// Counters a call needs.  They have to be 0 before a call, which leaves them 0; calls that may run at the same
+// time must not share them.
+int nt_paged_attn_counters(int sms);
 int nt_paged_attn(const PagedAttnArgs& a, cudaStream_t s);
 
 // Error word of this unit (reading clears it): 1 = a position behind the row's page table, 2 = a page number

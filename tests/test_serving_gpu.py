@@ -312,18 +312,20 @@ def test_delta_recurrent(dtype, kind, D, H, T, count, slots, l2norm):
 
 
 def test_delta_recurrent_in_pieces_and_zero_vectors():
-    """A run of tokens equals the same tokens in several calls; zero queries and keys stay zero under the norm."""
+    """A run of tokens equals the same tokens in several calls, bitwise where the cuts keep its blocks of eight and
+    within twice the bound of test_delta_recurrent elsewhere; zero queries and keys stay zero under the norm."""
     from nexttransformer_b200.ops.delta_recurrent import delta_recurrent
     torch.manual_seed(8)
     q, k, v = (torch.randn(2, 21, 2, 128, device=DEV) for _ in range(3))
     k[0, 3], q[1, 5] = 0.0, 0.0
     beta, g = torch.rand(2, 21, 2, device=DEV), -torch.rand(2, 21, 2, device=DEV)
     whole = torch.zeros(2, 2, 128, 128, device=DEV)
-    parts = whole.clone()
     o = delta_recurrent(q, k, v, whole, beta, g, l2norm=True)
-    cut = [delta_recurrent(*(x[:, a:b] for x in (q, k, v)), parts, beta[:, a:b], g[:, a:b], l2norm=True)
-           for a, b in ((0, 1), (1, 9), (9, 21))]
-    assert torch.equal(torch.cat(cut, 1), o) and torch.equal(parts, whole)
+    for cuts, slack in (((0, 8, 16, 21), 0.0), ((0, 1, 9, 21), 4e-6 * (21 + 4))):
+        state = torch.zeros_like(whole)
+        cut = [delta_recurrent(*(x[:, a:b] for x in (q, k, v)), state, beta[:, a:b], g[:, a:b], l2norm=True)
+               for a, b in zip(cuts, cuts[1:])]
+        assert (torch.cat(cut, 1) - o).abs().max() <= slack and (state - whole).abs().max() <= slack
     assert (o[1, 5] == 0).all() and torch.isfinite(o).all()
 
 
