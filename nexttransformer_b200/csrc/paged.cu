@@ -256,10 +256,10 @@ static int launch_append(const PagedAppendArgs& a, cudaStream_t s) {
 // equally and one long row uses all of them.  A warp that covers a whole (row, KV head) writes its result;
 // other pieces are joined in the CTA, and what crosses CTAs by the CTA that arrives last, up to 16 pieces at
 // a time.  Pieces are always joined in the order of the line, so results do not depend on timing.
-constexpr int WARPS = 8, TILE = 16, MIN_TILES = 4, FAN = 16;
+constexpr int WARPS = 8, TILE = 16, MIN_TILES = 2, CTA_SNAP = 32, WARP_SNAP = 2, FAN = 16;
 // Rows of the batch whose tiles a CTA lines up in shared memory; a larger batch has CTAs enough and gives
 // each (row, KV head) one.
-constexpr int MAX_ITEMS = 384;
+constexpr int MAX_ITEMS = 2048;
 
 template <int D, int NQ>
 struct Shape {
@@ -272,6 +272,7 @@ struct Shape {
   static constexpr int BLOCKS = NQ * (D / 16), PART = BLOCKS * 128 + NQ * 16;
   static constexpr int SMEM = WARPS * RING;
   static_assert(PART * 4 <= RING, "a warp's last piece lies in its own ring");
+  static_assert(SMEM + 12 * MAX_ITEMS + 1024 <= 227 * 1024, "shared memory of a CTA");
 };
 // Workspace: two pieces a CTA (1: a (row, KV head) that begins there, 0: one that began earlier), one piece
 // a warp (its first, where that is not its last), and three counters a CTA.
@@ -369,9 +370,17 @@ NT_DEVICE void load_pages(const PagedAttnArgs& a, Cursor& c, int lane) {
   const int col = c.column + lane;
   c.pages = col < a.cache.columns ? a.cache.table[static_cast<int64_t>(c.it.b) * a.cache.columns + col] : -1;
 }
-template <int NR>
+NT_DEVICE void prefetch_l1(const void* p) { asm volatile("prefetch.global.L1 [%0];" ::"l"(p)); }
+template <class T, int NR>
 NT_DEVICE void enter(const PagedAttnArgs& a, const Geometry& g, Cursor& c, int2 span, int lane) {
   c.it = get_item<NR>(a, g, c.id, span);
+  // the queries are wanted when the products get here, a ring later
+  const int r = c.it.r0 + (lane & (NR - 1)), i = token_of(r, g.inverse);
+  if (r < g.R && i < c.it.n) {
+    const T* q = static_cast<const T*>(a.q) + c.it.b * a.qs[0] + i * a.qs[1] + (c.hk * g.group + r - i * g.group) * a.qs[2];
+    prefetch_l1(q);
+    if (lane >= NR && a.D > 64) prefetch_l1(q + 64);
+  }
   const int key = (c.it.first & ~(TILE - 1)) + c.j * TILE;
   c.column = quotient(key, a.cache.page);
   c.slot = key - c.column * a.cache.page;
@@ -406,8 +415,8 @@ NT_DEVICE float4 join_block(int n, int blk, int lane, Piece piece, float4& stat)
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
       t[k] = make_float4(-INFINITY, 0.f, -INFINITY, 0.f);
-      if (from + k < n) {
-        const float* p = piece(from + k);
+      const float* p = from + k < n ? piece(from + k) : nullptr;
+      if (p) {
         t[k] = load(p + stats);
         v[k] = load(p + sums);
       }
@@ -469,7 +478,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
   using S = Shape<D, NQ>;
   constexpr int NR = S::NR, CHUNKS = D / 8;
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ int pre[MAX_ITEMS + 1];
+  __shared__ int pre[MAX_ITEMS + 1];  // tiles of a KV head before each item
   __shared__ int2 spans[MAX_ITEMS];
   __shared__ int warp_total[WARPS];
   __shared__ int part_id[2 * WARPS], part_flag[2 * WARPS];
@@ -481,34 +490,35 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
   const int Hk = a.Hk, me = blockIdx.x;
   float* ws_warp = ws + (static_cast<int64_t>(gridDim.x) * 2 + static_cast<int64_t>(me) * WARPS) * S::PART;
 
-  // ---- this CTA's piece [lo, hi) of the line: each of G has `each` tiles, the first `more` one more
-  int lo = 0, hi, G = 1, each = 0, more = 0, base_id = 0, base_hk = 0;
+  // ---- this CTA's piece of the line: each of G has `each` tiles, the first `more` one more, but a boundary that
+  // falls within CTA_SNAP tiles of a (row, KV head)'s start or end goes there, and between warps within WARP_SNAP
+  int G = 1, each = 0, more = 0;
+  int4 begin;  // of this warp's piece: place on the line, item, KV head, tile
+  int left;    // its tiles
+  if (tid < 2 * WARPS) part_id[tid] = -1;
   if (g.direct) {
-    base_id = me / Hk;
-    base_hk = me - base_id * Hk;
-    const int2 span = span_of(a, g, base_id);
-    const Item it = get_item<NR>(a, g, base_id, span);
-    hi = it.tiles;
+    const int id = me / Hk;
+    const int2 span = span_of(a, g, id);
+    const Item it = get_item<NR>(a, g, id, span);
     if (tid == 0) {
       spans[0] = span;
       if (it.n > 0 && static_cast<int64_t>(it.start) + it.n > g.capacity) record_error(1, it.b);
     }
+    const int few = it.tiles / WARPS, rest = it.tiles % WARPS, x = warp * few + min(warp, rest);
+    begin = make_int4(x, id, me - id * Hk, x);
+    left = few + (warp < rest ? 1 : 0);
     __syncthreads();
   } else {
-    constexpr int EACH = (MAX_ITEMS + WARPS * 32 - 1) / (WARPS * 32);
-    int own[EACH], sum = 0;
-#pragma unroll
-    for (int e = 0; e < EACH; ++e) {
-      const int id = tid * EACH + e;
-      own[e] = 0;
-      if (id < g.items) {
-        const int2 span = span_of(a, g, id);
-        const Item it = get_item<NR>(a, g, id, span);
-        spans[id] = span;
-        own[e] = it.tiles;
-        if (me == 0 && it.n > 0 && static_cast<int64_t>(it.start) + it.n > g.capacity) record_error(1, it.b);
-      }
-      sum += own[e];
+    // thread t lines up items t per .. (t + 1) per - 1
+    const int per = (g.items + WARPS * 32 - 1) / (WARPS * 32), from = tid * per, to = min(from + per, g.items);
+    int sum = 0;
+    for (int id = from; id < to; ++id) {
+      const int2 span = span_of(a, g, id);
+      const Item it = get_item<NR>(a, g, id, span);
+      spans[id] = span;
+      pre[id] = it.tiles;
+      sum += it.tiles;
+      if (me == 0 && it.n > 0 && static_cast<int64_t>(it.start) + it.n > g.capacity) record_error(1, it.b);
     }
     int scan = sum;
 #pragma unroll
@@ -518,50 +528,62 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
     }
     if (lane == 31) warp_total[warp] = scan;
     __syncthreads();
-    int before = scan - sum;
-    for (int w = 0; w < warp; ++w) before += warp_total[w];
+    int before = scan - sum, W = 0;
 #pragma unroll
-    for (int e = 0; e < EACH; ++e) {
-      const int id = tid * EACH + e;
-      if (id < g.items) {
-        pre[id] = before;
-        before += own[e];
-        if (id == g.items - 1) pre[g.items] = before;
-      }
+    for (int w = 0; w < WARPS; ++w) {
+      const int v = warp_total[w];
+      if (w < warp) before += v;
+      W += v;
     }
-    __syncthreads();
-    const int W = pre[g.items] * Hk;
-    G = max(1, min(static_cast<int>(gridDim.x), W / (WARPS * MIN_TILES)));
+    for (int id = from; id < to; ++id) {
+      const int n = pre[id];
+      pre[id] = before;
+      before += n;
+    }
+    if (tid == 0) pre[g.items] = W;
+    W *= Hk;
+    G = max(1, min(static_cast<int>(gridDim.x), max(W / (WARPS * MIN_TILES), (g.items * Hk + WARPS - 1) / WARPS)));
     if (me >= G) return;
     each = W / G;
     more = W - each * G;
-    lo = me * each + min(me, more);
-    hi = lo + each + (me < more ? 1 : 0);
+    __syncthreads();
+    auto snap = [&](int x, int reach) {
+      if (x >= W) return make_int4(W, g.items, 0, 0);
+      int id = 0, end = g.items;  // the last item whose tiles begin at or before x
+      while (end - id > 1) {
+        const int mid = (id + end) >> 1;
+        if (pre[mid] * Hk <= x) id = mid; else end = mid;
+      }
+      const int rest = x - pre[id] * Hk, n = pre[id + 1] - pre[id], hk = Hk == 1 ? 0 : quotient(rest, n), j = rest - hk * n;
+      if (j <= reach && j <= n - j) return make_int4(x - j, id, hk, 0);
+      if (n - j <= reach) return hk + 1 < Hk ? make_int4(x + n - j, id, hk + 1, 0) : make_int4(x + n - j, id + 1, 0, 0);
+      return make_int4(x, id, hk, j);
+    };
+    auto shfl4 = [](int4 v, int l) {
+      return make_int4(__shfl_sync(0xffffffffu, v.x, l), __shfl_sync(0xffffffffu, v.y, l), __shfl_sync(0xffffffffu, v.z, l),
+                       __shfl_sync(0xffffffffu, v.w, l));
+    };
+    // lanes 0 and 1 find the CTA's bounds, lanes 0 to 8 then the warps'
+    const int c = me + (lane & 1);
+    const int4 own = snap(c * each + min(c, more), CTA_SNAP), lo = shfl4(own, 0);
+    const int hi = __shfl_sync(0xffffffffu, own.x, 1);
+    if (lo.x == hi) return;
+    const int few = (hi - lo.x) / WARPS, rest = (hi - lo.x) % WARPS;  // fewer tiles than warps: the last have none
+    int4 at = snap(lo.x + lane * few + min(lane, rest), WARP_SNAP);
+    if (lane == 0 || at.x < lo.x) at = lo;
+    if (lane >= WARPS || at.x > hi) at.x = hi;
+    begin = shfl4(at, warp);
+    left = __shfl_sync(0xffffffffu, at.x, warp + 1) - begin.x;
   }
-  auto cta_of = [&](int x) { return x < more * (each + 1) ? quotient(x, each + 1) : more + quotient(x - more * (each + 1), each); };
   auto span_at = [&](int id) { return spans[g.direct ? 0 : id]; };
-  // a warp's piece of it; where there are fewer tiles than warps, the last warps have none
-  const int few = (hi - lo) / WARPS, rest_tiles = (hi - lo) % WARPS;
-  const int x0 = lo + warp * few + min(warp, rest_tiles), x1 = x0 + few + (warp < rest_tiles ? 1 : 0);
-  int fetch_left = x1 - x0, left = fetch_left;
-  if (lane < 2) part_id[2 * warp + lane] = -1;
+  int fetch_left = left;
 
   if (left > 0) {
     Cursor f;
-    if (g.direct) {
-      f.id = base_id; f.hk = base_hk; f.j = x0;
-    } else {
-      int l = 0, r = g.items;  // the last item whose tiles begin at or before x0
-      while (r - l > 1) {
-        const int mid = (l + r) >> 1;
-        if (pre[mid] * Hk <= x0) l = mid; else r = mid;
-      }
-      const int rest = x0 - pre[l] * Hk, n = pre[l + 1] - pre[l];
-      f.id = l;
-      f.hk = Hk == 1 ? 0 : quotient(rest, n);
-      f.j = rest - f.hk * n;
-    }
-    enter<NR>(a, g, f, span_at(f.id), lane);
+    f.id = begin.y;
+    f.hk = begin.z;
+    f.j = begin.w;
+    enter<T, NR>(a, g, f, span_at(f.id), lane);
     Cursor c = f;  // where the products stand (its page fields are unused)
 
     uint8_t* ring = smem + warp * S::RING;
@@ -614,7 +636,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
             ++f.id;
           }
           turn = true;
-          if (fetch_left > 0) enter<NR>(a, g, f, span_at(f.id), lane);
+          if (fetch_left > 0) enter<T, NR>(a, g, f, span_at(f.id), lane);
         } else if ((f.slot += TILE) == a.cache.page) {
           f.slot = 0;
           ++f.column;
@@ -830,12 +852,14 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
       const int end = 31 - __clz(mask), gid = __shfl_sync(0xffffffffu, id, leader);
       const bool begins = __shfl_sync(0xffffffffu, flag, leader) & 1, ends = __shfl_sync(0xffffffffu, flag, end) & 2;
       if (!(begins && ends)) open_id[begins ? 1 : 0] = gid;
-      // warps leader / 2 to end / 2 have one piece each
+      // warps leader / 2 to end / 2 have at most one piece each
       const int w0 = leader >> 1, n = (end >> 1) - w0 + 1;
       for (; blk < S::BLOCKS; blk += WARPS) {
         float4 stat;
         const float4 sum = join_block<D, NQ, false>(n, blk, lane, [&](int k) {
-          return (mask >> (2 * (w0 + k))) & 1u ? ws_warp + (w0 + k) * S::PART : reinterpret_cast<const float*>(smem + (w0 + k) * S::RING);
+          const int w = w0 + k;
+          if (!((mask >> (2 * w)) & 3u)) return static_cast<const float*>(nullptr);  // it has no tiles
+          return (mask >> (2 * w)) & 1u ? static_cast<const float*>(ws_warp + w * S::PART) : reinterpret_cast<const float*>(smem + w * S::RING);
         }, stat);
         if (!(begins && ends)) {
           store_block<D, NQ>(ws + (static_cast<int64_t>(me) * 2 + (begins ? 1 : 0)) * S::PART, blk, lane, sum, stat);
@@ -859,12 +883,14 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
     asm volatile("atom.acq_rel.gpu.global.inc.u32 %0, [%1], %2;" : "=r"(before) : "l"(counter), "r"(n - 1) : "memory");
     return before == static_cast<unsigned>(n - 1);
   };
+  auto cta_of = [&](int x) { return x < more * (each + 1) ? quotient(x, each + 1) : more + quotient(x - more * (each + 1), each); };
 #pragma unroll 1
   for (int side = 0; side < 2; ++side) {
     const int gid = open_id[side];
     if (gid < 0) continue;
     const int item = quotient(gid, Hk), hk = gid - item * Hk, tiles = pre[item + 1] - pre[item], x = pre[item] * Hk + hk * tiles;
-    const int c0 = cta_of(x), c1 = cta_of(x + tiles - 1), lead = c0 + ((me - c0) & ~(FAN - 1)), groups = (c1 - c0) / FAN + 1;
+    // boundaries within CTA_SNAP tiles of its ends went there
+    const int c0 = cta_of(x + CTA_SNAP), c1 = cta_of(x + tiles - 1 - CTA_SNAP), lead = c0 + ((me - c0) & ~(FAN - 1)), groups = (c1 - c0) / FAN + 1;
     const int b = g.row_tiles == 1 ? item : item / g.row_tiles, r0 = (item - b * g.row_tiles) * NR;
     auto at = [&](int c) { return ws + (static_cast<int64_t>(c) * 2 + (c == c0 ? 1 : 0)) * S::PART; };
     int first = lead, step = 1, n = min(FAN, c1 - lead + 1);
@@ -878,7 +904,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
       const bool done = level == 1 || groups == 1;
       for (int blk = warp; blk < S::BLOCKS; blk += WARPS) {
         float4 stat;
-        const float4 sum = join_block<D, NQ, true>(n, blk, lane, [&](int k) { return at(first + k * step); }, stat);
+        const float4 sum = join_block<D, NQ, true>(n, blk, lane, [&](int k) { return static_cast<const float*>(at(first + k * step)); }, stat);
         if (!done) {
           // into the leader's piece: its sums are read by this warp alone, its maxima and totals by all
           joined[blk * 32 + lane] = sum;
@@ -922,7 +948,7 @@ static Plan make_plan(const PagedAttnArgs& a) {
   if (a.window >= 0) tiles = std::min<int64_t>(tiles, (static_cast<int64_t>(a.window) + a.t) / TILE + 2);
   tiles = std::max<int64_t>(tiles, 1) * items * a.Hk;
   p.grid = static_cast<int>(g.direct ? std::min<int64_t>(items * a.Hk, INT32_MAX)
-                                     : std::max<int64_t>(1, std::min<int64_t>(std::min(a.sms, FAN * FAN), tiles / (WARPS * MIN_TILES))));
+                                     : std::max<int64_t>(1, std::min<int64_t>(std::min(a.sms, FAN * FAN), std::max(tiles / (WARPS * MIN_TILES), (items * a.Hk + WARPS - 1) / WARPS))));
   return p;
 }
 
