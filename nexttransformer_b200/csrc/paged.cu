@@ -256,6 +256,7 @@ static int launch_append(const PagedAppendArgs& a, cudaStream_t s) {
 // equally and one long row uses all of them.  A warp that covers a whole (row, KV head) writes its result;
 // other pieces are joined in the CTA, and what crosses CTAs by the CTA that arrives last, up to 16 pieces at
 // a time.  Pieces are always joined in the order of the line, so results do not depend on timing.
+constexpr float LAZY = 8.f;
 constexpr int WARPS = 8, TILE = 16, MIN_TILES = 2, CTA_SNAP = 32, WARP_SNAP = 2, FAN = 16;
 // Rows of the batch whose tiles a CTA lines up in shared memory; a larger batch has CTAs enough and gives
 // each (row, KV head) one.
@@ -705,7 +706,6 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
         __syncwarp();  // this stage has landed for every lane, and the stage before it is read by none
         int ahead = stage + S::STAGES - 1;
         if (ahead >= S::STAGES) ahead -= S::STAGES;
-        fetch(ahead);
         const uint32_t base = ring_u + stage * S::STAGE;
         if (++stage == S::STAGES) stage = 0;
 
@@ -721,9 +721,9 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
 #pragma unroll
           for (int nq = 0; nq < NQ; ++nq) Num<T>::mma(kk & 1 ? s2[nq] : s[nq], kf, qf[nq][kk][0], qf[nq][kk][1]);
         }
+        fetch(ahead);  // issued while the products finish
         const int key0 = (c.it.first & ~(TILE - 1)) + (j0 + tile) * TILE, key = key0 + qr;
         const bool edge = key0 < c.it.all_from || key0 < c.it.first || key0 + TILE > c.it.all_to;
-        uint32_t pf[NQ][2];
 #pragma unroll
         for (int nq = 0; nq < NQ; ++nq) {
 #pragma unroll
@@ -735,32 +735,49 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
               if (key + 8 > last[nq][e] || key + 8 < oldest[nq][e]) s[nq][e + 2] = -INFINITY;
             }
           }
-          float top[2] = {fmaxf(s[nq][0], s[nq][2]), fmaxf(s[nq][1], s[nq][3])};
+        }
+        // The reference m follows the maximum only when a score passes it by more than 2^LAZY, so that most tiles
+        // need neither a reduction over the lanes nor a rescaling; probabilities stay below 2^LAZY, far from the
+        // types' limits, and sums and pieces are relative to m all the same.
+        bool passed = false;
 #pragma unroll
-          for (int d = 4; d < 32; d <<= 1) {
-            top[0] = fmaxf(top[0], __shfl_xor_sync(0xffffffffu, top[0], d));
-            top[1] = fmaxf(top[1], __shfl_xor_sync(0xffffffffu, top[1], d));
-          }
-          const float m0 = fmaxf(m[nq][0], top[0]), m1 = fmaxf(m[nq][1], top[1]);
-          if (__any_sync(0xffffffffu, m0 != m[nq][0] || m1 != m[nq][1])) {
-            const float f0 = piece_weight(m[nq][0], m0), f1 = piece_weight(m[nq][1], m1);
-            m[nq][0] = m0;
-            m[nq][1] = m1;
-            l[nq][0] *= f0;
-            l[nq][1] *= f1;
+        for (int nq = 0; nq < NQ; ++nq)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) passed |= s[nq][e] > m[nq][e & 1] + LAZY;
+        if (__any_sync(0xffffffffu, passed)) {
+#pragma unroll
+          for (int nq = 0; nq < NQ; ++nq) {
+            float top[2] = {fmaxf(s[nq][0], s[nq][2]), fmaxf(s[nq][1], s[nq][3])};
+#pragma unroll
+            for (int d = 4; d < 32; d <<= 1) {
+              top[0] = fmaxf(top[0], __shfl_xor_sync(0xffffffffu, top[0], d));
+              top[1] = fmaxf(top[1], __shfl_xor_sync(0xffffffffu, top[1], d));
+            }
+            float f[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              top[e] = fmaxf(m[nq][e], top[e]);
+              f[e] = piece_weight(m[nq][e], top[e]);
+              m[nq][e] = top[e];
+              l[nq][e] *= f[e];
+            }
 #pragma unroll
             for (int d = 0; d < D / 16; ++d) {
-              o[nq][d][0] *= f0; o[nq][d][1] *= f1;
-              o[nq][d][2] *= f0; o[nq][d][3] *= f1;
+              o[nq][d][0] *= f[0]; o[nq][d][1] *= f[1];
+              o[nq][d][2] *= f[0]; o[nq][d][3] *= f[1];
             }
           }
-          const float r0 = m0 == -INFINITY ? 0.f : m0, r1 = m1 == -INFINITY ? 0.f : m1;
+        }
+        uint32_t pf[NQ][2];
+#pragma unroll
+        for (int nq = 0; nq < NQ; ++nq) {
+          const float r0 = m[nq][0] == -INFINITY ? 0.f : m[nq][0], r1 = m[nq][1] == -INFINITY ? 0.f : m[nq][1];
           s[nq][0] = exp2_fast(s[nq][0] - r0); s[nq][1] = exp2_fast(s[nq][1] - r1);
           s[nq][2] = exp2_fast(s[nq][2] - r0); s[nq][3] = exp2_fast(s[nq][3] - r1);
           l[nq][0] += s[nq][0] + s[nq][2];
           l[nq][1] += s[nq][1] + s[nq][3];
-          // probabilities are at most 1; rounding them to the cache's type costs no more than the rounding of
-          // V does (their sum stays in fp32)
+          // rounding the probabilities to the cache's type costs no more than the rounding of V did (their sum stays
+          // in fp32)
           pf[nq][0] = transpose8x8(Num<T>::pack(s[nq][0], s[nq][1]));
           pf[nq][1] = transpose8x8(Num<T>::pack(s[nq][2], s[nq][3]));
         }
