@@ -437,3 +437,40 @@ class LinearMixer(nn.Module):
         self.last_stats = {"state_precision": "fp32-carry" if chunked else str(acc_dtype(x)),
                            "backend": c.backend, "sequence_length": T}
         return self.c_proj(y)
+
+    def step(self, x, ve, conv, state, slots, count):
+        """Decoding: t new tokens ``x [B, t, d]`` of rows that carry their state (DeltaNet, GDN, KDA).
+
+        ``conv [rows, size - 1, 3 d]`` holds the last inputs of the short convolutions, ``state [rows, H, D, D]``
+        (fp32) the recurrent state; ``slots [B]`` are the rows' places in both, ``count [B]`` their real tokens.
+        Both are updated in place; what stands behind a row's count is ignored.
+        """
+        from nexttransformer_b200.ops.delta_recurrent import delta_recurrent
+        c = self.config
+        B, t, d = x.shape
+        H, D = c.heads, c.head_dim
+        convs = (self.q_conv, self.k_conv, self.v_conv)
+        rows, keep = slots.long(), convs[0].size - 1
+        seen = torch.cat((conv[rows].to(x.dtype), torch.cat((self.c_q(x), self.c_k(x), self.c_v(x)), -1)), 1)
+        weight = torch.cat([m.weight for m in convs]).to(x.dtype)
+        qkv = F.silu(F.conv1d(seen.transpose(1, 2), weight, groups=3 * d).transpose(1, 2).contiguous()).view(B, t, 3 * H, D)
+        last = count.long()[:, None] + torch.arange(keep, device=x.device)
+        conv[rows] = seen.gather(1, last[..., None].expand(-1, -1, 3 * d)).to(conv.dtype)
+        q, k, v = qkv[:, :, :H], qkv[:, :, H:2 * H], qkv[:, :, 2 * H:]
+        if ve is not None and self.ve_gate is not None:
+            v = v + (3 * torch.sigmoid(self.ve_gate(x[..., :12]))).unsqueeze(-1) * ve.reshape(B, t, H, D)
+        g = None
+        if self.kind == "gdn":
+            g = -self.log_decay.float().exp() * F.softplus(self.decay_proj(x).float() + self.dt_bias.float())
+        elif self.kind == "kda":
+            gate = self.gate_up(self.gate_down(x)).reshape(B, t, H, D)
+            g = -self.log_decay.float().exp() * F.softplus(gate.float() + self.dt_bias.float())
+        y = delta_recurrent(q, k, v, state, torch.sigmoid(self.beta_proj(x)), g, scale=D ** -.5, l2norm=True, slots=slots,
+                            count=count)
+        if self.kind == "deltanet":
+            return self.c_proj((norm(y) * self.output_gain.to(y.dtype)).reshape(B, t, d))
+        gate = self.output_gate(x).reshape(B, t, H, D)
+        if c.backend in CHUNK_BACKENDS and y.is_cuda:
+            from nexttransformer_b200.ops.linear_attention import gated_rms_norm as gated_rms_norm_cuda
+            return self.c_proj(gated_rms_norm_cuda(y, gate, self.output_gain).reshape(B, t, d))
+        return self.c_proj((norm(y) * self.output_gain.to(y.dtype) * F.silu(gate)).reshape(B, t, d))

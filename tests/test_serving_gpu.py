@@ -416,3 +416,94 @@ def test_adjust_logits_refusals():
             adjust_logits(**{"logits": x, **bad})
     with pytest.raises(RuntimeError, match="backward"):
         adjust_logits(x.clone().requires_grad_())
+
+
+# ------------------------------------------------------------------------------------------ together
+def test_operators_under_graph_capture():
+    """The operators can be captured; a replay on another stream, beside eager calls, sees the buffers' new contents."""
+    from nexttransformer_b200.ops.delta_recurrent import delta_recurrent
+    from nexttransformer_b200.ops.logits import adjust_logits
+    from nexttransformer_b200.ops.paged import paged_append, paged_attention
+    torch.manual_seed(11)
+    k, v, table = make_cache([3000, 40], 2, 16, 128, torch.bfloat16, fill=0.0)
+    start = torch.tensor([2990, 30], device=DEV, dtype=torch.int32)
+    angle = torch.rand(4096, 64, device=DEV)
+    cos, sin = angle.cos().bfloat16(), angle.sin().bfloat16()
+    new = torch.randn(2, 1, 8, 128, device=DEV).bfloat16()
+    state, beta = torch.zeros(2, 2, 128, 128, device=DEV), torch.rand(2, 1, 2, device=DEV)
+    tokens = torch.randint(0, 500, (2, 9), device=DEV, dtype=torch.int32)
+    two = torch.full((2,), 2.0, device=DEV)
+
+    def step():
+        q = paged_append(new[:, :, :4], new[:, :, 4:6], new[:, :, 6:], k, v, table, start, cos=cos, sin=sin, qk_scale=1.2)
+        y = paged_attention(q, k, v, table, start)
+        z = delta_recurrent(y[:, :, :2], y[:, :, 2:], y[:, :, :2], state, beta, l2norm=True)
+        return y, z, adjust_logits(z.reshape(2, -1), tokens=tokens, repetition=two)
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step()
+    side = torch.cuda.Stream()
+    for seed in (1, 2):
+        torch.manual_seed(seed)
+        new.copy_(torch.randn_like(new))
+        start += 1
+        state.zero_()
+        eager = [t.clone() for t in step()]
+        state.zero_()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            graph.replay()
+        torch.cuda.current_stream().wait_stream(side)
+        for a, b in zip(captured, eager):
+            assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("method,extra", [("dense", dict(layers=2, window_pattern="SL", kv_heads=1)),
+                                          ("gdn_hybrid_swa", dict(layers=4, backend="fla_chunk64", sliding_window=128)),
+                                          ("kda", dict(layers=2, backend="fla_chunk64"))])
+def test_paged_decode_of_a_model(method, extra):
+    """Prompts and steps through the kernels against the same weights in fp64: no further off than twice the plain
+    bf16 forward is, which measures what bf16 activations alone cost."""
+    from dataclasses import replace
+    from nexttransformer_b200.inference import PagedCache, decode_paged, generate_batch
+    from nexttransformer_b200.models import build_model
+    from nexttransformer_b200.models.config import candidate_config
+    from nexttransformer_b200.ops._ext import check_errors
+    from tests.test_families_gpu import compute_dtype
+    c = replace(candidate_config(method), width=256, heads=2, vocab_size=512, sequence_len=256, mlp_width=1024,
+                scale="custom", **{"window_pattern": "L", **extra})
+    with compute_dtype(torch.bfloat16):
+        m = build_model(c, DEV, seed=0).eval()
+    with torch.no_grad():
+        for b in m.transformer.h:
+            b.attn.c_proj.weight.normal_(0, .05)
+            b.mlp.c_proj.weight.normal_(0, .05)
+        m.smear_lambda.fill_(.5)
+        m.lm_head.weight.normal_(0, .2)
+    with compute_dtype(torch.float64):
+        oracle = build_model(c, "cpu", seed=0)
+        oracle.load_state_dict(m.state_dict())
+        oracle = oracle.double().eval()
+        oracle.cos, oracle.sin = m.cos.cpu().double(), m.sin.cpu().double()
+    torch.manual_seed(5)
+    ids = torch.randint(0, c.vocab_size, (3, 200), device=DEV)
+    have = [150, 1, 63]
+    cache = PagedCache(m, 3, 200, page=16)
+    with torch.no_grad():
+        got = [decode_paged(m, ids[:, :150], cache, have)]
+        for _ in range(2):
+            got.append(decode_paged(m, torch.stack([ids[r, n:n + 1] for r, n in enumerate(have)]), cache))
+            have = [n + 1 for n in have]
+        check_errors()
+        for step, n0 in ((0, [150, 1, 63]), (2, [152, 3, 65])):
+            for r, n in enumerate(n0):
+                with compute_dtype(torch.float64):
+                    ref = oracle(ids[r:r + 1, :n].cpu())[0, -1].float()
+                plain = (m(ids[r:r + 1, :n])[0, -1].cpu() - ref).norm() / ref.norm()
+                mine = (got[step][r].cpu() - ref).norm() / ref.norm()
+                assert mine <= 2 * plain + 2e-3, (step, r, mine.item(), plain.item())
+        answers = generate_batch(m, [ids[0, :9].tolist(), [1]], 5, temperature=.8, top_k=20, frequency=.5, repetition=1.1)
+    check_errors()
+    assert all(len(a) == 5 and all(0 <= t < c.vocab_size for t in a) for a in answers)
