@@ -1465,6 +1465,12 @@ Tensor delta_step(const Tensor& q, const Tensor& k, const Tensor& v, const Tenso
   const c10::cuda::CUDAGuard guard(q.device());
   Tensor o = at::empty({a.B, a.T, a.H, a.D}, q.options());
   a.o = o.data_ptr();
+  a.sms = num_sms(q);
+  Tensor ws;
+  if (const size_t bytes = nt_delta_step_workspace(a)) {
+    ws = at::empty({static_cast<int64_t>(bytes / sizeof(float))}, q.options().dtype(at::kFloat));
+    a.workspace = ws.data_ptr();
+  }
   ok(nt_delta_step(a, stream()), "delta_recurrent");
   C10_CUDA_KERNEL_LAUNCH_CHECK();
   return o;

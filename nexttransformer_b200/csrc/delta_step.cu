@@ -9,20 +9,23 @@
 // of its rows, so that every access is a full line; a thread's loads of the state are all in flight before the
 // first is used, and the quarters, the norms of q and k included, meet at one barrier.
 //
-// block_kernel (more tokens): eight tokens at a time.  With c_i the decay from the block's start through token i and
-// c_ij that behind token j through token i,
+// More tokens: eight at a time.  With c_i the decay from the block's start through token i and c_ij that behind token j
+// through token i,
 //   u_i = beta_i (v_i - (k_i c_i)^T S - sum_{j<i} M_ij u_j),     M_ij = k_i^T c_ij k_j
 //   o_i = (q_i c_i)^T S + sum_{j<=i} N_ij u_j,                   N_ij = q_i^T c_ij k_j
 //   S  <- c_7 S + sum_j (c_7j k_j) u_j^T
 // so the chain through S, its reduction and its update is walked once for eight tokens.  Decays are products of a
-// (never quotients or differences of sums), so none overflows and a decay of 0 is one.  Four warps hold the columns
-// in registers (a lane: CPL columns, an eighth of their rows) and read the block's vectors from shared memory, each
-// 16 bytes for 4 CPL products; four more prepare the next block meanwhile, a thread for each feature.  The state is
-// read once and written once.
+// (never quotients or differences of sums), so none overflows and a decay of 0 is one.
+// prepare_kernel forms what does not depend on S, for all blocks at once; block_kernel walks a row's blocks in order:
+// its warps hold the columns in registers (a lane: CPL columns, an eighth of their rows) and read the block's vectors
+// from shared memory, each 16 bytes for 4 CPL products, while bulk copies bring the next blocks.  The state is read
+// and written once a call (once for each segment of a long one).  The chain of a block bounds it.
 #include "delta_step.h"
 #include "common.cuh"
 
 #include <cuda_fp16.h>
+
+#include <algorithm>
 
 namespace nt {
 namespace dstep {
@@ -41,7 +44,7 @@ template <> NT_DEVICE float from_f(float v) { return v; }
 NT_DEVICE int tokens_of(const DeltaStepArgs& p, int b, bool report, int64_t& slot) {
   slot = p.slots ? p.slots[b] : b;
   if (slot >= 0 && slot < p.states) return p.count ? min(max(p.count[b], 0), p.T) : p.T;
-  if (slot >= p.states && report) record_error(1, b);
+  if (slot >= p.states && report) record_error(2, b);
   return 0;
 }
 template <class T>
@@ -127,18 +130,24 @@ __global__ void __launch_bounds__(128) step_kernel(const DeltaStepArgs p) {
 constexpr int PAIRS = C * (C + 1) / 2;  // (i, j) with j <= i, at i (i + 1) / 2 + j
 constexpr int SUMS = 2 * PAIRS + C;     // k_i c_ij k_j, q_i c_ij k_j, q_i q_i
 
-template <int D, int GATE, int COLS_>
-struct Block {  // eight tokens; the eighths of a vector lie in different banks
+// What block_kernel reads of eight tokens of a head.  The eighths of a vector lie in different banks.
+template <int D>
+struct Block {
   static constexpr int R = D / 8, SL = R + 4, ROW = 8 * SL;
-  alignas(16) float k[C][ROW];    // c_i k_i
-  alignas(16) float q[C][ROW];    // c_i q_i
-  alignas(16) float kc[C][ROW];   // c_7j k_j
-  alignas(16) float c7[GATE == 2 ? ROW : 4];
-  alignas(16) float Mt[C][C];     // Mt[j][i] = M_ij
-  alignas(16) float N[C][C];      // 0 above the diagonal
-  alignas(16) float beta[C];
-  float v[C][COLS_];
+  float k[C][ROW];    // c_i k_i
+  float q[C][ROW];    // c_i q_i
+  float kc[C][ROW];   // c_7j k_j
+  float c7[ROW];
+  float Mt[C][C];     // Mt[j][i] = M_ij
+  float N[C][C];      // 0 above the diagonal
+  float beta[C];
 };
+template <int D>
+struct Image {        // as it lies in the workspace
+  Block<D> block;
+  float v[D / 16][C][16];
+};
+static_assert(sizeof(Block<128>) % 16 == 0 && sizeof(Block<64>) % 16 == 0, "bulk copies take multiples of 16 bytes");
 
 // Sums of N values a lane over the warp: lane l (l % 16 for 16 values) gets the l-th sum.
 template <int N>
@@ -163,128 +172,129 @@ NT_DEVICE constexpr int pair_i(int e) {
 }
 NT_DEVICE constexpr int pair_j(int e) { return e - pair_i(e) * (pair_i(e) + 1) / 2; }
 
-template <class T, int D, int GATE, int CPL>
-__global__ void __launch_bounds__(256, 1) block_kernel(const DeltaStepArgs p) {
+// Block `blockIdx.x % rounds` of the segment for one (row, head): thread f has feature f of its eight tokens.
+template <class T, int D, int GATE>
+__global__ void __launch_bounds__(D) prepare_kernel(const DeltaStepArgs p, const int t0, const int rounds, Image<D>* images) {
+  constexpr int WARPS = D / 32;
+  __shared__ float partial[WARPS][SUMS], total[SUMS];
+  __shared__ float norm[2 * C];  // of k, of q
+  const int f = threadIdx.x, lane = f & 31, warp = f >> 5;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int bh = blockIdx.x / rounds, b = bh / p.H, h = bh - b * p.H, first = t0 + (blockIdx.x - bh * rounds) * C;
+  int64_t slot;
+  const int n = tokens_of(p, b, f == 0, slot);
+  if (first >= n) return;
+  Image<D>& im = images[blockIdx.x];
+  Block<D>& blk = im.block;
+  float k[C], q[C], c[C], ck[PAIRS];  // c: from the block's start; ck: c_ij k_j
+#pragma unroll
+  for (int i = 0; i < C; ++i) {
+    const int64_t t = first + i;
+    float a = 1.f, v = 0.f;
+    k[i] = q[i] = 0.f;
+    if (t < n) {  // behind the row's last token: nothing, with a decay of 1
+      k[i] = to_f(static_cast<const T*>(p.k)[b * p.ks[0] + t * p.ks[1] + h * p.ks[2] + f]);
+      q[i] = to_f(static_cast<const T*>(p.q)[b * p.qs[0] + t * p.qs[1] + h * p.qs[2] + f]);
+      v = to_f(static_cast<const T*>(p.v)[b * p.vs[0] + t * p.vs[1] + h * p.vs[2] + f]);
+      if (GATE) a = expf(p.g[b * p.gs[0] + t * p.gs[1] + h * p.gs[2] + (GATE == 2 ? f : 0)]);
+    }
+    im.v[f >> 4][i][f & 15] = v;
+    c[i] = i && GATE ? c[i - 1] * a : a;
+#pragma unroll
+    for (int j = 0; j <= i; ++j) {
+      const int e = i * (i + 1) / 2 + j;
+      ck[e] = j == i ? k[i] : GATE ? ck[(i - 1) * i / 2 + j] * a : k[j];
+    }
+  }
+  if (f < C) blk.beta[f] = first + f < n ? beta_of<T>(p, b * p.bs[0] + (first + f) * p.bs[1] + h * p.bs[2]) : 0.f;
+  {
+    float x[32], y[32], z[16];
+#pragma unroll
+    for (int e = 0; e < 32; ++e) x[e] = k[pair_i(e)] * ck[e];
+    partial[warp][lane] = reduce_scatter<32>(x, lane);
+#pragma unroll
+    for (int e = 0; e < 32; ++e) y[e] = q[pair_i(e)] * ck[e];
+    partial[warp][PAIRS + lane] = reduce_scatter<32>(y, lane);
+#pragma unroll
+    for (int e = 0; e < 16; ++e)
+      z[e] = e < 4 ? k[C - 1] * ck[32 + e] : e < 8 ? q[C - 1] * ck[28 + e] : q[e - 8] * q[e - 8];
+    const float last = reduce_scatter<16>(z, lane);
+    if (lane < 16) partial[warp][lane < 4 ? 32 + lane : lane < 8 ? PAIRS + 28 + lane : 2 * PAIRS + lane - 8] = last;
+  }
+  __syncthreads();
+  for (int e = f; e < SUMS; e += D) {
+    float x = partial[0][e];
+#pragma unroll
+    for (int w = 1; w < WARPS; ++w) x += partial[w][e];
+    total[e] = x;
+  }
+  __syncthreads();
+  if (f < 2 * C) {
+    const float x = total[f < C ? f * (f + 3) / 2 : 2 * PAIRS + f - C];
+    norm[f] = (f < C ? 1.f : p.scale) * (p.l2norm ? 1.f / fmaxf(sqrtf(x), 1e-12f) : 1.f);
+  }
+  __syncthreads();
+  if (f < C * C) {
+    const int i = f / C, j = f % C, e = i * (i + 1) / 2 + j;
+    blk.N[i][j] = j <= i ? total[PAIRS + e] * norm[C + i] * norm[j] : 0.f;
+    blk.Mt[j][i] = j < i ? total[e] * norm[i] * norm[j] : 0.f;
+  }
+  constexpr int R = Block<D>::R, SL = Block<D>::SL;
+  const int at = (f / R) * SL + f % R;
+#pragma unroll
+  for (int i = 0; i < C; ++i) {
+    blk.k[i][at] = k[i] * c[i] * norm[i];
+    blk.q[i][at] = q[i] * c[i] * norm[C + i];
+    blk.kc[i][at] = ck[(C - 1) * C / 2 + i] * norm[i];
+  }
+  blk.c7[at] = c[C - 1];
+}
+
+NT_DEVICE void bulk_load(void* dst, const void* src, int bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)),
+               "l"(src), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
+
+constexpr int BUFFERS = 4;
+template <int D, int CPL>
+struct Buffer {
+  Block<D> block;
+  float v[CPL][C][16];
+};
+
+// Tokens t0 .. t0 + tokens - 1 of one (row, head), 16 CPL columns a CTA.
+template <class T, int D, bool DECAY, int CPL>
+__global__ void __launch_bounds__(128) block_kernel(const DeltaStepArgs p, const int t0, const int tokens, const int rounds_all,
+                                                    const Image<D>* images) {
   constexpr int W = 16 * CPL, BLOCKS = D / W, R = D / 8;  // columns of a CTA; rows of a lane
-  using B = Block<D, GATE, W>;
-  __shared__ B blocks[2];
-  __shared__ float partial[D / 32][SUMS], total[SUMS];
-  __shared__ __align__(16) float norm[2 * C];  // of k, of q
-  const int lane = threadIdx.x & 31, warp = (threadIdx.x >> 5) & 3;
+  using B = Block<D>;
+  extern __shared__ __align__(128) uint8_t smem[];
+  Buffer<D, CPL>* buffers = reinterpret_cast<Buffer<D, CPL>*>(smem);
+  __shared__ uint64_t full[BUFFERS];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int cb = blockIdx.x % BLOCKS, bh = blockIdx.x / BLOCKS;
   const int b = bh / p.H, h = bh - b * p.H;
   int64_t slot;
-  const int n = tokens_of(p, b, threadIdx.x == 0, slot), rounds = (n + C - 1) / C;
-
-  if (threadIdx.x >= 128) {
-    // ---- the warps that prepare: thread f has feature f of the eight tokens
-    const int f = threadIdx.x - 128, at = (f / R) * B::SL + f % R;
-    const bool has = f < D;
-    T rk[C], rq[C], rv[CPL];
-    float rg[C], rbeta = 0.f;
-    const int vt = f >> 4, vc = (f & 15) * CPL;  // the value entries it brings
-    auto load = [&](int round) {
-#pragma unroll
-      for (int i = 0; i < C; ++i) {
-        const int64_t t = round * C + i;
-        rk[i] = rq[i] = from_f<T>(0.f);
-        rg[i] = 0.f;
-        if (t >= n) continue;  // behind the row's last token: nothing, with a decay of 1
-        if (has) {
-          rk[i] = static_cast<const T*>(p.k)[b * p.ks[0] + t * p.ks[1] + h * p.ks[2] + f];
-          rq[i] = static_cast<const T*>(p.q)[b * p.qs[0] + t * p.qs[1] + h * p.qs[2] + f];
-        }
-        const int64_t ga = b * p.gs[0] + t * p.gs[1] + h * p.gs[2];
-        if (GATE == 2 && has) rg[i] = p.g[ga + f];
-        if (GATE == 1) rg[i] = p.g[ga];
-      }
-      const int64_t t = round * C + vt;
-#pragma unroll
-      for (int e = 0; e < CPL; ++e)
-        rv[e] = t < n ? static_cast<const T*>(p.v)[b * p.vs[0] + t * p.vs[1] + h * p.vs[2] + cb * W + vc + e] : from_f<T>(0.f);
-      const int64_t tb = round * C + f;
-      rbeta = f < C && tb < n ? beta_of<T>(p, b * p.bs[0] + tb * p.bs[1] + h * p.bs[2]) : 0.f;
-    };
-    auto prepare = [&](int round) {
-      B& blk = blocks[round & 1];
-      float k[C], q[C], c[C], ck[PAIRS];  // c: from the block's start; ck: c_ij k_j
-#pragma unroll
-      for (int i = 0; i < C; ++i) {
-        k[i] = to_f(rk[i]);
-        q[i] = to_f(rq[i]);
-        const float a = GATE ? expf(rg[i]) : 1.f;
-        c[i] = i && GATE ? c[i - 1] * a : a;
-#pragma unroll
-        for (int j = 0; j <= i; ++j) {
-          const int e = i * (i + 1) / 2 + j;
-          ck[e] = j == i ? k[i] : GATE ? ck[(i - 1) * i / 2 + j] * a : k[j];
-        }
-      }
-#pragma unroll
-      for (int e = 0; e < CPL; ++e) blk.v[vt][vc + e] = to_f(rv[e]);
-      if (f < C) blk.beta[f] = rbeta;
-      if (round + 1 < rounds) load(round + 1);
-      if (has) {
-        float x[32], y[32], z[16];
-#pragma unroll
-        for (int e = 0; e < 32; ++e) x[e] = k[pair_i(e)] * ck[e];
-        partial[warp][lane] = reduce_scatter<32>(x, lane);
-#pragma unroll
-        for (int e = 0; e < 32; ++e) y[e] = q[pair_i(e)] * ck[e];
-        partial[warp][PAIRS + lane] = reduce_scatter<32>(y, lane);
-#pragma unroll
-        for (int e = 0; e < 16; ++e)
-          z[e] = e < 4 ? k[C - 1] * ck[32 + e] : e < 8 ? q[C - 1] * ck[28 + e] : q[e - 8] * q[e - 8];
-        const float last = reduce_scatter<16>(z, lane);
-        if (lane < 16) partial[warp][lane < 4 ? 32 + lane : lane < 8 ? PAIRS + 28 + lane : 2 * PAIRS + lane - 8] = last;
-      }
-      named_bar_sync(1, 128);
-      auto sum = [&](int e) {
-        float x = partial[0][e];
-#pragma unroll
-        for (int w = 1; w < D / 32; ++w) x += partial[w][e];
-        return x;
-      };
-      if (f < SUMS) total[f] = sum(f);
-      if (f >= 128 - 2 * C) {
-        const int e = f - (128 - 2 * C);
-        const float x = sum(e < C ? e * (e + 3) / 2 : 2 * PAIRS + e - C);
-        norm[e] = (e < C ? 1.f : p.scale) * (p.l2norm ? 1.f / fmaxf(sqrtf(x), 1e-12f) : 1.f);
-      }
-      named_bar_sync(1, 128);
-      if (f < C * C) {
-        const int i = f / C, j = f % C, e = i * (i + 1) / 2 + j;
-        blk.N[i][j] = j <= i ? total[PAIRS + e] * norm[C + i] * norm[j] : 0.f;
-        if (j < i) blk.Mt[j][i] = total[e] * norm[i] * norm[j];
-      }
-      if (has) {
-#pragma unroll
-        for (int i = 0; i < C; ++i) {
-          blk.k[i][at] = k[i] * c[i] * norm[i];
-          blk.q[i][at] = q[i] * c[i] * norm[C + i];
-          blk.kc[i][at] = ck[(C - 1) * C / 2 + i] * norm[i];
-        }
-        if (GATE == 2) blk.c7[at] = c[C - 1];
-        if (GATE == 1 && f == 0) blk.c7[0] = c[C - 1];
-      }
-    };
-    if (rounds > 0) {
-      load(0);
-      prepare(0);
-    }
-    __syncthreads();
-    for (int round = 0; round < rounds; ++round) {
-      if (round + 1 < rounds) prepare(round + 1);
-      __syncthreads();
-    }
-    return;
+  const int n = min(max(tokens_of(p, b, false, slot) - t0, 0), tokens), rounds = (n + C - 1) / C;
+  const Image<D>* im = images + static_cast<int64_t>(bh) * rounds_all;
+  auto bring = [&](int round) {
+    Buffer<D, CPL>& buf = buffers[round % BUFFERS];
+    uint64_t* bar = full + round % BUFFERS;
+    mbar_expect_tx(bar, sizeof(B) + sizeof(buf.v));
+    bulk_load(&buf.block, &im[round].block, sizeof(B), bar);
+    bulk_load(buf.v, im[round].v[cb * CPL], sizeof(buf.v), bar);
+  };
+  if (tid == 0) {
+    for (int i = 0; i < BUFFERS; ++i) mbar_init(full + i, 1);
+    fence_barrier_init();
   }
 
-  // ---- the warps that hold the state: lane (slice, lc) has rows slice R .. of columns col .. col + CPL - 1
-  const int slice = lane >> 2, mine = CPL == 2 ? slice & 1 : 0;  // the one of its columns that it solves for
-  const int local = warp * 4 * CPL + (lane & 3) * CPL, col = cb * W + local;
+  // lane (slice, lc) has rows slice R .. of columns col .. col + CPL - 1, and solves for column col + mine
+  const int slice = lane >> 2, mine = CPL == 2 ? slice & 1 : 0;
+  const int local = warp * 4 * CPL + (lane & 3) * CPL, col = cb * W + local, vg = (local + mine) >> 4, vc = (local + mine) & 15;
   float* sp = p.state + ((n ? slot : 0) * p.H + h) * D * D + static_cast<int64_t>(slice) * R * D + col;
-  T* op = static_cast<T*>(p.o) + (static_cast<int64_t>(b) * p.T * p.H + h) * D + col + mine;
+  T* op = static_cast<T*>(p.o) + ((static_cast<int64_t>(b) * p.T + t0) * p.H + h) * D + col + mine;
   const int64_t ostep = static_cast<int64_t>(p.H) * D;
   float2 S[CPL][R / 2];
   if (n > 0) {
@@ -293,9 +303,18 @@ __global__ void __launch_bounds__(256, 1) block_kernel(const DeltaStepArgs p) {
 #pragma unroll
       for (int e = 0; e < CPL; ++e) S[e][r] = make_float2(sp[2 * r * D + e], sp[(2 * r + 1) * D + e]);
   }
+  // launched while prepare_kernel runs: up to here nothing of its was read
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (tid == 0)
+    for (int r = 0; r < min(rounds, BUFFERS); ++r) bring(r);
   __syncthreads();
-  for (int round = 0; round < rounds; ++round) {
-    const B& blk = blocks[round & 1];
+  bool fine = true;
+  int round = 0;
+  for (; round < rounds; ++round) {
+    fine = mbar_wait(full + round % BUFFERS, (round / BUFFERS) & 1, 0xD50u);
+    __syncwarp();
+    const Buffer<D, CPL>& buf = buffers[round % BUFFERS];
+    const B& blk = buf.block;
     // products of the state with eight vectors, over this lane's rows
     auto products = [&](const float (&vec)[C][B::ROW], float (&x)[CPL][C]) {
       float2 acc[CPL][C];
@@ -321,7 +340,6 @@ __global__ void __launch_bounds__(256, 1) block_kernel(const DeltaStepArgs p) {
     };
     float x[CPL][C], y[CPL][C], u[CPL][C];
     products(blk.k, x);
-    products(blk.q, y);
     // the column's own sums, over the eight slices
     float own[C];
 #pragma unroll
@@ -330,13 +348,16 @@ __global__ void __launch_bounds__(256, 1) block_kernel(const DeltaStepArgs p) {
       else own[i] = x[0][i] + __shfl_xor_sync(0xffffffffu, x[0][i], 4);
       own[i] += __shfl_xor_sync(0xffffffffu, own[i], 8);
       own[i] += __shfl_xor_sync(0xffffffffu, own[i], 16);
-      own[i] = blk.v[i][local + mine] - own[i];
+      own[i] = buf.v[vg][i][vc] - own[i];
     }
+    products(blk.q, y);  // independent of the solution: fills its waits
 #pragma unroll
     for (int j = 0; j < C; ++j) {
+      const float4 m0 = *reinterpret_cast<const float4*>(&blk.Mt[j][0]), m1 = *reinterpret_cast<const float4*>(&blk.Mt[j][4]);
+      const float m[C] = {m0.x, m0.y, m0.z, m0.w, m1.x, m1.y, m1.z, m1.w};
       own[j] *= blk.beta[j];
 #pragma unroll
-      for (int i = j + 1; i < C; ++i) own[i] = fmaf(-blk.Mt[j][i], own[j], own[i]);
+      for (int i = j + 1; i < C; ++i) own[i] = fmaf(-m[i], own[j], own[i]);
     }
     // q sums: a lane keeps CPL tokens of its own column
     const bool b0 = slice & 1, b1 = slice & 2, b2 = slice & 4;
@@ -361,9 +382,10 @@ __global__ void __launch_bounds__(256, 1) block_kernel(const DeltaStepArgs p) {
 #pragma unroll
     for (int e = 0; e < CPL; ++e) {
       const int i = token + e;
+      const float4 n0 = *reinterpret_cast<const float4*>(&blk.N[i][0]), n1 = *reinterpret_cast<const float4*>(&blk.N[i][4]);
       float o = qs[e];
-#pragma unroll
-      for (int j = 0; j < C; ++j) o = fmaf(blk.N[i][j], own[j], o);
+      o = fmaf(n0.x, own[0], o); o = fmaf(n0.y, own[1], o); o = fmaf(n0.z, own[2], o); o = fmaf(n0.w, own[3], o);
+      o = fmaf(n1.x, own[4], o); o = fmaf(n1.y, own[5], o); o = fmaf(n1.z, own[6], o); o = fmaf(n1.w, own[7], o);
       if (round * C + i < n) op[(round * C + i) * ostep] = from_f<T>(o);
     }
 #pragma unroll
@@ -378,9 +400,8 @@ __global__ void __launch_bounds__(256, 1) block_kernel(const DeltaStepArgs p) {
     }
 #pragma unroll
     for (int r = 0; r < R / 4; ++r) {
-      if (GATE) {
-        const float4 c4 = GATE == 2 ? *reinterpret_cast<const float4*>(&blk.c7[slice * B::SL + r * 4])
-                                    : make_float4(blk.c7[0], blk.c7[0], blk.c7[0], blk.c7[0]);
+      if (DECAY) {
+        const float4 c4 = *reinterpret_cast<const float4*>(&blk.c7[slice * B::SL + r * 4]);
 #pragma unroll
         for (int e = 0; e < CPL; ++e) {
           S[e][2 * r] = mul2(S[e][2 * r], make_float2(c4.x, c4.y));
@@ -398,7 +419,12 @@ __global__ void __launch_bounds__(256, 1) block_kernel(const DeltaStepArgs p) {
         }
       }
     }
-    __syncthreads();
+    if (__syncthreads_or(!fine)) break;  // a wait that ran out ends the CTA
+    if (tid == 0 && round + BUFFERS < rounds) bring(round + BUFFERS);
+  }
+  if (round < rounds) {  // copies in flight land before the CTA's shared memory is given away
+    for (int r = round; r < min(round + BUFFERS, rounds); ++r) mbar_wait(full + r % BUFFERS, (r / BUFFERS) & 1, 0xD51u);
+    return;
   }
   if (n > 0) {
 #pragma unroll
@@ -410,26 +436,59 @@ __global__ void __launch_bounds__(256, 1) block_kernel(const DeltaStepArgs p) {
       }
   }
   if (slice < CPL)
-    for (int t = n; t < p.T; ++t) op[t * ostep] = from_f<T>(0.f);
+    for (int t = n; t < tokens; ++t) op[t * ostep] = from_f<T>(0.f);
+}
+
+template <class T, int D, bool DECAY, int CPL>
+static int launch_blocks(const DeltaStepArgs& a, int t0, int tokens, int rounds, const Image<D>* images, cudaStream_t s) {
+  static std::atomic<uint64_t> done{0};
+  constexpr int SMEM = BUFFERS * sizeof(Buffer<D, CPL>);
+  if (smem_limit(done, block_kernel<T, D, DECAY, CPL>, SMEM) != cudaSuccess) return -1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(a.B * a.H * (D / (16 * CPL))));
+  cfg.blockDim = dim3(128);
+  cfg.dynamicSmemBytes = SMEM;
+  cfg.stream = s;
+  cudaLaunchAttribute attr = {};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  // Launched early, the CTAs crowd on the SMs that prepare_kernel leaves first: 17 -> 14 us for 8 rows of 4 tokens,
+  // but 85 -> 142 us for one row of 389, where the walk through the blocks is all.
+  cfg.numAttrs = tokens <= 4 * C ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, block_kernel<T, D, DECAY, CPL>, a, t0, tokens, rounds, images) == cudaSuccess ? 0 : -1;
+}
+// Tokens of a segment: blocks that the workspace holds (64 MB, or one block of every head).
+static int64_t segment_rounds(const DeltaStepArgs& a) {
+  const int64_t image = a.D == 128 ? sizeof(Image<128>) : sizeof(Image<64>), heads = static_cast<int64_t>(a.B) * a.H;
+  return std::max<int64_t>(1, std::min<int64_t>((a.T + C - 1) / C, (int64_t{64} << 20) / (image * heads)));
 }
 
 template <class T, int D, int GATE>
-static void launch(const DeltaStepArgs& a, cudaStream_t s) {
-  if (a.T == 1) step_kernel<T, D, GATE><<<static_cast<unsigned>(a.B * a.H * (D / COLS)), 128, 0, s>>>(a);
-  else block_kernel<T, D, GATE, 2><<<static_cast<unsigned>(a.B * a.H * (D / 32)), 256, 0, s>>>(a);
+static int launch(const DeltaStepArgs& a, cudaStream_t s) {
+  if (a.T == 1) {
+    step_kernel<T, D, GATE><<<static_cast<unsigned>(a.B * a.H * (D / COLS)), 128, 0, s>>>(a);
+    return 0;
+  }
+  Image<D>* images = static_cast<Image<D>*>(a.workspace);
+  const int rounds = static_cast<int>(segment_rounds(a));
+  for (int t0 = 0; t0 < a.T; t0 += rounds * C) {
+    const int tokens = std::min(rounds * C, a.T - t0);
+    prepare_kernel<T, D, GATE><<<static_cast<unsigned>(a.B * a.H * rounds), D, 0, s>>>(a, t0, rounds, images);
+    // 32 columns a CTA use a vector twice as often as 16, which reach twice as many SMs
+    const int rc = a.B * a.H * (D / 32) < a.sms ? launch_blocks<T, D, GATE != 0, 1>(a, t0, tokens, rounds, images, s)
+                                                : launch_blocks<T, D, GATE != 0, 2>(a, t0, tokens, rounds, images, s);
+    if (rc) return rc;
+  }
+  return 0;
 }
 template <class T, int D>
-static void by_gate(const DeltaStepArgs& a, cudaStream_t s) {
-  if (a.gate == 0) launch<T, D, 0>(a, s);
-  else if (a.gate == 1) launch<T, D, 1>(a, s);
-  else launch<T, D, 2>(a, s);
+static int by_gate(const DeltaStepArgs& a, cudaStream_t s) {
+  return a.gate == 0 ? launch<T, D, 0>(a, s) : a.gate == 1 ? launch<T, D, 1>(a, s) : launch<T, D, 2>(a, s);
 }
 template <class T>
 static int by_width(const DeltaStepArgs& a, cudaStream_t s) {
-  if (a.D == 128) by_gate<T, 128>(a, s);
-  else if (a.D == 64) by_gate<T, 64>(a, s);
-  else return -1;
-  return 0;
+  return a.D == 128 ? by_gate<T, 128>(a, s) : a.D == 64 ? by_gate<T, 64>(a, s) : -1;
 }
 
 }  // namespace dstep
@@ -437,9 +496,14 @@ static int by_width(const DeltaStepArgs& a, cudaStream_t s) {
 
 using namespace nt::dstep;
 
+size_t nt_delta_step_workspace(const DeltaStepArgs& a) {
+  if (a.T <= 1 || (a.D != 64 && a.D != 128)) return 0;
+  return static_cast<size_t>(a.B) * a.H * segment_rounds(a) * (a.D == 128 ? sizeof(Image<128>) : sizeof(Image<64>));
+}
+
 int nt_delta_step(const DeltaStepArgs& a, cudaStream_t s) {
   if (a.B == 0 || a.T == 0 || a.H == 0) return 0;
-  if (static_cast<int64_t>(a.B) * a.H * 4 > INT32_MAX || a.gate < 0 || a.gate > 2) return -1;
+  if (static_cast<int64_t>(a.B) * a.H * std::max<int64_t>(8, segment_rounds(a)) > INT32_MAX || a.gate < 0 || a.gate > 2) return -1;
   if (a.type == DELTA_STEP_BF16) return by_width<__nv_bfloat16>(a, s);
   if (a.type == DELTA_STEP_FP16) return by_width<__half>(a, s);
   if (a.type == DELTA_STEP_FP32) return by_width<float>(a, s);

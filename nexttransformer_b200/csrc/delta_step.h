@@ -17,11 +17,13 @@ struct DeltaStepArgs {
   void* o = nullptr;
   const int *slots = nullptr, *count = nullptr;
   int64_t states = 0;
-  int B = 0, T = 0, H = 0, D = 0, gate = 0, type = 0;
+  int B = 0, T = 0, H = 0, D = 0, gate = 0, type = 0, sms = 0;
   bool beta_f32 = false, l2norm = false;
   float scale = 1.f;
+  void* workspace = nullptr;  // 16-byte aligned; holds nothing between calls
 };
+size_t nt_delta_step_workspace(const DeltaStepArgs& a);
 // 0, or -1 for an unsupported shape.
 int nt_delta_step(const DeltaStepArgs& a, cudaStream_t s);
-// Error word (reading clears it): 1 = a slot outside the states; `where` is the row.
+// Error word (reading clears it): 1 = a bounded device wait ran out, 2 = a slot outside the states, `where` is the row.
 int nt_delta_step_read_error(unsigned* where);

@@ -43,5 +43,7 @@ def check_errors():
         what = {1: "a position lies behind the row's page table", 2: "a page number lies outside the cache",
                 3: "a position lies behind the rotary table"}
         raise RuntimeError(f"paged cache: {what.get(p, f'code {p}')} (row {pw})")
+    if ds == 1:
+        raise RuntimeError(f"delta_recurrent: device pipeline wait expired ({dsw:#x})")
     if ds:
         raise RuntimeError(f"delta_recurrent: slot outside the states (row {dsw})")

@@ -284,6 +284,8 @@ def oracle_delta(q, k, v, state, beta, g, scale, l2norm, slots, count):
     ("kda", 64, 1, 17, [17, 16, 3], [0, 1, 2], True),
     ("deltanet", 128, 2, 70, [70, 41], [0, 1], True),
     ("gdn", 128, 1, 65, [65], [4], True),
+    ("gdn", 128, 30, 50, [50, 3, 50, 17, 50, 50], [5, 4, 3, 2, 1, 0], True),   # columns 32 a CTA
+    ("kda", 64, 40, 33, [33, 33, 8, 33, 33], [0, 1, 2, 3, 4], True),
 ])
 def test_delta_recurrent(dtype, kind, D, H, T, count, slots, l2norm):
     from nexttransformer_b200.ops._ext import check_errors
@@ -327,6 +329,22 @@ def test_delta_recurrent_in_pieces_and_zero_vectors():
                for a, b in zip(cuts, cuts[1:])]
         assert (torch.cat(cut, 1) - o).abs().max() <= slack and (state - whole).abs().max() <= slack
     assert (o[1, 5] == 0).all() and torch.isfinite(o).all()
+
+
+def test_delta_recurrent_in_segments():
+    """More blocks than the workspace holds: the state passes through memory between segments of a call."""
+    from nexttransformer_b200.ops.delta_recurrent import delta_recurrent
+    torch.manual_seed(12)
+    B, T, H, D = 8, 300, 16, 128
+    q, k, v = (torch.randn(B, T, H, D, device=DEV).bfloat16() for _ in range(3))
+    beta, g = torch.rand(B, T, H, device=DEV), -torch.rand(B, T, H, device=DEV)
+    count = [300, 1, 0, 199, 200, 201, 256, 77]
+    state = torch.randn(B, H, D, D, device=DEV) * 0.3
+    ref, ref_state = oracle_delta(q, k, v, state, beta, g, 1.0, True, list(range(B)), count)
+    got = delta_recurrent(q, k, v, state, beta, g, l2norm=True, count=torch.tensor(count, device=DEV, dtype=torch.int32))
+    slack = 2e-6 * (T + 4)
+    assert ((state.double() - ref_state).abs() <= slack).all()
+    assert ((got.double() - ref).abs() <= 1.02 * U[torch.bfloat16] * ref.abs() + slack).all()
 
 
 def test_delta_recurrent_state_behind_32_bits():
