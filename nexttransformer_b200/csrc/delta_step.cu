@@ -265,7 +265,7 @@ struct Buffer {
 
 // Tokens t0 .. t0 + tokens - 1 of one (row, head), 16 CPL columns a CTA.
 template <class T, int D, bool DECAY, int CPL>
-__global__ void __launch_bounds__(128) block_kernel(const DeltaStepArgs p, const int t0, const int tokens, const int rounds_all,
+__global__ void __launch_bounds__(160) block_kernel(const DeltaStepArgs p, const int t0, const int tokens, const int rounds_all,
                                                     const Image<D>* images) {
   constexpr int W = 16 * CPL, BLOCKS = D / W, R = D / 8;  // columns of a CTA; rows of a lane
   using B = Block<D>;
@@ -285,11 +285,26 @@ __global__ void __launch_bounds__(128) block_kernel(const DeltaStepArgs p, const
     bulk_load(&buf.block, &im[round].block, sizeof(B), bar);
     bulk_load(buf.v, im[round].v[cb * CPL], sizeof(buf.v), bar);
   };
-  if (tid == 0) {
+  if (tid == 128) {
     for (int i = 0; i < BUFFERS; ++i) mbar_init(full + i, 1);
     fence_barrier_init();
   }
 
+  if (warp == 4) {
+    // It only brings blocks (by a warp that also computes: 87 instead of 78 us for the longest listed run).  It may
+    // start while prepare_kernel runs, of which nothing was read up to here.
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (lane == 0)
+      for (int r = 0; r < min(rounds, BUFFERS); ++r) bring(r);
+    __syncthreads();
+    int round = 0;
+    for (; round < rounds; ++round) {
+      if (__syncthreads_or(0)) break;
+      if (lane == 0 && round + BUFFERS < rounds) bring(round + BUFFERS);
+      __syncwarp();
+    }
+    return;
+  }
   // lane (slice, lc) has rows slice R .. of columns col .. col + CPL - 1, and solves for column col + mine
   const int slice = lane >> 2, mine = CPL == 2 ? slice & 1 : 0;
   const int local = warp * 4 * CPL + (lane & 3) * CPL, col = cb * W + local, vg = (local + mine) >> 4, vc = (local + mine) & 15;
@@ -303,10 +318,6 @@ __global__ void __launch_bounds__(128) block_kernel(const DeltaStepArgs p, const
 #pragma unroll
       for (int e = 0; e < CPL; ++e) S[e][r] = make_float2(sp[2 * r * D + e], sp[(2 * r + 1) * D + e]);
   }
-  // launched while prepare_kernel runs: up to here nothing of its was read
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (tid == 0)
-    for (int r = 0; r < min(rounds, BUFFERS); ++r) bring(r);
   __syncthreads();
   bool fine = true;
   int round = 0;
@@ -420,7 +431,6 @@ __global__ void __launch_bounds__(128) block_kernel(const DeltaStepArgs p, const
       }
     }
     if (__syncthreads_or(!fine)) break;  // a wait that ran out ends the CTA
-    if (tid == 0 && round + BUFFERS < rounds) bring(round + BUFFERS);
   }
   if (round < rounds) {  // copies in flight land before the CTA's shared memory is given away
     for (int r = round; r < min(round + BUFFERS, rounds); ++r) mbar_wait(full + r % BUFFERS, (r / BUFFERS) & 1, 0xD51u);
@@ -446,7 +456,7 @@ static int launch_blocks(const DeltaStepArgs& a, int t0, int tokens, int rounds,
   if (smem_limit(done, block_kernel<T, D, DECAY, CPL>, SMEM) != cudaSuccess) return -1;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(a.B * a.H * (D / (16 * CPL))));
-  cfg.blockDim = dim3(128);
+  cfg.blockDim = dim3(160);
   cfg.dynamicSmemBytes = SMEM;
   cfg.stream = s;
   cudaLaunchAttribute attr = {};
