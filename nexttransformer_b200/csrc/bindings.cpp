@@ -1,6 +1,7 @@
 // Python bindings of the sm_100a kernels.  Only this file includes torch headers; the .cu
 // files export plain C++ launchers so that they compile quickly and stay independent of torch.
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
@@ -1254,6 +1255,15 @@ std::vector<int64_t> read_errors() {
 }
 
 // ------------------------------------------------------------------ serving
+void inference_only(std::initializer_list<const Tensor*> tensors) {
+  if (!at::GradMode::is_enabled()) return;
+  for (auto* t : tensors)
+    TORCH_CHECK(!t->requires_grad(), "serving operators have no backward: call them under torch.no_grad()");
+}
+// An uninitialised tensor from the caching allocator, without the dispatcher's detour.
+Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, const Tensor& like) {
+  return at::detail::empty_cuda(sizes, type, like.device(), c10::nullopt);
+}
 // A tensor of heads [B, t, heads, D]: its element strides of row, token and head.  `align` elements start a
 // 16-byte (or narrower) vector in the kernels.
 void head_strides(const Tensor& t, const char* name, int64_t align, int64_t (&s)[3]) {
@@ -1304,6 +1314,7 @@ PagedCacheArgs paged_cache(const Tensor& q, const Tensor& k, const Tensor& v, co
 Tensor paged_append(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& k_pages, const Tensor& v_pages,
                     const Tensor& table, const Tensor& start, const OptT& count, const Tensor& cos, const Tensor& sin,
                     c10::optional<double> qk_scale, const OptT& ve, const OptT& ve_gate) {
+  inference_only({&q, &k, &v});
   PagedAppendArgs a;
   a.cache = paged_cache(q, k_pages, v_pages, table);
   a.B = static_cast<int>(q.size(0));
@@ -1348,7 +1359,7 @@ Tensor paged_append(const Tensor& q, const Tensor& k, const Tensor& v, const Ten
   a.scale = static_cast<float>(qk_scale.value_or(1.0));
   a.fp16 = q.scalar_type() == at::kHalf;
   const c10::cuda::CUDAGuard guard(q.device());
-  Tensor out = at::empty({a.B, a.t, a.H, a.D}, q.options());
+  Tensor out = fresh({a.B, a.t, a.H, a.D}, q.scalar_type(), q);
   a.q_out = out.data_ptr();
   ok(nt_paged_append(a, stream()), "paged_append");
   C10_CUDA_KERNEL_LAUNCH_CHECK();
@@ -1386,6 +1397,7 @@ Tensor stream_counters(const Tensor& like, int n) {
 
 Tensor paged_attention(const Tensor& q, const Tensor& k_pages, const Tensor& v_pages, const Tensor& table,
                        const Tensor& start, const OptT& count, int64_t window, c10::optional<double> scale) {
+  inference_only({&q});
   PagedAttnArgs a;
   a.cache = paged_cache(q, k_pages, v_pages, table);
   a.B = static_cast<int>(q.size(0));
@@ -1402,12 +1414,12 @@ Tensor paged_attention(const Tensor& q, const Tensor& k_pages, const Tensor& v_p
   a.fp16 = q.scalar_type() == at::kHalf;
   a.sms = num_sms(q);
   const c10::cuda::CUDAGuard guard(q.device());
-  Tensor out = at::empty({a.B, a.t, a.H, a.D}, q.options());
+  Tensor out = fresh({a.B, a.t, a.H, a.D}, q.scalar_type(), q);
   if (out.numel() == 0) return out;
   a.out = out.data_ptr();
   Tensor ws, counters;
   if (const size_t bytes = nt_paged_attn_workspace(a)) {
-    ws = at::empty({static_cast<int64_t>(bytes / sizeof(float))}, q.options().dtype(at::kFloat));
+    ws = fresh({static_cast<int64_t>(bytes / sizeof(float))}, at::kFloat, q);
     a.workspace = ws.data_ptr<float>();
     counters = stream_counters(q, nt_paged_attn_counters(a.sms));
     a.counters = reinterpret_cast<unsigned*>(counters.data_ptr<int>());
@@ -1420,6 +1432,7 @@ Tensor paged_attention(const Tensor& q, const Tensor& k_pages, const Tensor& v_p
 Tensor delta_step(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& state, const Tensor& beta, const OptT& g,
                   double scale, bool l2norm, const OptT& slots, const OptT& count) {
   check_cuda(q, "q");
+  inference_only({&q, &k, &v});
   const auto type = q.scalar_type();
   TORCH_CHECK(type == at::kBFloat16 || type == at::kHalf || type == at::kFloat, "delta_recurrent takes bf16, fp16 or fp32");
   TORCH_CHECK(q.dim() == 4 && k.sizes() == q.sizes() && v.sizes() == q.sizes() && k.scalar_type() == type &&
@@ -1463,12 +1476,12 @@ Tensor delta_step(const Tensor& q, const Tensor& k, const Tensor& v, const Tenso
   a.scale = static_cast<float>(scale);
   a.type = type == at::kBFloat16 ? DELTA_STEP_BF16 : type == at::kHalf ? DELTA_STEP_FP16 : DELTA_STEP_FP32;
   const c10::cuda::CUDAGuard guard(q.device());
-  Tensor o = at::empty({a.B, a.T, a.H, a.D}, q.options());
+  Tensor o = fresh({a.B, a.T, a.H, a.D}, type, q);
   a.o = o.data_ptr();
   a.sms = num_sms(q);
   Tensor ws;
   if (const size_t bytes = nt_delta_step_workspace(a)) {
-    ws = at::empty({static_cast<int64_t>(bytes / sizeof(float))}, q.options().dtype(at::kFloat));
+    ws = fresh({static_cast<int64_t>(bytes / sizeof(float))}, at::kFloat, q);
     a.workspace = ws.data_ptr();
   }
   ok(nt_delta_step(a, stream()), "delta_recurrent");
@@ -1488,6 +1501,7 @@ Tensor adjust_logits(const Tensor& logits, const OptT& tokens, const OptT& lengt
                      const OptT& repetition, const OptT& presence, const OptT& frequency, const OptT& bias_ids,
                      const OptT& bias, const OptT& allowed) {
   check_cuda(logits, "logits");
+  inference_only({&logits});
   const auto type = logits.scalar_type();
   TORCH_CHECK(type == at::kBFloat16 || type == at::kHalf || type == at::kFloat, "logits must be bf16, fp16 or fp32");
   TORCH_CHECK(logits.dim() == 2 && (logits.stride(1) == 1 || logits.size(1) == 1), "logits must be [B, V] with contiguous rows");
@@ -1528,7 +1542,7 @@ Tensor adjust_logits(const Tensor& logits, const OptT& tokens, const OptT& lengt
     a.words = static_cast<int>(allowed->size(1));
   }
   const c10::cuda::CUDAGuard guard(logits.device());
-  Tensor out = at::empty({B, V}, logits.options().dtype(at::kFloat));
+  Tensor out = fresh({B, V}, at::kFloat, logits);
   a.out = out.data_ptr<float>();
   ok(nt_adjust_logits(a, stream()), "adjust_logits");
   C10_CUDA_KERNEL_LAUNCH_CHECK();

@@ -25,9 +25,9 @@ def delta_recurrent(q, k, v, state, beta, g=None, *, scale=1.0, l2norm=False, sl
     row out; no two rows share one).  ``count [B]``: how many of a row's T tokens are real; the others change
     nothing and give zeros.
     """
-    _inference_only(q, k, v)
     if q.is_cuda:
         return ext().delta_step(q, k, v, state, beta, g, scale, l2norm, slots, count)
+    _inference_only(q, k, v)
     return _plain(q, k, v, state, beta, g, scale, l2norm, slots, count)
 
 

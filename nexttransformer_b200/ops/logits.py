@@ -23,10 +23,10 @@ def adjust_logits(logits, *, tokens=None, length=None, prompt=None, repetition=N
 
     ``repetition``, ``presence`` and ``frequency`` are fp32 ``[B]``; what is None is left out.
     """
-    _inference_only(logits)
     if logits.is_cuda:
         return ext().adjust_logits(logits, tokens, length, prompt, repetition, presence, frequency, bias_ids, bias,
                                    allowed)
+    _inference_only(logits)
     return _plain(logits, tokens, length, prompt, repetition, presence, frequency, bias_ids, bias, allowed)
 
 

@@ -33,9 +33,9 @@ def paged_append(q, k, v, k_pages, v_pages, table, start, count=None, *, cos, si
     ``qk_scale``, RMS-normalised and scaled by it.  ``ve`` (like ``v``) and ``ve_gate [B, t, Hk]``: values
     become ``v + 3 sigmoid(ve_gate) ve``.
     """
-    _inference_only(q, k, v)
     if q.is_cuda:
         return ext().paged_append(q, k, v, k_pages, v_pages, table, start, count, cos, sin, qk_scale, ve, ve_gate)
+    _inference_only(q, k, v)
     return _append_plain(q, k, v, k_pages, v_pages, table, start, count, cos, sin, qk_scale, ve, ve_gate)
 
 
@@ -45,9 +45,9 @@ def paged_attention(q, k_pages, v_pages, table, start, count=None, *, window=-1,
     Token ``i`` of a row stands at position ``start + i`` and sees the positions up to its own, with
     ``window >= 0`` at most ``window`` back.  ``scale`` defaults to ``D ** -0.5``.
     """
-    _inference_only(q)
     if q.is_cuda:
         return ext().paged_attention(q, k_pages, v_pages, table, start, count, window, scale)
+    _inference_only(q)
     return _attention_plain(q, k_pages, v_pages, table, start, count, window, scale)
 
 
