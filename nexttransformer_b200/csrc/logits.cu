@@ -57,11 +57,11 @@ __global__ void __launch_bounds__(THREADS) adjust_kernel(const LogitsArgs a) {
       if (allowed) word[i] = static_cast<uint32_t>(allowed[(c0 + at) >> 5]) >> (at & 31);
     }
   }
+  const int n = a.length ? min(a.length[b], a.L) : a.L, prompt = a.prompt ? a.prompt[b] : 0;
   const int* row = a.tokens + static_cast<int64_t>(b) * a.L;
   int early[EARLY];
 #pragma unroll
-  for (int i = 0; i < EARLY; ++i) early[i] = i * THREADS + tid < a.L ? row[i * THREADS + tid] : -1;
-  const int n = a.length ? min(a.length[b], a.L) : a.L, prompt = a.prompt ? a.prompt[b] : 0;
+  for (int i = 0; i < EARLY; ++i) early[i] = i * THREADS + tid < n ? row[i * THREADS + tid] : -1;
   const float r = a.repetition ? a.repetition[b] : 1.f;
   const float presence = a.presence ? a.presence[b] : 0.f, frequency = a.frequency ? a.frequency[b] : 0.f;
   const bool adds_bias = a.K && tid >= THREADS - 32;  // one warp: repeated ids are added in their order
@@ -76,14 +76,8 @@ __global__ void __launch_bounds__(THREADS) adjust_kernel(const LogitsArgs a) {
       else atomicAdd(counts + at, 1u);
     }
   };
-  if (a.tokens) {
+  if (a.tokens)
     for (int i = tid; i < PIECE / 4; i += THREADS) reinterpret_cast<uint4*>(counts)[i] = make_uint4(0, 0, 0, 0);
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < EARLY; ++i) count(i * THREADS + tid, early[i]);
-#pragma unroll 4
-    for (int i = EARLY * THREADS + tid; i < n; i += THREADS) count(i, row[i]);
-  }
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     const int at = (i * THREADS + tid) * VEC;
@@ -101,6 +95,13 @@ __global__ void __launch_bounds__(THREADS) adjust_kernel(const LogitsArgs a) {
   }
   if (!a.tokens && !a.K) return;
   __syncthreads();
+  if (a.tokens) {
+#pragma unroll
+    for (int i = 0; i < EARLY; ++i) count(i * THREADS + tid, early[i]);
+#pragma unroll 4
+    for (int i = EARLY * THREADS + tid; i < n; i += THREADS) count(i, row[i]);
+    __syncthreads();
+  }
 
   auto is_allowed = [&](uint32_t at) { return !allowed || (static_cast<uint32_t>(allowed[(c0 + at) >> 5]) >> ((c0 + at) & 31)) & 1u; };
   auto mend = [&](int i, int token) {  // whoever takes an entry's count mends it

@@ -768,7 +768,9 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
             }
           }
         }
-        uint32_t pf[NQ][2];
+        // A probability is the sum of two numbers of the cache's type, so that its rounding (2^-17 for bf16) does not
+        // show beside the output's; the second product costs nothing that the memory would not take.
+        uint32_t pf[NQ][2], pl[NQ][2];
 #pragma unroll
         for (int nq = 0; nq < NQ; ++nq) {
           const float r0 = m[nq][0] == -INFINITY ? 0.f : m[nq][0], r1 = m[nq][1] == -INFINITY ? 0.f : m[nq][1];
@@ -776,10 +778,13 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
           s[nq][2] = exp2_fast(s[nq][2] - r0); s[nq][3] = exp2_fast(s[nq][3] - r1);
           l[nq][0] += s[nq][0] + s[nq][2];
           l[nq][1] += s[nq][1] + s[nq][3];
-          // rounding the probabilities to the cache's type costs no more than the rounding of V did (their sum stays
-          // in fp32)
-          pf[nq][0] = transpose8x8(Num<T>::pack(s[nq][0], s[nq][1]));
-          pf[nq][1] = transpose8x8(Num<T>::pack(s[nq][2], s[nq][3]));
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const uint32_t high = Num<T>::pack(s[nq][2 * e], s[nq][2 * e + 1]);
+            const float2 h = Num<T>::unpack(high);
+            pf[nq][e] = transpose8x8(high);
+            pl[nq][e] = transpose8x8(Num<T>::pack(s[nq][2 * e] - h.x, s[nq][2 * e + 1] - h.y));
+          }
         }
 #pragma unroll
         for (int d = 0; d < D / 16; ++d) {
@@ -787,6 +792,8 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
           ldsm4t(vf, base + vat[d & 3] + (d >> 2) * 128);
 #pragma unroll
           for (int nq = 0; nq < NQ; ++nq) Num<T>::mma(o[nq][d], vf, pf[nq][0], pf[nq][1]);
+#pragma unroll
+          for (int nq = 0; nq < NQ; ++nq) Num<T>::mma(o[nq][d], vf, pl[nq][0], pl[nq][1]);
         }
       }
 
