@@ -52,13 +52,13 @@ NT_DEVICE void load_halves(const T* p, int half, uint2& lo, uint2& hi) {
   hi = __ldcs(reinterpret_cast<const uint2*>(p + half));
 }
 template <class T>
-NT_DEVICE void unpack4(uint2 u, float (&x)[4]) {
-  const float2 a = Num<T>::unpack(u.x), b = Num<T>::unpack(u.y);
-  x[0] = a.x; x[1] = a.y; x[2] = b.x; x[3] = b.y;
+NT_DEVICE void unpack4(uint2 u, float2 (&x)[2]) {
+  x[0] = Num<T>::unpack(u.x);
+  x[1] = Num<T>::unpack(u.y);
 }
 template <class T>
-NT_DEVICE uint2 pack4(const float (&x)[4]) {
-  return make_uint2(Num<T>::pack(x[0], x[1]), Num<T>::pack(x[2], x[3]));
+NT_DEVICE uint2 pack4(const float2 (&x)[2]) {
+  return make_uint2(Num<T>::pack(x[0].x, x[0].y), Num<T>::pack(x[1].x, x[1].y));
 }
 // x / n for 0 <= x < 2^31 and 0 < n: the float quotient is at most a few units off
 NT_DEVICE int quotient(int x, int n) {
@@ -75,7 +75,7 @@ NT_DEVICE int quotient(int x, int n) {
   return q;
 }
 template <class T, int D, int PER>
-__global__ void __launch_bounds__(256, 5) append_kernel(const PagedAppendArgs a, const int turning) {
+__global__ void __launch_bounds__(256, 4) append_kernel(const PagedAppendArgs a, const int turning) {
   constexpr int L = D / 8, HALF = D / 2;
   const int lane = threadIdx.x % L, tok = blockIdx.x * (256 / L) + threadIdx.x / L;
   const bool live = tok < a.B * a.t;  // whole warps stay for the shuffles
@@ -135,14 +135,16 @@ __global__ void __launch_bounds__(256, 5) append_kernel(const PagedAppendArgs a,
     for (int e = 0; e < PER; ++e) {
       if (e >= heads) break;
       if (a.ve) {
-        float x[4], y[4], w[4];
+        float2 x[2], y[2], u[2], w[2];
         const float f = 3.f / (1.f + __expf(-Num<T>::one(gate[e])));
-        unpack4<T>(lo[e], x); unpack4<T>(elo[e], w);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) x[j] = fmaf(f, w[j], x[j]);
+        const float2 ff = make_float2(f, f);
+        unpack4<T>(lo[e], x); unpack4<T>(elo[e], u);
         unpack4<T>(hi[e], y); unpack4<T>(ehi[e], w);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) y[j] = fmaf(f, w[j], y[j]);
+        for (int j = 0; j < 2; ++j) {
+          x[j] = fma2(ff, u[j], x[j]);
+          y[j] = fma2(ff, w[j], y[j]);
+        }
         lo[e] = pack4<T>(x);
         hi[e] = pack4<T>(y);
       }
@@ -174,7 +176,7 @@ __global__ void __launch_bounds__(256, 5) append_kernel(const PagedAppendArgs a,
       }
   }
   T* k_out = nullptr;
-  float c[4] = {}, s[4] = {};
+  float2 c[2] = {}, s[2] = {}, ns[2];
   if (real) {
     if (h0 + heads > a.H) {
       int slot;
@@ -186,27 +188,28 @@ __global__ void __launch_bounds__(256, 5) append_kernel(const PagedAppendArgs a,
     unpack4<T>(*reinterpret_cast<const uint2*>(static_cast<const T*>(a.sin) + static_cast<int64_t>(pos) * HALF + lane * 4), s);
   }
 #pragma unroll
+  for (int j = 0; j < 2; ++j) ns[j] = make_float2(-s[j].x, -s[j].y);
+#pragma unroll
   for (int e = 0; e < PER; ++e) {
     if (e >= heads) break;
-    float x[4], y[4], u[4], w[4], r = 1.f;
+    float2 x[2], y[2], u[2], w[2];
     unpack4<T>(lo[e], x);
     unpack4<T>(hi[e], y);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      u[j] = fmaf(y[j], s[j], x[j] * c[j]);
-      w[j] = fmaf(-x[j], s[j], y[j] * c[j]);
+    for (int j = 0; j < 2; ++j) {
+      u[j] = fma2(y[j], s[j], mul2(x[j], c[j]));
+      w[j] = fma2(x[j], ns[j], mul2(y[j], c[j]));
     }
     if (a.norm) {
-      float sum = 0.f;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) sum = fmaf(u[j], u[j], fmaf(w[j], w[j], sum));
+      const float2 pair = fma2(w[1], w[1], fma2(u[1], u[1], fma2(w[0], w[0], mul2(u[0], u[0]))));
+      float sum = pair.x + pair.y;
 #pragma unroll
       for (int o = L / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      r = a.scale * rsqrtf(sum * (1.f / D) + EPS);
+      const float r = a.scale * rsqrtf(sum * (1.f / D) + EPS);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        u[j] *= r;
-        w[j] *= r;
+      for (int j = 0; j < 2; ++j) {
+        u[j] = mul2(u[j], make_float2(r, r));
+        w[j] = mul2(w[j], make_float2(r, r));
       }
     }
     T* dst;
@@ -235,9 +238,10 @@ template <class T, int D>
 static int launch_append(const PagedAppendArgs& a, cudaStream_t s) {
   const int64_t tokens = static_cast<int64_t>(a.B) * a.t, per_block = 256 / (D / 8), blocks = (tokens + per_block - 1) / per_block;
   if (tokens > INT32_MAX - per_block) return -1;
-  // four heads a thread keep enough bytes in flight and share a token's address work; with few tokens, one head
-  // a thread reaches more SMs
-  return blocks * ((a.H + 2 * a.Hk + 3) / 4) >= 2 * a.sms ? launch_append<T, D, 4>(a, static_cast<unsigned>(blocks), s)
+  // Five heads a thread keep enough bytes in flight and share a token's address work (8 prompts of 2048 tokens: 28.8 us;
+  // with four 30.8, with three 31, with one 65); with few tokens, one head a thread reaches more SMs (one token: 2.4 us
+  // on the device).
+  return blocks * ((a.H + 2 * a.Hk + 4) / 5) >= 2 * a.sms ? launch_append<T, D, 5>(a, static_cast<unsigned>(blocks), s)
                                                           : launch_append<T, D, 1>(a, static_cast<unsigned>(blocks), s);
 }
 
