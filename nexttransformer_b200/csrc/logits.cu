@@ -9,6 +9,11 @@
 // for nothing but its loads; meanwhile it counts the row's tokens that fall into the piece in shared memory
 // (whole-number atomics: their order does not matter) and then mends the few entries that tokens or biases
 // concern.  Reading and writing V (in + 4) bytes a row bounds it; the token list is read again by each piece, from L2.
+//
+// Measured on one B200, 224 rows of 65536 bf16 logits, up to 2048 tokens, 48 biases, a mask: 23 us, where its 92 MB
+// take 14 at the copy rate; without tokens, biases and mask the stream alone takes 20.  One row of 32768: 3 us.  With
+// counts and biases applied inside the stream it took 43 us (every piece waited for its counts).  Entries of 4 a thread
+// let a warp store whole lines (8 a thread: 21 instead of 20 us for the stream).
 #include "logits.h"
 #include "common.cuh"
 
@@ -161,7 +166,8 @@ static int launch(const LogitsArgs& a, cudaStream_t s) {
 }
 template <class T>
 static int by_piece(const LogitsArgs& a, cudaStream_t s) {
-  // large pieces read the token list less often, small ones reach more SMs
+  // large pieces read the token list less often (224 x 65536: 6 % faster than pieces of 4096), small ones reach
+  // more SMs (1 x 32768: 16 instead of 4)
   if (static_cast<int64_t>(a.B) * ((a.V + 8191) / 8192) >= 2 * a.sms) return launch<T, 8192>(a, s);
   return launch<T, 2048>(a, s);
 }

@@ -1,9 +1,9 @@
 """Serving operators (paged append and attention, recurrent delta rule, logits adjustment) against 64-bit definitions.
 
 Tolerances follow from the roundings: u is half a unit in the last place of the output type (2^-8 bf16, 2^-11 fp16).
-Attention rounds its probabilities (at most 1) to the cache's type before it multiplies them by V, which moves an
-output by at most u max|v| (fp16: and 2^-25 max|v| a key where they fall below the normal range), and rounds the
-output once.  Everything else is fp32.
+Attention may round its probabilities to the cache's type before it multiplies them by V, which moves an output by
+at most u max|v| (fp16: and 2^-25 max|v| a key where they fall below the normal range), and rounds the output once.
+Everything else is fp32.
 """
 import math
 
