@@ -11,9 +11,9 @@
 // concern.  Reading and writing V (in + 4) bytes a row bounds it; the token list is read again by each piece, from L2.
 //
 // Measured on one B200, 224 rows of 65536 bf16 logits, up to 2048 tokens, 48 biases, a mask: 23 us, where its 92 MB
-// take 14 at the copy rate; without tokens, biases and mask the stream alone takes 20.  One row of 32768: 3 us.  With
+// take 14 at the copy rate; an earlier build took 20 without tokens, biases and mask.  One row of 32768: 3 us.  With
 // counts and biases applied inside the stream it took 43 us (every piece waited for its counts).  Entries of 4 a thread
-// let a warp store whole lines (8 a thread: 21 instead of 20 us for the stream).
+// let a warp store whole lines.
 #include "logits.h"
 #include "common.cuh"
 

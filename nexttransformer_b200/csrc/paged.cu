@@ -1,4 +1,4 @@
-// K22: the paged key-value cache of the decoding engine.
+// K24: the paged key-value cache of the decoding engine.
 //
 // append     k' = s rope(k) / rms(rope(k)), v' = v + 3 sigmoid(gate) ve into the pages, q' = s rope(q) / rms(rope(q))
 // attention  o = softmax(scale q K^T) V over the pages, a few new tokens per row, GQA, left window
@@ -47,8 +47,8 @@ template <> struct Num<__half> {
 // both members of its rotated pairs.  They take PER heads of their token, whose loads are all in flight at once
 // and which share the token's angles and place in the cache.  Blocks with small y turn queries and keys, the
 // others mix values.  One pass: every input element is read once and every output element written once, and what is
-// no token is not read.  8 prompts of up to 2048 tokens, 10 + 5 heads of 128: 27 us where its 117 MB (and 18 MB of
-// zeros) take 21 at the copy rate; instruction issue (0.7 a cycle and scheduler) is the next limit.  One token: 2.4 us,
+// no token is not read.  8 prompts of up to 2048 tokens, 10 + 5 heads of 128: 27 us where its 117 MB (and 17 MB of
+// zeros) would take 21 at the copy rate; instruction issue (0.7 a cycle and scheduler) is the next limit.  One token: 2.4 us,
 // the chain from the row's length over its page to the store.
 template <class T>
 NT_DEVICE void load_halves(const T* p, int half, uint2& lo, uint2& hi) {
@@ -242,8 +242,8 @@ template <class T, int D>
 static int launch_append(const PagedAppendArgs& a, cudaStream_t s) {
   const int64_t tokens = static_cast<int64_t>(a.B) * a.t, per_block = 256 / (D / 8), blocks = (tokens + per_block - 1) / per_block;
   if (tokens > INT32_MAX - per_block) return -1;
-  // Five heads a thread keep enough bytes in flight and share a token's address work (8 prompts of 2048 tokens, back to back: 28.8
-  // us, with four heads 30.8); with few tokens, one head a thread reaches more SMs (one token: 2.4 us).
+  // Five heads a thread keep enough bytes in flight and share a token's address work (8 prompts of 2048 tokens, back
+  // to back: 28.8 us, with four heads 30.8); with few tokens, one head a thread reaches more SMs (one token: 2.4 us).
   return blocks * ((a.H + 2 * a.Hk + 4) / 5) >= 2 * a.sms ? launch_append<T, D, 5>(a, static_cast<unsigned>(blocks), s)
                                                           : launch_append<T, D, 1>(a, static_cast<unsigned>(blocks), s);
 }
@@ -266,12 +266,13 @@ static int launch_append(const PagedAppendArgs& a, cudaStream_t s) {
 // order of the line, so results do not depend on timing.
 //
 // Measured: 16 rows of 32768 keys, 10 / 5 heads of 128: 208 us, 6.45 TB/s.  64 rows of 512 to 8192 keys, 16 / 1 heads:
-// 28 us for 89 MB; the tiles themselves pass in 13 us (6.5 TB/s), the rest is the launch, the way to the first tile
-// (4 us: length, page, key, each a trip to memory) and the joins (6 us).  One row of 1001 keys: 11 us, a (row, KV head)
-// a CTA, at the 64 bytes a cycle that an SM takes in.  Smallest calls: 6 us.
+// 28.7 us for 89 MB.  Clock stamps of an earlier build, same case: the first tile is there after 4 us (length, page and
+// key are a trip to memory each), the tiles are done after 16 us in half of the CTAs and 20 in all; joins and launch
+// take what remains.  One row of 1001 keys: 11.5 us, few (row, KV
+// head) pairs on few SMs.
 // Tried and not kept: a second kernel for the join (10 us for one row, but two launches, 9 instead of 6 us on the
-// host), joins spread over rows instead of accumulator blocks, smaller reaches for the boundaries (8 and 16 tiles: the
-// same within 1 %), at least 4 tiles a warp (3 % slower over drawn calls).
+// host), joins spread over rows instead of accumulator blocks, smaller reaches for the boundaries (16
+// tiles 1 %, 8 tiles 2 % slower over a set of calls), at least 4 tiles a warp (4 % slower over it; 1: 2 % faster).
 constexpr float LAZY = 8.f;  // see the softmax
 constexpr int WARPS = 8, TILE = 16, MIN_TILES = 2, CTA_SNAP = 32, WARP_SNAP = 2, FAN = 16;
 // Rows of the batch whose tiles a CTA lines up in shared memory; a larger batch has CTAs enough and gives
