@@ -96,7 +96,7 @@ def test_paged_attention(dtype, D, H, Hk, page, t, window, rows):
 
 
 def test_paged_attention_many_rows():
-    """More rows than one CTA lines up: a CTA for each (row, KV head)."""
+    """More rows than a CTA has threads to line them up."""
     from nexttransformer_b200.ops.paged import paged_attention
     torch.manual_seed(2)
     rows = [(b * 7) % 90 for b in range(500)]
@@ -104,6 +104,33 @@ def test_paged_attention_many_rows():
     q = torch.randn(500, 1, 4, 64, device=DEV).bfloat16()
     got = paged_attention(q, k, v, table, torch.tensor(rows, device=DEV, dtype=torch.int32))
     check_attention(got, oracle_attention(q, k, v, table, rows, [1] * 500, -1), v, 90)
+
+
+@pytest.mark.parametrize("dtype,D,H,Hk,page,t,window,rows", [
+    (torch.bfloat16, 128, 12, 3, 16, 5, -1, [(0, 5), (1200, 5), (77, 1), (640, 4)]),        # 20 query rows: 2 strips
+    (torch.float16, 64, 10, 5, 48, 9, 30, [(0, 9), (500, 9), (31, 8), (32, 0)]),            # 18: the second almost empty
+    (torch.bfloat16, 128, 16, 4, 64, 9, -1, [(3000, 9), (5, 9)]),                           # 36: 4 strips, one empty
+    (torch.float16, 128, 16, 1, 32, 5, 100, [(0, 5), (2500, 5), (95, 5), (300, 1)]),        # 80: 8, three empty
+    (torch.bfloat16, 64, 16, 1, 128, 8, -1, [(9000, 8)]),                                   # 128: 8 strips over many CTAs
+    (torch.bfloat16, 128, 16, 1, 64, 11, -1, [(40, 11), (700, 2), (0, 11)]),                # 176: two items a row
+    (torch.float16, 128, 8, 2, 16, 50, 64, [(0, 50), (333, 41), (20, 33)]),                 # 200, windowed
+])
+def test_paged_attention_strips(dtype, D, H, Hk, page, t, window, rows):
+    """More query rows a KV head than one warp holds: warps beside each other, items behind each other."""
+    test_paged_attention(dtype, D, H, Hk, page, t, window, rows)
+
+
+@pytest.mark.parametrize("B,t,H,Hk", [(2100, 1, 4, 2), (2060, 5, 4, 1)])
+def test_paged_attention_of_more_rows_than_a_line_holds(B, t, H, Hk):
+    """More rows than the CTAs line up: a CTA for each (row, KV head).  Every 97th row is compared."""
+    from nexttransformer_b200.ops.paged import paged_attention
+    torch.manual_seed(12)
+    rows = [(b * 7) % 90 for b in range(B)]
+    k, v, table = make_cache([r + t for r in rows], Hk, 16, 64, torch.bfloat16)
+    q = torch.randn(B, t, H, 64, device=DEV).bfloat16()
+    got = paged_attention(q, k, v, table, torch.tensor(rows, device=DEV, dtype=torch.int32))
+    some = list(range(0, B, 97)) + [B - 1]
+    check_attention(got[some], oracle_attention(q[some], k, v, table[some], [rows[b] for b in some], [t] * len(some), -1), v, 95)
 
 
 def test_paged_attention_layouts_scale_and_stream():
