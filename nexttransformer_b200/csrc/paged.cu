@@ -273,6 +273,10 @@ static int launch_append(const PagedAppendArgs& a, cudaStream_t s) {
 // Tried and not kept: a second kernel for the join (10 us for one row, but two launches, 9 instead of 6 us on the
 // host), joins spread over rows instead of accumulator blocks, smaller reaches for the boundaries (16
 // tiles 1 %, 8 tiles 2 % slower over a set of calls), at least 4 tiles a warp (4 % slower over it; 1: 2 % faster).
+// More than 16 query rows a KV head are row tiles that each read the keys again: 248 rows of 5 tokens, 12 / 3 heads, 1709
+// keys take 237 us where one reading takes 102.  Warps of a CTA side by side on the row tiles of the same keys: 179 us,
+// but 5 % more for every call with one row tile and 12 % more over a set with several; row tiles outermost on the
+// line: 183 us and 1 % less over the set, but 1039 instead of 700 us for 8 prompts of 2048 tokens.  Neither was kept.
 constexpr float LAZY = 8.f;  // see the softmax
 constexpr int WARPS = 8, TILE = 16, MIN_TILES = 2, CTA_SNAP = 32, WARP_SNAP = 2, FAN = 16;
 // Rows of the batch whose tiles a CTA lines up in shared memory; a larger batch has CTAs enough and gives

@@ -6,7 +6,8 @@ feature) token by token on ``state [states, H, D, D]`` (fp32, updated in place):
     S <- diag(e^g) S,   S <- S + k (beta (v - k^T S))^T,   o = q^T S
 
 It is the form for decoding and for prompts that have to leave their final state; training uses the chunk
-form of ``ops.linear_attention``.  CUDA tensors run ``csrc/delta_step.cu`` (bf16, fp16 or fp32, heads of 64 or
+form of ``ops.linear_attention``.  On CUDA a run of tokens is taken eight at a time from the call's start, so a run
+cut elsewhere than behind a multiple of eight gives the same up to rounding, not bit for bit.  CUDA tensors run ``csrc/delta_step.cu`` (bf16, fp16 or fp32, heads of 64 or
 128), CPU tensors ``models.linear.recurrent_scan``.  It has no backward.
 """
 import torch

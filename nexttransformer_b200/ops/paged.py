@@ -43,7 +43,9 @@ def paged_attention(q, k_pages, v_pages, table, start, count=None, *, window=-1,
     """Attention of the new tokens ``q [B, t, H, D]`` over the pages, which hold their keys already.
 
     Token ``i`` of a row stands at position ``start + i`` and sees the positions up to its own, with
-    ``window >= 0`` at most ``window`` back.  ``scale`` defaults to ``D ** -0.5``.
+    ``window >= 0`` at most ``window`` back.  ``scale`` defaults to ``D ** -0.5``.  Keys and values that one of a
+    call's tokens sees have to be finite: one that only some of them see meets the others with probability zero,
+    which does not remove a NaN.  What no token sees (behind the row's tokens, before every window) may hold anything.
     """
     if q.is_cuda:
         return ext().paged_attention(q, k_pages, v_pages, table, start, count, window, scale)
