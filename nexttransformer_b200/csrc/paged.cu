@@ -371,7 +371,8 @@ NT_DEVICE float exp2_fast(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// Weight of a piece with maximum m in a sum with maximum top (both in powers of two; -inf: no keys).
+// Weight of a piece with maximum m in a sum with maximum top (both in powers of two; -inf: no keys; inf: the total is
+// NaN, and so is the weight).
 NT_DEVICE float piece_weight(float m, float top) { return top == -INFINITY ? 0.f : exp2_fast(m - top); }
 // A row without keys gives zeros; a total of NaN stays NaN.
 NT_DEVICE float inverse_total(float l) { return l == 0.f ? 0.f : 1.f / l; }
@@ -828,6 +829,8 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
           if (last[nq][e] < 0) {
             l[nq][e] = 0.f;
             m[nq][e] = -INFINITY;
+          } else if (isnan(l[nq][e])) {
+            m[nq][e] = INFINITY;  // maxima pass over a NaN; this one gives every join a weight of NaN
           }
         }
       const bool begins = j0 == 0, ends = j0 + n == c.it.tiles;
