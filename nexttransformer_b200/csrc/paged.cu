@@ -622,9 +622,11 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
     const int64_t kstep = ROWS * a.cache.slot_stride_k, vstep = ROWS * a.cache.slot_stride_v;
 
     bool turn = true;
+    unsigned gone = 0;  // bit of a stage: its tile's page is not in the cache
     auto fetch = [&](int stage) {
       if (fetch_left > 0) {
         if (turn) turn_page<T>(a, f, kc, vc, lane);
+        gone = (gone & ~(1u << stage)) | (f.there ? 0u : 1u << stage);
         const int key = (f.it.first & ~(TILE - 1)) + f.j * TILE;
         const T *ks = static_cast<const T*>(f.k), *vs = static_cast<const T*>(f.v);
         const uint32_t dst = ring_u + stage * S::STAGE;
@@ -729,6 +731,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
         int ahead = stage + S::STAGES - 1;
         if (ahead >= S::STAGES) ahead -= S::STAGES;
         const uint32_t base = ring_u + stage * S::STAGE;
+        const bool lost = (gone >> stage) & 1u;
         if (++stage == S::STAGES) stage = 0;
 
         float s[NQ][4], s2[NQ][4];  // two chains of products
@@ -744,8 +747,9 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
           for (int nq = 0; nq < NQ; ++nq) Num<T>::mma(kk & 1 ? s2[nq] : s[nq], kf, qf[nq][kk][0], qf[nq][kk][1]);
         }
         fetch(ahead);  // issued while the products finish
-        const int key0 = (c.it.first & ~(TILE - 1)) + (j0 + tile) * TILE, key = key0 + qr;
-        const bool edge = key0 < c.it.all_from || key0 < c.it.first || key0 + TILE > c.it.all_to;
+        const int key0 = (c.it.first & ~(TILE - 1)) + (j0 + tile) * TILE;
+        const int key = lost ? INT32_MAX - TILE : key0 + qr;  // a tile without a page lies behind every query
+        const bool edge = lost || key0 < c.it.all_from || key0 < c.it.first || key0 + TILE > c.it.all_to;
 #pragma unroll
         for (int nq = 0; nq < NQ; ++nq) {
 #pragma unroll

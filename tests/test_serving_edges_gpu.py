@@ -45,3 +45,49 @@ def test_attention_of_a_query_that_is_not_finite(keys, bad, dtype, heads, kv_hea
     assert torch.isnan(got[hit]).all()
     top = v.float().nan_to_num(0.0).abs().max()
     assert ((got - clean)[~hit].abs() <= 1.02 * U[dtype] * clean[~hit].abs() + 2.0 ** -15 * top).all()
+
+
+@pytest.mark.parametrize("dtype,D,H,Hk,page,t,window,rows,bad", [
+    # bad: (row, page column, number in the table)
+    (torch.bfloat16, 128, 10, 5, 64, 1, -1, [(1000, 1), (300, 1)], [(0, 7, -1), (0, 15, 1 << 30)]),
+    (torch.float16, 64, 4, 4, 16, 1, -1, [(40, 1), (9, 1)], [(0, 0, -5)]),
+    (torch.bfloat16, 128, 16, 1, 32, 5, 200, [(500, 5), (12, 3), (95, 5)], [(0, 12, -1), (0, 11, 99999), (2, 1, -1)]),
+    (torch.float16, 128, 6, 2, 48, 33, -1, [(0, 33), (200, 20)], [(1, 2, -1)]),
+    (torch.bfloat16, 64, 12, 3, 16, 1, -1, [(9000, 1)], [(0, j, -1) for j in range(100, 300)]),
+    (torch.bfloat16, 128, 2, 1, 64, 1, -1, [(70, 1), (70, 1)], [(0, 0, -1), (0, 1, -1)]),   # nothing is left of row 0
+])
+def test_attention_leaves_out_what_has_no_page(dtype, D, H, Hk, page, t, window, rows, bad):
+    """Keys whose page is not in the cache take no part; the others' softmax is theirs alone, and the error is reported.
+
+    Bound: probabilities held to 2^-16 (and in fp16 to 2^-25 of the largest a key), of values weighed with them, and u of the
+    output.
+    """
+    from nexttransformer_b200.ops._ext import check_errors
+    from nexttransformer_b200.ops.paged import paged_attention
+    torch.manual_seed(23)
+    k, v, table = make_cache([s + c for s, c in rows], Hk, page, D, dtype)
+    q = (torch.randn(len(rows), t, H, D, device=DEV) * 1.2).to(dtype)
+    missing = torch.zeros(len(rows), table.shape[1] * page, dtype=torch.bool, device=DEV)
+    broken = table.clone()
+    for b, column, number in bad:
+        broken[b, column] = number
+        missing[b, column * page:(column + 1) * page] = True
+    check_errors()
+    got = paged_attention(q, k, v, broken, ints(*(s for s, _ in rows)), ints(*(c for _, c in rows)), window=window)
+    with pytest.raises(RuntimeError, match="page number"):
+        check_errors()
+    top = v.float().nan_to_num(0.0).abs().max().double()
+    for b, (s, c) in enumerate(rows):
+        for i in range(c):
+            key = torch.arange(max(0, s + i - window) if window >= 0 else 0, s + i + 1, device=DEV)
+            key = key[~missing[b, key]]
+            if not len(key):
+                assert (got[b, i] == 0).all()
+                continue
+            at = table[b].long()[key // page], slice(None), key % page
+            K, V = k[at].double(), v[at].double()
+            p = torch.softmax(torch.einsum("hgd,khd->hgk", q[b, i].double().view(Hk, H // Hk, D), K) * D ** -0.5, -1)
+            ref, held = (torch.einsum("hgk,khd->hgd", p, x).reshape(H, D) for x in (V, V.abs()))
+            slack = 2.0 ** -15 * held + (len(key) * 2.0 ** -25 * top if dtype == torch.float16 else 0)
+            assert ((got[b, i].double() - ref).abs() <= 1.02 * U[dtype] * ref.abs() + slack).all(), (b, i)
+        assert (got[b, c:] == 0).all()
