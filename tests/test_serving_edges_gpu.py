@@ -91,3 +91,30 @@ def test_attention_leaves_out_what_has_no_page(dtype, D, H, Hk, page, t, window,
             slack = 2.0 ** -15 * held + (len(key) * 2.0 ** -25 * top if dtype == torch.float16 else 0)
             assert ((got[b, i].double() - ref).abs() <= 1.02 * U[dtype] * ref.abs() + slack).all(), (b, i)
         assert (got[b, c:] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("gap", [0, 6, 10, 12, 14, 16])
+@pytest.mark.parametrize("keys,B", [(32, 64), (700, 1), (5000, 300)])
+def test_attention_beside_a_key_that_takes_nearly_all(dtype, gap, keys, B):
+    """A first key with value zero whose score lies `gap` above the others': the output is made of small probabilities only.
+
+    Scores are exact up to their rounding in powers of two, below 2^-20, and exp2 is good to 2^-22.  A probability is held to
+    2^-16 of itself in bf16 and to 2^-22 in fp16, there with at most 2^-32 of the largest lost; sums of up to 5000 equal
+    numbers in fp32 may drift by 2^-24 for each 16 of them, 2^-15.7.  In all 2^-14 of the output besides its rounding, and
+    2^-32 of the value a key.
+    """
+    from nexttransformer_b200.ops.paged import paged_attention
+    K, V = torch.zeros(keys, 64), torch.full((keys, 64), 1000.0)
+    K[0, 0], V[0] = gap, 0
+    V[1::2, 1] = -500.0
+    k, v, table = pages_of(K, V, 16, dtype)
+    q = torch.zeros(B, 1, 1, 64, device=DEV, dtype=dtype)
+    q[..., 0] = 1
+    got = paged_attention(q, k, v, table.expand(B, -1).contiguous(), torch.full((B,), keys - 1, device=DEV, dtype=torch.int32),
+                          scale=1.0).double().cpu()[:, 0, 0]
+    p = torch.softmax(k.reshape(-1, 64)[:keys, 0].double().cpu(), 0)
+    values = v.reshape(-1, 64)[:keys].double().cpu()
+    ref, held = p @ values, p @ values.abs()
+    slack = 2.0 ** -14 * held + (keys * 2.0 ** -32 * 1000 * p[0] if dtype == torch.float16 else 0)
+    assert ((got - ref).abs() <= 1.02 * U[dtype] * ref.abs() + slack).all(), ((got - ref).abs() / ref.abs()).max().item()
