@@ -153,15 +153,17 @@ class PagedCache:
         self.held = [[] for _ in range(rows)]
 
     def reserve(self, counts):
-        """Pages for ``counts[row]`` more tokens of every row; raises when the pool is empty."""
-        new = []
+        """Pages for ``counts[row]`` more tokens of every row; raises when the pool is empty, and then takes none."""
+        needs = []
         for row, n in enumerate(counts):
-            need = -(-(self.lengths[row] + n) // self.page) - len(self.held[row])
             if n and self.lengths[row] + n > self.columns * self.page:
                 raise ValueError(f"row {row} would pass the cache's {self.columns * self.page} tokens")
-            if need > len(self.free):
-                raise RuntimeError("the paged cache has no free pages left")
-            for _ in range(max(0, need)):
+            needs.append(max(0, -(-(self.lengths[row] + n) // self.page) - len(self.held[row])))
+        if sum(needs) > len(self.free):
+            raise RuntimeError("the paged cache has no free pages left")
+        new = []
+        for row, need in enumerate(needs):
+            for _ in range(need):
                 new.append((row, len(self.held[row]), self.free[-1]))
                 self.held[row].append(self.free.pop())
         if new:
