@@ -249,7 +249,8 @@ def generate_batch(model, prompts, max_tokens, temperature=1.0, top_k=None, seed
     A row ends behind a token of ``stop``.  ``repetition``, ``presence`` and ``frequency`` are numbers, ``bias`` a
     dict from token to what is added to its logit, ``allowed`` a callable that gets the answers so far (a list
     of lists) and returns the grammar's bit masks for the next tokens, int32 ``[rows, ceil(V / 32)]`` (see
-    ``ops.logits.adjust_logits``).
+    ``ops.logits.adjust_logits``).  A row that it allows nothing ends there; rows that have ended may have any mask.  A
+    bias of inf settles the choice; a NaN among a row's logits raises.
     """
     if not prompts or any(not p for p in prompts):
         raise ValueError("every prompt needs at least one token")
@@ -279,13 +280,18 @@ def generate_batch(model, prompts, max_tokens, temperature=1.0, top_k=None, seed
             v, _ = torch.topk(logits, min(top_k, logits.size(-1)))
             logits = logits.masked_fill(logits < v[:, [-1]], -float("inf"))
         if temperature > 0:
-            nxt = torch.multinomial(F.softmax(logits / temperature, -1), 1, generator=g)
-        else:
-            nxt = logits.argmax(-1, keepdim=True)
-        for row, token in enumerate(nxt[:, 0].tolist()):
-            if live[row]:
+            logits = logits / temperature
+        # a row whose largest logit is not finite has a softmax of NaN, which sampling on CUDA answers with a device
+        # assert: its largest logits share the choice, and rows that have none are told apart below
+        top = logits.amax(-1, keepdim=True)
+        logits = torch.where(top.isfinite(), logits, torch.where(top.isnan() | (logits == top), 0.0, -torch.inf))
+        nxt = torch.multinomial(F.softmax(logits, -1), 1, generator=g) if temperature > 0 else logits.argmax(-1, keepdim=True)
+        for row, (token, nothing, broken) in enumerate(torch.cat((nxt, top == -torch.inf, top.isnan()), 1).tolist()):
+            if live[row] and broken:
+                raise RuntimeError(f"NaN among the logits of row {row}")
+            if live[row] and not nothing:
                 answers[row].append(token)
-                live[row] = token not in stop
+            live[row] = live[row] and not nothing and token not in stop
         if step + 1 == max_tokens or not any(live):
             break
         counts = [int(alive) for alive in live]

@@ -38,3 +38,41 @@ def test_a_refused_reservation_takes_nothing(method, fault):
     for _ in range(2):
         assert torch.equal(decode_paged(m, new, cache, counts)[:2], decode_paged(m, new, calm, counts)[:2])
     assert sorted(cache.free + sum(cache.held, [])) == list(range(len(cache.free) + sum(map(len, cache.held))))
+
+
+@pytest.mark.parametrize("temperature", [0, 1.0])
+@pytest.mark.parametrize("top_k", [None, 5])
+def test_a_grammar_that_allows_nothing(temperature, top_k):
+    """An ended answer's mask does not matter; a running answer that may not go on ends without a token; the others go on."""
+    from nexttransformer_b200.inference import generate_batch
+    c, m = _model("dense")
+    prompts, words = [[3, 1, 4], [9, 2], [6]], -(-c.vocab_size // 32)
+
+    def one(token):
+        mask = [0] * words
+        mask[token // 32] = 1 << (token % 32)
+        return mask
+
+    def grammar(done):   # row 0: 7 then stop token 8, then nothing; row 1: 5 for ever; row 2: 10, 11, then nothing
+        first = [one(7), one(8)][len(done[0])] if len(done[0]) < 2 else [0] * words
+        last = [one(10), one(11)][len(done[2])] if len(done[2]) < 2 else [0] * words
+        return torch.tensor([first, one(5), last], dtype=torch.int32)
+    got = generate_batch(m, prompts, 6, temperature=temperature, top_k=top_k, page=16, stop=(8,), allowed=grammar)
+    assert got == [[7, 8], [5] * 6, [10, 11]]
+    nothing = generate_batch(m, prompts, 6, temperature=temperature, top_k=top_k, page=16,
+                             allowed=lambda done: torch.zeros(3, words, dtype=torch.int32))
+    assert nothing == [[], [], []]
+
+
+@pytest.mark.parametrize("temperature", [0, 1.0])
+def test_logits_that_are_not_finite(temperature):
+    """NaN names its row; an infinite bias settles the choice."""
+    from nexttransformer_b200.inference import generate_batch
+    c, m = _model("dense")
+    with torch.no_grad():
+        m.transformer.wte.weight[7] = math.nan
+    with pytest.raises(RuntimeError, match="row 1"):
+        generate_batch(m, [[3, 1], [7], [2]], 2, temperature=temperature, page=16)
+    for bias in ({7: -1e9, 5: 1e6}, {7: -math.inf, 5: math.inf}, {7: -1e38, 5: 3e38}):
+        assert generate_batch(m, [[3, 1], [2]], 2, temperature=temperature, top_k=3, page=16, bias=bias) == [[5, 5]] * 2
+    assert generate_batch(m, [[3, 1]], 2, temperature=temperature * 1e-40, page=16, bias={7: -math.inf, 5: 9.0}) == [[5, 5]]
