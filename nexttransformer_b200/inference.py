@@ -279,13 +279,13 @@ def generate_batch(model, prompts, max_tokens, temperature=1.0, top_k=None, seed
         if top_k:
             v, _ = torch.topk(logits, min(top_k, logits.size(-1)))
             logits = logits.masked_fill(logits < v[:, [-1]], -float("inf"))
-        if temperature > 0:
-            logits = logits / temperature
-        # a row whose largest logit is not finite has a softmax of NaN, which sampling on CUDA answers with a device
-        # assert: its largest logits share the choice, and rows that have none are told apart below
+        # a row whose largest logit is not finite (over a small temperature, too) has a softmax of NaN, which sampling on
+        # CUDA answers with a device assert: its largest logits share the choice; rows that have none are told apart below
         top = logits.amax(-1, keepdim=True)
-        logits = torch.where(top.isfinite(), logits, torch.where(top.isnan() | (logits == top), 0.0, -torch.inf))
-        nxt = torch.multinomial(F.softmax(logits, -1), 1, generator=g) if temperature > 0 else logits.argmax(-1, keepdim=True)
+        scaled = logits / temperature if temperature > 0 else logits
+        scaled = torch.where(scaled.amax(-1, keepdim=True).isfinite(), scaled,
+                             torch.where(top.isnan() | (logits == top), 0.0, -torch.inf))
+        nxt = torch.multinomial(F.softmax(scaled, -1), 1, generator=g) if temperature > 0 else scaled.argmax(-1, keepdim=True)
         for row, (token, nothing, broken) in enumerate(torch.cat((nxt, top == -torch.inf, top.isnan()), 1).tolist()):
             if live[row] and broken:
                 raise RuntimeError(f"NaN among the logits of row {row}")
