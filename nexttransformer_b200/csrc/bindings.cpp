@@ -1255,10 +1255,14 @@ std::vector<int64_t> read_errors() {
 }
 
 // ------------------------------------------------------------------ serving
-void inference_only(std::initializer_list<const Tensor*> tensors) {
+void inference_only(std::initializer_list<const Tensor*> tensors, std::initializer_list<const OptT*> optional = {}) {
   if (!at::GradMode::is_enabled()) return;
-  for (auto* t : tensors)
-    TORCH_CHECK(!t->requires_grad(), "serving operators have no backward: call them under torch.no_grad()");
+  auto check = [](const Tensor& t) {
+    TORCH_CHECK(!t.requires_grad(), "serving operators have no backward: call them under torch.no_grad()");
+  };
+  for (auto* t : tensors) check(*t);
+  for (auto* t : optional)
+    if (t->has_value() && (*t)->defined()) check(**t);
 }
 // An uninitialised tensor from the caching allocator, without the dispatcher's detour.
 Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, const Tensor& like) {
@@ -1314,7 +1318,7 @@ PagedCacheArgs paged_cache(const Tensor& q, const Tensor& k, const Tensor& v, co
 Tensor paged_append(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& k_pages, const Tensor& v_pages,
                     const Tensor& table, const Tensor& start, const OptT& count, const Tensor& cos, const Tensor& sin,
                     c10::optional<double> qk_scale, const OptT& ve, const OptT& ve_gate) {
-  inference_only({&q, &k, &v});
+  inference_only({&q, &k, &v, &k_pages, &v_pages, &cos, &sin}, {&ve, &ve_gate});
   PagedAppendArgs a;
   a.cache = paged_cache(q, k_pages, v_pages, table);
   a.B = static_cast<int>(q.size(0));
@@ -1397,7 +1401,7 @@ Tensor stream_counters(const Tensor& like, int n) {
 
 Tensor paged_attention(const Tensor& q, const Tensor& k_pages, const Tensor& v_pages, const Tensor& table,
                        const Tensor& start, const OptT& count, int64_t window, c10::optional<double> scale) {
-  inference_only({&q});
+  inference_only({&q, &k_pages, &v_pages});
   PagedAttnArgs a;
   a.cache = paged_cache(q, k_pages, v_pages, table);
   a.B = static_cast<int>(q.size(0));
@@ -1432,7 +1436,7 @@ Tensor paged_attention(const Tensor& q, const Tensor& k_pages, const Tensor& v_p
 Tensor delta_step(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& state, const Tensor& beta, const OptT& g,
                   double scale, bool l2norm, const OptT& slots, const OptT& count) {
   check_cuda(q, "q");
-  inference_only({&q, &k, &v});
+  inference_only({&q, &k, &v, &state, &beta}, {&g});
   const auto type = q.scalar_type();
   TORCH_CHECK(type == at::kBFloat16 || type == at::kHalf || type == at::kFloat, "delta_recurrent takes bf16, fp16 or fp32");
   TORCH_CHECK(q.dim() == 4 && k.sizes() == q.sizes() && v.sizes() == q.sizes() && k.scalar_type() == type &&
@@ -1501,7 +1505,7 @@ Tensor adjust_logits(const Tensor& logits, const OptT& tokens, const OptT& lengt
                      const OptT& repetition, const OptT& presence, const OptT& frequency, const OptT& bias_ids,
                      const OptT& bias, const OptT& allowed) {
   check_cuda(logits, "logits");
-  inference_only({&logits});
+  inference_only({&logits}, {&repetition, &presence, &frequency, &bias});
   const auto type = logits.scalar_type();
   TORCH_CHECK(type == at::kBFloat16 || type == at::kHalf || type == at::kFloat, "logits must be bf16, fp16 or fp32");
   TORCH_CHECK(logits.dim() == 2 && (logits.stride(1) == 1 || logits.size(1) == 1), "logits must be [B, V] with contiguous rows");

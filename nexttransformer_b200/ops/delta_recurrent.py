@@ -28,7 +28,7 @@ def delta_recurrent(q, k, v, state, beta, g=None, *, scale=1.0, l2norm=False, sl
     """
     if q.is_cuda:
         return ext().delta_step(q, k, v, state, beta, g, scale, l2norm, slots, count)
-    _inference_only(q, k, v)
+    _inference_only(q, k, v, state, beta, g)
     return _plain(q, k, v, state, beta, g, scale, l2norm, slots, count)
 
 

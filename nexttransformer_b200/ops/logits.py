@@ -26,7 +26,7 @@ def adjust_logits(logits, *, tokens=None, length=None, prompt=None, repetition=N
     if logits.is_cuda:
         return ext().adjust_logits(logits, tokens, length, prompt, repetition, presence, frequency, bias_ids, bias,
                                    allowed)
-    _inference_only(logits)
+    _inference_only(logits, repetition, presence, frequency, bias)
     return _plain(logits, tokens, length, prompt, repetition, presence, frequency, bias_ids, bias, allowed)
 
 

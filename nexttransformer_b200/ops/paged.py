@@ -20,7 +20,7 @@ from nexttransformer_b200.ops._ext import ext
 
 
 def _inference_only(*tensors):
-    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         raise RuntimeError("serving operators have no backward: call them under torch.no_grad()")
 
 
@@ -35,7 +35,7 @@ def paged_append(q, k, v, k_pages, v_pages, table, start, count=None, *, cos, si
     """
     if q.is_cuda:
         return ext().paged_append(q, k, v, k_pages, v_pages, table, start, count, cos, sin, qk_scale, ve, ve_gate)
-    _inference_only(q, k, v)
+    _inference_only(q, k, v, k_pages, v_pages, cos, sin, ve, ve_gate)
     return _append_plain(q, k, v, k_pages, v_pages, table, start, count, cos, sin, qk_scale, ve, ve_gate)
 
 
@@ -49,7 +49,7 @@ def paged_attention(q, k_pages, v_pages, table, start, count=None, *, window=-1,
     """
     if q.is_cuda:
         return ext().paged_attention(q, k_pages, v_pages, table, start, count, window, scale)
-    _inference_only(q)
+    _inference_only(q, k_pages, v_pages)
     return _attention_plain(q, k_pages, v_pages, table, start, count, window, scale)
 
 

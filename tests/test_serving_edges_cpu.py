@@ -76,3 +76,44 @@ def test_logits_that_are_not_finite(temperature):
     for bias in ({7: -1e9, 5: 1e6}, {7: -math.inf, 5: math.inf}, {7: -1e38, 5: 3e38}):
         assert generate_batch(m, [[3, 1], [2]], 2, temperature=temperature, top_k=3, page=16, bias=bias) == [[5, 5]] * 2
     assert generate_batch(m, [[3, 1]], 2, temperature=temperature * 1e-40, page=16, bias={7: -math.inf, 5: 9.0}) == [[5, 5]]
+
+
+# what each operator is called with where every tensor that may carry a gradient is given
+def _serving_calls(device, dtype):
+    from nexttransformer_b200.ops.delta_recurrent import delta_recurrent
+    from nexttransformer_b200.ops.logits import adjust_logits
+    from nexttransformer_b200.ops.paged import paged_append, paged_attention
+
+    def ones(*shape, dtype=dtype):
+        return torch.ones(*shape, device=device, dtype=dtype)
+
+    def zeros(*shape):
+        return torch.zeros(*shape, device=device, dtype=torch.int32)
+    q, kv, pages, rope = ones(1, 1, 4, 64), ones(1, 1, 2, 64), ones(1, 2, 16, 64), ones(16, 32)
+    cache = dict(k_pages=pages, v_pages=pages.clone(), table=zeros(1, 1), start=zeros(1))
+    per_row = ones(1, dtype=torch.float32)
+    return {
+        "append": (paged_append, dict(q=q, k=kv, v=kv, cos=rope, sin=rope, ve=kv, ve_gate=kv[..., 0], **cache)),
+        "attention": (paged_attention, dict(q=q, **cache)),
+        "delta": (delta_recurrent, dict(q=kv, k=kv, v=kv, beta=kv[..., 0], g=ones(1, 1, 2, dtype=torch.float32),
+                                        state=ones(1, 2, 64, 64, dtype=torch.float32))),
+        "logits": (adjust_logits, dict(logits=ones(1, 32), tokens=zeros(1, 3), repetition=per_row, presence=per_row,
+                                       frequency=per_row, bias_ids=zeros(1, 1), bias=ones(1, 1, dtype=torch.float32))),
+    }
+
+
+@pytest.mark.parametrize("op,name", [
+    *(("append", n) for n in ("q", "k", "v", "k_pages", "v_pages", "cos", "sin", "ve", "ve_gate")),
+    *(("attention", n) for n in ("q", "k_pages", "v_pages")),
+    *(("delta", n) for n in ("q", "k", "v", "beta", "g", "state")),
+    *(("logits", n) for n in ("logits", "repetition", "presence", "frequency", "bias")),
+])
+def test_no_gradient_is_dropped(op, name):
+    """Whichever argument wants a gradient is refused while gradients are recorded, and welcome under no_grad."""
+    call, args = _serving_calls("cpu", torch.float32)[op]
+    call(**args)
+    args[name] = args[name].detach().clone().requires_grad_()
+    with pytest.raises(RuntimeError, match="backward"):
+        call(**args)
+    with torch.no_grad():
+        call(**args)

@@ -118,3 +118,22 @@ def test_attention_beside_a_key_that_takes_nearly_all(dtype, gap, keys, B):
     ref, held = p @ values, p @ values.abs()
     slack = 2.0 ** -14 * held + (keys * 2.0 ** -32 * 1000 * p[0] if dtype == torch.float16 else 0)
     assert ((got - ref).abs() <= 1.02 * U[dtype] * ref.abs() + slack).all(), ((got - ref).abs() / ref.abs()).max().item()
+
+
+
+@pytest.mark.parametrize("op,name", [
+    *(("append", n) for n in ("q", "k", "v", "k_pages", "v_pages", "cos", "sin", "ve", "ve_gate")),
+    *(("attention", n) for n in ("q", "k_pages", "v_pages")),
+    *(("delta", n) for n in ("q", "k", "v", "beta", "g", "state")),
+    *(("logits", n) for n in ("logits", "repetition", "presence", "frequency", "bias")),
+])
+def test_no_gradient_is_dropped(op, name):
+    """Whichever argument wants a gradient is refused while gradients are recorded, and welcome under no_grad."""
+    from tests.test_serving_edges_cpu import _serving_calls
+    call, args = _serving_calls(DEV, torch.bfloat16)[op]
+    call(**args)
+    args[name] = args[name].detach().clone().requires_grad_()
+    with pytest.raises(RuntimeError, match="backward"):
+        call(**args)
+    with torch.no_grad():
+        call(**args)
