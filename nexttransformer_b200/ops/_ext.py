@@ -6,6 +6,8 @@ plain-PyTorch restatement of each op (the oracle the kernels are tested against)
 """
 import importlib
 
+import torch
+
 _lib = None
 _err = None
 
@@ -33,17 +35,24 @@ def available():
 
 
 def check_errors():
-    """Raise if a bounded device-side wait in a kernel gave up (see csrc/common.cuh)."""
+    """Raise for what the kernels launched so far, on any stream of the current device, have recorded: bounded waits that
+    gave up (see csrc/common.cuh), and positions, page numbers and slots that the serving operators refused.  Reading
+    clears the record, so everything in it is told at once."""
+    if torch.cuda.is_initialized():
+        torch.cuda.synchronize()  # the words are read on the default stream, which waits for no other
     g, gw, a, aw, d, dw, sp, sw = ext().read_errors()
-    if g or a or d or sp:
-        raise RuntimeError(f"device pipeline wait expired: gemm code {g} at {gw:#x}, attention code {a} at {aw:#x}, "
-                           f"delta scan code {d} at {dw:#x}, sparse attention code {sp} at {sw:#x}")
     p, pw, ds, dsw = ext().read_serving_errors()
+    said = []
+    if g or a or d or sp:
+        said.append(f"device pipeline wait expired: gemm code {g} at {gw:#x}, attention code {a} at {aw:#x}, "
+                    f"delta scan code {d} at {dw:#x}, sparse attention code {sp} at {sw:#x}")
     if p:
         what = {1: "a position lies behind the row's page table", 2: "a page number lies outside the cache",
                 3: "a position lies behind the rotary table"}
-        raise RuntimeError(f"paged cache: {what.get(p, f'code {p}')} (row {pw})")
+        said.append(f"paged cache: {what.get(p, f'code {p}')} (row {pw})")
     if ds == 1:
-        raise RuntimeError(f"delta_recurrent: device pipeline wait expired ({dsw:#x})")
-    if ds:
-        raise RuntimeError(f"delta_recurrent: slot outside the states (row {dsw})")
+        said.append(f"delta_recurrent: device pipeline wait expired ({dsw:#x})")
+    elif ds:
+        said.append(f"delta_recurrent: slot outside the states (row {dsw})")
+    if said:
+        raise RuntimeError("; ".join(said))

@@ -117,3 +117,25 @@ def test_no_gradient_is_dropped(op, name):
         call(**args)
     with torch.no_grad():
         call(**args)
+
+
+def test_check_errors_tells_everything_at_once(monkeypatch):
+    """Reading clears the records, so an error that is read and not told would be lost."""
+    from nexttransformer_b200.ops import _ext
+
+    class Recorded:
+        gemm, serving = [7, 0x10, 0, 0, 0, 0, 0, 0], [2, 5, 2, 3]
+
+        def read_errors(self):
+            got, Recorded.gemm = Recorded.gemm, [0] * 8
+            return got
+
+        def read_serving_errors(self):
+            got, Recorded.serving = Recorded.serving, [0] * 4
+            return got
+    monkeypatch.setattr(_ext, "ext", Recorded)
+    with pytest.raises(RuntimeError) as said:
+        _ext.check_errors()
+    for words in ("gemm code 7 at 0x10", "page number lies outside the cache (row 5)", "slot outside the states (row 3)"):
+        assert words in str(said.value)
+    _ext.check_errors()

@@ -137,3 +137,22 @@ def test_no_gradient_is_dropped(op, name):
         call(**args)
     with torch.no_grad():
         call(**args)
+
+
+def test_check_errors_waits_for_other_streams():
+    """Streams of their own do not wait for the default stream, on which the error words are read, nor it for them."""
+    from nexttransformer_b200.ops._ext import check_errors
+    from nexttransformer_b200.ops.paged import paged_attention
+    k, v, table = make_cache([20], 2, 16, 64, torch.bfloat16, fill=0.0)
+    q = torch.ones(1, 1, 4, 64, device=DEV, dtype=torch.bfloat16)
+    start, bad = ints(3), torch.full_like(table, -1)
+    paged_attention(q, k, v, table, start)
+    check_errors()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        paged_attention(q, k, v, table, start)          # what a stream's first call sets up is not part of the wait
+        side.synchronize()
+        torch.cuda._sleep(200_000_000)                   # about a tenth of a second
+        paged_attention(q, k, v, bad, start)
+    with pytest.raises(RuntimeError, match="page number"):
+        check_errors()
