@@ -16,6 +16,7 @@ import torch.nn.functional as F
 
 from nexttransformer_b200.models.linear import LinearMixer
 from nexttransformer_b200.models.shell import Block, CausalSelfAttention, apply_rotary_emb, norm
+from nexttransformer_b200.ops._ext import check_errors
 from nexttransformer_b200.ops.logits import adjust_logits
 from nexttransformer_b200.ops.paged import paged_append, paged_attention
 
@@ -190,7 +191,8 @@ def decode_paged(model, idx, cache, counts=None):
     """Append ``idx [rows, t]`` to the cache and return logits ``[rows, V]`` of each row's last new token.
 
     ``counts`` (a list; t each by default) says how many of a row's t tokens are real; a row with 0 keeps its
-    state, and its logits mean nothing.
+    state, and its logits mean nothing.  It does not wait for the device; ``ops._ext.check_errors`` does, and raises
+    for what the kernels recorded.
     """
     B, t = idx.shape
     if B != cache.rows:
@@ -250,7 +252,8 @@ def generate_batch(model, prompts, max_tokens, temperature=1.0, top_k=None, seed
     dict from token to what is added to its logit, ``allowed`` a callable that gets the answers so far (a list
     of lists) and returns the grammar's bit masks for the next tokens, int32 ``[rows, ceil(V / 32)]`` (see
     ``ops.logits.adjust_logits``).  A row that it allows nothing ends there; rows that have ended may have any mask.  A
-    bias of inf settles the choice; a NaN among a row's logits raises.
+    bias of inf settles the choice; a NaN among a row's logits raises, as does at the end whatever the kernels recorded
+    (``ops._ext.check_errors``).
     """
     if not prompts or any(not p for p in prompts):
         raise ValueError("every prompt needs at least one token")
@@ -298,4 +301,6 @@ def generate_batch(model, prompts, max_tokens, temperature=1.0, top_k=None, seed
         history.scatter_(1, length.long()[:, None], nxt.int())
         length += torch.tensor(counts, dtype=torch.int32, device=dev)
         logits = decode_paged(model, nxt, cache, counts)
+    if history.is_cuda:
+        check_errors()
     return answers

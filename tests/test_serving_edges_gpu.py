@@ -156,3 +156,32 @@ def test_check_errors_waits_for_other_streams():
         paged_attention(q, k, v, bad, start)
     with pytest.raises(RuntimeError, match="page number"):
         check_errors()
+
+
+def small_model(**extra):
+    from dataclasses import replace
+    from nexttransformer_b200.models import build_model
+    from nexttransformer_b200.models.config import candidate_config
+    from tests.test_families_gpu import compute_dtype
+    c = replace(candidate_config("dense"), layers=2, width=256, heads=2, kv_heads=1, vocab_size=512, sequence_len=256,
+                mlp_width=1024, scale="custom", window_pattern="L", **extra)
+    with compute_dtype(torch.bfloat16):
+        return c, build_model(c, DEV, seed=0).eval()
+
+
+def test_generate_batch_raises_for_what_the_kernels_recorded(monkeypatch):
+    """A cache whose table loses a row's pages: the kernels leave them out, and the answers are not handed over."""
+    from nexttransformer_b200.inference import PagedCache, generate_batch
+    from nexttransformer_b200.ops._ext import check_errors
+    c, m = small_model()
+    check_errors()
+    assert [len(a) for a in generate_batch(m, [[1, 2, 3], [4]], 3)] == [3, 3]
+    reserve = PagedCache.reserve
+
+    def forgetful(cache, counts):
+        reserve(cache, counts)
+        cache.table[1] = -1
+    monkeypatch.setattr(PagedCache, "reserve", forgetful)
+    with pytest.raises(RuntimeError, match="page number lies outside the cache .row 1."):
+        generate_batch(m, [[1, 2, 3], [4]], 3)
+    check_errors()
