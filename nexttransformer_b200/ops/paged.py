@@ -111,7 +111,7 @@ def _attention_plain(q, k_pages, v_pages, table, start, count, window, scale):
     for b, (s, n) in enumerate(zip(starts, counts)):
         if not n:
             continue
-        key = torch.arange(s + n)
+        key = torch.arange(max(0, s - window) if window >= 0 else 0, s + n)   # what one of the tokens sees
         at = _pages_of(table, b, key, k_pages)
         K, V = k_pages[at].transpose(0, 1).float(), v_pages[at].transpose(0, 1).float()      # [Hk, keys, D]
         Q = q[b, :n].float().reshape(n, Hk, H // Hk, D).permute(1, 2, 0, 3)                  # [Hk, g, n, D]

@@ -139,3 +139,27 @@ def test_check_errors_tells_everything_at_once(monkeypatch):
     for words in ("gemm code 7 at 0x10", "page number lies outside the cache (row 5)", "slot outside the states (row 3)"):
         assert words in str(said.value)
     _ext.check_errors()
+
+
+@pytest.mark.parametrize("t,window", [(1, 0), (1, 20), (3, 20), (3, 100)])
+def test_plain_attention_reads_nothing_before_every_window(t, window):
+    """Pages before the oldest key that a token sees may have been given back, and their memory may hold anything."""
+    from nexttransformer_b200.ops.paged import paged_attention
+    torch.manual_seed(6)
+    n, H, Hk, D, page = 77, 4, 2, 8, 16
+    K, V = torch.randn(n, Hk, D), torch.randn(n, Hk, D)
+    q = torch.randn(1, t, H, D)
+    start = n - t
+    first = max(0, start - window)
+    kp, vp = (torch.full((5, Hk, page, D), math.nan) for _ in range(2))
+    for x, pages in ((K, kp), (V, vp)):
+        for p in range(first, n):
+            pages[p // page, :, p % page] = x[p]
+    table = torch.arange(5, dtype=torch.int32)[None]
+    table[0, :first // page] = -1
+    got = paged_attention(q, kp, vp, table, torch.tensor([start], dtype=torch.int32), window=window)
+    for i in range(t):
+        lo = max(0, start + i - window)
+        for h in range(H):
+            p = torch.softmax(K[lo:start + i + 1, h // 2].double() @ q[0, i, h].double() / math.sqrt(D), 0)
+            assert torch.allclose(got[0, i, h].double(), p @ V[lo:start + i + 1, h // 2].double(), atol=1e-5)
