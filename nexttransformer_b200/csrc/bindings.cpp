@@ -1448,8 +1448,8 @@ Tensor delta_step(const Tensor& q, const Tensor& k, const Tensor& v, const Tenso
   a.H = static_cast<int>(q.size(2));
   a.D = static_cast<int>(q.size(3));
   TORCH_CHECK(a.D == 64 || a.D == 128, "head dimension must be 64 or 128");
-  head_strides(q, "q", a.D / 32, a.qs);
-  head_strides(k, "k", a.D / 32, a.ks);
+  head_strides(q, "q", 1, a.qs);  // the kernels read single elements
+  head_strides(k, "k", 1, a.ks);
   head_strides(v, "v", 1, a.vs);
   a.q = q.data_ptr(); a.k = k.data_ptr(); a.v = v.data_ptr();
   TORCH_CHECK(beta.device() == q.device() && (beta.scalar_type() == type || beta.scalar_type() == at::kFloat) &&
@@ -1464,7 +1464,7 @@ Tensor delta_step(const Tensor& q, const Tensor& k, const Tensor& v, const Tenso
                 "g must be an fp32 log decay, [B, T, H] or [B, T, H, D]");
     a.g = g->data_ptr<float>();
     a.gate = g->dim() == 4 ? 2 : 1;
-    if (a.gate == 2) head_strides(*g, "g", a.D / 32, a.gs);
+    if (a.gate == 2) head_strides(*g, "g", 1, a.gs);
     else
       for (int i = 0; i < 3; ++i) a.gs[i] = g->stride(i);
   }

@@ -185,3 +185,20 @@ def test_generate_batch_raises_for_what_the_kernels_recorded(monkeypatch):
     with pytest.raises(RuntimeError, match="page number lies outside the cache .row 1."):
         generate_batch(m, [[1, 2, 3], [4]], 3)
     check_errors()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("T", [1, 11])
+def test_delta_recurrent_of_unaligned_views(dtype, T):
+    """Heads that start on any element, as slices of wider projections do: the same bits as from copies."""
+    from nexttransformer_b200.ops.delta_recurrent import delta_recurrent
+    torch.manual_seed(24)
+    B, H, D = 2, 3, 128
+    q, k, v = (torch.randn(B, T, H, D + 5, device=DEV).to(dtype)[..., i:D + i] for i in (1, 2, 3))
+    g = -torch.rand(B, T, H, D + 5, device=DEV)[..., 3:D + 3]
+    beta = torch.rand(B, T, H, device=DEV)
+    state = torch.randn(B, H, D, D, device=DEV) * .3
+    copy = state.clone()
+    got = delta_recurrent(q, k, v, state, beta, g, l2norm=True)
+    assert torch.equal(got, delta_recurrent(*(x.contiguous() for x in (q, k, v)), copy, beta, g.contiguous(), l2norm=True))
+    assert torch.equal(state, copy)
