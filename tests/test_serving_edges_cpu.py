@@ -163,3 +163,9 @@ def test_plain_attention_reads_nothing_before_every_window(t, window):
         for h in range(H):
             p = torch.softmax(K[lo:start + i + 1, h // 2].double() @ q[0, i, h].double() / math.sqrt(D), 0)
             assert torch.allclose(got[0, i, h].double(), p @ V[lo:start + i + 1, h // 2].double(), atol=1e-5)
+
+
+def test_paged_decode_of_a_mixture_of_experts():
+    """Ragged prompts and pausing rows: what stands behind a row's count changes no other token's experts."""
+    from tests.test_serving_cpu import test_paged_decode_matches_full_forward
+    test_paged_decode_matches_full_forward("moe")
