@@ -464,3 +464,25 @@ def test_attention_captured_without_counters_set_aside():
     import sys
     done = subprocess.run([sys.executable, "-c", CAPTURE], capture_output=True, text=True, timeout=240)
     assert done.returncode == 0 and done.stdout.split()[-1] == "fine", done.stderr[-2000:]
+
+
+@pytest.mark.parametrize("T", [1, 4, 300])
+def test_delta_recurrent_captured(T):
+    """A graph keeps the early launch of the walk through the blocks (T = 4), and segments (T = 300 of 128 heads)."""
+    from nexttransformer_b200.ops.delta_recurrent import delta_recurrent
+    torch.manual_seed(31)
+    B, H, D = 8, 16, 128
+    q, k, v = (torch.randn(B, T, H, D, device=DEV).bfloat16() for _ in range(3))
+    beta, g = torch.rand(B, T, H, device=DEV), -torch.rand(B, T, H, device=DEV)
+    first = torch.randn(B, H, D, D, device=DEV) * .3
+    alone = first.clone()
+    want = [delta_recurrent(q, k, v, alone, beta, g, l2norm=True) for _ in range(3)]
+    state = first.clone()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = [delta_recurrent(q, k, v, state, beta, g, l2norm=True) for _ in range(3)]
+    for _ in range(2):
+        state.copy_(first)
+        graph.replay()
+        assert all(torch.equal(a, b) for a, b in zip(held, want)) and torch.equal(state, alone)
