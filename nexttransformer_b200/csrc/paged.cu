@@ -19,7 +19,7 @@ constexpr float EPS = 1.1920929e-07f;  // FLT_EPSILON, as the shell's RMSNorm
 
 template <class T> struct Num;
 template <> struct Num<__nv_bfloat16> {
-  static constexpr float RAISE = 1.f;  // of probabilities, see the softmax
+  static constexpr float RAISE = 0.f;  // of probabilities, in powers of two, see the softmax
   static NT_DEVICE float2 unpack(uint32_t v) { return unpack_bf16x2(v); }
   static NT_DEVICE uint32_t pack(float lo, float hi) { return pack_bf16x2(lo, hi); }
   static NT_DEVICE float one(__nv_bfloat16 v) { return __bfloat162float(v); }
@@ -30,7 +30,7 @@ template <> struct Num<__nv_bfloat16> {
   }
 };
 template <> struct Num<__half> {
-  static constexpr float RAISE = 128.f;
+  static constexpr float RAISE = 7.f;
   static NT_DEVICE float2 unpack(uint32_t v) { return __half22float2(*reinterpret_cast<__half2*>(&v)); }
   static NT_DEVICE uint32_t pack(float lo, float hi) {
     __half2 h = __floats2half2_rn(lo, hi);
@@ -625,7 +625,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
     const int64_t kstep = ROWS * a.cache.slot_stride_k, vstep = ROWS * a.cache.slot_stride_v;
 
     bool turn = true;
-    unsigned gone = 0;  // bit of a stage: its tile's page is not in the cache (0.9 % over a set of calls)
+    unsigned gone = 0;  // bit of a stage: its tile's page is not in the cache (0.8 % over a set of calls)
     auto fetch = [&](int stage) {
       if (fetch_left > 0) {
         if (turn) turn_page<T>(a, f, kc, vc, lane);
@@ -750,9 +750,9 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
           for (int nq = 0; nq < NQ; ++nq) Num<T>::mma(kk & 1 ? s2[nq] : s[nq], kf, qf[nq][kk][0], qf[nq][kk][1]);
         }
         fetch(ahead);  // issued while the products finish
-        const int key0 = (c.it.first & ~(TILE - 1)) + (j0 + tile) * TILE;
-        const int key = lost ? INT32_MAX - TILE : key0 + qr;  // behind every query
-        const bool edge = lost || key0 < c.it.all_from || key0 + TILE > c.it.all_to;
+        // a tile without a page lies behind every query
+        const int key0 = lost ? INT32_MAX - 2 * TILE : (c.it.first & ~(TILE - 1)) + (j0 + tile) * TILE, key = key0 + qr;
+        const bool edge = key0 < c.it.all_from || key0 + TILE > c.it.all_to;
 #pragma unroll
         for (int nq = 0; nq < NQ; ++nq) {
 #pragma unroll
@@ -766,13 +766,14 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
           }
         }
         // The reference m follows the maximum only when a score passes it by more than 2^LAZY, so that most tiles
-        // need neither a reduction over the lanes nor a rescaling; probabilities stay below 2^LAZY, far from the
+        // need neither a reduction over the lanes nor a rescaling; probabilities stay below 2^(RAISE + LAZY), inside the
         // types' limits, and sums and pieces are relative to m all the same.
+        constexpr float RAISE = Num<T>::RAISE;
         bool passed = false;
 #pragma unroll
         for (int nq = 0; nq < NQ; ++nq)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) passed |= s[nq][e] > m[nq][e & 1] + LAZY;
+          for (int e = 0; e < 4; ++e) passed |= s[nq][e] > m[nq][e & 1] + (RAISE + LAZY);
         if (__any_sync(0xffffffffu, passed)) {
 #pragma unroll
           for (int nq = 0; nq < NQ; ++nq) {
@@ -785,7 +786,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
             float f[2];
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-              top[e] = fmaxf(m[nq][e], top[e]);
+              top[e] = fmaxf(m[nq][e], top[e] - RAISE);
               f[e] = piece_weight(m[nq][e], top[e]);
               m[nq][e] = top[e];
               l[nq][e] *= f[e];
@@ -800,16 +801,15 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
         // A probability is the sum of two numbers of the cache's type: 16 bits for bf16, 22 for fp16.  The error against 64
         // bits stays that of the output's rounding (1.66e-3 of the norm for 1 x 1001 bf16 keys, as with fp32 probabilities;
         // three bf16 numbers, which hold all 24 bits, change results by 1e-4 of the norm and cost 2.3 % over a set of
-        // calls).  fp16 ends at 2^-24, where the second number of a probability below 2^-14 is lost, so fp16 probabilities
-        // are raised to the type's top, up to 2^LAZY RAISE = 2^15, in products and totals alike: what is then lost is
-        // 2^-32 of the reference a key.
+        // calls).  fp16 ends at 2^-24, where the second number of a probability below 2^-14 is lost, so its reference m lies
+        // RAISE below the maximum that it follows: probabilities reach 2^(RAISE + LAZY) = 2^15, the type's top, in products and
+        // totals alike, and what is then lost is 2^-32 of the largest a key.
         uint32_t pf[NQ][2], pl[NQ][2];
 #pragma unroll
         for (int nq = 0; nq < NQ; ++nq) {
           const float r0 = m[nq][0] == -INFINITY ? 0.f : m[nq][0], r1 = m[nq][1] == -INFINITY ? 0.f : m[nq][1];
-          constexpr float RAISE = Num<T>::RAISE;
-          s[nq][0] = RAISE * exp2_fast(s[nq][0] - r0); s[nq][1] = RAISE * exp2_fast(s[nq][1] - r1);
-          s[nq][2] = RAISE * exp2_fast(s[nq][2] - r0); s[nq][3] = RAISE * exp2_fast(s[nq][3] - r1);
+          s[nq][0] = exp2_fast(s[nq][0] - r0); s[nq][1] = exp2_fast(s[nq][1] - r1);
+          s[nq][2] = exp2_fast(s[nq][2] - r0); s[nq][3] = exp2_fast(s[nq][3] - r1);
           l[nq][0] += s[nq][0] + s[nq][2];
           l[nq][1] += s[nq][1] + s[nq][3];
 #pragma unroll
