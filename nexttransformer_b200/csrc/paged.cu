@@ -50,7 +50,7 @@ template <> struct Num<__half> {
 // and which share the token's angles and place in the cache.  Blocks with small y turn queries and keys, the
 // others mix values.  One pass: every input element is read once and every output element written once, and what is
 // no token is not read.  8 prompts of up to 2048 tokens, 10 + 5 heads of 128: 27 us where its 117 MB (and 17 MB of
-// zeros) would take 21 at the copy rate; instruction issue (0.7 a cycle and scheduler) is the next limit.  One token: 2.4 us,
+// zeros) would take 21 at the copy rate; instruction issue (0.7 a cycle and scheduler) is the next limit.  One token: 2.5 us,
 // the chain from the row's length over its page to the store.
 template <class T>
 NT_DEVICE void load_halves(const T* p, int half, uint2& lo, uint2& hi) {
@@ -244,8 +244,11 @@ template <class T, int D>
 static int launch_append(const PagedAppendArgs& a, cudaStream_t s) {
   const int64_t tokens = static_cast<int64_t>(a.B) * a.t, per_block = 256 / (D / 8), blocks = (tokens + per_block - 1) / per_block;
   if (tokens > INT32_MAX - per_block) return -1;
-  // Five heads a thread keep enough bytes in flight and share a token's address work (8 prompts of 2048 tokens, back
-  // to back: 28.8 us, with four heads 30.8); with few tokens, one head a thread reaches more SMs (one token: 2.4 us).
+  // Five heads a thread keep enough bytes in flight and share a token's address work; with few tokens, one head a thread
+  // reaches more SMs.  Device times at 10 / 5, 16 / 1, 12 / 12, 8 / 2, 6 / 6 and 12 / 3 heads of 64 and 128: 8 prompts of 2048
+  // tokens take 11 to 49 us with five, 22 to 34 % more with one, up to 8 % more with four (6 / 6: 4 to 6 % less, its last
+  // group is half empty) and up to 19 % more with three; a prompt of 400 tokens takes 2.8 to 3.7 us with one and
+  // 14 to 32 % more with five.  At two thirds of the limit five take 0 to 14 % more than one, just above it 0 to 14 % less.
   return blocks * ((a.H + 2 * a.Hk + 4) / 5) >= 2 * a.sms ? launch_append<T, D, 5>(a, static_cast<unsigned>(blocks), s)
                                                           : launch_append<T, D, 1>(a, static_cast<unsigned>(blocks), s);
 }
@@ -267,18 +270,21 @@ static int launch_append(const PagedAppendArgs& a, cudaStream_t s) {
 // and what crosses CTAs by the CTA that arrives last, up to 16 pieces at a time.  Pieces are always joined in the
 // order of the line, so results do not depend on timing.
 //
-// Measured: 16 rows of 32768 keys, 10 / 5 heads of 128: 208 us, 6.45 TB/s.  64 rows of 512 to 8192 keys, 16 / 1 heads:
-// 28.7 us for 89 MB.  Clock stamps of an earlier build, same case: the first tile is there after 4 us (length, page and
-// key are a trip to memory each), the tiles are done after 16 us in half of the CTAs and 20 in all; joins and launch
-// take what remains.  One row of 1001 keys: 11.5 us, few (row, KV
-// head) pairs on few SMs.
+// Measured: 16 rows of 32768 keys, 10 / 5 heads of 128: 208.8 us, 6.43 TB/s.  64 rows of 512 to 8192 keys, 16 / 1 heads:
+// 28.5 us for 89 MB.  Clock stamps of a first warp a CTA, same case: the first tile is there after 4.1 us (length, page and
+// key are a trip to memory each), the tiles are done after 16 us in half of the CTAs and 23 in all, the CTAs' joins
+// after 18.7 and 25.9 us and those across CTAs after 27.  One row of 1001 keys: 11.5 us, few (row, KV head) pairs on few
+// SMs; first tile 2.9, tiles 7.9, join 9.7 us.
 // Tried and not kept: a second kernel for the join (10 us for one row, but two launches, 9 instead of 6 us on the
 // host), joins spread over rows instead of accumulator blocks, smaller reaches for the boundaries (16
 // tiles 1 %, 8 tiles 2 % slower over a set of calls), at least 4 tiles a warp (4 % slower over it; 1: 2 % faster).
-// More than 16 query rows a KV head are row tiles that each read the keys again: 248 rows of 5 tokens, 12 / 3 heads, 1709
-// keys take 237 us where one reading takes 102.  Warps of a CTA side by side on the row tiles of the same keys: 179 us,
-// but 5 % more for every call with one row tile and 12 % more over a set with several; row tiles outermost on the
-// line: 183 us and 1 % less over the set, but 1039 instead of 700 us for 8 prompts of 2048 tokens.  Neither was kept.
+// More than 16 query rows a KV head are row tiles that each read the keys again, by instructions made for 8 queries: 8
+// prompts of 2048 tokens, 10 / 5 heads of 128, take 715 us, where the training attention on tcgen05 takes 146 for the same
+// contiguous keys and the arithmetic 51; 4 prompts of 512 take 52 against 26.  248 rows of 5 tokens, 12 / 3 heads, 1709
+// keys take 236 us where one reading takes 102.  Ways to read them once, in an earlier build (237 us): warps of a CTA side
+// by side on the row tiles of the same keys: 179 us, but 5 % more for every call with one row tile and 12 % more over a set
+// with several; row tiles outermost on the line: 183 us and 1 % less over the set, but 1039 instead of 700 us for 8
+// prompts of 2048 tokens.  Neither was kept.
 constexpr float LAZY = 8.f;  // see the softmax
 constexpr int WARPS = 8, TILE = 16, MIN_TILES = 2, CTA_SNAP = 32, WARP_SNAP = 2, FAN = 16;
 // Rows of the batch whose tiles a CTA lines up in shared memory; a larger batch has CTAs enough and gives

@@ -2,8 +2,9 @@
 
 Keys and values lie in pages ``[P, Hk, page, D]`` (bf16 or fp16, heads of 64 or 128, ``page`` a multiple of
 16): token ``p`` of row ``b`` is in page ``table[b, p // page]`` at slot ``p % page``.  ``start [B]`` (int32)
-is how many tokens a row holds before the call, ``count [B]`` how many of the call's ``t`` tokens are real
-(all by default); what stands behind a row's count is neither written nor attended to and gives zeros.
+is how many tokens a row holds before the call (negative: the row is left out), ``count [B]`` how many of the call's
+``t`` tokens are real (all by default); what stands behind a row's count is neither written nor attended to and gives
+zeros.  Strides are free as long as rows, tokens and heads start on 16-byte boundaries.
 
 * ``paged_append``    rotates and QK-normalises new queries and keys, adds the gated value embedding, writes
   keys and values into the pages and returns the queries;
@@ -11,8 +12,9 @@ is how many tokens a row holds before the call, ``count [B]`` how many of the ca
   window.
 
 CUDA tensors run the kernels of ``csrc/paged.cu``; CPU tensors the plain form below, in any float type.  The
-kernels check positions and page numbers themselves: a bad one is skipped, and ``ops._ext.check_errors``
-raises for it.  Neither operator has a backward.
+kernels check positions and page numbers themselves: nothing is written to a page outside the cache, keys in one (or
+behind the table) take no part in the softmax, and ``ops._ext.check_errors`` raises for it; the plain form raises at once.
+Neither operator has a backward.
 """
 import torch
 
@@ -28,7 +30,7 @@ def paged_append(q, k, v, k_pages, v_pages, table, start, count=None, *, cos, si
                  ve_gate=None):
     """Write the new tokens' keys and values into the pages; return the rotated queries ``[B, t, H, D]``.
 
-    ``q [B, t, H, D]``, ``k`` / ``v [B, t, Hk, D]``: raw projections, any row / token / head strides.
+    ``q [B, t, H, D]``, ``k`` / ``v [B, t, Hk, D]``: raw projections, which may be slices of one.
     ``cos`` / ``sin [positions, D / 2]``: queries and keys are rotated by -theta at their position, then, with
     ``qk_scale``, RMS-normalised and scaled by it.  ``ve`` (like ``v``) and ``ve_gate [B, t, Hk]``: values
     become ``v + 3 sigmoid(ve_gate) ve``.
@@ -46,6 +48,7 @@ def paged_attention(q, k_pages, v_pages, table, start, count=None, *, window=-1,
     ``window >= 0`` at most ``window`` back.  ``scale`` defaults to ``D ** -0.5``.  Keys and values that one of a
     call's tokens sees have to be finite: one that only some of them see meets the others with probability zero,
     which does not remove a NaN.  What no token sees (behind the row's tokens, before every window) may hold anything.
+    A query with a NaN or an infinity gives NaN.
     """
     if q.is_cuda:
         return ext().paged_attention(q, k_pages, v_pages, table, start, count, window, scale)
