@@ -48,7 +48,8 @@ def paged_attention(q, k_pages, v_pages, table, start, count=None, *, window=-1,
     ``window >= 0`` at most ``window`` back.  ``scale`` defaults to ``D ** -0.5``.  Keys and values that one of a
     call's tokens sees have to be finite: one that only some of them see meets the others with probability zero,
     which does not remove a NaN.  What no token sees (behind the row's tokens, before every window) may hold anything.
-    A query with a NaN or an infinity gives NaN.
+    A query with a NaN gives NaN, and so does one with a score of inf; where every score is -inf the kernel gives zeros, as
+    for a token without keys (the plain form NaN).
     """
     if q.is_cuda:
         return ext().paged_attention(q, k_pages, v_pages, table, start, count, window, scale)

@@ -28,8 +28,8 @@ def pages_of(K, V, page, dtype):
 @pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
 @pytest.mark.parametrize("dtype,heads,kv_heads,t", [(torch.bfloat16, 10, 5, 1), (torch.float16, 16, 1, 1), (torch.bfloat16, 4, 2, 3)])
 def test_attention_of_a_query_that_is_not_finite(keys, bad, dtype, heads, kv_heads, t):
-    """Its scores are NaN or infinite whatever the keys are, so its output is NaN, in one piece or joined from many; the
-    other queries' outputs stay what they are (up to roundings: probabilities to 2^-16, the output to u)."""
+    """Its scores are NaN, or infinite of both signs with these keys, so its output is NaN, in one piece or joined from many;
+    the other queries' outputs stay what they are (up to roundings: probabilities to 2^-16, the output to u)."""
     from nexttransformer_b200.ops.paged import paged_attention
     torch.manual_seed(22)
     rows = [keys, keys, 17 + t]
