@@ -1289,10 +1289,13 @@ const int* row_ints(const OptT& t, const Tensor& like, int64_t rows, const char*
   TORCH_CHECK(t->size(0) == rows, name, " must have one entry for each row");
   return t->data_ptr<int>();
 }
-PagedCacheArgs paged_cache(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& table) {
+PagedCacheArgs paged_cache(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& table, const OptT& k_scale,
+                           const OptT& v_scale) {
   TORCH_CHECK(q.is_cuda() && k.device() == q.device() && v.device() == q.device(), "queries and pages must be on one CUDA device");
   TORCH_CHECK(q.scalar_type() == at::kBFloat16 || q.scalar_type() == at::kHalf, "paged attention takes bf16 or fp16");
-  TORCH_CHECK(k.scalar_type() == q.scalar_type() && v.scalar_type() == q.scalar_type(), "pages must have the queries' type");
+  const bool f8 = k.scalar_type() == at::kFloat8_e4m3fn && v.scalar_type() == at::kFloat8_e4m3fn;
+  TORCH_CHECK(f8 || (k.scalar_type() == q.scalar_type() && v.scalar_type() == q.scalar_type()),
+              "pages must have the queries' type, or both be float8_e4m3fn");
   TORCH_CHECK(q.dim() == 4 && k.dim() == 4 && v.dim() == 4 && k.sizes() == v.sizes(),
               "q [B, t, H, D] and pages [P, Hk, page, D] expected");
   TORCH_CHECK(k.size(3) == q.size(3) && (k.size(3) == 64 || k.size(3) == 128), "head dimension must be 64 or 128");
@@ -1302,8 +1305,8 @@ PagedCacheArgs paged_cache(const Tensor& q, const Tensor& k, const Tensor& v, co
   TORCH_CHECK(table.size(0) == q.size(0), "table must have one line for each row");
   PagedCacheArgs c;
   int64_t ks[3], vs[3];
-  head_strides(k, "k_pages", 8, ks);
-  head_strides(v, "v_pages", 8, vs);
+  head_strides(k, "k_pages", f8 ? 16 : 8, ks);
+  head_strides(v, "v_pages", f8 ? 16 : 8, vs);
   c.k = k.data_ptr();
   c.v = v.data_ptr();
   c.page_stride_k = ks[0]; c.head_stride_k = ks[1]; c.slot_stride_k = ks[2];
@@ -1312,15 +1315,29 @@ PagedCacheArgs paged_cache(const Tensor& q, const Tensor& k, const Tensor& v, co
   c.columns = static_cast<int>(table.size(1));
   c.pages = k.size(0);
   c.page = static_cast<int>(k.size(2));
+  const bool ks_there = k_scale.has_value() && k_scale->defined(), vs_there = v_scale.has_value() && v_scale->defined();
+  TORCH_CHECK(ks_there == f8 && vs_there == f8, "float8_e4m3fn pages go with k_scale and v_scale, other pages without");
+  if (f8) {
+    const auto check = [&](const Tensor& t, const char* name, int64_t (&strides)[3]) {
+      TORCH_CHECK(t.device() == q.device() && t.scalar_type() == at::kFloat && t.dim() == 3 && t.size(0) == k.size(0) &&
+                      t.size(1) == k.size(1) && t.size(2) == k.size(2) / 16,
+                  name, " must be fp32 [P, Hk, page / 16] on the pages' device");
+      for (int i = 0; i < 3; ++i) strides[i] = t.stride(i);
+    };
+    check(*k_scale, "k_scale", c.k_scale_strides);
+    check(*v_scale, "v_scale", c.v_scale_strides);
+    c.k_scale = k_scale->data_ptr<float>();
+    c.v_scale = v_scale->data_ptr<float>();
+  }
   return c;
 }
 
 Tensor paged_append(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& k_pages, const Tensor& v_pages,
                     const Tensor& table, const Tensor& start, const OptT& count, const Tensor& cos, const Tensor& sin,
-                    c10::optional<double> qk_scale, const OptT& ve, const OptT& ve_gate) {
-  inference_only({&q, &k, &v, &k_pages, &v_pages, &cos, &sin}, {&ve, &ve_gate});
+                    c10::optional<double> qk_scale, const OptT& ve, const OptT& ve_gate, const OptT& k_scale, const OptT& v_scale) {
+  inference_only({&q, &k, &v, &k_pages, &v_pages, &cos, &sin}, {&ve, &ve_gate, &k_scale, &v_scale});
   PagedAppendArgs a;
-  a.cache = paged_cache(q, k_pages, v_pages, table);
+  a.cache = paged_cache(q, k_pages, v_pages, table, k_scale, v_scale);
   a.B = static_cast<int>(q.size(0));
   a.t = static_cast<int>(q.size(1));
   a.H = static_cast<int>(q.size(2));
@@ -1400,10 +1417,11 @@ Tensor stream_counters(const Tensor& like, int n) {
 }
 
 Tensor paged_attention(const Tensor& q, const Tensor& k_pages, const Tensor& v_pages, const Tensor& table,
-                       const Tensor& start, const OptT& count, int64_t window, c10::optional<double> scale) {
-  inference_only({&q, &k_pages, &v_pages});
+                       const Tensor& start, const OptT& count, int64_t window, c10::optional<double> scale, const OptT& k_scale,
+                       const OptT& v_scale) {
+  inference_only({&q, &k_pages, &v_pages}, {&k_scale, &v_scale});
   PagedAttnArgs a;
-  a.cache = paged_cache(q, k_pages, v_pages, table);
+  a.cache = paged_cache(q, k_pages, v_pages, table, k_scale, v_scale);
   a.B = static_cast<int>(q.size(0));
   a.t = static_cast<int>(q.size(1));
   a.H = static_cast<int>(q.size(2));

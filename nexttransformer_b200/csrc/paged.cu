@@ -11,6 +11,7 @@
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <type_traits>
 
 namespace nt {
 namespace paged {
@@ -291,11 +292,17 @@ constexpr int WARPS = 8, TILE = 16, MIN_TILES = 2, CTA_SNAP = 32, WARP_SNAP = 2,
 // each (row, KV head) one.
 constexpr int MAX_ITEMS = 2048;
 
-template <int D, int NQ>
+struct E4M3 {  // a cache in 8 bits, with a scale for each 16 tokens and KV head
+  uint8_t code;
+};
+
+template <class C, int D, int NQ>
 struct Shape {
+  static constexpr bool F8 = sizeof(C) == 1;
   static constexpr int NR = NQ * 8;
-  static constexpr int HALF = TILE * D * 2, STAGE = 2 * HALF;  // bytes of K, of K and V
-  static constexpr int STAGES = D == 128 ? 3 : 6;              // 24 KB a warp, 192 KB an SM
+  static constexpr int LINE = D * static_cast<int>(sizeof(C));  // bytes of a key
+  static constexpr int HALF = TILE * LINE, STAGE = 2 * HALF + (F8 ? 16 : 0);  // bytes of K, of K and V (and their scales)
+  static constexpr int STAGES = 24 * 1024 / (2 * HALF);        // 24 KB a warp, 192 KB an SM
   static constexpr int RING = STAGES * STAGE;
   // Floats of a piece, in the order of the accumulators: NQ x D / 16 blocks of 32 lanes x 4 sums, then for each
   // NQ and lane % 4 the maxima and totals of that lane's two queries
@@ -358,6 +365,9 @@ NT_DEVICE void cp_async16(uint32_t dst, const void* src) {
 NT_DEVICE void cp_async16_or_zero(uint32_t dst, const void* src, bool valid) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
 }
+NT_DEVICE void cp_async4_or_zero(uint32_t dst, const void* src, bool valid) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(valid ? 4 : 0) : "memory");
+}
 NT_DEVICE void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 NT_DEVICE void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
@@ -369,6 +379,18 @@ NT_DEVICE void ldsm4t(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
+// What a line's chunk numbers are turned by, so that eight lines' equal chunks lie in different banks.
+template <int LINE>
+NT_DEVICE int turned(int row) { return LINE == 64 ? (row >> 1) & 3 : row & 7; }
+// Two e4m3 numbers (the lower or upper half of v) as two fp16 numbers, which hold them exactly.
+NT_DEVICE uint32_t widen(uint16_t v) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(v));
+  return r;
+}
+NT_DEVICE uint32_t widen_low(uint32_t v) { return widen(static_cast<uint16_t>(v)); }
+NT_DEVICE uint32_t widen_high(uint32_t v) { return widen(static_cast<uint16_t>(v >> 16)); }
+NT_DEVICE float power_of_two(int e) { return __int_as_float((e + 127) << 23); }  // -126 <= e <= 127
 NT_DEVICE uint32_t transpose8x8(uint32_t v) {
   uint32_t r;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
@@ -393,6 +415,7 @@ struct Cursor {
   int seen, pages;     // lane l holds the page of column seen + l
   bool there;          // the page lies in the cache
   const void *k, *v;   // this lane's first element of the tile
+  const float *ks, *vs;  // the tile's scales (8 bits)
 };
 
 NT_DEVICE void load_pages(const PagedAttnArgs& a, Cursor& c, int lane) {
@@ -417,8 +440,8 @@ NT_DEVICE void enter(const PagedAttnArgs& a, const Geometry& g, Cursor& c, int2 
   load_pages(a, c, lane);
 }
 // The tile's page is the next of the list (or the item's first).
-template <class T>
-NT_DEVICE void turn_page(const PagedAttnArgs& a, Cursor& c, const T* kc, const T* vc, int lane) {
+template <class C>
+NT_DEVICE void turn_page(const PagedAttnArgs& a, Cursor& c, const C* kc, const C* vc, int lane) {
   if (c.column - c.seen >= 32) load_pages(a, c, lane);
   const int page = __shfl_sync(0xffffffffu, c.pages, c.column - c.seen);
   c.there = page >= 0 && page < a.cache.pages;
@@ -426,13 +449,17 @@ NT_DEVICE void turn_page(const PagedAttnArgs& a, Cursor& c, const T* kc, const T
   const int64_t p = c.there ? page : 0;
   c.k = kc + p * a.cache.page_stride_k + c.hk * a.cache.head_stride_k + c.slot * a.cache.slot_stride_k;
   c.v = vc + p * a.cache.page_stride_v + c.hk * a.cache.head_stride_v + c.slot * a.cache.slot_stride_v;
+  if (sizeof(C) == 1) {
+    c.ks = a.cache.k_scale + p * a.cache.k_scale_strides[0] + c.hk * a.cache.k_scale_strides[1] + (c.slot / TILE) * a.cache.k_scale_strides[2];
+    c.vs = a.cache.v_scale + p * a.cache.v_scale_strides[0] + c.hk * a.cache.v_scale_strides[1] + (c.slot / TILE) * a.cache.v_scale_strides[2];
+  }
 }
 
 // Joins block blk of up to 16 pieces; piece(k) is the k-th, in the order of the line.  stat gets the maxima and
 // totals of the lane's two queries.
-template <int D, int NQ, bool L2, class Piece>
+template <class C, int D, int NQ, bool L2, class Piece>
 NT_DEVICE float4 join_block(int n, int blk, int lane, Piece piece, float4& stat) {
-  using S = Shape<D, NQ>;
+  using S = Shape<C, D, NQ>;
   auto load = [](const float* p) {
     return L2 ? __ldcg(reinterpret_cast<const float4*>(p)) : *reinterpret_cast<const float4*>(p);
   };
@@ -479,36 +506,41 @@ NT_DEVICE float4 join_block(int n, int blk, int lane, Piece piece, float4& stat)
   }
   return sum;
 }
-template <int D, int NQ>
+template <class C, int D, int NQ>
 NT_DEVICE void store_block(float* piece, int blk, int lane, const float4& sum, const float4& stat) {
-  using S = Shape<D, NQ>;
+  using S = Shape<C, D, NQ>;
   *reinterpret_cast<float4*>(piece + blk * 128 + lane * 4) = sum;
   if (blk % (D / 16) == 0 && lane < 4)
     *reinterpret_cast<float4*>(piece + S::BLOCKS * 128 + (blk / (D / 16)) * 16 + lane * 4) = stat;
 }
 // The output rows of a block of 8 queries: to the row of the query that a lane holds after the transpose.
-template <class T, int D>
+template <class T, class C, int D>
 NT_DEVICE T* output_row(const PagedAttnArgs& a, const Geometry& g, int b, int r, int hk, int lane) {
   r = min(r, g.R - 1);
   const int i = token_of(r, g.inverse);
   return static_cast<T*>(a.out) +
-         ((static_cast<int64_t>(b) * a.t + i) * a.H + hk * g.group + (r - i * g.group)) * D + (lane & 3) * 2;
+         ((static_cast<int64_t>(b) * a.t + i) * a.H + hk * g.group + (r - i * g.group)) * D + (lane & 3) * (sizeof(C) == 1 ? 4 : 2);
 }
-template <class T>
+template <class T, class C>
 NT_DEVICE void write_block(T* row, bool live, int d, const float4& sum, float w0, float w1) {
   const uint32_t u0 = transpose8x8(Num<T>::pack(weighted(w0, sum.x), weighted(w1, sum.y)));
   const uint32_t u1 = transpose8x8(Num<T>::pack(weighted(w0, sum.z), weighted(w1, sum.w)));
-  if (live) {
+  if (!live) return;
+  if (sizeof(C) == 1) {  // the rows of the products are the even channels of the block, then the odd ones
+    *reinterpret_cast<uint2*>(row + d * 16) = make_uint2(__byte_perm(u0, u1, 0x5410), __byte_perm(u0, u1, 0x7632));
+  } else {
     *reinterpret_cast<uint32_t*>(row + d * 16) = u0;
     *reinterpret_cast<uint32_t*>(row + d * 16 + 8) = u1;
   }
 }
 
-template <class T, int D, int NQ>
+template <class T, class C, int D, int NQ>
 __global__ void __launch_bounds__(WARPS * 32, 1)
     attn_kernel(const PagedAttnArgs a, const Geometry g, float* ws, unsigned* counters) {
-  using S = Shape<D, NQ>;
-  constexpr int NR = S::NR, CHUNKS = D / 8;
+  using S = Shape<C, D, NQ>;
+  using M = std::conditional_t<S::F8, __half, T>;  // what the products multiply
+  constexpr bool F8 = S::F8;
+  constexpr int NR = S::NR, LINE = S::LINE, CHUNKS = LINE / 16;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ int pre[MAX_ITEMS + 1];  // tiles of a KV head before each item
   __shared__ int2 spans[MAX_ITEMS];
@@ -625,24 +657,24 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
     constexpr int PERIOD = 8 / ROWS;        // copies after which the swizzle repeats
     uint32_t to[PERIOD];
 #pragma unroll
-    for (int e = 0; e < PERIOD; ++e) to[e] = (e * ROWS + lrow) * (D * 2) + ((lch ^ ((e * ROWS + lrow) & 7)) << 4);
-    const T* kc = static_cast<const T*>(a.cache.k) + lrow * a.cache.slot_stride_k + lch * 8;
-    const T* vc = static_cast<const T*>(a.cache.v) + lrow * a.cache.slot_stride_v + lch * 8;
+    for (int e = 0; e < PERIOD; ++e) to[e] = (e * ROWS + lrow) * LINE + ((lch ^ turned<LINE>(e * ROWS + lrow)) << 4);
+    const C* kc = static_cast<const C*>(a.cache.k) + lrow * a.cache.slot_stride_k + lch * (16 / sizeof(C));
+    const C* vc = static_cast<const C*>(a.cache.v) + lrow * a.cache.slot_stride_v + lch * (16 / sizeof(C));
     const int64_t kstep = ROWS * a.cache.slot_stride_k, vstep = ROWS * a.cache.slot_stride_v;
 
     bool turn = true;
     unsigned gone = 0;  // bit of a stage: its tile's page is not in the cache (0.8 % over a set of calls)
     auto fetch = [&](int stage) {
       if (fetch_left > 0) {
-        if (turn) turn_page<T>(a, f, kc, vc, lane);
+        if (turn) turn_page<C>(a, f, kc, vc, lane);
         gone = (gone & ~(1u << stage)) | (f.there ? 0u : 1u << stage);
         const int key = (f.it.first & ~(TILE - 1)) + f.j * TILE;
-        const T *ks = static_cast<const T*>(f.k), *vs = static_cast<const T*>(f.v);
+        const C *ks = static_cast<const C*>(f.k), *vs = static_cast<const C*>(f.v);
         const uint32_t dst = ring_u + stage * S::STAGE;
         if (f.there && key >= f.it.first && key + TILE <= f.it.end) {
 #pragma unroll
           for (int e = 0; e < TILE / ROWS; ++e) {
-            const uint32_t at = dst + to[e % PERIOD] + (e / PERIOD) * (8 * D * 2);
+            const uint32_t at = dst + to[e % PERIOD] + (e / PERIOD) * (8 * LINE);
             cp_async16(at, ks);
             cp_async16(at + S::HALF, vs);
             ks += kstep;
@@ -654,13 +686,14 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
           for (int e = 0; e < TILE / ROWS; ++e) {
             const int row = e * ROWS + lrow;
             const bool valid = f.there && key + row >= f.it.first && key + row < f.it.end;
-            const uint32_t at = dst + row * (D * 2) + ((lch ^ (row & 7)) << 4);
+            const uint32_t at = dst + row * LINE + ((lch ^ turned<LINE>(row)) << 4);
             cp_async16_or_zero(at, valid ? ks : kc, valid);
             cp_async16_or_zero(at + S::HALF, valid ? vs : vc, valid);
             ks += kstep;
             vs += vstep;
           }
         }
+        if (F8 && lane < 2) cp_async4_or_zero(dst + 2 * S::HALF + lane * 4, lane ? f.vs : f.ks, f.there);
         --fetch_left;
         turn = false;
         if (++f.j == f.it.tiles) {
@@ -676,8 +709,12 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
           ++f.column;
           turn = true;
         } else {
-          f.k = static_cast<const T*>(f.k) + TILE * a.cache.slot_stride_k;
-          f.v = static_cast<const T*>(f.v) + TILE * a.cache.slot_stride_v;
+          f.k = static_cast<const C*>(f.k) + TILE * a.cache.slot_stride_k;
+          f.v = static_cast<const C*>(f.v) + TILE * a.cache.slot_stride_v;
+          if (F8) {
+            f.ks += a.cache.k_scale_strides[2];
+            f.vs += a.cache.v_scale_strides[2];
+          }
         }
       }
       cp_commit();
@@ -692,28 +729,64 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const int krow = lane & 15, vrow = (lane & 7) + ((lane >> 4) << 3);
-      kat[e] = krow * (D * 2) + (((e * 2 + (lane >> 4)) ^ (krow & 7)) << 4);
-      vat[e] = S::HALF + vrow * (D * 2) + (((e * 2 + ((lane >> 3) & 1)) ^ (vrow & 7)) << 4);
+      // 8 bits: both products take a line's 16-byte chunks in pairs, keys 0 to 7 before keys 8 to 15
+      kat[e] = krow * LINE + (((e * 2 + (lane >> 4)) ^ turned<LINE>(krow)) << 4);
+      vat[e] = F8 ? S::HALF + kat[e] : S::HALF + vrow * LINE + (((e * 2 + ((lane >> 3) & 1)) ^ turned<LINE>(vrow)) << 4);
     }
 
     while (left > 0) {
       // ---- one piece: tiles [c.j, c.j + n) of (c.id, c.hk)
       const int n = min(left, c.it.tiles - c.j), j0 = c.j;
       uint32_t qf[NQ][D / 16][2];
+      float to_log[NQ][2];            // 8 bits: the factor of this lane's two queries' products
+      float v_top = 0.f, v_less = 0.f;  // 8 bits: the largest scale of values so far, to which sums are relative, and its inverse
       int last[NQ][2], oldest[NQ][2];  // newest and oldest key that this lane's two queries see
 #pragma unroll
       for (int nq = 0; nq < NQ; ++nq) {
         const int r = c.it.r0 + nq * 8 + qr, i = token_of(r, g.inverse);
         const bool live = r < g.R && i < c.it.n;
         const T* qp = static_cast<const T*>(a.q) + c.it.b * a.qs[0] + (live ? i : 0) * a.qs[1] +
-                      (c.hk * g.group + (live ? r - i * g.group : 0)) * a.qs[2] + qc * 2;
+                      (c.hk * g.group + (live ? r - i * g.group : 0)) * a.qs[2] + qc * (F8 ? 4 : 2);
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) {
-          qf[nq][kk][0] = live ? *reinterpret_cast<const uint32_t*>(qp + kk * 16) : 0u;
-          qf[nq][kk][1] = live ? *reinterpret_cast<const uint32_t*>(qp + kk * 16 + 8) : 0u;
+          if (F8) {  // a lane's four neighbouring channels, as it finds them in a key's line
+            const uint2 u = live ? *reinterpret_cast<const uint2*>(qp + kk * 16) : make_uint2(0u, 0u);
+            qf[nq][kk][0] = u.x;
+            qf[nq][kk][1] = u.y;
+          } else {
+            qf[nq][kk][0] = live ? *reinterpret_cast<const uint32_t*>(qp + kk * 16) : 0u;
+            qf[nq][kk][1] = live ? *reinterpret_cast<const uint32_t*>(qp + kk * 16 + 8) : 0u;
+          }
+        }
+        float own = scale2;  // what takes this lane's query row's products to powers of two
+        if (F8 && !std::is_same_v<T, M>) {
+          // bf16 queries become fp16: a power of two a row brings their largest to [2^12, 2^13), so that nothing is lost but
+          // what lies 2^-37 below it
+          float top = 0.f;
+#pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const float2 x = Num<T>::unpack(qf[nq][kk][e]);
+              top = fmaxf(top, fmaxf(fabsf(x.x), fabsf(x.y)));
+            }
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+          // an infinite element stays one, and the finite beside it become small
+          const int by = min(100, 139 - static_cast<int>(__float_as_uint(top) >> 23));
+          const float f = power_of_two(by);
+          own = scale2 * power_of_two(-by);
+#pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const float2 x = Num<T>::unpack(qf[nq][kk][e]);
+              qf[nq][kk][e] = Num<M>::pack(x.x * f, x.y * f);
+            }
         }
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
+          if (F8) to_log[nq][e] = __shfl_sync(0xffffffffu, own, (qc * 2 + e) * 4);
           const int rc = c.it.r0 + nq * 8 + qc * 2 + e, ic = token_of(rc, g.inverse);
           const bool lc = rc < g.R && ic < c.it.n;
           last[nq][e] = lc ? min(c.it.start + ic, c.it.end - 1) : -1;
@@ -748,12 +821,28 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
         for (int nq = 0; nq < NQ; ++nq)
 #pragma unroll
           for (int e = 0; e < 4; ++e) s[nq][e] = s2[nq][e] = 0.f;
+        float2 scales = make_float2(1.f, 1.f);
+        if constexpr (F8) {
+          scales = *reinterpret_cast<const float2*>(smem + (base - smem_u32(smem)) + 2 * S::HALF);
 #pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) {
-          uint32_t kf[4];
-          ldsm4(kf, base + kat[kk & 3] + (kk >> 2) * 128);
+          for (int kk = 0; kk < D / 16; kk += 2) {
+            uint32_t c4[4];  // chunk kk of keys 0 to 7, of keys 8 to 15, then chunk kk + 1
+            ldsm4(c4, base + kat[kk >> 1]);
 #pragma unroll
-          for (int nq = 0; nq < NQ; ++nq) Num<T>::mma(kk & 1 ? s2[nq] : s[nq], kf, qf[nq][kk][0], qf[nq][kk][1]);
+            for (int e = 0; e < 2; ++e) {
+              const uint32_t kf[4] = {widen_low(c4[2 * e]), widen_low(c4[2 * e + 1]), widen_high(c4[2 * e]), widen_high(c4[2 * e + 1])};
+#pragma unroll
+              for (int nq = 0; nq < NQ; ++nq) Num<M>::mma(e ? s2[nq] : s[nq], kf, qf[nq][kk + e][0], qf[nq][kk + e][1]);
+            }
+          }
+        } else {
+#pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk) {
+            uint32_t kf[4];
+            ldsm4(kf, base + kat[kk & 3] + (kk >> 2) * 128);
+#pragma unroll
+            for (int nq = 0; nq < NQ; ++nq) Num<M>::mma(kk & 1 ? s2[nq] : s[nq], kf, qf[nq][kk][0], qf[nq][kk][1]);
+          }
         }
         fetch(ahead);  // issued while the products finish
         // a tile without a page lies behind every query
@@ -762,7 +851,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
 #pragma unroll
         for (int nq = 0; nq < NQ; ++nq) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) s[nq][e] = (s[nq][e] + s2[nq][e]) * scale2;
+          for (int e = 0; e < 4; ++e) s[nq][e] = (s[nq][e] + s2[nq][e]) * (F8 ? to_log[nq][e & 1] * scales.x : scale2);
           if (edge) {
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
@@ -774,7 +863,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
         // The reference m follows the maximum only when a score passes it by more than 2^LAZY, so that most tiles
         // need neither a reduction over the lanes nor a rescaling; probabilities stay below 2^(RAISE + LAZY), inside the
         // types' limits, and sums and pieces are relative to m all the same.
-        constexpr float RAISE = Num<T>::RAISE;
+        constexpr float RAISE = Num<M>::RAISE;
         bool passed = false;
 #pragma unroll
         for (int nq = 0; nq < NQ; ++nq)
@@ -811,6 +900,18 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
         // RAISE below the maximum that it follows: probabilities reach 2^(RAISE + LAZY) = 2^15, the type's top, in products and
         // totals alike, and what is then lost is 2^-32 of the largest a key.
         uint32_t pf[NQ][2], pl[NQ][2];
+        if (F8 && scales.y > v_top) {  // (the same for the whole warp)
+          const float f = v_top / scales.y;
+          v_top = scales.y;
+          v_less = 1.f / scales.y;
+#pragma unroll
+          for (int nq = 0; nq < NQ; ++nq)
+#pragma unroll
+            for (int d = 0; d < D / 16; ++d)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) o[nq][d][e] *= f;
+        }
+        const float weight = scales.y * v_less;
 #pragma unroll
         for (int nq = 0; nq < NQ; ++nq) {
           const float r0 = m[nq][0] == -INFINITY ? 0.f : m[nq][0], r1 = m[nq][1] == -INFINITY ? 0.f : m[nq][1];
@@ -820,22 +921,50 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
           l[nq][1] += s[nq][1] + s[nq][3];
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            const uint32_t high = Num<T>::pack(s[nq][2 * e], s[nq][2 * e + 1]);
-            const float2 h = Num<T>::unpack(high);
+            if (F8) {
+              s[nq][2 * e] *= weight;
+              s[nq][2 * e + 1] *= weight;
+            }
+            const uint32_t high = Num<M>::pack(s[nq][2 * e], s[nq][2 * e + 1]);
+            const float2 h = Num<M>::unpack(high);
             pf[nq][e] = transpose8x8(high);
-            pl[nq][e] = transpose8x8(Num<T>::pack(s[nq][2 * e] - h.x, s[nq][2 * e + 1] - h.y));
+            pl[nq][e] = transpose8x8(Num<M>::pack(s[nq][2 * e] - h.x, s[nq][2 * e + 1] - h.y));
           }
         }
+        if constexpr (F8) {
+#pragma unroll
+          for (int d = 0; d < D / 16; d += 2) {
+            uint32_t c4[4];  // a lane has two channels of two keys; chunk d of keys 0 to 7, of keys 8 to 15, then chunk d + 1
+            ldsm4t(c4, base + vat[d >> 1]);
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const uint32_t x = __byte_perm(c4[2 * e], 0u, 0x3120), y = __byte_perm(c4[2 * e + 1], 0u, 0x3120);
+              const uint32_t vf[4] = {widen_low(x), widen_high(x), widen_low(y), widen_high(y)};
+#pragma unroll
+              for (int nq = 0; nq < NQ; ++nq) Num<M>::mma(o[nq][d + e], vf, pf[nq][0], pf[nq][1]);
+#pragma unroll
+              for (int nq = 0; nq < NQ; ++nq) Num<M>::mma(o[nq][d + e], vf, pl[nq][0], pl[nq][1]);
+            }
+          }
+        } else {
 #pragma unroll
         for (int d = 0; d < D / 16; ++d) {
           uint32_t vf[4];
           ldsm4t(vf, base + vat[d & 3] + (d >> 2) * 128);
 #pragma unroll
-          for (int nq = 0; nq < NQ; ++nq) Num<T>::mma(o[nq][d], vf, pf[nq][0], pf[nq][1]);
+          for (int nq = 0; nq < NQ; ++nq) Num<M>::mma(o[nq][d], vf, pf[nq][0], pf[nq][1]);
 #pragma unroll
-          for (int nq = 0; nq < NQ; ++nq) Num<T>::mma(o[nq][d], vf, pl[nq][0], pl[nq][1]);
+          for (int nq = 0; nq < NQ; ++nq) Num<M>::mma(o[nq][d], vf, pl[nq][0], pl[nq][1]);
+        }
         }
       }
+      if (F8)
+#pragma unroll
+        for (int nq = 0; nq < NQ; ++nq)
+#pragma unroll
+          for (int d = 0; d < D / 16; ++d)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[nq][d][e] *= v_top;
 
       // ---- the piece's end; rows that are no tokens have no keys
 #pragma unroll
@@ -855,11 +984,11 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
 #pragma unroll
         for (int nq = 0; nq < NQ; ++nq) {
           const int r = c.it.r0 + nq * 8 + qr;
-          T* row = output_row<T, D>(a, g, c.it.b, r, c.hk, lane);
+          T* row = output_row<T, C, D>(a, g, c.it.b, r, c.hk, lane);
           const float w0 = inverse_total(l[nq][0]), w1 = inverse_total(l[nq][1]);
 #pragma unroll
           for (int d = 0; d < D / 16; ++d)
-            write_block<T>(row, r < g.R, d, make_float4(o[nq][d][0], o[nq][d][1], o[nq][d][2], o[nq][d][3]), w0, w1);
+            write_block<T, C>(row, r < g.R, d, make_float4(o[nq][d][0], o[nq][d][1], o[nq][d][2], o[nq][d][3]), w0, w1);
         }
       } else {
         const bool final_piece = left == 0;
@@ -872,7 +1001,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
         for (int nq = 0; nq < NQ; ++nq)
 #pragma unroll
           for (int d = 0; d < D / 16; ++d)
-            store_block<D, NQ>(part, nq * (D / 16) + d, lane, make_float4(o[nq][d][0], o[nq][d][1], o[nq][d][2], o[nq][d][3]),
+            store_block<C, D, NQ>(part, nq * (D / 16) + d, lane, make_float4(o[nq][d][0], o[nq][d][1], o[nq][d][2], o[nq][d][3]),
                                make_float4(m[nq][0], l[nq][0], m[nq][1], l[nq][1]));
         if (lane == 0) {
           const int slot = 2 * warp + (final_piece ? 1 : 0);
@@ -920,17 +1049,17 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
       const int w0 = leader >> 1, n = (end >> 1) - w0 + 1;
       for (; blk < S::BLOCKS; blk += WARPS) {
         float4 stat;
-        const float4 sum = join_block<D, NQ, false>(n, blk, lane, [&](int k) {
+        const float4 sum = join_block<C, D, NQ, false>(n, blk, lane, [&](int k) {
           const int w = w0 + k;
           if (!((mask >> (2 * w)) & 3u)) return static_cast<const float*>(nullptr);  // it has no tiles
           return (mask >> (2 * w)) & 1u ? static_cast<const float*>(ws_warp + w * S::PART) : reinterpret_cast<const float*>(smem + w * S::RING);
         }, stat);
         if (!(begins && ends)) {
-          store_block<D, NQ>(ws + (static_cast<int64_t>(me) * 2 + (begins ? 1 : 0)) * S::PART, blk, lane, sum, stat);
+          store_block<C, D, NQ>(ws + (static_cast<int64_t>(me) * 2 + (begins ? 1 : 0)) * S::PART, blk, lane, sum, stat);
         } else {
           const int item = quotient(gid, Hk), b = g.row_tiles == 1 ? item : item / g.row_tiles;
           const int r = (item - b * g.row_tiles) * NR + (blk / (D / 16)) * 8 + (lane >> 2);
-          write_block<T>(output_row<T, D>(a, g, b, r, gid - item * Hk, lane), r < g.R, blk % (D / 16), sum, inverse_total(stat.y),
+          write_block<T, C>(output_row<T, C, D>(a, g, b, r, gid - item * Hk, lane), r < g.R, blk % (D / 16), sum, inverse_total(stat.y),
                          inverse_total(stat.w));
         }
       }
@@ -968,26 +1097,280 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
       const bool done = level == 1 || groups == 1;
       for (int blk = warp; blk < S::BLOCKS; blk += WARPS) {
         float4 stat;
-        const float4 sum = join_block<D, NQ, true>(n, blk, lane, [&](int k) { return static_cast<const float*>(at(first + k * step)); }, stat);
+        const float4 sum = join_block<C, D, NQ, true>(n, blk, lane, [&](int k) { return static_cast<const float*>(at(first + k * step)); }, stat);
         if (!done) {
           // into the leader's piece: its sums are read by this warp alone, its maxima and totals by all
           joined[blk * 32 + lane] = sum;
           if (blk % (D / 16) == 0 && lane < 4) joined_stat[(blk / (D / 16)) * 4 + lane] = stat;
         } else {
           const int r = r0 + (blk / (D / 16)) * 8 + (lane >> 2);
-          write_block<T>(output_row<T, D>(a, g, b, r, hk, lane), r < g.R, blk % (D / 16), sum, inverse_total(stat.y), inverse_total(stat.w));
+          write_block<T, C>(output_row<T, C, D>(a, g, b, r, hk, lane), r < g.R, blk % (D / 16), sum, inverse_total(stat.y), inverse_total(stat.w));
         }
       }
       if (done) break;
       __syncthreads();
       for (int blk = warp; blk < S::BLOCKS; blk += WARPS)
-        store_block<D, NQ>(at(lead), blk, lane, joined[blk * 32 + lane], joined_stat[(blk / (D / 16)) * 4 + (lane & 3)]);
+        store_block<C, D, NQ>(at(lead), blk, lane, joined[blk * 32 + lane], joined_stat[(blk / (D / 16)) * 4 + (lane & 3)]);
       first = c0;
       step = FAN;
       n = groups;
       counter = counters + c0 * COUNTERS + 2;
     }
   }
+}
+
+// ----------------------------------------------------------------------------- append, 8 bits
+// x is held as the e4m3 number next to x / S, S a power of two for each block of 16 tokens of a row (by position) and KV
+// head: the smallest whose 448-fold reaches the block's largest |x|.  A power of two moves no digits, so a block that
+// gets a larger token is written again with a larger S at the loss of nothing but what falls under the smallest step.
+// S never falls while a block is filled; a call that begins a block chooses it anew.  What is not finite becomes NaN
+// and does not count for S.
+//
+// A warp owns a block of one KV head, its keys or its values, so that nobody else writes its scale: all of its tokens are in
+// registers before the scale is known, and are read once.  The CTAs behind these turn the queries.
+NT_DEVICE uint32_t to_e4m3(const float (&x)[4]) {
+  uint16_t lo, hi;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(x[1]), "f"(x[0]));
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(x[3]), "f"(x[2]));
+  return static_cast<uint32_t>(lo) | (static_cast<uint32_t>(hi) << 16);
+}
+NT_DEVICE void from_e4m3(uint32_t v, float (&x)[4]) {
+  const float2 a = Num<__half>::unpack(widen_low(v)), b = Num<__half>::unpack(widen_high(v));
+  x[0] = a.x; x[1] = a.y; x[2] = b.x; x[3] = b.y;
+}
+// The smallest power of two, 2^-100 to 2^120, whose 448-fold (1.75 2^8) reaches top >= 0.
+NT_DEVICE float block_scale(float top) {
+  const uint32_t u = __float_as_uint(top);
+  const int e = static_cast<int>(u >> 23) - 127 - 8 + ((u & 0x7fffffu) > 0x600000u ? 1 : 0);
+  return power_of_two(max(-100, min(120, e)));
+}
+// Rotation by -theta and, if asked for, the RMS norm of a head that L lanes hold: 4 channels of each half a lane.
+template <int L, int D>
+NT_DEVICE void turn_head(const float2 (&x)[2], const float2 (&y)[2], const float2 (&c)[2], const float2 (&s)[2], bool norm, float scale,
+                         float2 (&u)[2], float2 (&w)[2]) {
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    u[j] = fma2(y[j], s[j], mul2(x[j], c[j]));
+    w[j] = fma2(x[j], make_float2(-s[j].x, -s[j].y), mul2(y[j], c[j]));
+  }
+  if (!norm) return;
+  const float2 pair = fma2(w[1], w[1], fma2(u[1], u[1], fma2(w[0], w[0], mul2(u[0], u[0]))));
+  float sum = pair.x + pair.y;
+#pragma unroll
+  for (int o = L / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  const float r = scale * rsqrtf(sum * (1.f / D) + EPS);
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    u[j] = mul2(u[j], make_float2(r, r));
+    w[j] = mul2(w[j], make_float2(r, r));
+  }
+}
+template <class T, int D, int PER>
+__global__ void __launch_bounds__(256) append8_kernel(const PagedAppendArgs a, const int blocks, const int64_t writing) {
+  constexpr int L = D / 8, HALF = D / 2, ABREAST = 32 / L, STEPS = TILE / ABREAST;
+  const int lane = threadIdx.x & 31, mine = lane % L;
+  const int64_t item = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+
+  if (blockIdx.x >= writing) {
+    // ---- queries: PER heads of a token a group of L lanes
+    const int64_t tokens = static_cast<int64_t>(a.B) * a.t, at = (item - writing * 8) * ABREAST + lane / L;
+    const int groups = (a.H + PER - 1) / PER;
+    const int64_t tok = at / groups;
+    const int h0 = static_cast<int>(at - tok * groups) * PER, heads = min(PER, a.H - h0);
+    const bool live = tok < tokens;
+    const int b = live ? static_cast<int>(tok / a.t) : 0, i = live ? static_cast<int>(tok - static_cast<int64_t>(b) * a.t) : 0;
+    const int start = a.start[b], n = a.count ? a.count[b] : a.t;
+    const bool real = live && i < n && start >= 0 && start < a.rope_rows - i;
+    uint2 lo[PER], hi[PER];
+    float2 c[2] = {}, s[2] = {};
+#pragma unroll
+    for (int e = 0; e < PER; ++e) lo[e] = hi[e] = make_uint2(0, 0);
+    if (real) {
+      const T* src = static_cast<const T*>(a.q) + b * a.qs[0] + i * a.qs[1] + h0 * a.qs[2] + mine * 4;
+#pragma unroll
+      for (int e = 0; e < PER; ++e)
+        if (e < heads) {
+          load_halves(src, HALF, lo[e], hi[e]);
+          src += a.qs[2];
+        }
+      const int64_t angle = static_cast<int64_t>(start + i) * HALF + mine * 4;
+      unpack4<T>(*reinterpret_cast<const uint2*>(static_cast<const T*>(a.cos) + angle), c);
+      unpack4<T>(*reinterpret_cast<const uint2*>(static_cast<const T*>(a.sin) + angle), s);
+    }
+    T* dst = static_cast<T*>(a.q_out) + (tok * a.H + h0) * D + mine * 4;
+#pragma unroll
+    for (int e = 0; e < PER; ++e) {
+      float2 x[2], y[2], u[2], w[2];
+      unpack4<T>(lo[e], x);
+      unpack4<T>(hi[e], y);
+      turn_head<L, D>(x, y, c, s, a.norm, a.scale, u, w);
+      if (live && e < heads) {  // tokens behind a row's count have zeros in, and give zeros
+        *reinterpret_cast<uint2*>(dst) = pack4<T>(u);
+        *reinterpret_cast<uint2*>(dst + HALF) = pack4<T>(w);
+      }
+      dst += D;
+    }
+    return;
+  }
+
+  // ---- a block of keys or values; the whole warp goes on or returns
+  const bool values = item & 1;
+  const int64_t rest = item >> 1, line = rest / a.Hk;
+  const int hk = static_cast<int>(rest - line * a.Hk), b = static_cast<int>(line / blocks), j = static_cast<int>(line - static_cast<int64_t>(b) * blocks);
+  if (b >= a.B) return;
+  const int start = a.start[b];
+  int n = a.count ? min(a.count[b], a.t) : a.t;
+  if (start < 0 || n <= 0) return;
+  if (start > a.rope_rows - n) {
+    if (lane == 0) record_error(3, b);
+    n = a.rope_rows - start;
+    if (n <= 0) return;
+  }
+  const int64_t first = (start & ~(TILE - 1)) + static_cast<int64_t>(j) * TILE;
+  if (first >= start + n) return;
+  const PagedCacheArgs& m = a.cache;
+  const int p0 = static_cast<int>(first), column = quotient(p0, m.page), slot0 = p0 - column * m.page;
+  if (column >= m.columns) {
+    if (lane == 0) record_error(1, b);
+    return;
+  }
+  const int page = m.table[static_cast<int64_t>(b) * m.columns + column];
+  if (page < 0 || page >= m.pages) {
+    if (lane == 0) record_error(2, b);
+    return;
+  }
+  const int64_t* scale_strides = values ? m.v_scale_strides : m.k_scale_strides;
+  float* scale_at = (values ? m.v_scale : m.k_scale) + page * scale_strides[0] + hk * scale_strides[1] + (slot0 / TILE) * scale_strides[2];
+  const bool continued = start > p0;
+  const float old = continued ? *scale_at : 0.f;
+
+  const int i0 = p0 + lane / L - start;  // the call's token in this lane's first slot
+  uint2 lo[STEPS], hi[STEPS];
+  const int64_t* strides = values ? a.vs : a.ks;
+  const T* src = static_cast<const T*>(values ? a.vin : a.kin) + b * strides[0] + hk * strides[2] + mine * 4;
+#pragma unroll
+  for (int e = 0; e < STEPS; ++e) {
+    const int i = i0 + e * ABREAST;
+    lo[e] = hi[e] = make_uint2(0, 0);
+    if (i >= 0 && i < n) load_halves(src + i * strides[1], HALF, lo[e], hi[e]);
+  }
+  float x[STEPS][8];
+  if (values) {
+    uint2 elo[STEPS], ehi[STEPS];
+    T gate[STEPS];
+    if (a.ve) {
+      const T* es = static_cast<const T*>(a.ve) + b * a.es[0] + hk * a.es[2] + mine * 4;
+      const T* gs = static_cast<const T*>(a.ve_gate) + b * a.gs[0] + hk * a.gs[2];
+#pragma unroll
+      for (int e = 0; e < STEPS; ++e) {
+        const int i = i0 + e * ABREAST;
+        if (i >= 0 && i < n) {
+          load_halves(es + i * a.es[1], HALF, elo[e], ehi[e]);
+          gate[e] = gs[i * a.gs[1]];
+        }
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < STEPS; ++e) {
+      const int i = i0 + e * ABREAST;
+      float2 u[2], w[2];
+      unpack4<T>(lo[e], u);
+      unpack4<T>(hi[e], w);
+      if (a.ve && i >= 0 && i < n) {
+        float2 y[2], z[2];
+        const float f = 3.f / (1.f + expf(-Num<T>::one(gate[e])));
+        unpack4<T>(elo[e], y);
+        unpack4<T>(ehi[e], z);
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          u[k] = fma2(make_float2(f, f), y[k], u[k]);
+          w[k] = fma2(make_float2(f, f), z[k], w[k]);
+        }
+      }
+      x[e][0] = u[0].x; x[e][1] = u[0].y; x[e][2] = u[1].x; x[e][3] = u[1].y;
+      x[e][4] = w[0].x; x[e][5] = w[0].y; x[e][6] = w[1].x; x[e][7] = w[1].y;
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < STEPS; ++e) {
+      const int i = i0 + e * ABREAST;
+      float2 c[2] = {}, s[2] = {}, y[2], z[2], u[2], w[2];
+      if (i >= 0 && i < n) {
+        const int64_t angle = static_cast<int64_t>(start + i) * HALF + mine * 4;
+        unpack4<T>(*reinterpret_cast<const uint2*>(static_cast<const T*>(a.cos) + angle), c);
+        unpack4<T>(*reinterpret_cast<const uint2*>(static_cast<const T*>(a.sin) + angle), s);
+      }
+      unpack4<T>(lo[e], y);
+      unpack4<T>(hi[e], z);
+      turn_head<L, D>(y, z, c, s, a.norm, a.scale, u, w);
+      x[e][0] = u[0].x; x[e][1] = u[0].y; x[e][2] = u[1].x; x[e][3] = u[1].y;
+      x[e][4] = w[0].x; x[e][5] = w[0].y; x[e][6] = w[1].x; x[e][7] = w[1].y;
+    }
+  }
+  // slots without a new token hold zeros here
+  float top = 0.f;
+  bool odd = false;
+#pragma unroll
+  for (int e = 0; e < STEPS; ++e)
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const bool fine = fabsf(x[e][k]) < INFINITY;
+      top = fmaxf(top, fine ? fabsf(x[e][k]) : 0.f);
+      odd |= !fine;
+    }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  if (odd)
+#pragma unroll
+    for (int e = 0; e < STEPS; ++e)
+#pragma unroll
+      for (int k = 0; k < 8; ++k) x[e][k] = fabsf(x[e][k]) < INFINITY ? x[e][k] : NAN;
+  const float scale = fmaxf(old, block_scale(top)), by = 1.f / scale;
+  const bool again = continued && scale != old;
+  uint8_t* codes = values ? static_cast<uint8_t*>(m.v) + page * m.page_stride_v + hk * m.head_stride_v + static_cast<int64_t>(slot0) * m.slot_stride_v
+                          : static_cast<uint8_t*>(m.k) + page * m.page_stride_k + hk * m.head_stride_k + static_cast<int64_t>(slot0) * m.slot_stride_k;
+  const int64_t step = values ? m.slot_stride_v : m.slot_stride_k;
+#pragma unroll
+  for (int e = 0; e < STEPS; ++e) {
+    const int i = i0 + e * ABREAST;
+    uint8_t* at = codes + (e * ABREAST + lane / L) * step + mine * 4;
+    float u[4], w[4];
+    float f = by;
+    if (i < 0) {
+      if (!again) continue;
+      from_e4m3(*reinterpret_cast<const uint32_t*>(at), u);
+      from_e4m3(*reinterpret_cast<const uint32_t*>(at + HALF), w);
+      f *= old;
+    } else {
+      if (i >= n) continue;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        u[k] = x[e][k];
+        w[k] = x[e][k + 4];
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      u[k] *= f;
+      w[k] *= f;
+    }
+    *reinterpret_cast<uint32_t*>(at) = to_e4m3(u);
+    *reinterpret_cast<uint32_t*>(at + HALF) = to_e4m3(w);
+  }
+  if (lane == 0) *scale_at = scale;
+}
+
+template <class T, int D, int PER>
+static int launch_append8(const PagedAppendArgs& a, cudaStream_t s) {
+  const int64_t tokens = static_cast<int64_t>(a.B) * a.t, blocks = (a.t + 2 * (TILE - 1)) / TILE, abreast = 32 / (D / 8);
+  const int64_t writing = (a.B * blocks * a.Hk * 2 + 7) / 8, turning = (tokens * ((a.H + PER - 1) / PER) + 8 * abreast - 1) / (8 * abreast);
+  if (writing + turning > INT32_MAX) return -1;
+  append8_kernel<T, D, PER><<<static_cast<unsigned>(writing + turning), 256, 0, s>>>(a, static_cast<int>(blocks), writing);
+  return 0;
+}
+template <class T, int D>
+static int launch_append8(const PagedAppendArgs& a, cudaStream_t s) {
+  return static_cast<int64_t>(a.B) * a.t * a.H >= 16384 ? launch_append8<T, D, 5>(a, s) : launch_append8<T, D, 1>(a, s);
 }
 
 struct Plan {
@@ -1016,14 +1399,20 @@ static Plan make_plan(const PagedAttnArgs& a) {
   return p;
 }
 
-template <class T, int D, int NQ>
+template <class T, class C, int D, int NQ>
 static int launch_attn(const PagedAttnArgs& a, const Plan& p, cudaStream_t s) {
-  using S = Shape<D, NQ>;
+  using S = Shape<C, D, NQ>;
   static std::atomic<uint64_t> done{0};
-  auto kern = attn_kernel<T, D, NQ>;
+  auto kern = attn_kernel<T, C, D, NQ>;
   if (smem_limit(done, kern, S::SMEM) != cudaSuccess) return -1;
   kern<<<p.grid, WARPS * 32, S::SMEM, s>>>(a, p.g, a.workspace, a.counters);
   return 0;
+}
+
+template <class T, class C>
+static int launch_attn(const PagedAttnArgs& a, const Plan& p, cudaStream_t s) {
+  if (a.D == 128) return p.NR == 8 ? launch_attn<T, C, 128, 1>(a, p, s) : launch_attn<T, C, 128, 2>(a, p, s);
+  return p.NR == 8 ? launch_attn<T, C, 64, 1>(a, p, s) : launch_attn<T, C, 64, 2>(a, p, s);
 }
 
 }  // namespace paged
@@ -1033,6 +1422,11 @@ using namespace nt::paged;
 
 int nt_paged_append(const PagedAppendArgs& a, cudaStream_t s) {
   if (a.B == 0 || a.t == 0) return 0;
+  if (a.cache.k_scale) {
+    if (a.D == 128) return a.fp16 ? launch_append8<__half, 128>(a, s) : launch_append8<__nv_bfloat16, 128>(a, s);
+    if (a.D == 64) return a.fp16 ? launch_append8<__half, 64>(a, s) : launch_append8<__nv_bfloat16, 64>(a, s);
+    return -1;
+  }
   if (a.D == 128) return a.fp16 ? launch_append<__half, 128>(a, s) : launch_append<__nv_bfloat16, 128>(a, s);
   if (a.D == 64) return a.fp16 ? launch_append<__half, 64>(a, s) : launch_append<__nv_bfloat16, 64>(a, s);
   return -1;
@@ -1052,13 +1446,8 @@ int nt_paged_attn(const PagedAttnArgs& a, cudaStream_t s) {
       static_cast<int64_t>(p.g.R) * p.g.group >= (int64_t{1} << 32) - 16 * p.g.group ||
       static_cast<int64_t>(a.t) * p.g.group > INT32_MAX / 2)
     return -1;
-  if (a.fp16) {
-    if (a.D == 128) return p.NR == 8 ? launch_attn<__half, 128, 1>(a, p, s) : launch_attn<__half, 128, 2>(a, p, s);
-    return p.NR == 8 ? launch_attn<__half, 64, 1>(a, p, s) : launch_attn<__half, 64, 2>(a, p, s);
-  }
-  if (a.D == 128)
-    return p.NR == 8 ? launch_attn<__nv_bfloat16, 128, 1>(a, p, s) : launch_attn<__nv_bfloat16, 128, 2>(a, p, s);
-  return p.NR == 8 ? launch_attn<__nv_bfloat16, 64, 1>(a, p, s) : launch_attn<__nv_bfloat16, 64, 2>(a, p, s);
+  if (a.fp16) return a.cache.k_scale ? launch_attn<__half, E4M3>(a, p, s) : launch_attn<__half, __half>(a, p, s);
+  return a.cache.k_scale ? launch_attn<__nv_bfloat16, E4M3>(a, p, s) : launch_attn<__nv_bfloat16, __nv_bfloat16>(a, p, s);
 }
 
 int nt_paged_read_error(unsigned* where) {

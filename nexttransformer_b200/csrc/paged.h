@@ -15,6 +15,10 @@ struct PagedCacheArgs {
   int columns = 0;
   int64_t pages = 0;
   int page = 0;                // tokens per page, a multiple of 16
+  // 8-bit (e4m3) pages: a scale for each block of 16 tokens and KV head, [P, Hk, page / 16] (null: 16-bit pages)
+  float* k_scale = nullptr;
+  float* v_scale = nullptr;
+  int64_t k_scale_strides[3] = {}, v_scale_strides[3] = {};
 };
 
 struct PagedAppendArgs {

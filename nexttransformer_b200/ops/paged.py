@@ -6,6 +6,12 @@ is how many tokens a row holds before the call (negative: the row is left out), 
 ``t`` tokens are real (all by default); what stands behind a row's count is neither written nor attended to and gives
 zeros.  Strides are free as long as rows, tokens and heads start on 16-byte boundaries.
 
+Pages may also be held in 8 bits (``float8_e4m3fn``) beside bf16 or fp16 queries.  Then ``k_scale`` and ``v_scale``, fp32
+``[P, Hk, page / 16]``, go with them: 16 tokens of a page and head share a scale, and a key is its code times its scale.
+``paged_append`` chooses it: the smallest power of two (2^-100 to 2^120) whose 448-fold reaches the largest number that the
+block's tokens had so far; a call that begins a block chooses anew, one that continues it may raise the scale, and then
+the block's earlier codes are written again.  What is not finite becomes NaN and does not count for the scale.
+
 * ``paged_append``    rotates and QK-normalises new queries and keys, adds the gated value embedding, writes
   keys and values into the pages and returns the queries;
 * ``paged_attention`` attends from the new tokens to the row's keys, causally and through an optional left
@@ -27,7 +33,7 @@ def _inference_only(*tensors):
 
 
 def paged_append(q, k, v, k_pages, v_pages, table, start, count=None, *, cos, sin, qk_scale=None, ve=None,
-                 ve_gate=None):
+                 ve_gate=None, k_scale=None, v_scale=None):
     """Write the new tokens' keys and values into the pages; return the rotated queries ``[B, t, H, D]``.
 
     ``q [B, t, H, D]``, ``k`` / ``v [B, t, Hk, D]``: raw projections, which may be slices of one.
@@ -36,12 +42,13 @@ def paged_append(q, k, v, k_pages, v_pages, table, start, count=None, *, cos, si
     become ``v + 3 sigmoid(ve_gate) ve``.
     """
     if q.is_cuda:
-        return ext().paged_append(q, k, v, k_pages, v_pages, table, start, count, cos, sin, qk_scale, ve, ve_gate)
-    _inference_only(q, k, v, k_pages, v_pages, cos, sin, ve, ve_gate)
-    return _append_plain(q, k, v, k_pages, v_pages, table, start, count, cos, sin, qk_scale, ve, ve_gate)
+        return ext().paged_append(q, k, v, k_pages, v_pages, table, start, count, cos, sin, qk_scale, ve, ve_gate, k_scale,
+                                  v_scale)
+    _inference_only(q, k, v, k_pages, v_pages, cos, sin, ve, ve_gate, k_scale, v_scale)
+    return _append_plain(q, k, v, k_pages, v_pages, table, start, count, cos, sin, qk_scale, ve, ve_gate, k_scale, v_scale)
 
 
-def paged_attention(q, k_pages, v_pages, table, start, count=None, *, window=-1, scale=None):
+def paged_attention(q, k_pages, v_pages, table, start, count=None, *, window=-1, scale=None, k_scale=None, v_scale=None):
     """Attention of the new tokens ``q [B, t, H, D]`` over the pages, which hold their keys already.
 
     Token ``i`` of a row stands at position ``start + i`` and sees the positions up to its own, with
@@ -52,19 +59,28 @@ def paged_attention(q, k_pages, v_pages, table, start, count=None, *, window=-1,
     for a token without keys (the plain form NaN).
     """
     if q.is_cuda:
-        return ext().paged_attention(q, k_pages, v_pages, table, start, count, window, scale)
-    _inference_only(q, k_pages, v_pages)
-    return _attention_plain(q, k_pages, v_pages, table, start, count, window, scale)
+        return ext().paged_attention(q, k_pages, v_pages, table, start, count, window, scale, k_scale, v_scale)
+    _inference_only(q, k_pages, v_pages, k_scale, v_scale)
+    return _attention_plain(q, k_pages, v_pages, table, start, count, window, scale, k_scale, v_scale)
 
 
 # ------------------------------------------------------------------------------ plain form (CPU)
-def _check_plain(q, k_pages, v_pages, table, start, count):
+BLOCK = 16  # tokens that share a scale
+
+
+def _check_plain(q, k_pages, v_pages, table, start, count, k_scale, v_scale):
     if q.dim() != 4 or k_pages.dim() != 4 or k_pages.shape != v_pages.shape or k_pages.shape[3] != q.shape[3]:
         raise RuntimeError("q [B, t, H, D] and pages [P, Hk, page, D] expected")
     if q.shape[2] % k_pages.shape[1]:
         raise RuntimeError("KV heads must divide query heads")
     if k_pages.shape[2] % 16:
         raise RuntimeError("tokens per page must be a multiple of 16")
+    f8 = k_pages.dtype == torch.float8_e4m3fn
+    if (v_pages.dtype == torch.float8_e4m3fn) != f8 or f8 != (k_scale is not None) or f8 != (v_scale is not None):
+        raise RuntimeError("float8_e4m3fn pages go with k_scale and v_scale, other pages without")
+    for s in (k_scale, v_scale) if f8 else ():
+        if s.dtype != torch.float32 or s.shape != (*k_pages.shape[:2], k_pages.shape[2] // BLOCK):
+            raise RuntimeError("k_scale and v_scale must be fp32 [P, Hk, page / 16]")
     B, t = q.shape[:2]
     if table.shape[0] != B or start.shape != (B,) or (count is not None and count.shape != (B,)):
         raise RuntimeError("table, start and count must have one entry for each row")
@@ -83,9 +99,35 @@ def _pages_of(table, b, positions, k_pages):
     return at, slice(None), positions % page
 
 
-def _append_plain(q, k, v, k_pages, v_pages, table, start, count, cos, sin, qk_scale, ve, ve_gate):
+def _append_coded(x, pages, scale, at, first):
+    """Tokens ``x [n, Hk, D]`` of a row, the first at slot ``first`` of a block, into 8-bit pages at ``at``."""
+    page, head, slot = at
+    for low in range(-first, len(x), BLOCK):                     # a block's first slot, as a token of the call
+        new = slice(max(low, 0), low + BLOCK)
+        p, begin = page[new][0], int(slot[new][0]) // BLOCK * BLOCK
+        y = x[new].float().transpose(0, 1)                       # [Hk, tokens, D]
+        y = torch.where(y.isfinite(), y, torch.nan)
+        fraction, exponent = torch.frexp(y.abs().nan_to_num(0.0).amax((1, 2)))
+        need = torch.where(fraction > 0, exponent - 9 + (fraction > 0.875).int(), -100).clamp(-100, 120)  # 448 = 0.875 2^9
+        need = torch.ldexp(torch.ones(len(need)), need)
+        if low < 0:
+            old = scale[p, :, begin // BLOCK].clone()
+            need = torch.maximum(need, old)
+            codes = pages[p, :, begin:begin - low].float() * (old / need)[:, None, None]
+            pages[p, :, begin:begin - low] = codes.to(pages.dtype)
+        scale[p, :, begin // BLOCK] = need
+        pages[p, :, int(slot[new][0]):int(slot[new][0]) + y.shape[1]] = (y / need[:, None, None]).to(pages.dtype)
+
+
+def _decoded(pages, scale, at):
+    """Keys or values at ``at`` of 8-bit pages, as the numbers that they stand for."""
+    page, head, slot = at
+    return pages.view(torch.uint8)[at].view(pages.dtype).float() * scale[page, :, slot // BLOCK][..., None]
+
+
+def _append_plain(q, k, v, k_pages, v_pages, table, start, count, cos, sin, qk_scale, ve, ve_gate, k_scale, v_scale):
     from nexttransformer_b200.models.shell import apply_rotary_emb, norm
-    starts, counts = _check_plain(q, k_pages, v_pages, table, start, count)
+    starts, counts = _check_plain(q, k_pages, v_pages, table, start, count, k_scale, v_scale)
     if (ve is None) != (ve_gate is None):
         raise RuntimeError("ve and ve_gate go together")
     if ve is not None:
@@ -101,13 +143,18 @@ def _append_plain(q, k, v, k_pages, v_pages, table, start, count, cos, sin, qk_s
             qb, kb = norm(qb) * qk_scale, norm(kb) * qk_scale
         at = _pages_of(table, b, positions, k_pages)
         out[b, :n] = qb
+        if k_scale is not None:
+            if n:
+                _append_coded(kb, k_pages, k_scale, at, s % BLOCK)
+                _append_coded(v[b, :n], v_pages, v_scale, at, s % BLOCK)
+            continue
         k_pages[at] = kb.to(k_pages.dtype)
         v_pages[at] = v[b, :n].to(v_pages.dtype)
     return out
 
 
-def _attention_plain(q, k_pages, v_pages, table, start, count, window, scale):
-    starts, counts = _check_plain(q, k_pages, v_pages, table, start, count)
+def _attention_plain(q, k_pages, v_pages, table, start, count, window, scale, k_scale, v_scale):
+    starts, counts = _check_plain(q, k_pages, v_pages, table, start, count, k_scale, v_scale)
     B, t, H, D = q.shape
     Hk = k_pages.shape[1]
     scale = D ** -0.5 if scale is None else scale
@@ -117,7 +164,10 @@ def _attention_plain(q, k_pages, v_pages, table, start, count, window, scale):
             continue
         key = torch.arange(max(0, s - window) if window >= 0 else 0, s + n)   # what one of the tokens sees
         at = _pages_of(table, b, key, k_pages)
-        K, V = k_pages[at].transpose(0, 1).float(), v_pages[at].transpose(0, 1).float()      # [Hk, keys, D]
+        if k_scale is not None:
+            K, V = _decoded(k_pages, k_scale, at).transpose(0, 1), _decoded(v_pages, v_scale, at).transpose(0, 1)
+        else:
+            K, V = k_pages[at].transpose(0, 1).float(), v_pages[at].transpose(0, 1).float()  # [Hk, keys, D]
         Q = q[b, :n].float().reshape(n, Hk, H // Hk, D).permute(1, 2, 0, 3)                  # [Hk, g, n, D]
         position = torch.arange(s, s + n)[:, None]
         seen = key <= position
