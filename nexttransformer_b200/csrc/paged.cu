@@ -1126,8 +1126,8 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
 // S never falls while a block is filled; a call that begins a block chooses it anew.  What is not finite becomes NaN
 // and does not count for S.
 //
-// A warp owns a block of one KV head, its keys or its values, so that nobody else writes its scale: all of its tokens are in
-// registers before the scale is known, and are read once.  The CTAs behind these turn the queries.
+// A block of one KV head, its keys or its values, is written by one group of lanes or warps, so that nobody else writes
+// its scale: all of its new tokens are in registers before the scale is known, and are read once.
 NT_DEVICE uint32_t to_e4m3(const float (&x)[4]) {
   uint16_t lo, hi;
   asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(x[1]), "f"(x[0]));
@@ -1144,233 +1144,330 @@ NT_DEVICE float block_scale(float top) {
   const int e = static_cast<int>(u >> 23) - 127 - 8 + ((u & 0x7fffffu) > 0x600000u ? 1 : 0);
   return power_of_two(max(-100, min(120, e)));
 }
-// Rotation by -theta and, if asked for, the RMS norm of a head that L lanes hold: 4 channels of each half a lane.
-template <int L, int D>
-NT_DEVICE void turn_head(const float2 (&x)[2], const float2 (&y)[2], const float2 (&c)[2], const float2 (&s)[2], bool norm, float scale,
-                         float2 (&u)[2], float2 (&w)[2]) {
-#pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    u[j] = fma2(y[j], s[j], mul2(x[j], c[j]));
-    w[j] = fma2(x[j], make_float2(-s[j].x, -s[j].y), mul2(y[j], c[j]));
+// Where a block of a row and KV head lies: its codes and its scale.
+struct BlockAt {
+  uint8_t* codes;   // null: nowhere
+  int64_t step;     // from token to token
+  float* scale;
+};
+NT_DEVICE BlockAt find_block(const PagedAppendArgs& a, int b, int position, int hk, bool values, bool tells) {
+  const PagedCacheArgs& m = a.cache;
+  const int column = quotient(position, m.page), slot = position - column * m.page;
+  int fault = 1;
+  if (column < m.columns) {
+    const int page = m.table[static_cast<int64_t>(b) * m.columns + column];
+    fault = 2;
+    if (page >= 0 && page < m.pages) {
+      if (values)
+        return {static_cast<uint8_t*>(m.v) + page * m.page_stride_v + hk * m.head_stride_v + slot * m.slot_stride_v, m.slot_stride_v,
+                m.v_scale + page * m.v_scale_strides[0] + hk * m.v_scale_strides[1] + (slot / TILE) * m.v_scale_strides[2]};
+      return {static_cast<uint8_t*>(m.k) + page * m.page_stride_k + hk * m.head_stride_k + slot * m.slot_stride_k, m.slot_stride_k,
+              m.k_scale + page * m.k_scale_strides[0] + hk * m.k_scale_strides[1] + (slot / TILE) * m.k_scale_strides[2]};
+    }
   }
-  if (!norm) return;
-  const float2 pair = fma2(w[1], w[1], fma2(u[1], u[1], fma2(w[0], w[0], mul2(u[0], u[0]))));
+  if (tells) record_error(fault, b);
+  return {nullptr, 0, nullptr};
+}
+// D / 16 lanes hold a head of a token, lane j channels 8 j to 8 j + 7 of each half, so that it has both members of its
+// rotated pairs.
+enum Kind { QUERY, KEY, VALUE };
+struct Raw {
+  uint4 lo, hi;    // the head's halves
+  uint4 lo2, hi2;  // cosines and sines; of a value the halves of its embedding
+};
+template <class T>
+NT_DEVICE void load16(const T* p, int half, uint4& lo, uint4& hi) {
+  lo = __ldcs(reinterpret_cast<const uint4*>(p));
+  hi = __ldcs(reinterpret_cast<const uint4*>(p + half));
+}
+template <class T>
+NT_DEVICE void load_angles(const PagedAppendArgs& a, int position, int half, int mine, Raw& r) {
+  const int64_t at = static_cast<int64_t>(position) * half + mine * 8;
+  r.lo2 = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.cos) + at);
+  r.hi2 = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.sin) + at);
+}
+template <class T>
+NT_DEVICE void unpack8(const uint4& u, float2 (&x)[4]) {
+  x[0] = Num<T>::unpack(u.x);
+  x[1] = Num<T>::unpack(u.y);
+  x[2] = Num<T>::unpack(u.z);
+  x[3] = Num<T>::unpack(u.w);
+}
+// Both halves of what becomes of a head; zeros stay zeros.  Whole warps call it for queries and keys.
+template <class T, int D>
+NT_DEVICE void turn_raw(const PagedAppendArgs& a, const Raw& r, float2 (&x)[8]) {
+  float2 y[4], z[4], c[4], s[4];
+  unpack8<T>(r.lo, y);
+  unpack8<T>(r.hi, z);
+  unpack8<T>(r.lo2, c);
+  unpack8<T>(r.hi2, s);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    x[k] = fma2(z[k], s[k], mul2(y[k], c[k]));
+    x[k + 4] = fma2(y[k], make_float2(-s[k].x, -s[k].y), mul2(z[k], c[k]));
+  }
+  if (!a.norm) return;
+  float2 pair = mul2(x[0], x[0]);
+#pragma unroll
+  for (int k = 1; k < 8; ++k) pair = fma2(x[k], x[k], pair);
   float sum = pair.x + pair.y;
 #pragma unroll
-  for (int o = L / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  const float r = scale * rsqrtf(sum * (1.f / D) + EPS);
+  for (int o = D / 32; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  const float f = a.scale * rsqrtf(sum * (1.f / D) + EPS);
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    u[j] = mul2(u[j], make_float2(r, r));
-    w[j] = mul2(w[j], make_float2(r, r));
+  for (int k = 0; k < 8; ++k) x[k] = mul2(x[k], make_float2(f, f));
+}
+// gate: 3 sigmoid of it is the embedding's share
+NT_DEVICE float share_of(float gate) { return __fdividef(3.f, 1.f + expf(-gate)); }
+template <class T>
+NT_DEVICE void mix_raw(const Raw& r, bool embedded, float share, float2 (&x)[8]) {
+  float2 u[4], w[4], y[4], z[4];
+  unpack8<T>(r.lo, u);
+  unpack8<T>(r.hi, w);
+  unpack8<T>(r.lo2, y);
+  unpack8<T>(r.hi2, z);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    x[k] = embedded ? fma2(make_float2(share, share), y[k], u[k]) : u[k];
+    x[k + 4] = embedded ? fma2(make_float2(share, share), z[k], w[k]) : w[k];
   }
 }
-template <class T, int D, int PER>
-__global__ void __launch_bounds__(256) append8_kernel(const PagedAppendArgs a, const int blocks, const int64_t writing) {
-  constexpr int L = D / 8, HALF = D / 2, ABREAST = 32 / L, STEPS = TILE / ABREAST;
-  const int lane = threadIdx.x & 31, mine = lane % L;
-  const int64_t item = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+// The largest finite |x|; the others become NaN.
+template <int N>
+NT_DEVICE float finite_top(float2 (&x)[N][8]) {
+  constexpr uint32_t INF = 0x7f800000u;
+  uint32_t top = 0;  // magnitudes are ordered as their bits are
+  auto bits = [](float v) { return __float_as_uint(v) & 0x7fffffffu; };
+#pragma unroll
+  for (int e = 0; e < N; ++e)
+#pragma unroll
+    for (int k = 0; k < 8; ++k) top = max(top, max(bits(x[e][k].x), bits(x[e][k].y)));
+  if (top >= INF) {
+    top = 0;
+    auto mend = [&](float& v) {
+      if (bits(v) < INF) top = max(top, bits(v));
+      else v = NAN;
+    };
+#pragma unroll
+    for (int e = 0; e < N; ++e)
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        mend(x[e][k].x);
+        mend(x[e][k].y);
+      }
+  }
+  return __uint_as_float(top);
+}
+NT_DEVICE void write_codes(uint8_t* at, int half, const float2 (&x)[8], float by) {
+  uint32_t u[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const float2 y = mul2(x[2 * k], make_float2(by, by)), z = mul2(x[2 * k + 1], make_float2(by, by));
+    const float four[4] = {y.x, y.y, z.x, z.y};
+    u[k] = to_e4m3(four);
+  }
+  *reinterpret_cast<uint2*>(at) = make_uint2(u[0], u[1]);
+  *reinterpret_cast<uint2*>(at + half) = make_uint2(u[2], u[3]);
+}
+NT_DEVICE void rescale_codes(uint8_t* at, int half, float by) {
+  const uint2 lo = *reinterpret_cast<const uint2*>(at), hi = *reinterpret_cast<const uint2*>(at + half);
+  const uint32_t u[4] = {lo.x, lo.y, hi.x, hi.y};
+  float2 x[8];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    x[2 * k] = Num<__half>::unpack(widen_low(u[k]));
+    x[2 * k + 1] = Num<__half>::unpack(widen_high(u[k]));
+  }
+  write_codes(at, half, x, by);
+}
+template <class T, int D>
+NT_DEVICE void store_query(const PagedAppendArgs& a, int tok, int head, int mine, const float2 (&x)[8]) {
+  T* dst = static_cast<T*>(a.q_out) + (static_cast<int64_t>(tok) * a.H + head) * D + mine * 8;
+  uint32_t u[8];
+#pragma unroll
+  for (int k = 0; k < 8; ++k) u[k] = Num<T>::pack(x[k].x, x[k].y);
+  *reinterpret_cast<uint4*>(dst) = make_uint4(u[0], u[1], u[2], u[3]);
+  *reinterpret_cast<uint4*>(dst + D / 2) = make_uint4(u[4], u[5], u[6], u[7]);
+}
 
-  if (blockIdx.x >= writing) {
-    // ---- queries: PER heads of a token a group of L lanes
-    const int64_t tokens = static_cast<int64_t>(a.B) * a.t, at = (item - writing * 8) * ABREAST + lane / L;
-    const int groups = (a.H + PER - 1) / PER;
-    const int64_t tok = at / groups;
-    const int h0 = static_cast<int>(at - tok * groups) * PER, heads = min(PER, a.H - h0);
-    const bool live = tok < tokens;
-    const int b = live ? static_cast<int>(tok / a.t) : 0, i = live ? static_cast<int>(tok - static_cast<int64_t>(b) * a.t) : 0;
+// One token a row: D / 16 lanes a head, of the queries, keys and values in turn.
+template <class T, int D>
+__global__ void __launch_bounds__(256) append8_one_kernel(const PagedAppendArgs a) {
+  constexpr int L = D / 16, HALF = D / 2;
+  const int mine = threadIdx.x % L, at = blockIdx.x * (256 / L) + threadIdx.x / L, heads = a.H + 2 * a.Hk;
+  const bool live = at < a.B * heads;  // whole warps stay for the shuffles
+  const int b = live ? quotient(at, heads) : 0, h = live ? at - b * heads : 0;
+  const Kind kind = h < a.H ? QUERY : h < a.H + a.Hk ? KEY : VALUE;
+  const int head = h - (kind == QUERY ? 0 : kind == KEY ? a.H : a.H + a.Hk);
+  const int start = a.start[b];
+  bool real = live && start >= 0 && (!a.count || a.count[b] > 0);
+  if (real && start >= a.rope_rows) {
+    if (mine == 0) record_error(3, b);
+    real = false;
+  }
+  Raw r = {};
+  BlockAt block = {};
+  float old = 0.f, gate = 0.f;
+  const int before = start & (TILE - 1);
+  if (real) {
+    const T* src = kind == QUERY ? static_cast<const T*>(a.q) + b * a.qs[0] + head * a.qs[2]
+                 : kind == KEY ? static_cast<const T*>(a.kin) + b * a.ks[0] + head * a.ks[2]
+                               : static_cast<const T*>(a.vin) + b * a.vs[0] + head * a.vs[2];
+    load16(src + mine * 8, HALF, r.lo, r.hi);
+    if (kind != VALUE) {
+      load_angles<T>(a, start, HALF, mine, r);
+    } else if (a.ve) {
+      load16(static_cast<const T*>(a.ve) + b * a.es[0] + head * a.es[2] + mine * 8, HALF, r.lo2, r.hi2);
+      gate = Num<T>::one(static_cast<const T*>(a.ve_gate)[b * a.gs[0] + head * a.gs[2]]);
+    }
+    if (kind != QUERY) {
+      block = find_block(a, b, start - before, head, kind == VALUE, mine == 0);
+      if (block.codes && before) old = *block.scale;
+    }
+  }
+  float2 x[1][8];
+  turn_raw<T, D>(a, r, x[0]);  // lanes of a warp differ in their kind: all pass the shuffles
+  if (kind == VALUE) mix_raw<T>(r, a.ve, share_of(gate), x[0]);
+  float top = 0.f;
+  if (kind != QUERY) top = finite_top(x);
+#pragma unroll
+  for (int o = L / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  if (kind == QUERY) {
+    if (live) store_query<T, D>(a, b, head, mine, x[0]);  // what is no token has zeros in, and gives zeros
+    return;
+  }
+  if (!block.codes) return;
+  const float scale = fmaxf(old, block_scale(top)), by = 1.f / scale;
+  if (before && scale != old)
+#pragma unroll 1
+    for (int e = 0; e < before; ++e) rescale_codes(block.codes + e * block.step + mine * 8, HALF, old * by);
+  write_codes(block.codes + before * block.step + mine * 8, HALF, x[0], by);
+  if (mine == 0) *block.scale = scale;
+}
+
+// More tokens: WIDE warps a block of a KV head's keys or values, so that a thread holds STEPS tokens' 16 channels; the CTAs
+// behind these turn the queries, PER heads of a token a group of lanes.
+template <class T, int D, int PER, int STEPS>
+__global__ void __launch_bounds__(256) append8_kernel(const PagedAppendArgs a, const int blocks, const int writing) {
+  constexpr int L = D / 16, HALF = D / 2, ABREAST = 32 / L, WIDE = TILE / (ABREAST * STEPS);
+  __shared__ float tops[8];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, mine = lane % L;
+
+  if (static_cast<int>(blockIdx.x) >= writing) {
+    const int groups = (a.H + PER - 1) / PER, at = (blockIdx.x - writing) * (256 / L) + threadIdx.x / L;
+    const int tok = PER >= a.H ? at : quotient(at, groups), h0 = (at - tok * groups) * PER;
+    const bool live = tok < a.B * a.t;
+    const int b = live ? quotient(tok, a.t) : 0, i = live ? tok - b * a.t : 0;
     const int start = a.start[b], n = a.count ? a.count[b] : a.t;
     const bool real = live && i < n && start >= 0 && start < a.rope_rows - i;
-    uint2 lo[PER], hi[PER];
-    float2 c[2] = {}, s[2] = {};
-#pragma unroll
-    for (int e = 0; e < PER; ++e) lo[e] = hi[e] = make_uint2(0, 0);
-    if (real) {
-      const T* src = static_cast<const T*>(a.q) + b * a.qs[0] + i * a.qs[1] + h0 * a.qs[2] + mine * 4;
-#pragma unroll
-      for (int e = 0; e < PER; ++e)
-        if (e < heads) {
-          load_halves(src, HALF, lo[e], hi[e]);
-          src += a.qs[2];
-        }
-      const int64_t angle = static_cast<int64_t>(start + i) * HALF + mine * 4;
-      unpack4<T>(*reinterpret_cast<const uint2*>(static_cast<const T*>(a.cos) + angle), c);
-      unpack4<T>(*reinterpret_cast<const uint2*>(static_cast<const T*>(a.sin) + angle), s);
-    }
-    T* dst = static_cast<T*>(a.q_out) + (tok * a.H + h0) * D + mine * 4;
+    uint4 lo[PER], hi[PER];
+    Raw r = {};
+    const T* src = static_cast<const T*>(a.q) + b * a.qs[0] + i * a.qs[1] + h0 * a.qs[2] + mine * 8;
 #pragma unroll
     for (int e = 0; e < PER; ++e) {
-      float2 x[2], y[2], u[2], w[2];
-      unpack4<T>(lo[e], x);
-      unpack4<T>(hi[e], y);
-      turn_head<L, D>(x, y, c, s, a.norm, a.scale, u, w);
-      if (live && e < heads) {  // tokens behind a row's count have zeros in, and give zeros
-        *reinterpret_cast<uint2*>(dst) = pack4<T>(u);
-        *reinterpret_cast<uint2*>(dst + HALF) = pack4<T>(w);
-      }
-      dst += D;
+      lo[e] = hi[e] = make_uint4(0, 0, 0, 0);
+      if (real && h0 + e < a.H) load16(src, HALF, lo[e], hi[e]);
+      src += a.qs[2];
+    }
+    if (real) load_angles<T>(a, start + i, HALF, mine, r);
+#pragma unroll
+    for (int e = 0; e < PER; ++e) {
+      float2 x[8];
+      r.lo = lo[e];
+      r.hi = hi[e];
+      turn_raw<T, D>(a, r, x);
+      if (live && h0 + e < a.H) store_query<T, D>(a, tok, h0 + e, mine, x);
     }
     return;
   }
 
-  // ---- a block of keys or values; the whole warp goes on or returns
+  // ---- a block; its warps go on or return together
+  const int item = blockIdx.x * (8 / WIDE) + warp / WIDE, part = warp % WIDE;
   const bool values = item & 1;
-  const int64_t rest = item >> 1, line = rest / a.Hk;
-  const int hk = static_cast<int>(rest - line * a.Hk), b = static_cast<int>(line / blocks), j = static_cast<int>(line - static_cast<int64_t>(b) * blocks);
+  const int line = quotient(item >> 1, a.Hk), hk = (item >> 1) - line * a.Hk, b = quotient(line, blocks), j = line - b * blocks;
   if (b >= a.B) return;
   const int start = a.start[b];
   int n = a.count ? min(a.count[b], a.t) : a.t;
+  const bool tells = lane == 0 && part == 0;
   if (start < 0 || n <= 0) return;
   if (start > a.rope_rows - n) {
-    if (lane == 0) record_error(3, b);
+    if (tells) record_error(3, b);
     n = a.rope_rows - start;
     if (n <= 0) return;
   }
   const int64_t first = (start & ~(TILE - 1)) + static_cast<int64_t>(j) * TILE;
   if (first >= start + n) return;
-  const PagedCacheArgs& m = a.cache;
-  const int p0 = static_cast<int>(first), column = quotient(p0, m.page), slot0 = p0 - column * m.page;
-  if (column >= m.columns) {
-    if (lane == 0) record_error(1, b);
-    return;
-  }
-  const int page = m.table[static_cast<int64_t>(b) * m.columns + column];
-  if (page < 0 || page >= m.pages) {
-    if (lane == 0) record_error(2, b);
-    return;
-  }
-  const int64_t* scale_strides = values ? m.v_scale_strides : m.k_scale_strides;
-  float* scale_at = (values ? m.v_scale : m.k_scale) + page * scale_strides[0] + hk * scale_strides[1] + (slot0 / TILE) * scale_strides[2];
-  const bool continued = start > p0;
-  const float old = continued ? *scale_at : 0.f;
-
-  const int i0 = p0 + lane / L - start;  // the call's token in this lane's first slot
-  uint2 lo[STEPS], hi[STEPS];
-  const int64_t* strides = values ? a.vs : a.ks;
-  const T* src = static_cast<const T*>(values ? a.vin : a.kin) + b * strides[0] + hk * strides[2] + mine * 4;
+  const int p0 = static_cast<int>(first);
+  const int slot0 = part * (ABREAST * STEPS) + lane / L, i0 = p0 + slot0 - start;  // this lane's first slot, as a token of the call
+  Raw r[STEPS];
+  float gate[STEPS] = {};
+  const T* src = (values ? static_cast<const T*>(a.vin) + b * a.vs[0] + hk * a.vs[2] : static_cast<const T*>(a.kin) + b * a.ks[0] + hk * a.ks[2]) + mine * 8;
+  const int64_t step = values ? a.vs[1] : a.ks[1];
 #pragma unroll
   for (int e = 0; e < STEPS; ++e) {
     const int i = i0 + e * ABREAST;
-    lo[e] = hi[e] = make_uint2(0, 0);
-    if (i >= 0 && i < n) load_halves(src + i * strides[1], HALF, lo[e], hi[e]);
-  }
-  float x[STEPS][8];
-  if (values) {
-    uint2 elo[STEPS], ehi[STEPS];
-    T gate[STEPS];
-    if (a.ve) {
-      const T* es = static_cast<const T*>(a.ve) + b * a.es[0] + hk * a.es[2] + mine * 4;
-      const T* gs = static_cast<const T*>(a.ve_gate) + b * a.gs[0] + hk * a.gs[2];
-#pragma unroll
-      for (int e = 0; e < STEPS; ++e) {
-        const int i = i0 + e * ABREAST;
-        if (i >= 0 && i < n) {
-          load_halves(es + i * a.es[1], HALF, elo[e], ehi[e]);
-          gate[e] = gs[i * a.gs[1]];
-        }
-      }
-    }
-#pragma unroll
-    for (int e = 0; e < STEPS; ++e) {
-      const int i = i0 + e * ABREAST;
-      float2 u[2], w[2];
-      unpack4<T>(lo[e], u);
-      unpack4<T>(hi[e], w);
-      if (a.ve && i >= 0 && i < n) {
-        float2 y[2], z[2];
-        const float f = 3.f / (1.f + expf(-Num<T>::one(gate[e])));
-        unpack4<T>(elo[e], y);
-        unpack4<T>(ehi[e], z);
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          u[k] = fma2(make_float2(f, f), y[k], u[k]);
-          w[k] = fma2(make_float2(f, f), z[k], w[k]);
-        }
-      }
-      x[e][0] = u[0].x; x[e][1] = u[0].y; x[e][2] = u[1].x; x[e][3] = u[1].y;
-      x[e][4] = w[0].x; x[e][5] = w[0].y; x[e][6] = w[1].x; x[e][7] = w[1].y;
-    }
-  } else {
-#pragma unroll
-    for (int e = 0; e < STEPS; ++e) {
-      const int i = i0 + e * ABREAST;
-      float2 c[2] = {}, s[2] = {}, y[2], z[2], u[2], w[2];
-      if (i >= 0 && i < n) {
-        const int64_t angle = static_cast<int64_t>(start + i) * HALF + mine * 4;
-        unpack4<T>(*reinterpret_cast<const uint2*>(static_cast<const T*>(a.cos) + angle), c);
-        unpack4<T>(*reinterpret_cast<const uint2*>(static_cast<const T*>(a.sin) + angle), s);
-      }
-      unpack4<T>(lo[e], y);
-      unpack4<T>(hi[e], z);
-      turn_head<L, D>(y, z, c, s, a.norm, a.scale, u, w);
-      x[e][0] = u[0].x; x[e][1] = u[0].y; x[e][2] = u[1].x; x[e][3] = u[1].y;
-      x[e][4] = w[0].x; x[e][5] = w[0].y; x[e][6] = w[1].x; x[e][7] = w[1].y;
+    r[e] = {};
+    if (i < 0 || i >= n) continue;
+    load16(src + i * step, HALF, r[e].lo, r[e].hi);
+    if (!values) {
+      load_angles<T>(a, start + i, HALF, mine, r[e]);
+    } else if (a.ve) {
+      load16(static_cast<const T*>(a.ve) + b * a.es[0] + hk * a.es[2] + mine * 8 + i * a.es[1], HALF, r[e].lo2, r[e].hi2);
+      gate[e] = Num<T>::one((static_cast<const T*>(a.ve_gate) + b * a.gs[0] + hk * a.gs[2])[i * a.gs[1]]);
     }
   }
-  // slots without a new token hold zeros here
-  float top = 0.f;
-  bool odd = false;
+  const BlockAt block = find_block(a, b, p0, hk, values, tells);
+  if (!block.codes) return;
+  const float old = start > p0 ? *block.scale : 0.f;
+  float2 x[STEPS][8];
 #pragma unroll
-  for (int e = 0; e < STEPS; ++e)
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const bool fine = fabsf(x[e][k]) < INFINITY;
-      top = fmaxf(top, fine ? fabsf(x[e][k]) : 0.f);
-      odd |= !fine;
-    }
+  for (int e = 0; e < STEPS; ++e) {
+    if (values) mix_raw<T>(r[e], a.ve, share_of(gate[e]), x[e]);
+    else turn_raw<T, D>(a, r[e], x[e]);
+  }
+  float top = finite_top(x);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  if (odd)
+  if (WIDE > 1) {
+    if (lane == 0) tops[warp] = top;
+    named_bar_sync(1 + warp / WIDE, WIDE * 32);  // (the old scale is read by now, too)
 #pragma unroll
-    for (int e = 0; e < STEPS; ++e)
-#pragma unroll
-      for (int k = 0; k < 8; ++k) x[e][k] = fabsf(x[e][k]) < INFINITY ? x[e][k] : NAN;
+    for (int w = 0; w < WIDE; ++w) top = fmaxf(top, tops[warp - part + w]);
+  }
   const float scale = fmaxf(old, block_scale(top)), by = 1.f / scale;
-  const bool again = continued && scale != old;
-  uint8_t* codes = values ? static_cast<uint8_t*>(m.v) + page * m.page_stride_v + hk * m.head_stride_v + static_cast<int64_t>(slot0) * m.slot_stride_v
-                          : static_cast<uint8_t*>(m.k) + page * m.page_stride_k + hk * m.head_stride_k + static_cast<int64_t>(slot0) * m.slot_stride_k;
-  const int64_t step = values ? m.slot_stride_v : m.slot_stride_k;
 #pragma unroll
   for (int e = 0; e < STEPS; ++e) {
     const int i = i0 + e * ABREAST;
-    uint8_t* at = codes + (e * ABREAST + lane / L) * step + mine * 4;
-    float u[4], w[4];
-    float f = by;
+    uint8_t* at = block.codes + (slot0 + e * ABREAST) * block.step + mine * 8;
     if (i < 0) {
-      if (!again) continue;
-      from_e4m3(*reinterpret_cast<const uint32_t*>(at), u);
-      from_e4m3(*reinterpret_cast<const uint32_t*>(at + HALF), w);
-      f *= old;
-    } else {
-      if (i >= n) continue;
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        u[k] = x[e][k];
-        w[k] = x[e][k + 4];
-      }
+      if (scale != old) rescale_codes(at, HALF, old * by);
+    } else if (i < n) {
+      write_codes(at, HALF, x[e], by);
     }
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      u[k] *= f;
-      w[k] *= f;
-    }
-    *reinterpret_cast<uint32_t*>(at) = to_e4m3(u);
-    *reinterpret_cast<uint32_t*>(at + HALF) = to_e4m3(w);
   }
-  if (lane == 0) *scale_at = scale;
+  if (tells) *block.scale = scale;
 }
 
-template <class T, int D, int PER>
+template <class T, int D, int PER, int STEPS>
 static int launch_append8(const PagedAppendArgs& a, cudaStream_t s) {
-  const int64_t tokens = static_cast<int64_t>(a.B) * a.t, blocks = (a.t + 2 * (TILE - 1)) / TILE, abreast = 32 / (D / 8);
-  const int64_t writing = (a.B * blocks * a.Hk * 2 + 7) / 8, turning = (tokens * ((a.H + PER - 1) / PER) + 8 * abreast - 1) / (8 * abreast);
-  if (writing + turning > INT32_MAX) return -1;
-  append8_kernel<T, D, PER><<<static_cast<unsigned>(writing + turning), 256, 0, s>>>(a, static_cast<int>(blocks), writing);
+  constexpr int L = D / 16, PER_CTA = 8 * STEPS * (32 / L) / TILE;
+  const int64_t tokens = static_cast<int64_t>(a.B) * a.t, blocks = (a.t + 2 * (TILE - 1)) / TILE;
+  const int64_t writing = (a.B * blocks * a.Hk * 2 + PER_CTA - 1) / PER_CTA;
+  const int64_t turning = (tokens * ((a.H + PER - 1) / PER) + 256 / L - 1) / (256 / L);
+  if (writing * PER_CTA > INT32_MAX || turning * (256 / L) > INT32_MAX) return -1;
+  append8_kernel<T, D, PER, STEPS><<<static_cast<unsigned>(writing + turning), 256, 0, s>>>(a, static_cast<int>(blocks), static_cast<int>(writing));
   return 0;
 }
 template <class T, int D>
 static int launch_append8(const PagedAppendArgs& a, cudaStream_t s) {
-  return static_cast<int64_t>(a.B) * a.t * a.H >= 16384 ? launch_append8<T, D, 5>(a, s) : launch_append8<T, D, 1>(a, s);
+  if (a.t == 1) {
+    constexpr int PER_CTA = 256 / (D / 16);
+    const int64_t items = static_cast<int64_t>(a.B) * (a.H + 2 * a.Hk);
+    if (items > INT32_MAX - PER_CTA) return -1;
+    append8_one_kernel<T, D><<<static_cast<unsigned>((items + PER_CTA - 1) / PER_CTA), 256, 0, s>>>(a);
+    return 0;
+  }
+  return static_cast<int64_t>(a.B) * a.t * a.H >= 32768 ? launch_append8<T, D, 3, 2>(a, s) : launch_append8<T, D, 1, 1>(a, s);
 }
 
 struct Plan {
