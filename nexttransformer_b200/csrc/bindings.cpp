@@ -25,6 +25,7 @@
 #include "nsa_compress.h"
 #include "msar.h"
 #include "paged.h"
+#include "sampling.h"
 #include "plugin_ops.h"
 #include "probe_sm100.h"
 #include "residual.h"
@@ -1571,6 +1572,51 @@ Tensor adjust_logits(const Tensor& logits, const OptT& tokens, const OptT& lengt
   return out;
 }
 
+std::vector<Tensor> sample_logits(const Tensor& logits, const Tensor& uniform, const py::object& temperature, const py::object& top_k,
+                                  const py::object& top_p, const py::object& min_p) {
+  check_cuda(logits, "logits");
+  inference_only({&logits, &uniform});
+  const auto type = logits.scalar_type();
+  TORCH_CHECK(type == at::kBFloat16 || type == at::kHalf || type == at::kFloat, "logits must be bf16, fp16 or fp32");
+  TORCH_CHECK(logits.dim() == 2 && (logits.stride(1) == 1 || logits.size(1) == 1), "logits must be [B, V] with contiguous rows");
+  SampleArgs a;
+  const int64_t B = logits.size(0), V = logits.size(1);
+  TORCH_CHECK(V >= 1 && V <= nt_sample_most(), "sample_logits takes vocabularies of 1 to ", nt_sample_most(), " tokens");
+  TORCH_CHECK(B <= INT32_MAX / 8, "sample_logits: too many rows");
+  a.B = static_cast<int>(B);
+  a.V = static_cast<int>(V);
+  a.logits = logits.data_ptr();
+  a.row_stride = logits.stride(0);
+  a.type = type == at::kBFloat16 ? LOGITS_BF16 : type == at::kHalf ? LOGITS_FP16 : LOGITS_FP32;
+  a.sms = num_sms(logits);
+  a.uniform = row_floats(uniform, logits, B, "uniform");
+  // a number for all rows, a tensor with one for each, or None
+  const auto given = [&](const py::object& o, const char* name, bool whole, double none) {
+    RowValue v;
+    v.all = none;
+    if (o.is_none()) return v;
+    if (THPVariable_Check(o.ptr())) {
+      const Tensor& t = THPVariable_Unpack(o.ptr());
+      inference_only({&t});
+      v.rows = whole ? static_cast<const void*>(row_ints(t, logits, B, name)) : row_floats(t, logits, B, name);
+    } else {
+      v.all = whole ? static_cast<double>(std::min<int64_t>(o.cast<int64_t>(), INT32_MAX)) : o.cast<double>();
+    }
+    return v;
+  };
+  a.temperature = given(temperature, "temperature", false, 1.0);
+  a.top_k = given(top_k, "top_k", true, 0.0);
+  a.top_p = given(top_p, "top_p", false, 1.0);
+  a.min_p = given(min_p, "min_p", false, 0.0);
+  const c10::cuda::CUDAGuard guard(logits.device());
+  Tensor tokens = fresh({B}, at::kLong, logits), logprobs = fresh({B}, at::kFloat, logits);
+  a.tokens = tokens.data_ptr<int64_t>();
+  a.logprobs = logprobs.data_ptr<float>();
+  ok(nt_sample_logits(a, stream()), "sample_logits");
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  return {tokens, logprobs};
+}
+
 std::vector<int64_t> read_serving_errors() {
   unsigned wp = 0, wd = 0;
   const int p = nt_paged_read_error(&wp);
@@ -1660,6 +1706,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("paged_attention", &paged_attention, "attention of new tokens over a paged cache");
   m.def("delta_step", &delta_step, "recurrent gated delta rule with a carried fp32 state");
   m.def("adjust_logits", &adjust_logits, "penalties, biases and grammar mask on logits");
+  m.def("sample_logits", &sample_logits, "a token for each row: temperature, top-k, top-p, min-p");
   m.def("read_serving_errors", &read_serving_errors);
   m.def("read_comm_errors", &read_comm_errors);
   m.def("gemm_ce_dgrad", &gemm_ce_dgrad);

@@ -1,0 +1,724 @@
+// K25: one token for each row of logits, from a number u in [0, 1) that the caller draws.
+//
+//   w_i = exp((x_i - max x) / T); order: x falling, index rising among equals
+//   top-k: the first k.  top-p: those before which less than p of (the first k's) mass lies.  min-p: w_i >= min_p
+//   token = the smallest index up to which more than u of the kept mass lies (in the order of indices)
+//
+// Weights are whole numbers, 2^S w rounded (S = 62 - log2 V), from a 64-bit exp: sums are exact in any order, so atomics and
+// the split of a row change nothing, and a token differs from the one that real numbers give only when u lies within
+// about V 2^-S of a border.
+//
+// A row lies in the shared memory of a cluster of CTAs and is read from memory once.  A selection's border (the k-th, or the
+// one at which p is reached) is found by a histogram of 2048 bins of T / 32 below the maximum, whose bins the CTAs add up
+// through distributed shared memory; the few logits of the border's bin are then ranked among each other.  Where
+// they are many, further histograms split the bin by the numbers' bits, and equal logits by their indices.
+#include "sampling.h"
+#include "common.cuh"
+
+#include <cuda_fp16.h>
+#include <math.h>
+
+namespace nt {
+namespace sampling {
+
+constexpr int THREADS = 512, WARPS = THREADS / 32, BINS = 2048, CAP = 1024;
+constexpr int FEW = 2048, EACH = FEW / THREADS;  // a list that one CTA sorts; its entries a thread
+constexpr int SEGMENT_MOST = 45056;  // logits of a CTA: 176 KB
+constexpr int CLUSTER_MOST = 8;
+using u64 = unsigned long long;
+
+template <class T> NT_DEVICE float to_float(T v);
+template <> NT_DEVICE float to_float(float v) { return v; }
+template <> NT_DEVICE float to_float(__half v) { return __half2float(v); }
+template <> NT_DEVICE float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+
+// Whole numbers in the order of the floats (which have no -0 here).
+NT_DEVICE uint32_t key_of(float x) {
+  const uint32_t u = __float_as_uint(x);
+  return u ^ (static_cast<uint32_t>(static_cast<int>(u) >> 31) | 0x80000000u);
+}
+
+NT_DEVICE float value_of(uint32_t key) { return __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key); }
+
+struct Border {     // kept: keys above it, and those equal to it up to its index
+  uint32_t key;
+  int index;
+};
+struct Note {       // what a CTA tells the others
+  u64 mass;
+  uint32_t count, low, high;
+  int index;
+};
+
+struct Shared {
+  union {
+    u64 mass[BINS];
+    uint32_t count[BINS];
+    struct {
+      uint32_t key[CAP];
+      int index[CAP];
+      u64 weight[CAP];
+    } all;           // the border's bin, of every CTA
+    u64 sorted[FEW];  // what may be kept, of every CTA, in order
+  };
+  union {            // of this CTA
+    struct {
+      uint32_t key[CAP];
+      int index[CAP];
+    };
+    u64 list[FEW];
+    u64 by_index[FEW / 2];
+  };
+  Note note[2];
+  u64 scan[WARPS + 1], own[WARPS];
+  float top[WARPS];
+  int nan;
+  uint32_t listed, low, high;
+  int found;
+  u64 found_before, found_own;
+  Border border;
+};
+
+// The same address in CTA `rank` of the cluster.
+template <class P>
+NT_DEVICE P* peer(P* p, int rank) {
+  uint64_t r;
+  asm("mapa.u64 %0, %1, %2;" : "=l"(r) : "l"(reinterpret_cast<uint64_t>(p)), "r"(rank));
+  return reinterpret_cast<P*>(r);
+}
+
+struct Row {
+  float* x;          // this CTA's logits
+  int n, first, V;   // how many, index of the first
+  int ranks, rank;
+  float top;         // the row's largest
+  double inverse;    // log2(e) / T
+  float per_bin;     // bins a logit's distance from the top
+  int shift;         // S
+};
+
+// 2^S exp((x - top) / T), rounded; |error| below 1 + 2^(S - 48)
+NT_DEVICE double power(const Row& r, float x, int shift) {
+  const double t = (static_cast<double>(x) - static_cast<double>(r.top)) * r.inverse;
+  if (!(t > -70.0)) return 0.0;
+  constexpr double MAGIC = 6755399441055744.0;  // 1.5 2^52: adding it rounds to a whole number
+  const double whole = t + MAGIC, n = whole - MAGIC, z = (t - n) * 0.69314718055994530942;
+  // exp(z), |z| <= 0.347, by its series: the first term left out is 7e-15 (z^12 / 12!)
+  double p = 1.0 / 39916800.0;
+  p = fma(p, z, 1.0 / 3628800.0);
+  p = fma(p, z, 1.0 / 362880.0);
+  p = fma(p, z, 1.0 / 40320.0);
+  p = fma(p, z, 1.0 / 5040.0);
+  p = fma(p, z, 1.0 / 720.0);
+  p = fma(p, z, 1.0 / 120.0);
+  p = fma(p, z, 1.0 / 24.0);
+  p = fma(p, z, 1.0 / 6.0);
+  p = fma(p, z, 0.5);
+  p = fma(p, z, 1.0);
+  p = fma(p, z, 1.0);
+  const int e = __double2loint(whole) + shift;  // p 2^e; never below 2^-72, so that only the exponent's bits change
+  return __hiloint2double(__double2hiint(p) + (e << 20), __double2loint(p));
+}
+NT_DEVICE u64 weight_of(const Row& r, float x) {
+  const double v = power(r, x, r.shift) + 4503599627370496.0;  // 2^52: the whole number is in the lower bits
+  return static_cast<u64>(__double_as_longlong(v)) & 0xfffffffffffffull;
+}
+NT_DEVICE int bin_of(const Row& r, float x) {
+  // both operations keep the order of the logits; the last bin, from 64 T on, has no weight (-inf and NaN, of inf 0, too)
+  return static_cast<int>(fminf((r.top - x) * r.per_bin, static_cast<float>(BINS - 1)));
+}
+NT_DEVICE bool within(const Border& b, float x, int index) {
+  const uint32_t k = key_of(x);
+  return k > b.key || (k == b.key && index <= b.index);
+}
+
+template <class V>
+NT_DEVICE V warp_scan(V v, int lane) {  // inclusive
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const V w = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += w;
+  }
+  return v;
+}
+// Exclusive sum over the CTA's threads; `total` gets the whole.  Two barriers.
+NT_DEVICE u64 block_scan(u64 v, Shared& s, u64& total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const u64 upto = warp_scan(v, lane);
+  __syncthreads();
+  if (lane == 31) s.scan[warp] = upto;
+  __syncthreads();
+  u64 before = 0;
+  total = 0;
+#pragma unroll
+  for (int w = 0; w < WARPS; ++w) {
+    const u64 x = s.scan[w];
+    if (w < warp) before += x;
+    total += x;
+  }
+  return before + upto - v;
+}
+
+NT_DEVICE u64 share_of(float p, u64 total, bool up) {  // p total, 0 <= p < 1, to a whole number
+  const u64 f = static_cast<u64>(static_cast<double>(p) * 18446744073709551616.0);
+  return __umul64hi(f, total) + (up && f * total != 0 ? 1 : 0);
+}
+
+// Adds to a 64-bit sum in shared memory by its halves: the upper one is rarely touched.
+NT_DEVICE void add_to(u64* p, u64 w) {
+  uint32_t* half = reinterpret_cast<uint32_t*>(p);
+  const uint32_t lo = static_cast<uint32_t>(w), before = atomicAdd(half, lo);
+  const uint32_t hi = static_cast<uint32_t>(w >> 32) + (before + lo < lo ? 1u : 0u);
+  if (hi) atomicAdd(half + 1, hi);
+}
+template <bool MASS>
+NT_DEVICE void clear_bins(Shared& s) {
+  uint4* p = reinterpret_cast<uint4*>(s.mass);
+  for (int i = threadIdx.x; i < BINS * (MASS ? 8 : 4) / 16; i += THREADS) p[i] = make_uint4(0, 0, 0, 0);
+  __syncthreads();
+}
+template <bool MASS>
+NT_DEVICE void add_to_bin(const Row& r, Shared& s, int bin, float x) {
+  if (MASS) add_to(&s.mass[bin], weight_of(r, x));
+  else atomicAdd(&s.count[bin], 1u);
+}
+// The bin in which the sum over the cluster's bins reaches the target, or -1; `before`: the sum over those before it.  A target of
+// 0 is set to `share` of the whole first.
+template <bool MASS>
+NT_DEVICE int crossing(const Row& r, Shared& s, u64& target, float share, u64& before) {
+  constexpr int PER = BINS / THREADS;
+  const int tid = threadIdx.x;
+  u64 sum[PER] = {}, all = 0;
+  for (int c0 = 0; c0 < r.ranks; c0 += 4) {  // four CTAs' bins are asked for at once
+    if (MASS) {
+      ulonglong2 u[4], v[4];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        u[c] = v[c] = make_ulonglong2(0, 0);
+        if (c0 + c < r.ranks) {
+          const ulonglong2* m = reinterpret_cast<const ulonglong2*>(peer(s.mass, c0 + c)) + tid * 2;
+          u[c] = m[0];
+          v[c] = m[1];
+        }
+      }
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        sum[0] += u[c].x; sum[1] += u[c].y; sum[2] += v[c].x; sum[3] += v[c].y;
+      }
+    } else {
+      uint4 u[4];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        u[c] = make_uint4(0, 0, 0, 0);
+        if (c0 + c < r.ranks) u[c] = reinterpret_cast<const uint4*>(peer(s.count, c0 + c))[tid];
+      }
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        sum[0] += u[c].x; sum[1] += u[c].y; sum[2] += u[c].z; sum[3] += u[c].w;
+      }
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < PER; ++e) all += sum[e];
+  if (tid == 0) s.found = -1;
+  u64 total;
+  u64 at = block_scan(all, s, total);
+  if (MASS && target == 0) target = share > 0.f ? max(share_of(share, total, true), 1ull) : 1ull;
+#pragma unroll
+  for (int e = 0; e < PER; ++e) {
+    if (at < target && target <= at + sum[e]) {
+      s.found = tid * PER + e;
+      s.found_before = at;
+    }
+    at += sum[e];
+  }
+  __syncthreads();
+  before = s.found_before;
+  return s.found;
+}
+// A histogram of the elements within `outer` by their distance from the top, and its crossing.
+template <bool MASS>
+NT_DEVICE int first_crossing(const Row& r, Shared& s, const Border& outer, u64& target, float share, u64& before) {
+  clear_bins<MASS>(s);
+  const bool any = outer.key == 0;
+  for (int i = threadIdx.x; i < r.n; i += THREADS) {
+    const float x = r.x[i];
+    const int bin = bin_of(r, x);
+    if (bin < BINS - 1 && (any || within(outer, x, r.first + i))) add_to_bin<MASS>(r, s, bin, x);
+  }
+  cluster_sync();
+  return crossing<MASS>(r, s, target, share, before);
+}
+
+// The border of a selection: the element at which the sum (of weights, or of ones) over the order reaches `target`, which lies in
+// bin `chosen`, behind a sum of `done`.  Only elements within `outer` count.
+template <bool MASS>
+NT_DEVICE Border find_border(const Row& r, Shared& s, int& round, const Border& outer, u64 target, int chosen, u64 done) {
+  const int tid = threadIdx.x, lane = tid & 31;
+  uint32_t low = 0, high = 0xffffffffu;  // of the candidates' keys, after the first list
+  bool first = true;
+  auto candidate = [&](float x, int index) {
+    if (first) return bin_of(r, x) == chosen && within(outer, x, index);
+    const uint32_t k = key_of(x);
+    return k >= low && k <= high && within(outer, x, index);
+  };
+#pragma unroll 1
+  while (true) {
+    // ---- this CTA's candidates: a list, their number, and their extremes
+    if (tid == 0) {
+      s.listed = 0;
+      s.low = 0xffffffffu;
+      s.high = 0;
+    }
+    __syncthreads();
+    for (int i0 = 0; i0 < r.n; i0 += THREADS) {
+      const int i = i0 + tid;
+      const bool mine = i < r.n && candidate(r.x[i], r.first + i);
+      const unsigned who = __ballot_sync(0xffffffffu, mine);
+      if (!who) continue;
+      uint32_t at = 0;
+      if (lane == 0) at = atomicAdd(&s.listed, __popc(who));
+      at = __shfl_sync(0xffffffffu, at, 0) + __popc(who & ((1u << lane) - 1u));
+      const uint32_t k = mine ? key_of(r.x[i]) : 0u;
+      const uint32_t least = __reduce_min_sync(0xffffffffu, mine ? k : 0xffffffffu), most = __reduce_max_sync(0xffffffffu, k);
+      if (mine && at < CAP) {
+        s.key[at] = k;
+        s.index[at] = r.first + i;
+      }
+      if (lane == 0) {
+        atomicMin(&s.low, least);
+        atomicMax(&s.high, most);
+      }
+    }
+    __syncthreads();
+    if (tid == 0) {
+      Note& n = s.note[round & 1];
+      n.count = s.listed;
+      n.low = s.low;
+      n.high = s.high;
+    }
+    cluster_sync();
+    const Note* theirs = peer(&s.note[round & 1], min(lane, r.ranks - 1));
+    const uint32_t counts = lane < r.ranks ? theirs->count : 0u;  // lane c: CTA c's
+    const uint32_t many = __reduce_add_sync(0xffffffffu, counts);
+    low = __reduce_min_sync(0xffffffffu, theirs->low);
+    high = __reduce_max_sync(0xffffffffu, theirs->high);
+    ++round;
+    first = false;
+    if (many <= CAP) {
+      // ---- rank them among each other (each CTA by itself)
+      uint32_t at = 0;
+      for (int c = 0; c < r.ranks; ++c) {
+        const uint32_t n = __shfl_sync(0xffffffffu, counts, c);
+        for (uint32_t i = tid; i < n; i += THREADS) {
+          const uint32_t k = peer(s.key, c)[i];
+          s.all.key[at + i] = k;
+          s.all.index[at + i] = peer(s.index, c)[i];
+          if (MASS) s.all.weight[at + i] = weight_of(r, value_of(k));
+        }
+        at += n;
+      }
+      __syncthreads();
+      for (uint32_t i = tid; i < many; i += THREADS) {
+        const uint32_t k = s.all.key[i];
+        const int index = s.all.index[i];
+        u64 sum = done;
+        for (uint32_t j = 0; j < many; ++j) {
+          const uint32_t kj = s.all.key[j];
+          if (kj > k || (kj == k && s.all.index[j] < index)) sum += MASS ? s.all.weight[j] : 1ull;
+        }
+        if (sum < target && target <= sum + (MASS ? s.all.weight[i] : 1ull)) s.border = {k, index};
+      }
+      __syncthreads();
+      return s.border;
+    }
+    if (low == high) {
+      // ---- equal logits: the first of them by index.  The number of those that are kept:
+      const u64 each = MASS ? weight_of(r, value_of(low)) : 1ull;
+      u64 need = (target - done + each - 1) / each;  // at least 1
+      for (int c = 0; c < r.rank; ++c) {
+        const uint32_t n = __shfl_sync(0xffffffffu, counts, c);
+        need = need > n ? need - n : 0;  // 0 from the CTA on that has the last
+      }
+      // every warp takes a run of indices
+      const int run = (r.n + WARPS - 1) / WARPS, from = (tid >> 5) * run, to = min(r.n, from + run);
+      u64 mine = 0, total;
+      for (int i = from + lane; i < to; i += 32) mine += candidate(r.x[i], r.first + i) ? 1 : 0;
+      u64 prior = block_scan(mine, s, total);
+      prior = __shfl_sync(0xffffffffu, prior, 0);  // of the warps before
+      if (tid == 0) s.note[round & 1].index = -1;
+      __syncthreads();
+      if (need && need <= total) {
+        for (int i0 = from; i0 < to; i0 += 32) {
+          const int i = i0 + lane;
+          const bool is = i < to && candidate(r.x[i], r.first + i);
+          const unsigned who = __ballot_sync(0xffffffffu, is);
+          if (is && prior + __popc(who & ((2u << lane) - 1u)) == need) s.note[round & 1].index = r.first + i;
+          prior += __popc(who);
+        }
+      }
+      cluster_sync();
+      const int index = lane < r.ranks ? peer(&s.note[round & 1], lane)->index : -1;
+      ++round;
+      return {low, __reduce_max_sync(0xffffffffu, index)};
+    }
+    // ---- many that differ: a histogram of their keys, the largest first
+    const int shift = max(0, 32 - __clz(high - low) - 11);
+    clear_bins<MASS>(s);
+    for (int i = tid; i < r.n; i += THREADS) {
+      const float x = r.x[i];
+      if (candidate(x, r.first + i)) add_to_bin<MASS>(r, s, (high - key_of(x)) >> shift, x);
+    }
+    cluster_sync();
+    u64 rest = target - done, before;  // crossing() counts from the first bin
+    const int bin = crossing<MASS>(r, s, rest, 0.f, before);
+    done += before;
+    high = high - (static_cast<uint32_t>(bin) << shift);
+    low = max(low, shift ? high - ((1u << shift) - 1u) : high);
+  }
+}
+
+struct Filters {
+  int first;       // top-k (0x7fffffff: off)
+  float share;     // top-p (1: off)
+  double least;    // min-p
+  float number;    // u
+};
+
+NT_DEVICE void sort(u64* x, int n) {  // n a power of two, 64 at least; ascending
+  const int tid = threadIdx.x;
+#pragma unroll 1
+  for (int k = 2; k <= n; k <<= 1)
+#pragma unroll 1
+    for (int j = k >> 1; j > 0; j >>= 1) {
+      for (int p = tid; p < n / 2; p += THREADS) {
+        const int i = ((p & ~(j - 1)) << 1) | (p & (j - 1));
+        const u64 u = x[i], v = x[i + j];
+        if ((u > v) == ((i & k) == 0)) {
+          x[i] = v;
+          x[i + j] = u;
+        }
+      }
+      // up to a distance of 32 a warp's pairs lie in its own 64 entries
+      if (j > 32 || (j == 1 && k >= 64)) __syncthreads();
+      else __syncwarp();
+    }
+  __syncthreads();
+}
+
+// Where few elements can be kept (the bins up to `chosen`): one CTA sorts them and draws.  target: the mass at which p is reached, or
+// 0 where it is yet to be taken of the first k's.  False: they are many.
+NT_DEVICE bool draw_from_few(const SampleArgs& a, const Row& r, Shared& s, int& round, const Border& outer, int chosen, u64 target,
+                             const Filters& f, int b) {
+  const int tid = threadIdx.x, lane = tid & 31;
+  if (tid == 0) s.listed = 0;
+  __syncthreads();
+  const bool any = outer.key == 0;
+  for (int i0 = 0; i0 < r.n; i0 += THREADS) {
+    const int i = i0 + tid;
+    const float x = i < r.n ? r.x[i] : 0.f;
+    const bool mine = i < r.n && bin_of(r, x) <= chosen && (any || within(outer, x, r.first + i));
+    const unsigned who = __ballot_sync(0xffffffffu, mine);
+    if (!who) continue;
+    uint32_t at = 0;
+    if (lane == 0) at = atomicAdd(&s.listed, __popc(who));
+    at = __shfl_sync(0xffffffffu, at, 0) + __popc(who & ((1u << lane) - 1u));
+    if (mine && at < FEW) s.list[at] = (static_cast<u64>(~key_of(x)) << 32) | static_cast<uint32_t>(r.first + i);
+  }
+  __syncthreads();
+  if (tid == 0) s.note[round & 1].count = s.listed;
+  cluster_sync();
+  const uint32_t counts = lane < r.ranks ? peer(&s.note[round & 1], lane)->count : 0u;
+  const int many = static_cast<int>(__reduce_add_sync(0xffffffffu, counts));
+  ++round;
+  if (many > FEW) return false;
+  if (r.rank == 0) {
+    uint32_t at = 0;
+    for (int c = 0; c < r.ranks; ++c) {
+      const uint32_t n = __shfl_sync(0xffffffffu, counts, c);
+      for (uint32_t i = tid; i < n; i += THREADS) s.sorted[at + i] = peer(s.list, c)[i];
+      at += n;
+    }
+  }
+  cluster_sync();  // the lists are read: the other CTAs are done
+  if (r.rank != 0) return true;
+  int n = 64;
+  while (n < many) n <<= 1;
+  for (int i = many + tid; i < n; i += THREADS) s.sorted[i] = ~0ull;
+  __syncthreads();
+  sort(s.sorted, n);
+
+  // ---- masses in order, a thread's entries one after another; the kept ones are the first
+  u64 w[EACH], sum = 0, total;
+  uint32_t index[EACH];
+#pragma unroll
+  for (int e = 0; e < EACH; ++e) {
+    const int at = tid * EACH + e;
+    w[e] = 0;
+    index[e] = 0;
+    if (at >= min(many, f.first)) continue;
+    const u64 v = s.sorted[at];
+    const float x = value_of(~static_cast<uint32_t>(v >> 32));
+    index[e] = static_cast<uint32_t>(v);
+    w[e] = weight_of(r, x);
+    sum += w[e];
+    if (f.least > 0.0 && !(power(r, x, 0) >= f.least)) index[e] = 0xffffffffu;
+  }
+  u64 at = block_scan(sum, s, total);
+  if (target == 0) target = f.share < 1.f ? (f.share > 0.f ? max(share_of(f.share, total, true), 1ull) : 1ull) : total;
+  sum = 0;
+#pragma unroll
+  for (int e = 0; e < EACH; ++e) {
+    const u64 own = w[e];
+    if (at >= target || index[e] == 0xffffffffu) w[e] = 0;
+    at += own;
+    sum += w[e];
+  }
+  block_scan(sum, s, total);
+  // ---- the draw goes by index: runs of indices first, then the indices of the run
+  u64 aim = min(share_of(f.number, total, false), total - 1);
+  const int low_bits = max(0, 32 - __clz(r.V - 1) - 9);  // V <= 2^19: at most 1024 indices a run
+  for (int i = tid; i < THREADS; i += THREADS) s.by_index[i] = 0;
+  __syncthreads();
+#pragma unroll
+  for (int e = 0; e < EACH; ++e)
+    if (w[e]) add_to(&s.by_index[index[e] >> low_bits], w[e]);
+  __syncthreads();
+  u64 own = s.by_index[tid], ignored;
+  at = block_scan(own, s, ignored);
+  if (at <= aim && aim < at + own) {
+    s.found = tid;
+    s.found_before = at;
+  }
+  __syncthreads();
+  const uint32_t run = s.found;
+  aim -= s.found_before;
+  for (int i = tid; i < (1 << low_bits); i += THREADS) s.by_index[i] = 0;
+  __syncthreads();
+#pragma unroll
+  for (int e = 0; e < EACH; ++e)
+    if (w[e] && (index[e] >> low_bits) == run) s.by_index[index[e] & ((1u << low_bits) - 1u)] = w[e];
+  __syncthreads();
+  const u64 u = 2 * tid < (1 << low_bits) ? s.by_index[2 * tid] : 0, v = 2 * tid + 1 < (1 << low_bits) ? s.by_index[2 * tid + 1] : 0;
+  at = block_scan(u + v, s, ignored);
+  if (at <= aim && aim < at + u + v) {
+    const bool second = aim >= at + u;
+    a.tokens[b] = (static_cast<int64_t>(run) << low_bits) + 2 * tid + (second ? 1 : 0);
+    a.logprobs[b] = static_cast<float>(log(static_cast<double>(second ? v : u) / static_cast<double>(total)));
+  }
+  return true;
+}
+
+template <class T, bool VECTORS>
+__global__ void __launch_bounds__(THREADS) sample_kernel(const SampleArgs a, const int segment, const int ranks) {
+  extern __shared__ __align__(16) float values[];
+  __shared__ Shared s;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, b = blockIdx.x / ranks;
+  auto value = [&](const RowValue& v) { return v.rows ? static_cast<const float*>(v.rows)[b] : static_cast<float>(v.all); };
+  Row r;
+  r.x = values;
+  r.ranks = ranks;
+  r.rank = blockIdx.x % ranks;
+  r.V = a.V;
+  r.first = min(r.rank * segment, a.V);
+  r.n = min(segment, a.V - r.first);
+  const float heat = value(a.temperature), u = a.uniform[b], top_p = value(a.top_p), min_p = value(a.min_p);
+  const int top_k = a.top_k.rows ? static_cast<const int*>(a.top_k.rows)[b] : static_cast<int>(a.top_k.all);
+  int round = 0;
+
+  // ---- the row comes in; its largest logit
+  float top = -INFINITY;
+  bool nan = false;
+  auto take = [&](int i, float x) {
+    x += 0.f;  // -0 becomes 0
+    values[i] = x;
+    top = fmaxf(top, x);
+    nan |= isnan(x);
+  };
+  const T* in = static_cast<const T*>(a.logits) + b * a.row_stride + r.first;
+  if (VECTORS) {
+    constexpr int E = 16 / sizeof(T);
+    struct alignas(16) Vec { T x[E]; };
+    for (int i0 = 0; i0 < r.n; i0 += THREADS * E * 4) {
+      Vec v[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int i = i0 + (k * THREADS + tid) * E;
+        if (i < r.n) v[k] = *reinterpret_cast<const Vec*>(in + i);
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int i = i0 + (k * THREADS + tid) * E;
+        if (i < r.n)
+#pragma unroll
+          for (int e = 0; e < E; ++e) take(i + e, to_float(v[k].x[e]));
+      }
+    }
+  } else {
+    for (int i0 = 0; i0 < r.n; i0 += THREADS * 8) {
+      T v[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const int i = i0 + k * THREADS + tid;
+        if (i < r.n) v[k] = in[i];
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const int i = i0 + k * THREADS + tid;
+        if (i < r.n) take(i, to_float(v[k]));
+      }
+    }
+  }
+  if (tid == 0) s.nan = 0;
+  __syncthreads();
+  if (nan) s.nan = 1;
+  top = warp_max(top);
+  if (lane == 0) s.top[warp] = top;
+  __syncthreads();
+  if (tid == 0) {
+    for (int w = 1; w < WARPS; ++w) top = fmaxf(top, s.top[w]);
+    s.note[0].low = __float_as_uint(top);
+    s.note[0].index = s.nan;
+  }
+  cluster_sync();
+  {
+    const Note* n = peer(&s.note[0], min(lane, ranks - 1));  // lane c: CTA c's
+    nan = __any_sync(0xffffffffu, n->index != 0);
+    top = warp_max(__uint_as_float(n->low));
+  }
+  ++round;
+  if (nan || top == -INFINITY) {
+    if (r.rank == 0 && tid == 0) {
+      a.tokens[b] = nan ? -2 : -1;
+      a.logprobs[b] = nan ? NAN : -INFINITY;
+    }
+    cluster_sync();  // the others may still read this CTA's note
+    return;
+  }
+  if (top == INFINITY) {  // the infinite ones share the choice
+    for (int i = tid; i < r.n; i += THREADS) values[i] = values[i] == INFINITY ? 0.f : -INFINITY;
+    top = 0.f;
+    __syncthreads();
+  }
+  const bool greedy = !(heat > 0.f);
+  r.top = top;
+  r.inverse = greedy ? 0.0 : 1.4426950408889634074 / static_cast<double>(heat);
+  r.per_bin = fminf(32.f / heat, 3e38f);
+  r.shift = min(50, 30 + __clz(a.V));  // V 2^S <= 2^62
+
+  const Filters f = {top_k > 0 && top_k < a.V ? top_k : 0x7fffffff, top_p < 1.f ? top_p : 1.f,
+                     min_p > 0.f ? fmin(static_cast<double>(min_p), 1.0) : 0.0, u > 0.f ? fminf(u, 0.99999994f) : 0.f};
+
+  // ---- the order's kept part
+  Border kept = {0u, 0x7fffffff};
+  if (greedy) {
+    kept.key = key_of(top);  // its first index is found below
+  } else {
+    u64 target = f.first, before;
+    if (f.first < 0x7fffffff) {
+      const int chosen = first_crossing<false>(r, s, kept, target, 0.f, before);
+      if (chosen >= 0) {  // (else the k-th has no weight)
+        if (draw_from_few(a, r, s, round, kept, chosen, 0, f, b)) return;
+        kept = find_border<false>(r, s, round, kept, target, chosen, before);
+      }
+    }
+    if (f.share < 1.f) {
+      target = 0;
+      const int chosen = first_crossing<true>(r, s, kept, target, f.share, before);
+      if (draw_from_few(a, r, s, round, kept, chosen, target, {0x7fffffff, 1.f, f.least, f.number}, b)) return;
+      kept = find_border<true>(r, s, round, kept, target, chosen, before);
+    }
+  }
+  auto mass_of = [&](int i) -> u64 {
+    const float x = values[i];
+    if (!within(kept, x, r.first + i)) return 0ull;
+    if (greedy) return 1ull;
+    if (f.least > 0.0 && !(power(r, x, 0) >= f.least)) return 0ull;
+    return weight_of(r, x);
+  };
+
+  // ---- the draw: masses of the warps' runs of indices, the run that u falls into, the thread, the token
+  const int run = (r.n + WARPS - 1) / WARPS, from = min(r.n, warp * run), to = min(r.n, from + run);
+  u64 mine = 0;
+  for (int i = from + lane; i < to; i += 32) mine += mass_of(i);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+  if (lane == 0) s.own[warp] = mine;
+  __syncthreads();
+  if (tid == 0) {
+    u64 sum = 0;
+    for (int w = 0; w < WARPS; ++w) sum += s.own[w];
+    s.note[round & 1].mass = sum;
+  }
+  cluster_sync();
+  const u64 theirs = lane < ranks ? peer(&s.note[round & 1], lane)->mass : 0ull, upto = warp_scan(theirs, lane);  // lane c: CTA c's
+  const u64 total = __shfl_sync(0xffffffffu, upto, 31), own = __shfl_sync(0xffffffffu, theirs, r.rank);
+  const u64 prior = __shfl_sync(0xffffffffu, upto, r.rank) - own;
+  const u64 aim = greedy ? 0 : min(share_of(f.number, total, false), total - 1);
+  if (prior <= aim && aim < prior + own) {
+    int w = 0;
+    u64 at = prior;
+    while (w < WARPS - 1 && aim >= at + s.own[w]) at += s.own[w++];
+    const int begin = min(r.n, w * run), end = min(r.n, begin + run), each = (end - begin + THREADS - 1) / THREADS;
+    const int lo = min(end, begin + tid * each), hi = min(end, lo + each);
+    u64 sum = 0, ignored;
+    for (int i = lo; i < hi; ++i) sum += mass_of(i);
+    at += block_scan(sum, s, ignored);
+    if (at <= aim && aim < at + sum) {
+      int i = lo;
+      u64 m = mass_of(i);
+      while (aim >= at + m) {
+        at += m;
+        m = mass_of(++i);
+      }
+      a.tokens[b] = r.first + i;
+      a.logprobs[b] = greedy ? 0.f : static_cast<float>(log(static_cast<double>(m) / static_cast<double>(total)));
+    }
+  }
+  cluster_sync();  // nobody leaves while its notes are read
+}
+
+template <class T, bool VECTORS>
+static int launch(const SampleArgs& a, int segment, int ranks, cudaStream_t s) {
+  static std::atomic<uint64_t> done{0};
+  auto kern = sample_kernel<T, VECTORS>;
+  if (smem_limit(done, kern, SEGMENT_MOST * 4) != cudaSuccess) return -1;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = ranks;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(a.B) * ranks);
+  cfg.blockDim = dim3(THREADS);
+  cfg.dynamicSmemBytes = segment * 4;
+  cfg.stream = s;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kern, a, segment, ranks) == cudaSuccess ? 0 : -1;
+}
+template <class T>
+static int by_type(const SampleArgs& a, cudaStream_t s) {
+  constexpr int E = 16 / sizeof(T);
+  // Short segments spread a row over SMs, long ones spare exchanges.
+  int ranks = 1;
+  while (ranks < CLUSTER_MOST && ((a.V + ranks - 1) / ranks > 16384 || (static_cast<int64_t>(a.B) * ranks * 2 <= a.sms && a.V / ranks > 4096))) ranks *= 2;
+  const int segment = ((a.V + ranks - 1) / ranks + E - 1) / E * E;
+  const bool vectors = a.V % E == 0 && a.row_stride % E == 0 && reinterpret_cast<uintptr_t>(a.logits) % 16 == 0;
+  return vectors ? launch<T, true>(a, segment, ranks, s) : launch<T, false>(a, segment, ranks, s);
+}
+
+}  // namespace sampling
+}  // namespace nt
+
+using namespace nt::sampling;
+
+int nt_sample_most() { return SEGMENT_MOST * CLUSTER_MOST; }
+
+int nt_sample_logits(const SampleArgs& a, cudaStream_t s) {
+  if (a.B == 0) return 0;
+  if (a.V < 1 || a.V > nt_sample_most() || a.B > INT32_MAX / CLUSTER_MOST) return -1;
+  if (a.type == LOGITS_BF16) return by_type<__nv_bfloat16>(a, s);
+  if (a.type == LOGITS_FP16) return by_type<__half>(a, s);
+  if (a.type == LOGITS_FP32) return by_type<float>(a, s);
+  return -1;
+}
