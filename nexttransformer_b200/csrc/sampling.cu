@@ -182,14 +182,19 @@ NT_DEVICE void add_to_bin(const Row& r, Shared& s, int bin, float x) {
   if (MASS) add_to(&s.mass[bin], weight_of(r, x));
   else atomicAdd(&s.count[bin], 1u);
 }
-// The bin in which the sum over the cluster's bins reaches the target, or -1; `before`: the sum over those before it.  A target of
+// The bin in which the sum over the cluster's bins (`alone`: this CTA's) reaches the target, or -1; `before`: the sum over those before it.  A target of
 // 0 is set to `share` of the whole first.
 template <bool MASS>
-NT_DEVICE int crossing(const Row& r, Shared& s, u64& target, float share, u64& before) {
+NT_DEVICE int crossing(const Row& r, Shared& s, u64& target, float share, u64& before, bool alone = false) {
   constexpr int PER = BINS / THREADS;
   const int tid = threadIdx.x;
   u64 sum[PER] = {}, all = 0;
-  for (int c0 = 0; c0 < r.ranks; c0 += 4) {  // four CTAs' bins are asked for at once
+  alone |= r.ranks == 1;
+  if (alone) {
+#pragma unroll
+    for (int e = 0; e < PER; ++e) sum[e] = MASS ? s.mass[tid * PER + e] : s.count[tid * PER + e];
+  }
+  for (int c0 = 0; !alone && c0 < r.ranks; c0 += 4) {  // four CTAs' bins are asked for at once
     if (MASS) {
       ulonglong2 u[4], v[4];
 #pragma unroll
@@ -241,6 +246,7 @@ template <bool MASS>
 NT_DEVICE int first_crossing(const Row& r, Shared& s, const Border& outer, u64& target, float share, u64& before) {
   clear_bins<MASS>(s);
   const bool any = outer.key == 0;
+#pragma unroll 4
   for (int i = threadIdx.x; i < r.n; i += THREADS) {
     const float x = r.x[i];
     const int bin = bin_of(r, x);
@@ -385,107 +391,142 @@ struct Filters {
   float number;    // u
 };
 
-NT_DEVICE void sort(u64* x, int n) {  // n a power of two, 64 at least; ascending
+// The entry of the list at which the sum (of weights, or of ones) over the order reaches `target`.  `chosen`, `done`: its bin, and the
+// sum before that.  A thread has EACH entries; those up to `last` count.  Entries are ordered as their numbers are.
+template <bool MASS>
+NT_DEVICE u64 border_of_few(const Row& r, Shared& s, const u64 (&entry)[EACH], const u64 (&w)[EACH], u64 last, int chosen, u64 target,
+                            u64 done) {
   const int tid = threadIdx.x;
-#pragma unroll 1
-  for (int k = 2; k <= n; k <<= 1)
-#pragma unroll 1
-    for (int j = k >> 1; j > 0; j >>= 1) {
-      for (int p = tid; p < n / 2; p += THREADS) {
-        const int i = ((p & ~(j - 1)) << 1) | (p & (j - 1));
-        const u64 u = x[i], v = x[i + j];
-        if ((u > v) == ((i & k) == 0)) {
-          x[i] = v;
-          x[i + j] = u;
-        }
-      }
-      // up to a distance of 32 a warp's pairs lie in its own 64 entries
-      if (j > 32 || (j == 1 && k >= 64)) __syncthreads();
-      else __syncwarp();
+  if (tid == 0) s.listed = 0;
+  __syncthreads();
+  int mine = 0;
+#pragma unroll
+  for (int e = 0; e < EACH; ++e)
+    if (entry[e] <= last && bin_of(r, value_of(~static_cast<uint32_t>(entry[e] >> 32))) == chosen) mine |= 1 << e;
+  uint32_t at = mine ? atomicAdd(&s.listed, __popc(mine)) : 0u;
+#pragma unroll
+  for (int e = 0; e < EACH; ++e)
+    if ((mine >> e) & 1) {
+      s.sorted[at] = entry[e];
+      s.list[at++] = MASS ? w[e] : 1ull;
     }
   __syncthreads();
+  const int m = s.listed;
+  for (int i = tid; i < m; i += THREADS) {
+    const u64 own = s.sorted[i];
+    u64 sum = done;
+#pragma unroll 4
+    for (int j = 0; j < m; ++j)
+      if (s.sorted[j] < own) sum += s.list[j];
+    if (sum < target && target <= sum + s.list[i]) s.found_own = own;
+  }
+  __syncthreads();
+  return s.found_own;
 }
 
-// Where few elements can be kept (the bins up to `chosen`): one CTA sorts them and draws.  target: the mass at which p is reached, or
-// 0 where it is yet to be taken of the first k's.  False: they are many.
-NT_DEVICE bool draw_from_few(const SampleArgs& a, const Row& r, Shared& s, int& round, const Border& outer, int chosen, u64 target,
+// Where few elements can be kept (the bins up to `chosen`, `done` before it): one CTA gathers them and draws.  MASS: target is the mass
+// at which p is reached; else it is the k of top-k, and what p is reached at follows.  False: they are many.
+template <bool MASS>
+NT_DEVICE bool draw_from_few(const SampleArgs& a, const Row& r, Shared& s, int& round, const Border& outer, int chosen, u64 target, u64 done,
                              const Filters& f, int b) {
   const int tid = threadIdx.x, lane = tid & 31;
   if (tid == 0) s.listed = 0;
   __syncthreads();
   const bool any = outer.key == 0;
-  for (int i0 = 0; i0 < r.n; i0 += THREADS) {
-    const int i = i0 + tid;
-    const float x = i < r.n ? r.x[i] : 0.f;
-    const bool mine = i < r.n && bin_of(r, x) <= chosen && (any || within(outer, x, r.first + i));
-    const unsigned who = __ballot_sync(0xffffffffu, mine);
-    if (!who) continue;
+  for (int i0 = 0; i0 < r.n; i0 += THREADS * 4) {
+    unsigned mine = 0;
+    float x[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int i = i0 + e * THREADS + tid;
+      x[e] = i < r.n ? r.x[i] : -INFINITY;
+      if (bin_of(r, x[e]) <= chosen && (any || within(outer, x[e], r.first + i))) mine |= 1u << e;  // (-inf is in the last bin)
+    }
+    if (!__any_sync(0xffffffffu, mine)) continue;
+    const uint32_t upto = warp_scan(static_cast<uint32_t>(__popc(mine)), lane);
     uint32_t at = 0;
-    if (lane == 0) at = atomicAdd(&s.listed, __popc(who));
-    at = __shfl_sync(0xffffffffu, at, 0) + __popc(who & ((1u << lane) - 1u));
-    if (mine && at < FEW) s.list[at] = (static_cast<u64>(~key_of(x)) << 32) | static_cast<uint32_t>(r.first + i);
+    if (lane == 31) at = atomicAdd(&s.listed, upto);
+    at = __shfl_sync(0xffffffffu, at, 31) + upto - __popc(mine);
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if ((mine >> e) & 1u) {
+        if (at < FEW) s.list[at] = (static_cast<u64>(~key_of(x[e])) << 32) | static_cast<uint32_t>(r.first + i0 + e * THREADS + tid);
+        ++at;
+      }
   }
   __syncthreads();
   if (tid == 0) s.note[round & 1].count = s.listed;
   cluster_sync();
-  const uint32_t counts = lane < r.ranks ? peer(&s.note[round & 1], lane)->count : 0u;
-  const int many = static_cast<int>(__reduce_add_sync(0xffffffffu, counts));
+  const uint32_t counts = lane < r.ranks ? peer(&s.note[round & 1], lane)->count : 0u, upto = warp_scan(counts, lane);
+  const int many = static_cast<int>(__shfl_sync(0xffffffffu, upto, 31));
   ++round;
   if (many > FEW) return false;
+  // a thread's entries, straight from the lists (0xff..: none)
+  u64 entry[EACH];
   if (r.rank == 0) {
-    uint32_t at = 0;
-    for (int c = 0; c < r.ranks; ++c) {
-      const uint32_t n = __shfl_sync(0xffffffffu, counts, c);
-      for (uint32_t i = tid; i < n; i += THREADS) s.sorted[at + i] = peer(s.list, c)[i];
-      at += n;
+#pragma unroll
+    for (int e = 0; e < EACH; ++e) {
+      const int at = e * THREADS + tid;
+      entry[e] = ~0ull;
+      int c = 0;
+      uint32_t before = 0;
+      for (int o = 0; o < r.ranks; ++o) {
+        const uint32_t end = __shfl_sync(0xffffffffu, upto, o);
+        if (static_cast<uint32_t>(at) >= end) {
+          c = o + 1;
+          before = end;
+        }
+      }
+      if (at < many) entry[e] = peer(s.list, c)[at - before];
     }
   }
   cluster_sync();  // the lists are read: the other CTAs are done
   if (r.rank != 0) return true;
-  int n = 64;
-  while (n < many) n <<= 1;
-  for (int i = many + tid; i < n; i += THREADS) s.sorted[i] = ~0ull;
-  __syncthreads();
-  sort(s.sorted, n);
 
-  // ---- masses in order, a thread's entries one after another; the kept ones are the first
-  u64 w[EACH], sum = 0, total;
-  uint32_t index[EACH];
+  u64 w[EACH], total, last = ~0ull - 1;
 #pragma unroll
-  for (int e = 0; e < EACH; ++e) {
-    const int at = tid * EACH + e;
-    w[e] = 0;
-    index[e] = 0;
-    if (at >= min(many, f.first)) continue;
-    const u64 v = s.sorted[at];
-    const float x = value_of(~static_cast<uint32_t>(v >> 32));
-    index[e] = static_cast<uint32_t>(v);
-    w[e] = weight_of(r, x);
-    sum += w[e];
-    if (f.least > 0.0 && !(power(r, x, 0) >= f.least)) index[e] = 0xffffffffu;
+  for (int e = 0; e < EACH; ++e) w[e] = 0;
+  if (!MASS) last = border_of_few<false>(r, s, entry, w, last, chosen, target, done);
+  u64 sum = 0;
+#pragma unroll
+  for (int e = 0; e < EACH; ++e)
+    if (entry[e] <= last) {
+      w[e] = weight_of(r, value_of(~static_cast<uint32_t>(entry[e] >> 32)));
+      sum += w[e];
+    }
+  if (MASS) {
+    last = border_of_few<true>(r, s, entry, w, last, chosen, target, done);
+  } else if (f.share < 1.f) {
+    clear_bins<true>(s);
+#pragma unroll
+    for (int e = 0; e < EACH; ++e)
+      if (w[e]) add_to(&s.mass[bin_of(r, value_of(~static_cast<uint32_t>(entry[e] >> 32)))], w[e]);
+    __syncthreads();
+    target = 0;
+    const int bin = crossing<true>(r, s, target, f.share, done, true);
+    __syncthreads();  // the bins are read
+    last = border_of_few<true>(r, s, entry, w, last, bin, target, done);
   }
-  u64 at = block_scan(sum, s, total);
-  if (target == 0) target = f.share < 1.f ? (f.share > 0.f ? max(share_of(f.share, total, true), 1ull) : 1ull) : total;
+  uint32_t index[EACH];
   sum = 0;
 #pragma unroll
   for (int e = 0; e < EACH; ++e) {
-    const u64 own = w[e];
-    if (at >= target || index[e] == 0xffffffffu) w[e] = 0;
-    at += own;
+    const float x = value_of(~static_cast<uint32_t>(entry[e] >> 32));
+    index[e] = static_cast<uint32_t>(entry[e]);
+    if (entry[e] > last || (f.least > 0.0 && !(power(r, x, 0) >= f.least))) w[e] = 0;
     sum += w[e];
   }
   block_scan(sum, s, total);
   // ---- the draw goes by index: runs of indices first, then the indices of the run
   u64 aim = min(share_of(f.number, total, false), total - 1);
   const int low_bits = max(0, 32 - __clz(r.V - 1) - 9);  // V <= 2^19: at most 1024 indices a run
-  for (int i = tid; i < THREADS; i += THREADS) s.by_index[i] = 0;
+  s.by_index[tid] = 0;
   __syncthreads();
 #pragma unroll
   for (int e = 0; e < EACH; ++e)
     if (w[e]) add_to(&s.by_index[index[e] >> low_bits], w[e]);
   __syncthreads();
-  u64 own = s.by_index[tid], ignored;
-  at = block_scan(own, s, ignored);
+  u64 own = s.by_index[tid], ignored, at = block_scan(own, s, ignored);
   if (at <= aim && aim < at + own) {
     s.found = tid;
     s.found_before = at;
@@ -510,7 +551,7 @@ NT_DEVICE bool draw_from_few(const SampleArgs& a, const Row& r, Shared& s, int& 
 }
 
 template <class T, bool VECTORS>
-__global__ void __launch_bounds__(THREADS) sample_kernel(const SampleArgs a, const int segment, const int ranks) {
+__global__ void __launch_bounds__(THREADS, 2) sample_kernel(const SampleArgs a, const int segment, const int ranks) {
   extern __shared__ __align__(16) float values[];
   __shared__ Shared s;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, b = blockIdx.x / ranks;
@@ -618,14 +659,14 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(const SampleArgs a, con
     if (f.first < 0x7fffffff) {
       const int chosen = first_crossing<false>(r, s, kept, target, 0.f, before);
       if (chosen >= 0) {  // (else the k-th has no weight)
-        if (draw_from_few(a, r, s, round, kept, chosen, 0, f, b)) return;
+        if (draw_from_few<false>(a, r, s, round, kept, chosen, target, before, f, b)) return;
         kept = find_border<false>(r, s, round, kept, target, chosen, before);
       }
     }
     if (f.share < 1.f) {
       target = 0;
       const int chosen = first_crossing<true>(r, s, kept, target, f.share, before);
-      if (draw_from_few(a, r, s, round, kept, chosen, target, {0x7fffffff, 1.f, f.least, f.number}, b)) return;
+      if (draw_from_few<true>(a, r, s, round, kept, chosen, target, before, f, b)) return;
       kept = find_border<true>(r, s, round, kept, target, chosen, before);
     }
   }
