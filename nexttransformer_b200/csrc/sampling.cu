@@ -21,8 +21,9 @@
 namespace nt {
 namespace sampling {
 
-constexpr int THREADS = 512, WARPS = THREADS / 32, BINS = 2048, CAP = 1024;
-constexpr int FEW = 2048, EACH = FEW / THREADS;  // a list that one CTA sorts; its entries a thread
+constexpr int THREADS = 512, WARPS = THREADS / 32, BINS = 2048;
+constexpr int FEW = 2048, EACH = FEW / THREADS;  // a list that one CTA takes; its entries a thread
+constexpr int CAP = FEW / 2;                     // entries of one bin that are ranked among each other
 constexpr int SEGMENT_MOST = 45056;  // logits of a CTA: 176 KB
 constexpr int CLUSTER_MOST = 8;
 using u64 = unsigned long long;
@@ -40,6 +41,10 @@ NT_DEVICE uint32_t key_of(float x) {
 
 NT_DEVICE float value_of(uint32_t key) { return __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key); }
 
+// An entry of a list: its number grows along the order.
+NT_DEVICE u64 entry_of(uint32_t key, int index) { return (static_cast<u64>(~key) << 32) | static_cast<uint32_t>(index); }
+NT_DEVICE float value_in(u64 entry) { return value_of(~static_cast<uint32_t>(entry >> 32)); }
+
 struct Border {     // kept: keys above it, and those equal to it up to its index
   uint32_t key;
   int index;
@@ -54,19 +59,10 @@ struct Shared {
   union {
     u64 mass[BINS];
     uint32_t count[BINS];
-    struct {
-      uint32_t key[CAP];
-      int index[CAP];
-      u64 weight[CAP];
-    } all;           // the border's bin, of every CTA
-    u64 sorted[FEW];  // what may be kept, of every CTA, in order
+    u64 sorted[FEW];  // entries that are ranked (and their shares)
   };
-  union {            // of this CTA
-    struct {
-      uint32_t key[CAP];
-      int index[CAP];
-    };
-    u64 list[FEW];
+  union {
+    u64 list[FEW];    // this CTA's candidates
     u64 by_index[FEW / 2];
   };
   Note note[2];
@@ -76,7 +72,6 @@ struct Shared {
   uint32_t listed, low, high;
   int found;
   u64 found_before, found_own;
-  Border border;
 };
 
 // The same address in CTA `rank` of the cluster.
@@ -99,8 +94,8 @@ struct Row {
 
 // 2^S exp((x - top) / T), rounded; |error| below 1 + 2^(S - 48)
 NT_DEVICE double power(const Row& r, float x, int shift) {
-  const double t = (static_cast<double>(x) - static_cast<double>(r.top)) * r.inverse;
-  if (!(t > -70.0)) return 0.0;
+  const double exponent = (static_cast<double>(x) - static_cast<double>(r.top)) * r.inverse;
+  const double t = fmax(exponent, -100.0);  // of -inf and NaN, too
   constexpr double MAGIC = 6755399441055744.0;  // 1.5 2^52: adding it rounds to a whole number
   const double whole = t + MAGIC, n = whole - MAGIC, z = (t - n) * 0.69314718055994530942;
   // exp(z), |z| <= 0.347, by its series: the first term left out is 7e-15 (z^12 / 12!)
@@ -116,8 +111,9 @@ NT_DEVICE double power(const Row& r, float x, int shift) {
   p = fma(p, z, 0.5);
   p = fma(p, z, 1.0);
   p = fma(p, z, 1.0);
-  const int e = __double2loint(whole) + shift;  // p 2^e; never below 2^-72, so that only the exponent's bits change
-  return __hiloint2double(__double2hiint(p) + (e << 20), __double2loint(p));
+  const int e = __double2loint(whole) + shift;  // p 2^e; never below 2^-102, so that only the exponent's bits change
+  const double v = __hiloint2double(__double2hiint(p) + (e << 20), __double2loint(p));
+  return exponent > -70.0 ? v : 0.0;
 }
 NT_DEVICE u64 weight_of(const Row& r, float x) {
   const double v = power(r, x, r.shift) + 4503599627370496.0;  // 2^52: the whole number is in the lower bits
@@ -182,68 +178,64 @@ NT_DEVICE void add_to_bin(const Row& r, Shared& s, int bin, float x) {
   if (MASS) add_to(&s.mass[bin], weight_of(r, x));
   else atomicAdd(&s.count[bin], 1u);
 }
-// The bin in which the sum over the cluster's bins (`alone`: this CTA's) reaches the target, or -1; `before`: the sum over those before it.  A target of
-// 0 is set to `share` of the whole first.
+// The bin in which the sum over the cluster's bins (`alone`: this CTA's) reaches the target, or -1; `before`: the sum over those
+// before it.  A target of 0 is set to `share` of the whole first.  Each CTA adds up its part of the bins: if all of them read
+// all bins of eight CTAs, it takes 15 us instead of 4.
 template <bool MASS>
-NT_DEVICE int crossing(const Row& r, Shared& s, u64& target, float share, u64& before, bool alone = false) {
-  constexpr int PER = BINS / THREADS;
-  const int tid = threadIdx.x;
-  u64 sum[PER] = {}, all = 0;
-  alone |= r.ranks == 1;
-  if (alone) {
+NT_DEVICE int crossing(const Row& r, Shared& s, int& round, u64& target, float share, u64& before, bool alone = false) {
+  constexpr int MOST = BINS / THREADS;
+  const int tid = threadIdx.x, lane = tid & 31, ranks = alone ? 1 : r.ranks, part = BINS / ranks, per = max(1, part / THREADS);
+  const int from = (alone ? 0 : r.rank * part) + tid * per;
+  u64 sum[MOST] = {}, all = 0;
+  if (ranks == 1) {
 #pragma unroll
-    for (int e = 0; e < PER; ++e) sum[e] = MASS ? s.mass[tid * PER + e] : s.count[tid * PER + e];
-  }
-  for (int c0 = 0; !alone && c0 < r.ranks; c0 += 4) {  // four CTAs' bins are asked for at once
-    if (MASS) {
-      ulonglong2 u[4], v[4];
+    for (int e = 0; e < MOST; ++e) sum[e] = MASS ? s.mass[from + e] : s.count[from + e];
+  } else if (tid * per < part) {
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        u[c] = v[c] = make_ulonglong2(0, 0);
-        if (c0 + c < r.ranks) {
-          const ulonglong2* m = reinterpret_cast<const ulonglong2*>(peer(s.mass, c0 + c)) + tid * 2;
-          u[c] = m[0];
-          v[c] = m[1];
+    for (int e = 0; e < MOST; ++e)
+      if (e < per) {
+        u64 v[CLUSTER_MOST];
+#pragma unroll
+        for (int c = 0; c < CLUSTER_MOST; ++c) {
+          v[c] = 0;
+          if (c < ranks) v[c] = MASS ? peer(s.mass, c)[from + e] : peer(s.count, c)[from + e];
         }
-      }
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        sum[0] += u[c].x; sum[1] += u[c].y; sum[2] += v[c].x; sum[3] += v[c].y;
+        for (int c = 0; c < CLUSTER_MOST; ++c) sum[e] += v[c];
       }
-    } else {
-      uint4 u[4];
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        u[c] = make_uint4(0, 0, 0, 0);
-        if (c0 + c < r.ranks) u[c] = reinterpret_cast<const uint4*>(peer(s.count, c0 + c))[tid];
-      }
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        sum[0] += u[c].x; sum[1] += u[c].y; sum[2] += u[c].z; sum[3] += u[c].w;
-      }
-    }
   }
 #pragma unroll
-  for (int e = 0; e < PER; ++e) all += sum[e];
+  for (int e = 0; e < MOST; ++e) all += sum[e];
   if (tid == 0) s.found = -1;
   u64 total;
   u64 at = block_scan(all, s, total);
+  if (ranks > 1) {
+    if (tid == 0) s.note[round & 1].mass = total;
+    cluster_sync();
+    const u64 upto = warp_scan(lane < ranks ? peer(&s.note[round & 1], lane)->mass : 0ull, lane);
+    if (r.rank) at += __shfl_sync(0xffffffffu, upto, r.rank - 1);
+    total = __shfl_sync(0xffffffffu, upto, 31);
+    ++round;
+  }
   if (MASS && target == 0) target = share > 0.f ? max(share_of(share, total, true), 1ull) : 1ull;
 #pragma unroll
-  for (int e = 0; e < PER; ++e) {
-    if (at < target && target <= at + sum[e]) {
-      s.found = tid * PER + e;
-      s.found_before = at;
-    }
+  for (int e = 0; e < MOST; ++e) {
+    if (at < target && target <= at + sum[e])
+      for (int c = 0; c < ranks; ++c) {
+        Shared* to = ranks > 1 ? peer(&s, c) : &s;
+        to->found = from + e;
+        to->found_before = at;
+      }
     at += sum[e];
   }
-  __syncthreads();
+  if (ranks > 1) cluster_sync();
+  else __syncthreads();
   before = s.found_before;
   return s.found;
 }
 // A histogram of the elements within `outer` by their distance from the top, and its crossing.
 template <bool MASS>
-NT_DEVICE int first_crossing(const Row& r, Shared& s, const Border& outer, u64& target, float share, u64& before) {
+NT_DEVICE int first_crossing(const Row& r, Shared& s, int& round, const Border& outer, u64& target, float share, u64& before) {
   clear_bins<MASS>(s);
   const bool any = outer.key == 0;
 #pragma unroll 4
@@ -253,7 +245,31 @@ NT_DEVICE int first_crossing(const Row& r, Shared& s, const Border& outer, u64& 
     if (bin < BINS - 1 && (any || within(outer, x, r.first + i))) add_to_bin<MASS>(r, s, bin, x);
   }
   cluster_sync();
-  return crossing<MASS>(r, s, target, share, before);
+  return crossing<MASS>(r, s, round, target, share, before);
+}
+
+// Of m entries in any order and their shares: the one at which the sum over the order reaches the target.  As many lanes as
+// there are for it add up each entry's predecessors.
+NT_DEVICE u64 ranked(const u64* entry, const u64* share, int m, u64 target, u64 done, Shared& s) {
+  const int tid = threadIdx.x;
+  int lanes = 1;
+  while (lanes < 32 && 2 * lanes * m <= THREADS) lanes *= 2;
+  const int part = tid & (lanes - 1);
+  for (int i0 = 0; i0 < m; i0 += THREADS / lanes) {
+    const int i = i0 + tid / lanes;
+    const u64 own = i < m ? entry[i] : 0ull;
+    u64 sum = 0;
+#pragma unroll 4
+    for (int j = part; j < m; j += lanes) {
+      const u64 v = share[j];
+      sum += entry[j] < own ? v : 0ull;
+    }
+    for (int o = lanes / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    sum += done;
+    if (i < m && sum < target && target <= sum + share[i]) s.found_own = own;
+  }
+  __syncthreads();
+  return s.found_own;
 }
 
 // The border of a selection: the element at which the sum (of weights, or of ones) over the order reaches `target`, which lies in
@@ -287,10 +303,7 @@ NT_DEVICE Border find_border(const Row& r, Shared& s, int& round, const Border& 
       at = __shfl_sync(0xffffffffu, at, 0) + __popc(who & ((1u << lane) - 1u));
       const uint32_t k = mine ? key_of(r.x[i]) : 0u;
       const uint32_t least = __reduce_min_sync(0xffffffffu, mine ? k : 0xffffffffu), most = __reduce_max_sync(0xffffffffu, k);
-      if (mine && at < CAP) {
-        s.key[at] = k;
-        s.index[at] = r.first + i;
-      }
+      if (mine && at < FEW) s.list[at] = entry_of(k, r.first + i);
       if (lane == 0) {
         atomicMin(&s.low, least);
         atomicMax(&s.high, most);
@@ -317,26 +330,15 @@ NT_DEVICE Border find_border(const Row& r, Shared& s, int& round, const Border& 
       for (int c = 0; c < r.ranks; ++c) {
         const uint32_t n = __shfl_sync(0xffffffffu, counts, c);
         for (uint32_t i = tid; i < n; i += THREADS) {
-          const uint32_t k = peer(s.key, c)[i];
-          s.all.key[at + i] = k;
-          s.all.index[at + i] = peer(s.index, c)[i];
-          if (MASS) s.all.weight[at + i] = weight_of(r, value_of(k));
+          const u64 v = peer(s.list, c)[i];
+          s.sorted[at + i] = v;
+          s.sorted[CAP + at + i] = MASS ? weight_of(r, value_in(v)) : 1ull;
         }
         at += n;
       }
       __syncthreads();
-      for (uint32_t i = tid; i < many; i += THREADS) {
-        const uint32_t k = s.all.key[i];
-        const int index = s.all.index[i];
-        u64 sum = done;
-        for (uint32_t j = 0; j < many; ++j) {
-          const uint32_t kj = s.all.key[j];
-          if (kj > k || (kj == k && s.all.index[j] < index)) sum += MASS ? s.all.weight[j] : 1ull;
-        }
-        if (sum < target && target <= sum + (MASS ? s.all.weight[i] : 1ull)) s.border = {k, index};
-      }
-      __syncthreads();
-      return s.border;
+      const u64 v = ranked(s.sorted, s.sorted + CAP, static_cast<int>(many), target, done, s);
+      return {~static_cast<uint32_t>(v >> 32), static_cast<int>(static_cast<uint32_t>(v))};
     }
     if (low == high) {
       // ---- equal logits: the first of them by index.  The number of those that are kept:
@@ -377,7 +379,7 @@ NT_DEVICE Border find_border(const Row& r, Shared& s, int& round, const Border& 
     }
     cluster_sync();
     u64 rest = target - done, before;  // crossing() counts from the first bin
-    const int bin = crossing<MASS>(r, s, rest, 0.f, before);
+    const int bin = crossing<MASS>(r, s, round, rest, 0.f, before);
     done += before;
     high = high - (static_cast<uint32_t>(bin) << shift);
     low = max(low, shift ? high - ((1u << shift) - 1u) : high);
@@ -402,7 +404,7 @@ NT_DEVICE u64 border_of_few(const Row& r, Shared& s, const u64 (&entry)[EACH], c
   int mine = 0;
 #pragma unroll
   for (int e = 0; e < EACH; ++e)
-    if (entry[e] <= last && bin_of(r, value_of(~static_cast<uint32_t>(entry[e] >> 32))) == chosen) mine |= 1 << e;
+    if (entry[e] <= last && bin_of(r, value_in(entry[e])) == chosen) mine |= 1 << e;
   uint32_t at = mine ? atomicAdd(&s.listed, __popc(mine)) : 0u;
 #pragma unroll
   for (int e = 0; e < EACH; ++e)
@@ -411,17 +413,7 @@ NT_DEVICE u64 border_of_few(const Row& r, Shared& s, const u64 (&entry)[EACH], c
       s.list[at++] = MASS ? w[e] : 1ull;
     }
   __syncthreads();
-  const int m = s.listed;
-  for (int i = tid; i < m; i += THREADS) {
-    const u64 own = s.sorted[i];
-    u64 sum = done;
-#pragma unroll 4
-    for (int j = 0; j < m; ++j)
-      if (s.sorted[j] < own) sum += s.list[j];
-    if (sum < target && target <= sum + s.list[i]) s.found_own = own;
-  }
-  __syncthreads();
-  return s.found_own;
+  return ranked(s.sorted, s.list, s.listed, target, done, s);
 }
 
 // Where few elements can be kept (the bins up to `chosen`, `done` before it): one CTA gathers them and draws.  MASS: target is the mass
@@ -450,7 +442,7 @@ NT_DEVICE bool draw_from_few(const SampleArgs& a, const Row& r, Shared& s, int& 
 #pragma unroll
     for (int e = 0; e < 4; ++e)
       if ((mine >> e) & 1u) {
-        if (at < FEW) s.list[at] = (static_cast<u64>(~key_of(x[e])) << 32) | static_cast<uint32_t>(r.first + i0 + e * THREADS + tid);
+        if (at < FEW) s.list[at] = entry_of(key_of(x[e]), r.first + i0 + e * THREADS + tid);
         ++at;
       }
   }
@@ -491,7 +483,7 @@ NT_DEVICE bool draw_from_few(const SampleArgs& a, const Row& r, Shared& s, int& 
 #pragma unroll
   for (int e = 0; e < EACH; ++e)
     if (entry[e] <= last) {
-      w[e] = weight_of(r, value_of(~static_cast<uint32_t>(entry[e] >> 32)));
+      w[e] = weight_of(r, value_in(entry[e]));
       sum += w[e];
     }
   if (MASS) {
@@ -500,10 +492,10 @@ NT_DEVICE bool draw_from_few(const SampleArgs& a, const Row& r, Shared& s, int& 
     clear_bins<true>(s);
 #pragma unroll
     for (int e = 0; e < EACH; ++e)
-      if (w[e]) add_to(&s.mass[bin_of(r, value_of(~static_cast<uint32_t>(entry[e] >> 32)))], w[e]);
+      if (w[e]) add_to(&s.mass[bin_of(r, value_in(entry[e]))], w[e]);
     __syncthreads();
     target = 0;
-    const int bin = crossing<true>(r, s, target, f.share, done, true);
+    const int bin = crossing<true>(r, s, round, target, f.share, done, true);
     __syncthreads();  // the bins are read
     last = border_of_few<true>(r, s, entry, w, last, bin, target, done);
   }
@@ -511,7 +503,7 @@ NT_DEVICE bool draw_from_few(const SampleArgs& a, const Row& r, Shared& s, int& 
   sum = 0;
 #pragma unroll
   for (int e = 0; e < EACH; ++e) {
-    const float x = value_of(~static_cast<uint32_t>(entry[e] >> 32));
+    const float x = value_in(entry[e]);
     index[e] = static_cast<uint32_t>(entry[e]);
     if (entry[e] > last || (f.least > 0.0 && !(power(r, x, 0) >= f.least))) w[e] = 0;
     sum += w[e];
@@ -657,7 +649,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const SampleArgs a, 
   } else {
     u64 target = f.first, before;
     if (f.first < 0x7fffffff) {
-      const int chosen = first_crossing<false>(r, s, kept, target, 0.f, before);
+      const int chosen = first_crossing<false>(r, s, round, kept, target, 0.f, before);
       if (chosen >= 0) {  // (else the k-th has no weight)
         if (draw_from_few<false>(a, r, s, round, kept, chosen, target, before, f, b)) return;
         kept = find_border<false>(r, s, round, kept, target, chosen, before);
@@ -665,7 +657,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const SampleArgs a, 
     }
     if (f.share < 1.f) {
       target = 0;
-      const int chosen = first_crossing<true>(r, s, kept, target, f.share, before);
+      const int chosen = first_crossing<true>(r, s, round, kept, target, f.share, before);
       if (draw_from_few<true>(a, r, s, round, kept, chosen, target, before, f, b)) return;
       kept = find_border<true>(r, s, round, kept, target, chosen, before);
     }
