@@ -68,6 +68,7 @@ struct Shared {
   Note note[2];
   u64 scan[WARPS + 1], own[WARPS];
   float top[WARPS];
+  double sixteenths[16];
   int nan;
   uint32_t listed, low, high;
   int found;
@@ -87,42 +88,39 @@ struct Row {
   int n, first, V;   // how many, index of the first
   int ranks, rank;
   float top;         // the row's largest
-  double inverse;    // log2(e) / T
+  double inverse;    // 16 log2(e) / T
+  const double* sixteenths;  // 2^(i / 16)
   float per_bin;     // bins a logit's distance from the top
   int shift;         // S
 };
 
-// 2^S exp((x - top) / T), rounded; |error| below 1 + 2^(S - 48)
+// 2^shift exp((x - top) / T), to 2e-13 of it; 0 from 2^(shift - 70) down.  t = (x - top) log2(e) / T is n / 16 and a rest, 2^(n mod 16 / 16)
+// stands in a table, and the rest's power is its series: with z = rest ln 2, |z| <= 0.0217, the first term left out is z^6 / 720 = 1.5e-13.
 NT_DEVICE double power(const Row& r, float x, int shift) {
-  const double exponent = (static_cast<double>(x) - static_cast<double>(r.top)) * r.inverse;
-  const double t = fmax(exponent, -100.0);  // of -inf and NaN, too
+  const double exponent = (static_cast<double>(x) - static_cast<double>(r.top)) * r.inverse;  // 16 t
+  const double t = fmax(exponent, -1600.0);  // of -inf and NaN, too
   constexpr double MAGIC = 6755399441055744.0;  // 1.5 2^52: adding it rounds to a whole number
-  const double whole = t + MAGIC, n = whole - MAGIC, z = (t - n) * 0.69314718055994530942;
-  // exp(z), |z| <= 0.347, by its series: the first term left out is 7e-15 (z^12 / 12!)
-  double p = 1.0 / 39916800.0;
-  p = fma(p, z, 1.0 / 3628800.0);
-  p = fma(p, z, 1.0 / 362880.0);
-  p = fma(p, z, 1.0 / 40320.0);
-  p = fma(p, z, 1.0 / 5040.0);
-  p = fma(p, z, 1.0 / 720.0);
-  p = fma(p, z, 1.0 / 120.0);
+  const double whole = t + MAGIC, z = (t - (whole - MAGIC)) * (0.69314718055994530942 / 16);
+  double p = 1.0 / 120.0;
   p = fma(p, z, 1.0 / 24.0);
   p = fma(p, z, 1.0 / 6.0);
   p = fma(p, z, 0.5);
   p = fma(p, z, 1.0);
   p = fma(p, z, 1.0);
-  const int e = __double2loint(whole) + shift;  // p 2^e; never below 2^-102, so that only the exponent's bits change
-  const double v = __hiloint2double(__double2hiint(p) + (e << 20), __double2loint(p));
-  return exponent > -70.0 ? v : 0.0;
+  const int n = __double2loint(whole);
+  p *= r.sixteenths[n & 15];
+  // p 2^e; never below 2^-102, so that only the exponent's bits change
+  const double v = __hiloint2double(__double2hiint(p) + (((n >> 4) + shift) << 20), __double2loint(p));
+  return exponent > -1120.0 ? v : 0.0;
 }
 NT_DEVICE u64 weight_of(const Row& r, float x) {
   const double v = power(r, x, r.shift) + 4503599627370496.0;  // 2^52: the whole number is in the lower bits
   return static_cast<u64>(__double_as_longlong(v)) & 0xfffffffffffffull;
 }
-NT_DEVICE int bin_of(const Row& r, float x) {
-  // both operations keep the order of the logits; the last bin, from 64 T on, has no weight (-inf and NaN, of inf 0, too)
-  return static_cast<int>(fminf((r.top - x) * r.per_bin, static_cast<float>(BINS - 1)));
-}
+// Bins keep the order of the logits; the last, from 64 T on, has no weight (-inf and NaN, of inf 0, go there).  Adding 2^23 rounds
+// to a whole number, which is the sum's lower bits: a conversion would take an instruction of a quarter of the rate.
+NT_DEVICE float bin_sum(const Row& r, float x) { return fminf((r.top - x) * r.per_bin, static_cast<float>(BINS - 1)) + 8388608.f; }
+NT_DEVICE int bin_of(const Row& r, float x) { return __float_as_int(bin_sum(r, x)) & (BINS - 1); }
 NT_DEVICE bool within(const Border& b, float x, int index) {
   const uint32_t k = key_of(x);
   return k > b.key || (k == b.key && index <= b.index);
@@ -179,17 +177,27 @@ NT_DEVICE void add_to_bin(const Row& r, Shared& s, int bin, float x) {
   else atomicAdd(&s.count[bin], 1u);
 }
 // The bin in which the sum over the cluster's bins (`alone`: this CTA's) reaches the target, or -1; `before`: the sum over those
-// before it.  A target of 0 is set to `share` of the whole first.  Each CTA adds up its part of the bins: if all of them read
-// all bins of eight CTAs, it takes 15 us instead of 4.
+// before it.  A target of 0 is set to `share` of the whole first.  Counts of up to four
+// CTAs are read by all of them; else each adds up its part of the bins and tells the others (all masses of eight CTAs read by all took 15 us
+// instead of 4).
 template <bool MASS>
 NT_DEVICE int crossing(const Row& r, Shared& s, int& round, u64& target, float share, u64& before, bool alone = false) {
   constexpr int MOST = BINS / THREADS;
-  const int tid = threadIdx.x, lane = tid & 31, ranks = alone ? 1 : r.ranks, part = BINS / ranks, per = max(1, part / THREADS);
-  const int from = (alone ? 0 : r.rank * part) + tid * per;
+  const int tid = threadIdx.x, lane = tid & 31, ranks = alone ? 1 : r.ranks;
+  const bool apart = ranks > 4 || (MASS && ranks > 1);
+  const int part = apart ? BINS / ranks : BINS, per = max(1, part / THREADS), from = (apart ? r.rank * part : 0) + tid * per;
   u64 sum[MOST] = {}, all = 0;
   if (ranks == 1) {
 #pragma unroll
     for (int e = 0; e < MOST; ++e) sum[e] = MASS ? s.mass[from + e] : s.count[from + e];
+  } else if (!apart) {
+    uint4 u[4];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) u[c] = c < ranks ? reinterpret_cast<const uint4*>(peer(s.count, c))[tid] : make_uint4(0, 0, 0, 0);
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      sum[0] += u[c].x; sum[1] += u[c].y; sum[2] += u[c].z; sum[3] += u[c].w;
+    }
   } else if (tid * per < part) {
 #pragma unroll
     for (int e = 0; e < MOST; ++e)
@@ -209,7 +217,7 @@ NT_DEVICE int crossing(const Row& r, Shared& s, int& round, u64& target, float s
   if (tid == 0) s.found = -1;
   u64 total;
   u64 at = block_scan(all, s, total);
-  if (ranks > 1) {
+  if (apart) {
     if (tid == 0) s.note[round & 1].mass = total;
     cluster_sync();
     const u64 upto = warp_scan(lane < ranks ? peer(&s.note[round & 1], lane)->mass : 0ull, lane);
@@ -221,14 +229,14 @@ NT_DEVICE int crossing(const Row& r, Shared& s, int& round, u64& target, float s
 #pragma unroll
   for (int e = 0; e < MOST; ++e) {
     if (at < target && target <= at + sum[e])
-      for (int c = 0; c < ranks; ++c) {
-        Shared* to = ranks > 1 ? peer(&s, c) : &s;
+      for (int c = 0; c < (apart ? ranks : 1); ++c) {
+        Shared* to = apart ? peer(&s, c) : &s;
         to->found = from + e;
         to->found_before = at;
       }
     at += sum[e];
   }
-  if (ranks > 1) cluster_sync();
+  if (apart) cluster_sync();
   else __syncthreads();
   before = s.found_before;
   return s.found;
@@ -253,7 +261,7 @@ NT_DEVICE int first_crossing(const Row& r, Shared& s, int& round, const Border& 
 NT_DEVICE u64 ranked(const u64* entry, const u64* share, int m, u64 target, u64 done, Shared& s) {
   const int tid = threadIdx.x;
   int lanes = 1;
-  while (lanes < 32 && 2 * lanes * m <= THREADS) lanes *= 2;
+  while (lanes < 32 && 2 * lanes * m <= THREADS && 32 * lanes <= m) lanes *= 2;
   const int part = tid & (lanes - 1);
   for (int i0 = 0; i0 < m; i0 += THREADS / lanes) {
     const int i = i0 + tid / lanes;
@@ -272,6 +280,33 @@ NT_DEVICE u64 ranked(const u64* entry, const u64* share, int m, u64 target, u64 
   return s.found_own;
 }
 
+// Lists the elements that `is(x, index)` names, up to FEW of them, and counts all; ends with a barrier.  A thread looks at 32 before it asks
+// for room.
+template <class Is>
+NT_DEVICE void list_elements(const Row& r, Shared& s, Is is) {
+  const int tid = threadIdx.x, lane = tid & 31;
+  if (tid == 0) s.listed = 0;
+  __syncthreads();
+  for (int i0 = 0; i0 < r.n; i0 += THREADS * 32) {
+    unsigned mine = 0;
+#pragma unroll 8
+    for (int e = 0; e < 32; ++e) {
+      const int i = i0 + e * THREADS + tid;
+      if (i < r.n && is(r.x[i], r.first + i)) mine |= 1u << e;
+    }
+    if (!__any_sync(0xffffffffu, mine)) continue;
+    const uint32_t upto = warp_scan(static_cast<uint32_t>(__popc(mine)), lane);
+    uint32_t at = 0;
+    if (lane == 31) at = atomicAdd(&s.listed, upto);
+    at = __shfl_sync(0xffffffffu, at, 31) + upto - __popc(mine);
+    for (; mine; mine &= mine - 1, ++at) {
+      const int i = i0 + (__ffs(mine) - 1) * THREADS + tid;
+      if (at < FEW) s.list[at] = entry_of(key_of(r.x[i]), r.first + i);
+    }
+  }
+  __syncthreads();
+}
+
 // The border of a selection: the element at which the sum (of weights, or of ones) over the order reaches `target`, which lies in
 // bin `chosen`, behind a sum of `done`.  Only elements within `outer` count.
 template <bool MASS>
@@ -286,27 +321,31 @@ NT_DEVICE Border find_border(const Row& r, Shared& s, int& round, const Border& 
   };
 #pragma unroll 1
   while (true) {
-    // ---- this CTA's candidates: a list, their number, and their extremes
+    // ---- this CTA's candidates: a list, their number, and, where they are many, their extremes
     if (tid == 0) {
-      s.listed = 0;
       s.low = 0xffffffffu;
       s.high = 0;
     }
-    __syncthreads();
-    for (int i0 = 0; i0 < r.n; i0 += THREADS) {
-      const int i = i0 + tid;
-      const bool mine = i < r.n && candidate(r.x[i], r.first + i);
-      const unsigned who = __ballot_sync(0xffffffffu, mine);
-      if (!who) continue;
-      uint32_t at = 0;
-      if (lane == 0) at = atomicAdd(&s.listed, __popc(who));
-      at = __shfl_sync(0xffffffffu, at, 0) + __popc(who & ((1u << lane) - 1u));
-      const uint32_t k = mine ? key_of(r.x[i]) : 0u;
-      const uint32_t least = __reduce_min_sync(0xffffffffu, mine ? k : 0xffffffffu), most = __reduce_max_sync(0xffffffffu, k);
-      if (mine && at < FEW) s.list[at] = entry_of(k, r.first + i);
+    list_elements(r, s, candidate);
+    if (s.listed > CAP) {
+      uint32_t least = 0xffffffffu, most = 0;
+      for (int i = tid; i < r.n; i += THREADS)
+        if (candidate(r.x[i], r.first + i)) {
+          const uint32_t k = key_of(r.x[i]);
+          least = min(least, k);
+          most = max(most, k);
+        }
+      least = __reduce_min_sync(0xffffffffu, least);
+      most = __reduce_max_sync(0xffffffffu, most);
       if (lane == 0) {
         atomicMin(&s.low, least);
         atomicMax(&s.high, most);
+      }
+    } else {
+      for (uint32_t i = tid; i < s.listed; i += THREADS) {
+        const uint32_t k = ~static_cast<uint32_t>(s.list[i] >> 32);
+        atomicMin(&s.low, k);
+        atomicMax(&s.high, k);
       }
     }
     __syncthreads();
@@ -422,31 +461,9 @@ template <bool MASS>
 NT_DEVICE bool draw_from_few(const SampleArgs& a, const Row& r, Shared& s, int& round, const Border& outer, int chosen, u64 target, u64 done,
                              const Filters& f, int b) {
   const int tid = threadIdx.x, lane = tid & 31;
-  if (tid == 0) s.listed = 0;
-  __syncthreads();
   const bool any = outer.key == 0;
-  for (int i0 = 0; i0 < r.n; i0 += THREADS * 4) {
-    unsigned mine = 0;
-    float x[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int i = i0 + e * THREADS + tid;
-      x[e] = i < r.n ? r.x[i] : -INFINITY;
-      if (bin_of(r, x[e]) <= chosen && (any || within(outer, x[e], r.first + i))) mine |= 1u << e;  // (-inf is in the last bin)
-    }
-    if (!__any_sync(0xffffffffu, mine)) continue;
-    const uint32_t upto = warp_scan(static_cast<uint32_t>(__popc(mine)), lane);
-    uint32_t at = 0;
-    if (lane == 31) at = atomicAdd(&s.listed, upto);
-    at = __shfl_sync(0xffffffffu, at, 31) + upto - __popc(mine);
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if ((mine >> e) & 1u) {
-        if (at < FEW) s.list[at] = entry_of(key_of(x[e]), r.first + i0 + e * THREADS + tid);
-        ++at;
-      }
-  }
-  __syncthreads();
+  const float end = static_cast<float>(chosen) + 8388608.f;
+  list_elements(r, s, [&](float x, int index) { return bin_sum(r, x) <= end && (any || within(outer, x, index)); });
   if (tid == 0) s.note[round & 1].count = s.listed;
   cluster_sync();
   const uint32_t counts = lane < r.ranks ? peer(&s.note[round & 1], lane)->count : 0u, upto = warp_scan(counts, lane);
@@ -603,6 +620,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const SampleArgs a, 
     }
   }
   if (tid == 0) s.nan = 0;
+  if (tid < 16) s.sixteenths[tid] = exp2(tid / 16.0);
   __syncthreads();
   if (nan) s.nan = 1;
   top = warp_max(top);
@@ -635,7 +653,8 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const SampleArgs a, 
   }
   const bool greedy = !(heat > 0.f);
   r.top = top;
-  r.inverse = greedy ? 0.0 : 1.4426950408889634074 / static_cast<double>(heat);
+  r.inverse = greedy ? 0.0 : 16 * 1.4426950408889634074 / static_cast<double>(heat);
+  r.sixteenths = s.sixteenths;
   r.per_bin = fminf(32.f / heat, 3e38f);
   r.shift = min(50, 30 + __clz(a.V));  // V 2^S <= 2^62
 
