@@ -24,7 +24,8 @@ namespace sampling {
 constexpr int THREADS = 512, WARPS = THREADS / 32, BINS = 2048;
 constexpr int FEW = 2048, EACH = FEW / THREADS;  // a list that one CTA takes; its entries a thread
 constexpr int CAP = FEW / 2;                     // entries of one bin that are ranked among each other
-constexpr int SEGMENT_MOST = 45056;  // logits of a CTA: 176 KB
+constexpr int SEGMENT_MOST = 16384;  // logits that a CTA holds in shared memory, 64 KB, so that two CTAs fit an SM
+constexpr int VOCABULARY_MOST = 1 << 19;
 constexpr int CLUSTER_MOST = 8;
 using u64 = unsigned long long;
 
@@ -68,7 +69,7 @@ struct Shared {
   Note note[2];
   u64 scan[WARPS + 1], own[WARPS];
   float top[WARPS];
-  double sixteenths[16];
+  double table[64];
   int nan;
   uint32_t listed, low, high;
   int found;
@@ -83,44 +84,72 @@ NT_DEVICE P* peer(P* p, int rank) {
   return reinterpret_cast<P*>(r);
 }
 
+constexpr int TABLE = 64;  // 2^(i / 64)
+
+// A CTA's part of a row: in shared memory, or read again at each pass.
+template <class T, bool HELD>
 struct Row {
-  float* x;          // this CTA's logits
+  float* held;
+  const T* in;
   int n, first, V;   // how many, index of the first
   int ranks, rank;
   float top;         // the row's largest
-  double inverse;    // 16 log2(e) / T
-  const double* sixteenths;  // 2^(i / 16)
+  float none;        // smaller ones have no weight
+  bool infinite;     // the largest are inf: they count as 0, the others as -inf
+  double factor, offset;  // 64 log2(e) / T, and -top times it
+  const double* table;
   float per_bin;     // bins a logit's distance from the top
   int shift;         // S
+
+  NT_DEVICE float operator[](int i) const {
+    if (HELD) return held[i];
+    const float x = to_float(in[i]) + 0.f;  // -0 becomes 0
+    return infinite ? (x == INFINITY ? 0.f : -INFINITY) : x;
+  }
+  // f(x, i) for the CTA's logits; several are asked for at once.
+  template <class F>
+  NT_DEVICE void each(F f) const {
+    constexpr int U = HELD ? 4 : 8;
+    for (int i0 = threadIdx.x; i0 < n; i0 += THREADS * U) {
+      float x[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) x[u] = i0 + u * THREADS < n ? (*this)[i0 + u * THREADS] : 0.f;
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (i0 + u * THREADS < n) f(x[u], i0 + u * THREADS);
+    }
+  }
 };
 
-// 2^shift exp((x - top) / T), to 2e-13 of it; 0 from 2^(shift - 70) down.  t = (x - top) log2(e) / T is n / 16 and a rest, 2^(n mod 16 / 16)
-// stands in a table, and the rest's power is its series: with z = rest ln 2, |z| <= 0.0217, the first term left out is z^6 / 720 = 1.5e-13.
-NT_DEVICE double power(const Row& r, float x, int shift) {
-  const double exponent = (static_cast<double>(x) - static_cast<double>(r.top)) * r.inverse;  // 16 t
-  const double t = fmax(exponent, -1600.0);  // of -inf and NaN, too
-  constexpr double MAGIC = 6755399441055744.0;  // 1.5 2^52: adding it rounds to a whole number
-  const double whole = t + MAGIC, z = (t - (whole - MAGIC)) * (0.69314718055994530942 / 16);
-  double p = 1.0 / 120.0;
-  p = fma(p, z, 1.0 / 24.0);
-  p = fma(p, z, 1.0 / 6.0);
-  p = fma(p, z, 0.5);
-  p = fma(p, z, 1.0);
+// 2^shift exp((x - top) / T), to 1e-13 of it; 0 from 2^(shift - 70) down.  64 (x - top) log2(e) / T is n and a rest; 2^(n mod 64 / 64) stands
+// in a table, and the rest's power is its series: with z = rest ln 2 / 64, |z| <= 0.0054, the first term left out is z^5 / 120 = 4e-14.
+template <class R>
+NT_DEVICE double power(const R& r, float x, int shift) {
+  constexpr double LN = 0.69314718055994530942 / TABLE, MAGIC = 6755399441055744.0;  // 1.5 2^52: adding it rounds to a whole number
+  const double t = fma(static_cast<double>(fmaxf(x, r.none)), r.factor, r.offset);
+  const double whole = t + MAGIC, z = t - (whole - MAGIC);
+  double p = LN * LN * LN * LN / 24;
+  p = fma(p, z, LN * LN * LN / 6);
+  p = fma(p, z, LN * LN / 2);
+  p = fma(p, z, LN);
   p = fma(p, z, 1.0);
   const int n = __double2loint(whole);
-  p *= r.sixteenths[n & 15];
+  p *= r.table[n & (TABLE - 1)];
   // p 2^e; never below 2^-102, so that only the exponent's bits change
-  const double v = __hiloint2double(__double2hiint(p) + (((n >> 4) + shift) << 20), __double2loint(p));
-  return exponent > -1120.0 ? v : 0.0;
+  const double v = __hiloint2double(__double2hiint(p) + (((n >> 6) + shift) << 20), __double2loint(p));
+  return x < r.none ? 0.0 : v;
 }
-NT_DEVICE u64 weight_of(const Row& r, float x) {
+template <class R>
+NT_DEVICE u64 weight_of(const R& r, float x) {
   const double v = power(r, x, r.shift) + 4503599627370496.0;  // 2^52: the whole number is in the lower bits
   return static_cast<u64>(__double_as_longlong(v)) & 0xfffffffffffffull;
 }
 // Bins keep the order of the logits; the last, from 64 T on, has no weight (-inf and NaN, of inf 0, go there).  Adding 2^23 rounds
 // to a whole number, which is the sum's lower bits: a conversion would take an instruction of a quarter of the rate.
-NT_DEVICE float bin_sum(const Row& r, float x) { return fminf((r.top - x) * r.per_bin, static_cast<float>(BINS - 1)) + 8388608.f; }
-NT_DEVICE int bin_of(const Row& r, float x) { return __float_as_int(bin_sum(r, x)) & (BINS - 1); }
+template <class R>
+NT_DEVICE float bin_sum(const R& r, float x) { return fminf((r.top - x) * r.per_bin, static_cast<float>(BINS - 1)) + 8388608.f; }
+template <class R>
+NT_DEVICE int bin_of(const R& r, float x) { return __float_as_int(bin_sum(r, x)) & (BINS - 1); }
 NT_DEVICE bool within(const Border& b, float x, int index) {
   const uint32_t k = key_of(x);
   return k > b.key || (k == b.key && index <= b.index);
@@ -171,8 +200,8 @@ NT_DEVICE void clear_bins(Shared& s) {
   for (int i = threadIdx.x; i < BINS * (MASS ? 8 : 4) / 16; i += THREADS) p[i] = make_uint4(0, 0, 0, 0);
   __syncthreads();
 }
-template <bool MASS>
-NT_DEVICE void add_to_bin(const Row& r, Shared& s, int bin, float x) {
+template <bool MASS, class R>
+NT_DEVICE void add_to_bin(const R& r, Shared& s, int bin, float x) {
   if (MASS) add_to(&s.mass[bin], weight_of(r, x));
   else atomicAdd(&s.count[bin], 1u);
 }
@@ -180,8 +209,8 @@ NT_DEVICE void add_to_bin(const Row& r, Shared& s, int bin, float x) {
 // before it.  A target of 0 is set to `share` of the whole first.  Counts of up to four
 // CTAs are read by all of them; else each adds up its part of the bins and tells the others (all masses of eight CTAs read by all took 15 us
 // instead of 4).
-template <bool MASS>
-NT_DEVICE int crossing(const Row& r, Shared& s, int& round, u64& target, float share, u64& before, bool alone = false) {
+template <bool MASS, class R>
+NT_DEVICE int crossing(const R& r, Shared& s, int& round, u64& target, float share, u64& before, bool alone = false) {
   constexpr int MOST = BINS / THREADS;
   const int tid = threadIdx.x, lane = tid & 31, ranks = alone ? 1 : r.ranks;
   const bool apart = ranks > 4 || (MASS && ranks > 1);
@@ -242,16 +271,14 @@ NT_DEVICE int crossing(const Row& r, Shared& s, int& round, u64& target, float s
   return s.found;
 }
 // A histogram of the elements within `outer` by their distance from the top, and its crossing.
-template <bool MASS>
-NT_DEVICE int first_crossing(const Row& r, Shared& s, int& round, const Border& outer, u64& target, float share, u64& before) {
+template <bool MASS, class R>
+NT_DEVICE int first_crossing(const R& r, Shared& s, int& round, const Border& outer, u64& target, float share, u64& before) {
   clear_bins<MASS>(s);
   const bool any = outer.key == 0;
-#pragma unroll 4
-  for (int i = threadIdx.x; i < r.n; i += THREADS) {
-    const float x = r.x[i];
+  r.each([&](float x, int i) {
     const int bin = bin_of(r, x);
     if (bin < BINS - 1 && (any || within(outer, x, r.first + i))) add_to_bin<MASS>(r, s, bin, x);
-  }
+  });
   cluster_sync();
   return crossing<MASS>(r, s, round, target, share, before);
 }
@@ -282,17 +309,26 @@ NT_DEVICE u64 ranked(const u64* entry, const u64* share, int m, u64 target, u64 
 
 // Lists the elements that `is(x, index)` names, up to FEW of them, and counts all; ends with a barrier.  A thread looks at 32 before it asks
 // for room.
-template <class Is>
-NT_DEVICE void list_elements(const Row& r, Shared& s, Is is) {
+template <class R, class Is>
+NT_DEVICE void list_elements(const R& r, Shared& s, Is is) {
   const int tid = threadIdx.x, lane = tid & 31;
   if (tid == 0) s.listed = 0;
   __syncthreads();
   for (int i0 = 0; i0 < r.n; i0 += THREADS * 32) {
     unsigned mine = 0;
-#pragma unroll 8
-    for (int e = 0; e < 32; ++e) {
-      const int i = i0 + e * THREADS + tid;
-      if (i < r.n && is(r.x[i], r.first + i)) mine |= 1u << e;
+#pragma unroll 1
+    for (int e = 0; e < 32 && i0 + e * THREADS < r.n; e += 8) {
+      float x[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const int i = i0 + (e + u) * THREADS + tid;
+        x[u] = i < r.n ? r[i] : 0.f;
+      }
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const int i = i0 + (e + u) * THREADS + tid;
+        if (i < r.n && is(x[u], r.first + i)) mine |= 1u << (e + u);
+      }
     }
     if (!__any_sync(0xffffffffu, mine)) continue;
     const uint32_t upto = warp_scan(static_cast<uint32_t>(__popc(mine)), lane);
@@ -301,7 +337,7 @@ NT_DEVICE void list_elements(const Row& r, Shared& s, Is is) {
     at = __shfl_sync(0xffffffffu, at, 31) + upto - __popc(mine);
     for (; mine; mine &= mine - 1, ++at) {
       const int i = i0 + (__ffs(mine) - 1) * THREADS + tid;
-      if (at < FEW) s.list[at] = entry_of(key_of(r.x[i]), r.first + i);
+      if (at < FEW) s.list[at] = entry_of(key_of(r[i]), r.first + i);
     }
   }
   __syncthreads();
@@ -309,8 +345,8 @@ NT_DEVICE void list_elements(const Row& r, Shared& s, Is is) {
 
 // The border of a selection: the element at which the sum (of weights, or of ones) over the order reaches `target`, which lies in
 // bin `chosen`, behind a sum of `done`.  Only elements within `outer` count.
-template <bool MASS>
-NT_DEVICE Border find_border(const Row& r, Shared& s, int& round, const Border& outer, u64 target, int chosen, u64 done) {
+template <bool MASS, class R>
+NT_DEVICE Border find_border(const R& r, Shared& s, int& round, const Border& outer, u64 target, int chosen, u64 done) {
   const int tid = threadIdx.x, lane = tid & 31;
   uint32_t low = 0, high = 0xffffffffu;  // of the candidates' keys, after the first list
   bool first = true;
@@ -329,12 +365,11 @@ NT_DEVICE Border find_border(const Row& r, Shared& s, int& round, const Border& 
     list_elements(r, s, candidate);
     if (s.listed > CAP) {
       uint32_t least = 0xffffffffu, most = 0;
-      for (int i = tid; i < r.n; i += THREADS)
-        if (candidate(r.x[i], r.first + i)) {
-          const uint32_t k = key_of(r.x[i]);
-          least = min(least, k);
-          most = max(most, k);
-        }
+      r.each([&](float x, int i) {
+        if (!candidate(x, r.first + i)) return;
+        least = min(least, key_of(x));
+        most = max(most, key_of(x));
+      });
       least = __reduce_min_sync(0xffffffffu, least);
       most = __reduce_max_sync(0xffffffffu, most);
       if (lane == 0) {
@@ -390,7 +425,7 @@ NT_DEVICE Border find_border(const Row& r, Shared& s, int& round, const Border& 
       // every warp takes a run of indices
       const int run = (r.n + WARPS - 1) / WARPS, from = (tid >> 5) * run, to = min(r.n, from + run);
       u64 mine = 0, total;
-      for (int i = from + lane; i < to; i += 32) mine += candidate(r.x[i], r.first + i) ? 1 : 0;
+      for (int i = from + lane; i < to; i += 32) mine += candidate(r[i], r.first + i) ? 1 : 0;
       u64 prior = block_scan(mine, s, total);
       prior = __shfl_sync(0xffffffffu, prior, 0);  // of the warps before
       if (tid == 0) s.note[round & 1].index = -1;
@@ -398,7 +433,7 @@ NT_DEVICE Border find_border(const Row& r, Shared& s, int& round, const Border& 
       if (need && need <= total) {
         for (int i0 = from; i0 < to; i0 += 32) {
           const int i = i0 + lane;
-          const bool is = i < to && candidate(r.x[i], r.first + i);
+          const bool is = i < to && candidate(r[i], r.first + i);
           const unsigned who = __ballot_sync(0xffffffffu, is);
           if (is && prior + __popc(who & ((2u << lane) - 1u)) == need) s.note[round & 1].index = r.first + i;
           prior += __popc(who);
@@ -412,10 +447,9 @@ NT_DEVICE Border find_border(const Row& r, Shared& s, int& round, const Border& 
     // ---- many that differ: a histogram of their keys, the largest first
     const int shift = max(0, 32 - __clz(high - low) - 11);
     clear_bins<MASS>(s);
-    for (int i = tid; i < r.n; i += THREADS) {
-      const float x = r.x[i];
+    r.each([&](float x, int i) {
       if (candidate(x, r.first + i)) add_to_bin<MASS>(r, s, (high - key_of(x)) >> shift, x);
-    }
+    });
     cluster_sync();
     u64 rest = target - done, before;  // crossing() counts from the first bin
     const int bin = crossing<MASS>(r, s, round, rest, 0.f, before);
@@ -434,8 +468,8 @@ struct Filters {
 
 // The entry of the list at which the sum (of weights, or of ones) over the order reaches `target`.  `chosen`, `done`: its bin, and the
 // sum before that.  A thread has EACH entries; those up to `last` count.  Entries are ordered as their numbers are.
-template <bool MASS>
-NT_DEVICE u64 border_of_few(const Row& r, Shared& s, const u64 (&entry)[EACH], const u64 (&w)[EACH], u64 last, int chosen, u64 target,
+template <bool MASS, class R>
+NT_DEVICE u64 border_of_few(const R& r, Shared& s, const u64 (&entry)[EACH], const u64 (&w)[EACH], u64 last, int chosen, u64 target,
                             u64 done) {
   const int tid = threadIdx.x;
   if (tid == 0) s.listed = 0;
@@ -457,8 +491,8 @@ NT_DEVICE u64 border_of_few(const Row& r, Shared& s, const u64 (&entry)[EACH], c
 
 // Where few elements can be kept (the bins up to `chosen`, `done` before it): one CTA gathers them and draws.  MASS: target is the mass
 // at which p is reached; else it is the k of top-k, and what p is reached at follows.  False: they are many.
-template <bool MASS>
-NT_DEVICE bool draw_from_few(const SampleArgs& a, const Row& r, Shared& s, int& round, const Border& outer, int chosen, u64 target, u64 done,
+template <bool MASS, class R>
+NT_DEVICE bool draw_from_few(const SampleArgs& a, const R& r, Shared& s, int& round, const Border& outer, int chosen, u64 target, u64 done,
                              const Filters& f, int b) {
   const int tid = threadIdx.x, lane = tid & 31;
   const bool any = outer.key == 0;
@@ -559,19 +593,20 @@ NT_DEVICE bool draw_from_few(const SampleArgs& a, const Row& r, Shared& s, int& 
   return true;
 }
 
-template <class T, bool VECTORS>
+template <class T, bool HELD, bool VECTORS>
 __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const SampleArgs a, const int segment, const int ranks) {
   extern __shared__ __align__(16) float values[];
   __shared__ Shared s;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, b = blockIdx.x / ranks;
   auto value = [&](const RowValue& v) { return v.rows ? static_cast<const float*>(v.rows)[b] : static_cast<float>(v.all); };
-  Row r;
-  r.x = values;
+  Row<T, HELD> r;
+  r.held = values;
   r.ranks = ranks;
   r.rank = blockIdx.x % ranks;
   r.V = a.V;
   r.first = min(r.rank * segment, a.V);
   r.n = min(segment, a.V - r.first);
+  r.in = static_cast<const T*>(a.logits) + b * a.row_stride + r.first;
   const float heat = value(a.temperature), u = a.uniform[b], top_p = value(a.top_p), min_p = value(a.min_p);
   const int top_k = a.top_k.rows ? static_cast<const int*>(a.top_k.rows)[b] : static_cast<int>(a.top_k.all);
   int round = 0;
@@ -581,11 +616,11 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const SampleArgs a, 
   bool nan = false;
   auto take = [&](int i, float x) {
     x += 0.f;  // -0 becomes 0
-    values[i] = x;
+    if (HELD) values[i] = x;
     top = fmaxf(top, x);
     nan |= isnan(x);
   };
-  const T* in = static_cast<const T*>(a.logits) + b * a.row_stride + r.first;
+  const T* in = r.in;
   if (VECTORS) {
     constexpr int E = 16 / sizeof(T);
     struct alignas(16) Vec { T x[E]; };
@@ -620,7 +655,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const SampleArgs a, 
     }
   }
   if (tid == 0) s.nan = 0;
-  if (tid < 16) s.sixteenths[tid] = exp2(tid / 16.0);
+  if (tid < TABLE) s.table[tid] = exp2(static_cast<double>(tid) / TABLE);
   __syncthreads();
   if (nan) s.nan = 1;
   top = warp_max(top);
@@ -646,15 +681,19 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const SampleArgs a, 
     cluster_sync();  // the others may still read this CTA's note
     return;
   }
-  if (top == INFINITY) {  // the infinite ones share the choice
-    for (int i = tid; i < r.n; i += THREADS) values[i] = values[i] == INFINITY ? 0.f : -INFINITY;
+  r.infinite = top == INFINITY;  // the infinite ones share the choice
+  if (r.infinite) {
+    if (HELD)
+      for (int i = tid; i < r.n; i += THREADS) values[i] = values[i] == INFINITY ? 0.f : -INFINITY;
     top = 0.f;
     __syncthreads();
   }
   const bool greedy = !(heat > 0.f);
   r.top = top;
-  r.inverse = greedy ? 0.0 : 16 * 1.4426950408889634074 / static_cast<double>(heat);
-  r.sixteenths = s.sixteenths;
+  r.factor = greedy ? 0.0 : TABLE * 1.4426950408889634074 / static_cast<double>(heat);
+  r.offset = -r.factor * static_cast<double>(top);
+  r.table = s.table;
+  r.none = fmaxf(top - 48.f * heat, -3.4028235e38f);  // 2^-69
   r.per_bin = fminf(32.f / heat, 3e38f);
   r.shift = min(50, 30 + __clz(a.V));  // V 2^S <= 2^62
 
@@ -681,9 +720,10 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const SampleArgs a, 
       kept = find_border<true>(r, s, round, kept, target, chosen, before);
     }
   }
+  const bool all = kept.key == 0;
   auto mass_of = [&](int i) -> u64 {
-    const float x = values[i];
-    if (!within(kept, x, r.first + i)) return 0ull;
+    const float x = r[i];
+    if (!all && !within(kept, x, r.first + i)) return 0ull;
     if (greedy) return 1ull;
     if (f.least > 0.0 && !(power(r, x, 0) >= f.least)) return 0ull;
     return weight_of(r, x);
@@ -730,11 +770,11 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const SampleArgs a, 
   cluster_sync();  // nobody leaves while its notes are read
 }
 
-template <class T, bool VECTORS>
+template <class T, bool HELD, bool VECTORS>
 static int launch(const SampleArgs& a, int segment, int ranks, cudaStream_t s) {
   static std::atomic<uint64_t> done{0};
-  auto kern = sample_kernel<T, VECTORS>;
-  if (smem_limit(done, kern, SEGMENT_MOST * 4) != cudaSuccess) return -1;
+  auto kern = sample_kernel<T, HELD, VECTORS>;
+  if (HELD && smem_limit(done, kern, SEGMENT_MOST * 4) != cudaSuccess) return -1;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = ranks;
@@ -742,7 +782,7 @@ static int launch(const SampleArgs& a, int segment, int ranks, cudaStream_t s) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(a.B) * ranks);
   cfg.blockDim = dim3(THREADS);
-  cfg.dynamicSmemBytes = segment * 4;
+  cfg.dynamicSmemBytes = HELD ? segment * 4 : 0;
   cfg.stream = s;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
@@ -751,12 +791,14 @@ static int launch(const SampleArgs& a, int segment, int ranks, cudaStream_t s) {
 template <class T>
 static int by_type(const SampleArgs& a, cudaStream_t s) {
   constexpr int E = 16 / sizeof(T);
-  // Short segments spread a row over SMs, long ones spare exchanges.
+  // As many CTAs as hold the row on chip; few rows are spread further.  224 x 65536, a filter or three in each row: one CTA a row
+  // (read again at each pass) 163 us, two 116, four 84, eight 120; 1 x 32768: one 25 us, two 14.9, four 13.8, eight 14.5.
   int ranks = 1;
-  while (ranks < CLUSTER_MOST && ((a.V + ranks - 1) / ranks > 16384 || (static_cast<int64_t>(a.B) * ranks * 2 <= a.sms && a.V / ranks > 4096))) ranks *= 2;
+  while (ranks < CLUSTER_MOST && ((a.V + ranks - 1) / ranks > SEGMENT_MOST || (ranks < 4 && a.B * ranks * 2ll <= 2 * a.sms && a.V / ranks > 4096))) ranks *= 2;
   const int segment = ((a.V + ranks - 1) / ranks + E - 1) / E * E;
   const bool vectors = a.V % E == 0 && a.row_stride % E == 0 && reinterpret_cast<uintptr_t>(a.logits) % 16 == 0;
-  return vectors ? launch<T, true>(a, segment, ranks, s) : launch<T, false>(a, segment, ranks, s);
+  if (segment <= SEGMENT_MOST) return vectors ? launch<T, true, true>(a, segment, ranks, s) : launch<T, true, false>(a, segment, ranks, s);
+  return vectors ? launch<T, false, true>(a, segment, ranks, s) : launch<T, false, false>(a, segment, ranks, s);
 }
 
 }  // namespace sampling
@@ -764,7 +806,7 @@ static int by_type(const SampleArgs& a, cudaStream_t s) {
 
 using namespace nt::sampling;
 
-int nt_sample_most() { return SEGMENT_MOST * CLUSTER_MOST; }
+int nt_sample_most() { return VOCABULARY_MOST; }
 
 int nt_sample_logits(const SampleArgs& a, cudaStream_t s) {
   if (a.B == 0) return 0;

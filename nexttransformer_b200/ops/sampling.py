@@ -11,7 +11,7 @@ from nexttransformer_b200.ops.paged import _inference_only
 
 def sample_logits(logits, uniform, *, temperature=1.0, top_k=None, top_p=None, min_p=None):
     """``(tokens, logprobs)``, int64 and fp32 ``[B]``, of ``logits [B, V]`` (bf16, fp16 or fp32, any row stride; on CUDA
-    up to 360448 tokens) and ``uniform [B]``, fp32 numbers in [0, 1).
+    up to 524288 tokens) and ``uniform [B]``, fp32 numbers in [0, 1).
 
     With the weights ``w = exp((x - max x) / temperature)`` and tokens ordered by falling logit, equal ones by rising
     index, a row keeps
