@@ -20,6 +20,7 @@
 #include "logits.h"
 #include "moe.h"
 #include "moe_route.h"
+#include "moe_tokens.h"
 #include "sparse_attn.h"
 #include "sparse_teacher.h"
 #include "nsa_compress.h"
@@ -1617,6 +1618,79 @@ std::vector<Tensor> sample_logits(const Tensor& logits, const Tensor& uniform, c
   return {tokens, logprobs};
 }
 
+Tensor moe_tokens(const Tensor& x, const Tensor& router, const Tensor& w_fc, const Tensor& w_proj, int64_t top_k, const OptT& bias,
+                  const OptT& shared_fc, const OptT& shared_proj) {
+  check_cuda(x, "x");
+  inference_only({&x, &router, &w_fc, &w_proj}, {&bias, &shared_fc, &shared_proj});
+  const auto type = x.scalar_type();
+  TORCH_CHECK(type == at::kBFloat16 || type == at::kHalf, "moe_tokens takes bf16 or fp16");
+  TORCH_CHECK(x.dim() == 2 && x.size(0) <= NT_MOE_TOKENS_MOST, "x must be [T, d] with at most ", NT_MOE_TOKENS_MOST, " tokens");
+  const int64_t T = x.size(0), d = x.size(1);
+  TORCH_CHECK(d >= 8 && d % 8 == 0 && d <= NT_MOE_TOKENS_WIDTH, "the width must be a multiple of 8, at most ", NT_MOE_TOKENS_WIDTH);
+  TORCH_CHECK((x.stride(1) == 1) && (T <= 1 || x.stride(0) % 8 == 0), "x must have contiguous rows on 16-byte boundaries");
+  const auto aligned = [](const Tensor& t, const char* name) {
+    TORCH_CHECK(reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0, name, " must be 16-byte aligned");
+  };
+  aligned(x, "x");
+  TORCH_CHECK(router.device() == x.device() && router.scalar_type() == at::kFloat && router.is_contiguous() && router.dim() == 2 &&
+                  router.size(1) == d && router.size(0) >= 1 && router.size(0) <= NT_MOE_TOKENS_EXPERTS,
+              "router must be contiguous fp32 [E, d] on the device of x, with 1 to ", NT_MOE_TOKENS_EXPERTS, " experts");
+  aligned(router, "router");
+  const int64_t E = router.size(0);
+  TORCH_CHECK(top_k >= 1 && top_k <= E && top_k <= NT_MOE_TOKENS_CHOICES, "top_k must lie between 1 and the experts, at most ", NT_MOE_TOKENS_CHOICES);
+  const auto weight = [&](const Tensor& t, const char* name) {
+    TORCH_CHECK(t.device() == x.device() && t.scalar_type() == type && t.is_contiguous(), name, " must be contiguous, of x's type and device");
+    aligned(t, name);
+  };
+  weight(w_fc, "w_fc");
+  weight(w_proj, "w_proj");
+  TORCH_CHECK(w_fc.dim() == 3 && w_fc.size(0) == E && w_fc.size(2) == d && w_proj.dim() == 3 && w_proj.size(0) == E && w_proj.size(1) == d &&
+                  w_proj.size(2) == w_fc.size(1),
+              "w_fc [E, F, d] and w_proj [E, d, F] expected");
+  const int64_t F = w_fc.size(1);
+  TORCH_CHECK(F >= 8 && F % 8 == 0 && F <= 65536, "the experts' width must be a multiple of 8, at most 65536");
+  MoeTokensArgs a;
+  const bool shared = shared_fc.has_value() && shared_fc->defined();
+  TORCH_CHECK(shared == (shared_proj.has_value() && shared_proj->defined()), "shared_fc and shared_proj go together");
+  if (shared) {
+    weight(*shared_fc, "shared_fc");
+    weight(*shared_proj, "shared_proj");
+    TORCH_CHECK(shared_fc->dim() == 2 && shared_fc->size(1) == d && shared_proj->dim() == 2 && shared_proj->size(0) == d &&
+                    shared_proj->size(1) == shared_fc->size(0),
+                "shared_fc [Fs, d] and shared_proj [d, Fs] expected");
+    TORCH_CHECK(shared_fc->size(0) >= 8 && shared_fc->size(0) % 8 == 0 && shared_fc->size(0) <= 1048576, "the shared expert's width must be a multiple of 8");
+    a.Fs = static_cast<int>(shared_fc->size(0));
+    a.shared_fc = shared_fc->data_ptr();
+    a.shared_proj = shared_proj->data_ptr();
+  }
+  if (bias.has_value() && bias->defined()) {
+    TORCH_CHECK(bias->device() == x.device() && bias->scalar_type() == at::kFloat && bias->is_contiguous() && bias->dim() == 1 && bias->size(0) == E,
+                "bias must be fp32 [E]");
+    a.bias = bias->data_ptr<float>();
+  }
+  a.x = x.data_ptr();
+  a.x_stride = x.stride(0);
+  a.router = router.data_ptr<float>();
+  a.w_fc = w_fc.data_ptr();
+  a.w_proj = w_proj.data_ptr();
+  a.T = static_cast<int>(T);
+  a.d = static_cast<int>(d);
+  a.F = static_cast<int>(F);
+  a.E = static_cast<int>(E);
+  a.k = static_cast<int>(top_k);
+  a.sms = num_sms(x);
+  a.fp16 = type == at::kHalf;
+  const c10::cuda::CUDAGuard guard(x.device());
+  Tensor y = fresh({T, d}, type, x);
+  if (T == 0) return y;
+  Tensor ws = fresh({static_cast<int64_t>(nt_moe_tokens_workspace(a))}, at::kByte, x);
+  a.workspace = ws.data_ptr();
+  a.y = y.data_ptr();
+  ok(nt_moe_tokens(a, stream()), "moe_tokens");
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  return y;
+}
+
 std::vector<int64_t> read_serving_errors() {
   unsigned wp = 0, wd = 0;
   const int p = nt_paged_read_error(&wp);
@@ -1706,6 +1780,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("paged_attention", &paged_attention, "attention of new tokens over a paged cache");
   m.def("delta_step", &delta_step, "recurrent gated delta rule with a carried fp32 state");
   m.def("adjust_logits", &adjust_logits, "penalties, biases and grammar mask on logits");
+  m.def("moe_tokens", &moe_tokens, "a mixture-of-experts layer for a few tokens");
   m.def("sample_logits", &sample_logits, "a token for each row: temperature, top-k, top-p, min-p");
   m.def("read_serving_errors", &read_serving_errors);
   m.def("read_comm_errors", &read_comm_errors);

@@ -6,9 +6,7 @@
 // Both are bound by memory.  What each kernel does about it, and what it measured on one B200 (copies reach 6.46 TB/s
 // there), stands beside it; times are the device's.
 #include "paged.h"
-#include "common.cuh"
-
-#include <cuda_fp16.h>
+#include "warp_mma.cuh"
 
 #include <algorithm>
 #include <type_traits>
@@ -17,33 +15,9 @@ namespace nt {
 namespace paged {
 
 constexpr float EPS = 1.1920929e-07f;  // FLT_EPSILON, as the shell's RMSNorm
-
-template <class T> struct Num;
-template <> struct Num<__nv_bfloat16> {
-  static constexpr float RAISE = 0.f;  // of probabilities, in powers of two, see the softmax
-  static NT_DEVICE float2 unpack(uint32_t v) { return unpack_bf16x2(v); }
-  static NT_DEVICE uint32_t pack(float lo, float hi) { return pack_bf16x2(lo, hi); }
-  static NT_DEVICE float one(__nv_bfloat16 v) { return __bfloat162float(v); }
-  static NT_DEVICE void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-  }
-};
-template <> struct Num<__half> {
-  static constexpr float RAISE = 7.f;
-  static NT_DEVICE float2 unpack(uint32_t v) { return __half22float2(*reinterpret_cast<__half2*>(&v)); }
-  static NT_DEVICE uint32_t pack(float lo, float hi) {
-    __half2 h = __floats2half2_rn(lo, hi);
-    return *reinterpret_cast<uint32_t*>(&h);
-  }
-  static NT_DEVICE float one(__half v) { return __half2float(v); }
-  static NT_DEVICE void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-  }
-};
+// By how many powers of two probabilities are raised, see the softmax
+template <class T> constexpr float RAISE_OF = 0.f;
+template <> constexpr float RAISE_OF<__half> = 7.f;
 
 // ------------------------------------------------------------------------------------ append
 // D / 8 lanes hold one head of one token; lane j has channels 4 j to 4 j + 3 of each half, so that it holds
@@ -66,20 +40,6 @@ NT_DEVICE void unpack4(uint2 u, float2 (&x)[2]) {
 template <class T>
 NT_DEVICE uint2 pack4(const float2 (&x)[2]) {
   return make_uint2(Num<T>::pack(x[0].x, x[0].y), Num<T>::pack(x[1].x, x[1].y));
-}
-// x / n for 0 <= x < 2^31 and 0 < n: the float quotient is at most a few units off
-NT_DEVICE int quotient(int x, int n) {
-  int q = static_cast<int>(__fdividef(static_cast<float>(x), static_cast<float>(n)));
-  int rest = x - q * n;
-  while (rest < 0) {
-    --q;
-    rest += n;
-  }
-  while (rest >= n) {
-    ++q;
-    rest -= n;
-  }
-  return q;
 }
 template <class T, int D, int PER>
 __global__ void __launch_bounds__(256, 4) append_kernel(const PagedAppendArgs a, const int turning) {
@@ -359,26 +319,6 @@ NT_DEVICE Item get_item(const PagedAttnArgs& a, const Geometry& g, int id, int2 
   return it;
 }
 
-NT_DEVICE void cp_async16(uint32_t dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-}
-NT_DEVICE void cp_async16_or_zero(uint32_t dst, const void* src, bool valid) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
-}
-NT_DEVICE void cp_async4_or_zero(uint32_t dst, const void* src, bool valid) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(valid ? 4 : 0) : "memory");
-}
-NT_DEVICE void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-NT_DEVICE void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-NT_DEVICE void ldsm4(uint32_t (&r)[4], uint32_t addr) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
-}
-NT_DEVICE void ldsm4t(uint32_t (&r)[4], uint32_t addr) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
-}
 // What a line's chunk numbers are turned by, so that eight lines' equal chunks lie in different banks.
 template <int LINE>
 NT_DEVICE int turned(int row) { return LINE == 64 ? (row >> 1) & 3 : row & 7; }
@@ -391,11 +331,6 @@ NT_DEVICE uint32_t widen(uint16_t v) {
 NT_DEVICE uint32_t widen_low(uint32_t v) { return widen(static_cast<uint16_t>(v)); }
 NT_DEVICE uint32_t widen_high(uint32_t v) { return widen(static_cast<uint16_t>(v >> 16)); }
 NT_DEVICE float power_of_two(int e) { return __int_as_float((e + 127) << 23); }  // -126 <= e <= 127
-NT_DEVICE uint32_t transpose8x8(uint32_t v) {
-  uint32_t r;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
-  return r;
-}
 NT_DEVICE float exp2_fast(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -863,7 +798,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
         // The reference m follows the maximum only when a score passes it by more than 2^LAZY, so that most tiles
         // need neither a reduction over the lanes nor a rescaling; probabilities stay below 2^(RAISE + LAZY), inside the
         // types' limits, and sums and pieces are relative to m all the same.
-        constexpr float RAISE = Num<M>::RAISE;
+        constexpr float RAISE = RAISE_OF<M>;
         bool passed = false;
 #pragma unroll
         for (int nq = 0; nq < NQ; ++nq)

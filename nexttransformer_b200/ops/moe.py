@@ -159,3 +159,52 @@ def grouped_experts_state(x, choice, w, moe, pl=None):
     pl = pl or plan(choice, moe._w_fc.shape[0])
     return _GroupedExperts.apply(x, w, moe._w_fc, moe._w_proj, pl["row_of"], pl["src_of"], pl["grp_m"], pl["grp_k"],
                                  moe)
+
+
+# ------------------------------------------------------------------------------------- a few tokens (decoding)
+TOKENS_MOST = 64
+
+
+def moe_tokens(x, router, w_fc, w_proj, top_k, *, bias=None, shared_fc=None, shared_proj=None):
+    """The whole layer for ``x [T, d]``, up to 64 tokens (bf16 or fp16; on the CPU any float type and any T): ``[T, d]``.
+
+    Each token goes to the ``top_k`` experts with the largest ``softmax(router x) + bias`` (``router [E, d]`` and ``bias [E]``
+    fp32; ties to the lower expert), with the chosen probabilities, without the bias, normalised to a sum of 1.  Experts are
+    ``w_proj[e] relu(w_fc[e] x)^2`` with ``w_fc [E, F, d]`` and ``w_proj [E, d, F]`` in the type of x; the shared expert
+    ``shared_fc [Fs, d]``, ``shared_proj [d, Fs]`` is added for every token.  Widths are multiples of 8; d up to 8192, E up to 512,
+    top_k up to 16.  Logits and sums are fp32; a hidden value, times its share, is rounded to the type of x once (fp16: as 2^-6
+    of it, so it may reach 4e6).  A token with a NaN gives NaN and leaves the others alone.
+
+    Only the chosen experts' weights are read, each once (``csrc/moe_tokens.cu``).  It has no backward: training takes
+    ``fused_route`` and ``grouped_experts``.
+    """
+    if x.is_cuda:
+        return ext().moe_tokens(x, router, w_fc, w_proj, top_k, bias, shared_fc, shared_proj)
+    from nexttransformer_b200.ops.paged import _inference_only
+    _inference_only(x, router, w_fc, w_proj, bias, shared_fc, shared_proj)
+    return _tokens_plain(x, router, w_fc, w_proj, top_k, bias, shared_fc, shared_proj)
+
+
+def _tokens_plain(x, router, w_fc, w_proj, top_k, bias, shared_fc, shared_proj):
+    if x.dim() != 2 or router.dim() != 2 or router.shape[1] != x.shape[1]:
+        raise RuntimeError("x [T, d] and router [E, d] expected")
+    E, d = router.shape
+    if w_fc.dim() != 3 or w_fc.shape[0] != E or w_fc.shape[2] != d or w_proj.shape != (E, d, w_fc.shape[1]):
+        raise RuntimeError("w_fc [E, F, d] and w_proj [E, d, F] expected")
+    if not 1 <= top_k <= E:
+        raise RuntimeError("top_k must lie between 1 and the experts")
+    if (shared_fc is None) != (shared_proj is None):
+        raise RuntimeError("shared_fc and shared_proj go together")
+    p = torch.softmax(x.float() @ router.float().T, -1)
+    score = (p if bias is None else p + bias).nan_to_num(-3e38)
+    choice = torch.sort(score, dim=-1, descending=True, stable=True).indices[:, :top_k]
+    share = p.gather(1, choice)
+    share = share / share.sum(-1, keepdim=True)
+
+    def expert(rows, fc, proj):
+        return torch.relu(rows.float() @ fc.float().T).square() @ proj.float().T
+    y = expert(x, shared_fc, shared_proj) if shared_fc is not None else torch.zeros(x.shape)
+    for e in choice.unique().tolist():
+        rows, slot = (choice == e).nonzero(as_tuple=True)
+        y[rows] += share[rows, slot, None] * expert(x[rows], w_fc[e], w_proj[e])
+    return y.to(x.dtype)
