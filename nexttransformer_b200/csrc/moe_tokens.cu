@@ -22,7 +22,7 @@ namespace moe_tokens {
 
 constexpr int ROUTE_WARPS = 8, ROUTE_THREADS = ROUTE_WARPS * 32;
 constexpr int WARPS = 4, THREADS = WARPS * 32;
-constexpr int STAGE = 2048, STAGES = 12, RING = STAGE * STAGES;  // 24 KB a warp; two CTAs an SM
+constexpr int STAGE = 2048, STAGES = 10, RING = STAGE * STAGES;  // 20 KB a warp; two CTAs an SM
 constexpr int SMEM = WARPS * RING;
 constexpr int MOST = NT_MOE_TOKENS_MOST, EXPERTS = NT_MOE_TOKENS_EXPERTS, CHOICES = NT_MOE_TOKENS_CHOICES;
 // Hidden values are held in the weights' type.  fp16 ends at 65504, which a square passes where its root is 256: they
@@ -34,7 +34,7 @@ struct Workspace {
   int* choice;    // [T, k]
   float* share;   // [T, E], set where chosen
   uint2* x;       // [ceil(d / 16), blocks of 8 tokens, 32]: a lane's part of a 16 x 8 operand
-  uint2* h;       // [pairs of an expert and a block of 8 of its tokens, ceil(F / 16), 32]
+  uint2* h;       // [pairs of an expert and a block of 8 of its tokens, ceil(F / 16), 2, 32]
   int pairs;      // of routed experts; the shared expert's blocks, of ceil(Fs / 16) each, come behind them
 };
 static int blocks_of(int n, int by) { return (n + by - 1) / by; }
@@ -51,7 +51,7 @@ static size_t layout(const MoeTokensArgs& a, Workspace& w) {
   w.choice = reinterpret_cast<int*>(take(static_cast<size_t>(a.T) * a.k * 4));
   w.share = reinterpret_cast<float*>(take(static_cast<size_t>(a.T) * a.E * 4));
   w.x = reinterpret_cast<uint2*>(take(static_cast<size_t>(blocks_of(a.d, 16)) * nb * 256));
-  w.h = reinterpret_cast<uint2*>(take(static_cast<size_t>(w.pairs) * blocks_of(a.F, 16) * 256 + static_cast<size_t>(nb) * blocks_of(a.Fs, 16) * 256));
+  w.h = reinterpret_cast<uint2*>(take((static_cast<size_t>(w.pairs) * blocks_of(a.F, 16) + static_cast<size_t>(nb) * blocks_of(a.Fs, 16)) * 512));
   return at;
 }
 
@@ -59,7 +59,7 @@ NT_DEVICE void dependents_may_start() { asm volatile("griddepcontrol.launch_depe
 NT_DEVICE void wait_for_predecessor() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 // ------------------------------------------------------------------------------------ route
-template <class T>
+template <class T, int PER>  // experts a lane
 __global__ void __launch_bounds__(ROUTE_THREADS) route_kernel(const MoeTokensArgs a, const Workspace w, const int ranks) {
   extern __shared__ __align__(16) float x[];
   __shared__ float logits[EXPERTS];
@@ -100,7 +100,6 @@ __global__ void __launch_bounds__(ROUTE_THREADS) route_kernel(const MoeTokensArg
   }
   cluster_sync();
   if (rank != 0 || warp != 0) return;
-  constexpr int PER = EXPERTS / 32;
   float p[PER], score[PER], top = -INFINITY, sum = 0.f;
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
@@ -135,22 +134,17 @@ __global__ void __launch_bounds__(ROUTE_THREADS) route_kernel(const MoeTokensArg
         its = p[i];
         at = lane + 32 * i;
       }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      const float other = __shfl_xor_sync(0xffffffffu, best, o), theirs = __shfl_xor_sync(0xffffffffu, its, o);
-      const int where = __shfl_xor_sync(0xffffffffu, at, o);
-      if (other > best || (other == best && where < at)) {
-        best = other;
-        its = theirs;
-        at = where;
-      }
-    }
+    // the largest as a whole number in the order of the floats, then the lowest expert that has it
+    const uint32_t u = __float_as_uint(best + 0.f), key = u ^ (static_cast<uint32_t>(static_cast<int>(u) >> 31) | 0x80000000u);
+    const uint32_t most = __reduce_max_sync(0xffffffffu, key);
+    const int winner = __reduce_min_sync(0xffffffffu, key == most ? at : 0x7fffffff);
+    const float winners = __shfl_sync(0xffffffffu, its, winner & 31);
 #pragma unroll
     for (int i = 0; i < PER; ++i)
-      if (lane + 32 * i == at) score[i] = -INFINITY;
+      if (lane + 32 * i == winner) score[i] = -INFINITY;
     if (lane == j) {
-      chosen = at;
-      chosen_p = its;
+      chosen = winner;
+      chosen_p = winners;
     }
   }
   const float all = warp_sum(lane < a.k ? chosen_p : 0.f);
@@ -161,53 +155,58 @@ __global__ void __launch_bounds__(ROUTE_THREADS) route_kernel(const MoeTokensArg
 }
 
 // ------------------------------------------------------------------------------------ the experts
-// Who wants which expert, from the choices: one bit a token, the wanted experts in order, and their first block of 8 tokens.
+// What the products run over: entries of an expert and up to 16 of its tokens, experts in order and the shared one (E) last.
+constexpr int ENTRIES = EXPERTS + MOST * CHOICES / 16 + MOST / 16;
 struct Lists {
-  unsigned long long mask[EXPERTS + 1];  // [E]: the shared expert's, all tokens
-  uint16_t expert[EXPERTS + 1];          // wanted ones; the shared expert (E) comes last
-  uint16_t block[EXPERTS + 1];           // their first block
-  int wanted;
+  unsigned long long mask[EXPERTS + 1];  // an expert's tokens; [E]: the shared expert's, all
+  uint16_t expert[ENTRIES], block[ENTRIES];  // an entry's expert, and its first block of 8 tokens in h
+  uint8_t first[ENTRIES];                // the first of its tokens, counted among the expert's
+  int routed, entries;
 };
 NT_DEVICE void make_lists(const MoeTokensArgs& a, const Workspace& w, Lists& l) {
   const int tid = threadIdx.x, lane = tid & 31;
   for (int e = tid; e <= a.E; e += THREADS) l.mask[e] = 0;
   __syncthreads();
-  for (int i = tid; i < a.T * a.k; i += THREADS) atomicOr(&l.mask[__ldcg(w.choice + i)], 1ull << (i / a.k));
+  for (int i = tid; i < a.T * a.k; i += THREADS) atomicOr(&l.mask[__ldcg(w.choice + i)], 1ull << quotient(i, a.k));
   __syncthreads();
   if (tid < 32) {
     int n = 0, blocks = 0;
     for (int e0 = 0; e0 < a.E; e0 += 32) {
-      const int e = e0 + lane;
-      const int own = e < a.E ? (__popcll(l.mask[e]) + 7) >> 3 : 0;
-      const unsigned who = __ballot_sync(0xffffffffu, own > 0);
+      const int e = e0 + lane, tokens = e < a.E ? __popcll(l.mask[e]) : 0;
+      const int own = ((tokens + 15) >> 4) | (((tokens + 7) >> 3) << 16);  // entries, blocks
       int upto = own;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const int v = __shfl_up_sync(0xffffffffu, upto, o);
         if (lane >= o) upto += v;
       }
-      if (own) {
-        const int at = n + __popc(who & ((1u << lane) - 1u));
+      for (int i = 0; i < (own & 0xffff); ++i) {
+        const int at = n + ((upto - own) & 0xffff) + i;
         l.expert[at] = static_cast<uint16_t>(e);
-        l.block[at] = static_cast<uint16_t>(blocks + upto - own);
+        l.block[at] = static_cast<uint16_t>(blocks + ((upto - own) >> 16) + 2 * i);
+        l.first[at] = static_cast<uint8_t>(16 * i);
       }
-      n += __popc(who);
-      blocks += __shfl_sync(0xffffffffu, upto, 31);
+      const int all = __shfl_sync(0xffffffffu, upto, 31);
+      n += all & 0xffff;
+      blocks += all >> 16;
+    }
+    const int own = a.Fs ? (a.T + 15) >> 4 : 0;
+    if (lane < own) {
+      l.expert[n + lane] = static_cast<uint16_t>(a.E);
+      l.block[n + lane] = static_cast<uint16_t>(2 * lane);
+      l.first[n + lane] = static_cast<uint8_t>(16 * lane);
     }
     if (lane == 0) {
-      if (a.Fs) {
-        l.mask[a.E] = a.T == 64 ? ~0ull : (1ull << a.T) - 1;
-        l.expert[n] = static_cast<uint16_t>(a.E);
-        l.block[n] = 0;
-        ++n;
-      }
-      l.wanted = n;
+      l.mask[a.E] = a.T == 64 ? ~0ull : (1ull << a.T) - 1;
+      l.routed = n;
+      l.entries = n + own;
     }
   }
   __syncthreads();
 }
 // The n-th token (from 0) of a mask, or -1.
 NT_DEVICE int nth_token(unsigned long long m, int n) {
+  if ((m & (m + 1)) == 0) return n < __popcll(m) ? n : -1;  // all of the first
   for (int i = 0; i < n && m; ++i) m &= m - 1;
   return m ? __ffsll(static_cast<long long>(m)) - 1 : -1;
 }
@@ -249,6 +248,106 @@ NT_DEVICE void copy_stage(Ring& r, const char* p, int64_t stride, int rows, bool
   if (++r.stage_in == STAGES) r.stage_in = 0;
 }
 
+// A row tile of an entry: what a warp goes through, a stage of 64 inner elements after the other.
+struct Piece {
+  int entry, expert, tile;
+  int inner, rows;    // elements of a weight row; rows of the tile (16, or fewer at the end)
+  int stage, stages;  // the next one; the first behind the piece
+};
+
+// Goes through a warp's pieces: weights come `STAGES - 1` stages ahead, the other operand one.
+//   first(piece) / next(piece) set a piece and say whether there is one (the copies, the operand and the products each go through them);
+//   base(piece): the tile's first weight; operand(piece, pointers): this lane's part of the 16 x 8 tiles of stage 0 of each block of
+//   8 tokens (null: none), `step` apart from tile to tile of 16; ready(): what has to be waited for before the operand is read;
+//   done(piece, sums): a piece's products are complete.
+template <class T, int NB, class First, class Next, class Base, class Operand, class Ready, class Done>
+NT_DEVICE void stream(const MoeTokensArgs& a, const void* smem, First first, Next next, Base base, Operand operand, Ready ready, Done done) {
+  Ring r = make_ring(smem);
+  const int lane = threadIdx.x & 31, row = lane >> 3, chunk = lane & 7;
+  Piece f, o, c;  // where the copies, the operand and the products stand
+  bool f_more = first(f);
+  const char* f_at = nullptr;
+  auto enter = [&]() {
+    if (f_more) f_at = reinterpret_cast<const char*>(static_cast<const T*>(base(f)) + static_cast<int64_t>(row) * f.inner + f.stage * 64 + chunk * 8);
+  };
+  enter();
+  auto fetch = [&]() {
+    if (f_more) {
+      copy_stage(r, f_at, static_cast<int64_t>(f.inner) * sizeof(T), f.rows, f.stage * 64 + chunk * 8 < f.inner, a.x);
+      f_at += 128;
+      if (++f.stage == f.stages) {
+        f_more = next(f);
+        enter();
+      }
+    }
+    cp_commit();
+  };
+#pragma unroll 1
+  for (int i = 0; i < STAGES - 1; ++i) fetch();
+  ready();
+
+  bool o_more = first(o), c_more = first(c);
+  const uint2* at[NB];
+  int64_t step = 0;
+  int tiles = 0;  // of 16 inner elements
+  auto point = [&]() {
+    if (o_more) {
+      step = operand(o, at);
+      tiles = (o.inner + 15) >> 4;
+    }
+  };
+  uint2 ahead[4][NB];
+  auto load = [&]() {
+    if (!o_more) return;
+#pragma unroll
+    for (int s = 0; s < 4; ++s)
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) {
+        const int g = o.stage * 4 + s;
+        ahead[s][nb] = make_uint2(0u, 0u);
+        if (at[nb] && g < tiles) ahead[s][nb] = __ldcg(at[nb] + g * step);
+      }
+    if (++o.stage == o.stages) {
+      o_more = next(o);
+      point();
+    }
+  };
+  point();
+  load();
+  float acc[NB][4] = {};
+#pragma unroll 1
+  while (c_more) {
+    uint2 b[4][NB];
+#pragma unroll
+    for (int s = 0; s < 4; ++s)
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) b[s][nb] = ahead[s][nb];
+    load();
+    cp_wait<STAGES - 2>();
+    __syncwarp();  // this stage has landed for every lane, and the stage before it is read by none
+    const uint32_t from = r.base + r.stage_out * STAGE;
+    if (++r.stage_out == STAGES) r.stage_out = 0;
+    uint32_t w[4][4];
+#pragma unroll
+    for (int s = 0; s < 4; ++s) ldsm4(w[s], from + r.at[s]);
+    fetch();
+#pragma unroll
+    for (int s = 0; s < 4; ++s)
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) Num<T>::mma(acc[nb], w[s], b[s][nb].x, b[s][nb].y);
+    if (++c.stage == c.stages) {
+      done(c, acc);
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[nb][e] = 0.f;
+      c_more = next(c);
+    }
+  }
+  cp_wait<0>();
+}
+
+// NB blocks of 8 tokens an entry: 1 where there are no more than 8 tokens, else 2.
 template <class T, int NB>
 __global__ void __launch_bounds__(THREADS, 2) fc_kernel(const MoeTokensArgs a, const Workspace w) {
   extern __shared__ __align__(128) uint8_t smem[];
@@ -257,284 +356,164 @@ __global__ void __launch_bounds__(THREADS, 2) fc_kernel(const MoeTokensArgs a, c
   wait_for_predecessor();
   dependents_may_start();
   make_lists(a, w, l);
-  const int tiles = (a.F + 15) / 16, shared_tiles = (a.Fs + 15) / 16, stages = (a.d + 63) / 64, groups = (a.d + 15) / 16, nb_x = (a.T + 7) / 8;
-  const int routed = l.wanted - (a.Fs ? 1 : 0), items = routed * tiles + shared_tiles;
-  const int first = warp * gridDim.x + blockIdx.x, step = gridDim.x * WARPS;
-  if (first >= items) return;
-  Ring r = make_ring(smem);
-  const int row = lane >> 3, chunk = lane & 7, width = a.d;
-
-  struct Item {
-    int e, at, tile, hidden;  // expert, its place in the list, row tile, rows in all
+  const int tiles = (a.F + 15) / 16, shared_tiles = (a.Fs + 15) / 16, nb_x = (a.T + 7) / 8;
+  const int routed = l.routed * tiles, items = routed + (l.entries - l.routed) * shared_tiles, by = gridDim.x * WARPS;
+  // (the first items go to different SMs)
+  auto set = [&](Piece& p, int item) {
+    if (item >= items) return false;
+    const bool shared = item >= routed;
+    const int i = shared ? item - routed : item, per = shared ? shared_tiles : tiles, n = quotient(i, per);
+    p.entry = (shared ? l.routed : 0) + n;
+    p.tile = i - n * per;
+    p.expert = l.expert[p.entry];
+    p.inner = a.d;
+    p.rows = min(16, (shared ? a.Fs : a.F) - p.tile * 16);
+    p.stage = 0;
+    p.stages = (a.d + 63) / 64;
+    return true;
   };
-  auto item_of = [&](int i) {
-    Item it;
-    if (i < routed * tiles) {
-      it.at = quotient(i, tiles);
-      it.tile = i - it.at * tiles;
-      it.hidden = a.F;
-    } else {
-      it.at = routed;
-      it.tile = i - routed * tiles;
-      it.hidden = a.Fs;
-    }
-    it.e = l.expert[it.at];
-    return it;
+  auto item_at = [&](const Piece& p) {
+    return p.entry >= l.routed ? routed + (p.entry - l.routed) * shared_tiles + p.tile : p.entry * tiles + p.tile;
   };
-  // ---- the copies' place
-  int f_item = first, f_stage = 0, f_rows = 0;
-  const char* f_at = nullptr;
-  auto enter = [&]() {
-    const Item it = item_of(f_item);
-    const T* base = it.e == a.E ? static_cast<const T*>(a.shared_fc) : static_cast<const T*>(a.w_fc) + static_cast<int64_t>(it.e) * a.F * a.d;
-    f_at = reinterpret_cast<const char*>(base + (static_cast<int64_t>(it.tile) * 16 + row) * a.d + chunk * 8);
-    f_rows = min(16, it.hidden - it.tile * 16);
-  };
-  enter();
-  auto fetch = [&]() {
-    if (f_item < items) {
-      copy_stage(r, f_at, static_cast<int64_t>(a.d) * sizeof(T), f_rows, f_stage * 64 + chunk * 8 < width, a.x);
-      f_at += 128;
-      if (++f_stage == stages) {
-        f_stage = 0;
-        f_item += step;
-        if (f_item < items) enter();
-      }
-    }
-    cp_commit();
-  };
-#pragma unroll 1
-  for (int i = 0; i < STAGES - 1; ++i) fetch();
-
-#pragma unroll 1
-  for (int item = first; item < items; item += step) {
-    const Item it = item_of(item);
-    const unsigned long long mask = l.mask[it.e];
-    const int blocks = (__popcll(mask) + 7) >> 3;  // of 8 of the expert's tokens
-    const uint2* xs[NB];
-#pragma unroll
-    for (int nb = 0; nb < NB; ++nb) {
-      const int t = nb < blocks ? max(0, nth_token(mask, nb * 8 + (lane >> 2))) : 0;
-      xs[nb] = w.x + (t >> 3) * 32 + (t & 7) * 4 + (lane & 3);
-    }
-    float acc[NB][4];
-#pragma unroll
-    for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) acc[nb][e] = 0.f;
-#pragma unroll 1
-    for (int st = 0; st < stages; ++st) {
-      uint2 b[4][NB];
-#pragma unroll
-      for (int s = 0; s < 4; ++s) {
-        const int g = st * 4 + s;
+  stream<T, NB>(
+      a, smem, [&](Piece& p) { return set(p, warp * gridDim.x + blockIdx.x); }, [&](Piece& p) { return set(p, item_at(p) + by); },
+      [&](const Piece& p) -> const void* {
+        const T* e = p.expert == a.E ? static_cast<const T*>(a.shared_fc) : static_cast<const T*>(a.w_fc) + static_cast<int64_t>(p.expert) * a.F * a.d;
+        return e + static_cast<int64_t>(p.tile) * 16 * a.d;
+      },
+      [&](const Piece& p, const uint2* (&at)[NB]) {
+        const unsigned long long mask = l.mask[p.expert];
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
-          b[s][nb] = make_uint2(0u, 0u);
-          if (nb < blocks && g < groups) b[s][nb] = xs[nb][static_cast<int64_t>(g) * nb_x * 32];
+          const int t = nth_token(mask, l.first[p.entry] + nb * 8 + (lane >> 2));
+          at[nb] = t < 0 ? nullptr : w.x + (t >> 3) * 32 + (t & 7) * 4 + (lane & 3);
         }
-      }
-      cp_wait<STAGES - 2>();
-      __syncwarp();  // this stage has landed for every lane, and the stage before it is read by none
-      const uint32_t base = r.base + r.stage_out * STAGE;
-      if (++r.stage_out == STAGES) r.stage_out = 0;
-      uint32_t wf[4][4];
+        return static_cast<int64_t>(nb_x) * 32;
+      },
+      [] {},
+      [&](const Piece& p, const float (&acc)[NB][4]) {
+        // h, in the order in which it is an operand: rows of the tile become the products' inner dimension.  It is held as two
+        // numbers of its type, so that nothing but the output is rounded.
+        const bool shared = p.expert == a.E;
+        const unsigned long long mask = l.mask[p.expert];
+        const int left = __popcll(mask) - l.first[p.entry], inner = shared ? shared_tiles : tiles;
+        uint2* h = w.h + (shared ? static_cast<int64_t>(w.pairs) * tiles * 2 : 0ll) * 32;
 #pragma unroll
-      for (int s = 0; s < 4; ++s) ldsm4(wf[s], base + r.at[s]);
-      fetch();
+        for (int nb = 0; nb < NB; ++nb) {
+          if (nb * 8 >= left) break;
+          float v[4];
 #pragma unroll
-      for (int s = 0; s < 4; ++s)
+          for (int e = 0; e < 2; ++e) {
+            const int t = nth_token(mask, l.first[p.entry] + nb * 8 + (lane & 3) * 2 + e);
+            const float c = t < 0 ? 0.f : shared ? LOWER<T> : LOWER<T> * __ldcg(w.share + static_cast<int64_t>(t) * a.E + p.expert);
 #pragma unroll
-        for (int nb = 0; nb < NB; ++nb)
-          if (nb < blocks) Num<T>::mma(acc[nb], wf[s], b[s][nb].x, b[s][nb].y);
-    }
-    // ---- h, in the order in which it is an operand: rows of the tile become the products' inner dimension
-    const int inner = it.e == a.E ? shared_tiles : tiles;
-    uint2* h = w.h + (it.e == a.E ? static_cast<int64_t>(w.pairs) * tiles : static_cast<int64_t>(l.block[it.at]) * tiles) * 32;
-#pragma unroll
-    for (int nb = 0; nb < NB; ++nb) {
-      if (nb >= blocks) break;
-      float v[4];
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int t = nth_token(mask, nb * 8 + (lane & 3) * 2 + e);
-        const float c = t < 0 ? 0.f : it.e == a.E ? LOWER<T> : LOWER<T> * w.share[static_cast<int64_t>(t) * a.E + it.e];
-        const float u = fmaxf(acc[nb][e], 0.f), z = fmaxf(acc[nb][e + 2], 0.f);
-        // a NaN has to stay one; columns that are no token's give zero
-        v[e] = t < 0 ? 0.f : c * (isnan(acc[nb][e]) ? acc[nb][e] : u * u);
-        v[e + 2] = t < 0 ? 0.f : c * (isnan(acc[nb][e + 2]) ? acc[nb][e + 2] : z * z);
-      }
-      h[(static_cast<int64_t>(nb) * inner + it.tile) * 32 + lane] =
-          make_uint2(transpose8x8(Num<T>::pack(v[0], v[1])), transpose8x8(Num<T>::pack(v[2], v[3])));
-    }
-  }
-  cp_wait<0>();
+            for (int k = e; k < 4; k += 2) {
+              const float u = acc[nb][k] < 0.f ? 0.f : acc[nb][k];  // a NaN stays one
+              v[k] = t < 0 ? 0.f : c * (u * u);
+            }
+          }
+          uint2* to = h + ((static_cast<int64_t>(l.block[p.entry]) + nb) * inner + p.tile) * 64 + lane;
+          const uint32_t hi0 = Num<T>::pack(v[0], v[1]), hi1 = Num<T>::pack(v[2], v[3]);
+          const float2 f0 = Num<T>::unpack(hi0), f1 = Num<T>::unpack(hi1);
+          // (of an infinite value the rest is NaN, and so would the sum be)
+          const uint32_t lo0 = Num<T>::pack(isinf(f0.x) ? 0.f : v[0] - f0.x, isinf(f0.y) ? 0.f : v[1] - f0.y);
+          const uint32_t lo1 = Num<T>::pack(isinf(f1.x) ? 0.f : v[2] - f1.x, isinf(f1.y) ? 0.f : v[3] - f1.y);
+          to[0] = make_uint2(transpose8x8(hi0), transpose8x8(hi1));
+          to[32] = make_uint2(transpose8x8(lo0), transpose8x8(lo1));
+        }
+      });
 }
 
 template <class T, int NB>
 __global__ void __launch_bounds__(THREADS, 2) proj_kernel(const MoeTokensArgs a, const Workspace w, const int parts) {
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ Lists l;
+  __shared__ float sums[WARPS][MOST][17];  // a warp's, of the tile's 16 channels for each token
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, part = blockIdx.x % parts, tile = blockIdx.x / parts;
+  for (int i = tid; i < WARPS * MOST * 17; i += THREADS) (&sums[0][0][0])[i] = 0.f;
   make_lists(a, w, l);  // (the route kernel ended before the one before this began its work)
   const int per = (a.F + 63) / 64, shared_per = (a.Fs + 63) / 64, tiles = (a.F + 15) / 16, shared_tiles = (a.Fs + 15) / 16;
-  const int routed = l.wanted - (a.Fs ? 1 : 0), all = routed * per + shared_per;
-  // an equal run of the stages of all wanted experts
+  // an equal run of the stages of all entries
+  const int routed = l.routed * per, all = routed + (l.entries - l.routed) * shared_per;
   const int runs = parts * WARPS, run = part * WARPS + warp, few = all / runs, more = all % runs;
   const int first = run * few + min(run, more), last = first + few + (run < more ? 1 : 0);
-  Ring r = make_ring(smem);
-  const int row = lane >> 3, chunk = lane & 7, rows = min(16, a.d - tile * 16);
-  float acc[NB][4];
-#pragma unroll
-  for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) acc[nb][e] = 0.f;
-
-  struct Place {
-    int at, stage, stages, hidden;
+  auto set = [&](Piece& p, int at) {
+    if (at >= last) return false;
+    const bool shared = at >= routed;
+    const int i = shared ? at - routed : at, n = quotient(i, shared ? shared_per : per);
+    p.entry = (shared ? l.routed : 0) + n;
+    p.tile = tile;
+    p.expert = l.expert[p.entry];
+    p.inner = shared ? a.Fs : a.F;
+    p.rows = min(16, a.d - tile * 16);
+    p.stage = i - n * (shared ? shared_per : per);
+    p.stages = min(shared ? shared_per : per, p.stage + last - at);
+    return true;
   };
-  auto place_of = [&](int i) {
-    Place p;
-    if (i < routed * per) {
-      p.at = quotient(i, per);
-      p.stage = i - p.at * per;
-      p.stages = per;
-      p.hidden = a.F;
-    } else {
-      p.at = routed;
-      p.stage = i - routed * per;
-      p.stages = shared_per;
-      p.hidden = a.Fs;
-    }
-    return p;
+  auto end_of = [&](const Piece& p) {  // the stage behind it, among all
+    return p.entry >= l.routed ? routed + (p.entry - l.routed) * shared_per + p.stages : p.entry * per + p.stages;
   };
-  if (first < last) {
-    Place f = place_of(first);
-    const char* f_at = nullptr;
-    int f_left = last - first;
-    auto enter = [&]() {
-      const int e = l.expert[f.at];
-      const T* base = e == a.E ? static_cast<const T*>(a.shared_proj) : static_cast<const T*>(a.w_proj) + static_cast<int64_t>(e) * a.d * a.F;
-      f_at = reinterpret_cast<const char*>(base + (static_cast<int64_t>(tile) * 16 + row) * f.hidden + f.stage * 64 + chunk * 8);
-    };
-    enter();
-    auto fetch = [&]() {
-      if (f_left > 0) {
-        copy_stage(r, f_at, static_cast<int64_t>(f.hidden) * sizeof(T), rows, f.stage * 64 + chunk * 8 < f.hidden, a.x);
-        f_at += 128;
-        --f_left;
-        if (++f.stage == f.stages) {
-          f.stage = 0;
-          ++f.at;
-          if (f_left > 0) {
-            f.stages = f.at < routed ? per : shared_per;
-            f.hidden = f.at < routed ? a.F : a.Fs;
-            enter();
-          }
+  // the two numbers of a hidden value stand beside each other: blocks nb and NB + nb
+  stream<T, 2 * NB>(
+      a, smem, [&](Piece& p) { return set(p, first); }, [&](Piece& p) { return set(p, end_of(p)); },
+      [&](const Piece& p) -> const void* {
+        const T* e = p.expert == a.E ? static_cast<const T*>(a.shared_proj) : static_cast<const T*>(a.w_proj) + static_cast<int64_t>(p.expert) * a.d * a.F;
+        return e + static_cast<int64_t>(tile) * 16 * p.inner;
+      },
+      [&](const Piece& p, const uint2* (&at)[2 * NB]) {
+        const bool shared = p.expert == a.E;
+        const int left = __popcll(l.mask[p.expert]) - l.first[p.entry], inner = shared ? shared_tiles : tiles;
+        const uint2* h = w.h + (shared ? static_cast<int64_t>(w.pairs) * tiles * 2 : 0ll) * 32;
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+          at[nb] = nb * 8 < left ? h + (static_cast<int64_t>(l.block[p.entry]) + nb) * inner * 64 + lane : nullptr;
+          at[NB + nb] = at[nb] ? at[nb] + 32 : nullptr;
         }
-      }
-      cp_commit();
-    };
-#pragma unroll 1
-    for (int i = 0; i < STAGES - 1; ++i) fetch();
-    wait_for_predecessor();  // weights may come before, h may not
-
-    Place c = place_of(first);
-    int left = last - first;
-#pragma unroll 1
-    while (left > 0) {
-      const int e = l.expert[c.at], n = min(left, c.stages - c.stage), inner = e == a.E ? shared_tiles : tiles;
-      const unsigned long long mask = l.mask[e];
-      const uint2* h = w.h + (e == a.E ? static_cast<int64_t>(w.pairs) * tiles : static_cast<int64_t>(l.block[c.at]) * tiles) * 32;
-      // columns are tokens here, which an expert's blocks hold one after another
-      const uint2* hs[NB];
+        return static_cast<int64_t>(64);
+      },
+      [] { wait_for_predecessor(); },  // weights may come before, h may not
+      [&](const Piece& p, const float (&acc)[2 * NB][4]) {
+        const unsigned long long mask = l.mask[p.expert];
 #pragma unroll
-      for (int nb = 0; nb < NB; ++nb) {
-        const int t = nb * 8 + (lane >> 2);
-        const bool is = (mask >> t) & 1ull;
-        const int place = __popcll(mask & ((1ull << t) - 1ull));
-        hs[nb] = is ? h + static_cast<int64_t>(place >> 3) * inner * 32 + (place & 7) * 4 + (lane & 3) : nullptr;
-      }
-#pragma unroll 1
-      for (int st = c.stage; st < c.stage + n; ++st) {
-        uint2 b[4][NB];
+        for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-        for (int s = 0; s < 4; ++s) {
-          const int g = st * 4 + s;
-#pragma unroll
-          for (int nb = 0; nb < NB; ++nb) {
-            b[s][nb] = make_uint2(0u, 0u);
-            if (hs[nb] && g < inner) b[s][nb] = __ldcg(hs[nb] + g * 32);
+          for (int e = 0; e < 2; ++e) {
+            const int t = nth_token(mask, l.first[p.entry] + nb * 8 + (lane & 3) * 2 + e);
+            if (t < 0) continue;
+            float* to = &sums[warp][t][lane >> 2];
+            to[0] += acc[nb][e] + acc[NB + nb][e];
+            to[8] += acc[nb][e + 2] + acc[NB + nb][e + 2];
           }
-        }
-        cp_wait<STAGES - 2>();
-        __syncwarp();
-        const uint32_t base = r.base + r.stage_out * STAGE;
-        if (++r.stage_out == STAGES) r.stage_out = 0;
-        uint32_t wf[4][4];
-#pragma unroll
-        for (int s = 0; s < 4; ++s) ldsm4(wf[s], base + r.at[s]);
-        fetch();
-#pragma unroll
-        for (int s = 0; s < 4; ++s)
-#pragma unroll
-          for (int nb = 0; nb < NB; ++nb)
-            if ((mask >> (nb * 8)) & 0xffull) Num<T>::mma(acc[nb], wf[s], b[s][nb].x, b[s][nb].y);
-      }
-      left -= n;
-      c.stage += n;
-      if (c.stage == c.stages) {
-        c.stage = 0;
-        ++c.at;
-        c.stages = c.at < routed ? per : shared_per;
-        c.hidden = c.at < routed ? a.F : a.Fs;
-      }
-    }
-    cp_wait<0>();
-  } else {
-    wait_for_predecessor();
-  }
+        __syncwarp();  // the next entry's lanes may hold this one's tokens elsewhere
+      });
 
   // ---- the warps' sums, then the parts', in their order
   __syncthreads();
-  float4* sums = reinterpret_cast<float4*>(smem);  // [warp][nb][lane]
+  float(*whole)[17] = sums[0];
+  for (int i = tid; i < a.T * 16; i += THREADS) {
+    float v = 0.f;
 #pragma unroll
-  for (int nb = 0; nb < NB; ++nb) sums[(warp * NB + nb) * 32 + lane] = make_float4(acc[nb][0], acc[nb][1], acc[nb][2], acc[nb][3]);
-  __syncthreads();
-  float4* whole = sums + WARPS * NB * 32;
-  for (int i = tid; i < NB * 32; i += THREADS) {
-    float4 v = sums[i];
-#pragma unroll
-    for (int k = 1; k < WARPS; ++k) {
-      const float4 u = sums[k * NB * 32 + i];
-      v.x += u.x; v.y += u.y; v.z += u.z; v.w += u.w;
-    }
-    whole[i] = v;
+    for (int k = 0; k < WARPS; ++k) v += sums[k][i >> 4][i & 15];
+    whole[i >> 4][i & 15] = v;
   }
   if (parts > 1) cluster_sync();
   else __syncthreads();
   if (part == 0) {
-    for (int i = tid; i < NB * 32; i += THREADS) {
-      float4 v = whole[i];
+    for (int i = tid; i < a.T * 8; i += THREADS) {  // a pair of channels of a token
+      const int t = i >> 3, ch = (i & 7) * 2;
+      float2 v = make_float2(whole[t][ch], whole[t][ch + 1]);
       for (int c = 1; c < parts; ++c) {
         uint32_t remote;
-        float4 u;
-        asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(smem_u32(whole + i)), "r"(c));
-        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(u.x), "=f"(u.y), "=f"(u.z), "=f"(u.w) : "r"(remote) : "memory");
-        v.x += u.x; v.y += u.y; v.z += u.z; v.w += u.w;
+        float2 u;
+        asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(smem_u32(&whole[t][ch])), "r"(c));
+        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(u.x) : "r"(remote) : "memory");
+        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(u.y) : "r"(remote + 4) : "memory");
+        v.x += u.x;
+        v.y += u.y;
       }
-      // a lane has channels g and g + 8 of tokens 2 c and 2 c + 1
-      const int t = (i >> 5) * 8 + (i & 3) * 2, ch = tile * 16 + ((i & 31) >> 2);
-      T* y = static_cast<T*>(a.y);
       const float f = 1.f / LOWER<T>;
-      const uint32_t lo = Num<T>::pack(v.x * f, v.z * f), hi = Num<T>::pack(v.y * f, v.w * f);
-      auto put = [&](int token, int at, uint32_t u) {
-        if (token < a.T && at < a.d) reinterpret_cast<uint16_t*>(y)[static_cast<int64_t>(token) * a.d + at] = static_cast<uint16_t>(u);
-      };
-      put(t, ch, lo);
-      put(t, ch + 8, lo >> 16);
-      put(t + 1, ch, hi);
-      put(t + 1, ch + 8, hi >> 16);
+      if (tile * 16 + ch < a.d)  // (d is even)
+        *reinterpret_cast<uint32_t*>(static_cast<T*>(a.y) + static_cast<int64_t>(t) * a.d + tile * 16 + ch) = Num<T>::pack(v.x * f, v.y * f);
     }
   }
   if (parts > 1) cluster_sync();  // nobody leaves while its sums are read
@@ -572,19 +551,12 @@ static int launch(const MoeTokensArgs& a, cudaStream_t s) {
   layout(a, w);
   int ranks = 8;
   while (ranks > 1 && a.T * ranks > 2 * a.sms) ranks /= 2;
-  if (start(route_kernel<T>, a.T * ranks, ROUTE_THREADS, a.d * sizeof(float), ranks, false, s, a, w, ranks)) return -1;
+  const auto route = a.E <= 64 ? route_kernel<T, 2> : a.E <= 256 ? route_kernel<T, 8> : route_kernel<T, EXPERTS / 32>;
+  if (start(route, a.T * ranks, ROUTE_THREADS, a.d * sizeof(float), ranks, false, s, a, w, ranks)) return -1;
   if (start(fc_kernel<T, NB>, 2 * a.sms, THREADS, SMEM, 1, true, s, a, w)) return -1;
   const int tiles = (a.d + 15) / 16, parts = std::max(1, std::min(8, 2 * a.sms / tiles));
   return start(proj_kernel<T, NB>, tiles * parts, THREADS, SMEM, parts, true, s, a, w, parts);
 }
-template <class T>
-static int by_tokens(const MoeTokensArgs& a, cudaStream_t s) {
-  if (a.T <= 8) return launch<T, 1>(a, s);
-  if (a.T <= 16) return launch<T, 2>(a, s);
-  if (a.T <= 32) return launch<T, 4>(a, s);
-  return launch<T, 8>(a, s);
-}
-
 }  // namespace moe_tokens
 }  // namespace nt
 
@@ -600,5 +572,6 @@ int nt_moe_tokens(const MoeTokensArgs& a, cudaStream_t s) {
   if (a.T > MOST || a.E < 1 || a.E > EXPERTS || a.k < 1 || a.k > CHOICES || a.k > a.E || a.d < 8 || a.d % 8 || a.d > NT_MOE_TOKENS_WIDTH ||
       a.F < 8 || a.F % 8 || a.Fs % 8 || static_cast<int64_t>(a.E) * ((a.F + 15) / 16) + a.Fs > INT32_MAX / 2)
     return -1;
-  return a.fp16 ? by_tokens<__half>(a, s) : by_tokens<__nv_bfloat16>(a, s);
+  if (a.fp16) return a.T <= 8 ? launch<__half, 1>(a, s) : launch<__half, 2>(a, s);
+  return a.T <= 8 ? launch<__nv_bfloat16, 1>(a, s) : launch<__nv_bfloat16, 2>(a, s);
 }
