@@ -21,8 +21,8 @@ namespace nt {
 namespace moe_tokens {
 
 constexpr int ROUTE_WARPS = 8, ROUTE_THREADS = ROUTE_WARPS * 32;
-constexpr int WARPS = 4, THREADS = WARPS * 32;
-constexpr int STAGE = 2048, STAGES = 10, RING = STAGE * STAGES;  // 20 KB a warp; two CTAs an SM
+constexpr int WARPS = 8, THREADS = WARPS * 32;
+constexpr int STAGE = 2048, STAGES = 4, RING = STAGE * STAGES;  // 8 KB a warp, 16 warps an SM
 constexpr int SMEM = WARPS * RING;
 constexpr int MOST = NT_MOE_TOKENS_MOST, EXPERTS = NT_MOE_TOKENS_EXPERTS, CHOICES = NT_MOE_TOKENS_CHOICES;
 // Hidden values are held in the weights' type.  fp16 ends at 65504, which a square passes where its root is 256: they
@@ -33,10 +33,12 @@ template <> constexpr float LOWER<__half> = 1.f / 64;
 struct Workspace {
   int* choice;    // [T, k]
   float* share;   // [T, E], set where chosen
-  uint2* x;       // [ceil(d / 16), blocks of 8 tokens, 32]: a lane's part of a 16 x 8 operand
-  uint2* h;       // [pairs of an expert and a block of 8 of its tokens, ceil(F / 16), 2, 32]
-  int pairs;      // of routed experts; the shared expert's blocks, of ceil(Fs / 16) each, come behind them
+  uint2* x;       // [groups of d, blocks of 8 tokens, 32]: a lane's part of a 16 x 8 operand
+  uint4* h;       // [pairs of an expert and a block of 8 of its tokens, groups of F, 32]: the same of a value's two numbers
+  int pairs;      // of routed experts; the shared expert's blocks, of groups of Fs each, come behind them
 };
+// 16 inner elements each, a whole number of stages; what lies behind the inner dimension is zero.
+__host__ __device__ static int groups_of(int n) { return (n + 63) / 64 * 4; }
 static int blocks_of(int n, int by) { return (n + by - 1) / by; }
 static size_t layout(const MoeTokensArgs& a, Workspace& w) {
   size_t at = 0;
@@ -50,8 +52,8 @@ static size_t layout(const MoeTokensArgs& a, Workspace& w) {
   w.pairs = static_cast<int>(std::min<int64_t>(static_cast<int64_t>(a.T) * a.k, static_cast<int64_t>(a.E) * nb));
   w.choice = reinterpret_cast<int*>(take(static_cast<size_t>(a.T) * a.k * 4));
   w.share = reinterpret_cast<float*>(take(static_cast<size_t>(a.T) * a.E * 4));
-  w.x = reinterpret_cast<uint2*>(take(static_cast<size_t>(blocks_of(a.d, 16)) * nb * 256));
-  w.h = reinterpret_cast<uint2*>(take((static_cast<size_t>(w.pairs) * blocks_of(a.F, 16) + static_cast<size_t>(nb) * blocks_of(a.Fs, 16)) * 512));
+  w.x = reinterpret_cast<uint2*>(take(static_cast<size_t>(groups_of(a.d)) * nb * 256));
+  w.h = reinterpret_cast<uint4*>(take((static_cast<size_t>(w.pairs) * groups_of(a.F) + static_cast<size_t>(nb) * groups_of(a.Fs)) * 512));
   return at;
 }
 
@@ -73,10 +75,10 @@ __global__ void __launch_bounds__(ROUTE_THREADS) route_kernel(const MoeTokensArg
     for (int e = 0; e < 4; ++e) *reinterpret_cast<float2*>(x + i + 2 * e) = Num<T>::unpack(v[e]);
   }
   // x as an operand: lane 4 n + c of a 16 x 8 tile has token n's channels 2 c, 2 c + 1 and 2 c + 8, 2 c + 9
-  const int nb = (a.T + 7) / 8, groups = (a.d + 15) / 16;
+  const int nb = (a.T + 7) / 8, groups = groups_of(a.d);
   for (int i = rank * ROUTE_THREADS + tid; i < groups * 4; i += ranks * ROUTE_THREADS) {
     const int g = i >> 2, at = g * 16 + (i & 3) * 2;
-    const uint32_t lo = *reinterpret_cast<const uint32_t*>(src + at), hi = at + 8 < a.d ? *reinterpret_cast<const uint32_t*>(src + at + 8) : 0u;
+    const uint32_t lo = at < a.d ? *reinterpret_cast<const uint32_t*>(src + at) : 0u, hi = at + 8 < a.d ? *reinterpret_cast<const uint32_t*>(src + at + 8) : 0u;
     w.x[(static_cast<int64_t>(g) * nb + t / 8) * 32 + (t % 8) * 4 + (i & 3)] = make_uint2(lo, hi);
   }
   cluster_sync();  // x is there, and the first CTA, which gets the logits
@@ -213,16 +215,16 @@ NT_DEVICE int nth_token(unsigned long long m, int n) {
 
 // A warp's ring: 16 rows of 64 elements a stage, chunk c of row r at c ^ (r & 7).
 struct Ring {
-  uint32_t base, to;     // of the ring; this lane's first place in a stage
-  int stage_in, stage_out;
-  uint32_t at[4];        // this lane's matrix row of the four 16-column tiles
+  uint32_t base, in, out;  // addresses of the ring, of the stage that is filled next and of the one that is read next
+  uint32_t to[2];          // this lane's place in a stage for rows r and r + 4 (r < 4); 1024 further on for r + 8 and r + 12
+  uint32_t at[4];          // this lane's matrix row of the four 16-column tiles
 };
 NT_DEVICE Ring make_ring(const void* smem) {
   Ring r;
   const int lane = threadIdx.x & 31, row = lane >> 3, chunk = lane & 7;
-  r.base = smem_u32(smem) + (threadIdx.x >> 5) * RING;
-  r.to = row * 128 + ((chunk ^ row) << 4);  // rows row + 4 e have the chunk at the same place, or across (chunk ^ 4)
-  r.stage_in = r.stage_out = 0;
+  r.base = r.in = r.out = smem_u32(smem) + (threadIdx.x >> 5) * RING;
+  r.to[0] = row * 128 + ((chunk ^ row) << 4);
+  r.to[1] = (row + 4) * 128 + ((chunk ^ (row + 4)) << 4);
 #pragma unroll
   for (int s = 0; s < 4; ++s) {
     const int m = lane & 15;
@@ -230,50 +232,54 @@ NT_DEVICE Ring make_ring(const void* smem) {
   }
   return r;
 }
-// Rows [0, rows) of a tile at p (this lane's row and chunk), stride bytes apart; `inside`: the lane's chunk is.  What is not
-// there becomes zero (and names an address that is).
-NT_DEVICE void copy_stage(Ring& r, const char* p, int64_t stride, int rows, bool inside, const void* there) {
-  const uint32_t dst = r.base + r.stage_in * STAGE + r.to;
-  const int row = (threadIdx.x & 31) >> 3;
-  if (rows == 16 && inside) {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) cp_async16((dst + e * 512) ^ ((e & 1) << 6), p + e * 4 * stride);
-  } else {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const bool valid = inside && row + 4 * e < rows;
-      cp_async16_or_zero((dst + e * 512) ^ ((e & 1) << 6), valid ? p + e * 4 * stride : there, valid);
-    }
-  }
-  if (++r.stage_in == STAGES) r.stage_in = 0;
-}
+NT_DEVICE void turn(uint32_t& stage, const Ring& r) { stage = stage == r.base + (STAGES - 1) * STAGE ? r.base : stage + STAGE; }
 
 // A row tile of an entry: what a warp goes through, a stage of 64 inner elements after the other.
 struct Piece {
   int entry, expert, tile;
   int inner, rows;    // elements of a weight row; rows of the tile (16, or fewer at the end)
+  int blocks;         // of 8 tokens
   int stage, stages;  // the next one; the first behind the piece
 };
 
 // Goes through a warp's pieces: weights come `STAGES - 1` stages ahead, the other operand one.
 //   first(piece) / next(piece) set a piece and say whether there is one (the copies, the operand and the products each go through them);
-//   base(piece): the tile's first weight; operand(piece, pointers): this lane's part of the 16 x 8 tiles of stage 0 of each block of
-//   8 tokens (null: none), `step` apart from tile to tile of 16; ready(): what has to be waited for before the operand is read;
-//   done(piece, sums): a piece's products are complete.
-template <class T, int NB, class First, class Next, class Base, class Operand, class Ready, class Done>
-NT_DEVICE void stream(const MoeTokensArgs& a, const void* smem, First first, Next next, Base base, Operand operand, Ready ready, Done done) {
+//   base(piece): the tile's first weight; operand(piece, pointers): this lane's part of the 16 x 8 tile of the piece's next stage, of
+//   each block of 8 tokens, `step` apart from tile to tile (a Frag of 16 bytes holds two numbers for each value); ready(): what has to
+//   be waited for before the operand is read; done(piece, sums): a piece's products are complete.
+// With 8 warps an SM and 187 instructions a stage the first product took 60 us for 12 tokens (3.7 TB/s): a warp's instructions wait
+// for each other, so there are 16 warps, and what a stage needs is counted on.
+template <class T, int NB, class Frag, class First, class Next, class Base, class Operand, class Ready, class Done>
+NT_DEVICE void stream(const MoeTokensArgs& a, const void* smem, const int step, First first, Next next, Base base, Operand operand, Ready ready,
+                      Done done) {
+  constexpr bool TWO = sizeof(Frag) == 16;
   Ring r = make_ring(smem);
   const int lane = threadIdx.x & 31, row = lane >> 3, chunk = lane & 7;
   Piece f, o, c;  // where the copies, the operand and the products stand
   bool f_more = first(f);
   const char* f_at = nullptr;
+  int64_t f_step = 0;  // four rows
   auto enter = [&]() {
-    if (f_more) f_at = reinterpret_cast<const char*>(static_cast<const T*>(base(f)) + static_cast<int64_t>(row) * f.inner + f.stage * 64 + chunk * 8);
+    if (!f_more) return;
+    f_at = reinterpret_cast<const char*>(static_cast<const T*>(base(f)) + static_cast<int64_t>(row) * f.inner + f.stage * 64 + chunk * 8);
+    f_step = static_cast<int64_t>(f.inner) * (4 * sizeof(T));
   };
   enter();
   auto fetch = [&]() {
     if (f_more) {
-      copy_stage(r, f_at, static_cast<int64_t>(f.inner) * sizeof(T), f.rows, f.stage * 64 + chunk * 8 < f.inner, a.x);
+      const bool inside = f.stage * 64 + chunk * 8 < f.inner;
+      if (f.rows == 16 && (f.stage + 1) * 64 <= f.inner) {
+        const char* p = f_at;
+#pragma unroll
+        for (int e = 0; e < 4; ++e, p += f_step) cp_async16(r.in + r.to[e & 1] + (e >> 1) * 1024, p);
+      } else {  // what is not there becomes zero
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const bool valid = inside && row + 4 * e < f.rows;
+          cp_async16_or_zero(r.in + r.to[e & 1] + (e >> 1) * 1024, valid ? f_at + e * f_step : static_cast<const char*>(a.x), valid);
+        }
+      }
+      turn(r.in, r);
       f_at += 128;
       if (++f.stage == f.stages) {
         f_more = next(f);
@@ -287,54 +293,40 @@ NT_DEVICE void stream(const MoeTokensArgs& a, const void* smem, First first, Nex
   ready();
 
   bool o_more = first(o), c_more = first(c);
-  const uint2* at[NB];
-  int64_t step = 0;
-  int tiles = 0;  // of 16 inner elements
-  auto point = [&]() {
-    if (o_more) {
-      step = operand(o, at);
-      tiles = (o.inner + 15) >> 4;
-    }
-  };
-  uint2 ahead[4][NB];
-  auto load = [&]() {
+  const Frag* at[NB];
+  if (o_more) operand(o, at);
+  auto load = [&](Frag (&b)[4][NB]) {
     if (!o_more) return;
 #pragma unroll
-    for (int s = 0; s < 4; ++s)
+    for (int nb = 0; nb < NB; ++nb)
+      if (nb == 0 || nb < o.blocks) {
 #pragma unroll
-      for (int nb = 0; nb < NB; ++nb) {
-        const int g = o.stage * 4 + s;
-        ahead[s][nb] = make_uint2(0u, 0u);
-        if (at[nb] && g < tiles) ahead[s][nb] = __ldcg(at[nb] + g * step);
+        for (int s = 0; s < 4; ++s) b[s][nb] = __ldcg(at[nb] + s * step);
+        at[nb] += 4 * step;
       }
     if (++o.stage == o.stages) {
       o_more = next(o);
-      point();
+      if (o_more) operand(o, at);
     }
   };
-  point();
-  load();
   float acc[NB][4] = {};
-#pragma unroll 1
-  while (c_more) {
-    uint2 b[4][NB];
-#pragma unroll
-    for (int s = 0; s < 4; ++s)
-#pragma unroll
-      for (int nb = 0; nb < NB; ++nb) b[s][nb] = ahead[s][nb];
-    load();
+  auto multiply = [&](const Frag (&b)[4][NB], Frag (&ahead)[4][NB]) {
+    load(ahead);
     cp_wait<STAGES - 2>();
     __syncwarp();  // this stage has landed for every lane, and the stage before it is read by none
-    const uint32_t from = r.base + r.stage_out * STAGE;
-    if (++r.stage_out == STAGES) r.stage_out = 0;
     uint32_t w[4][4];
 #pragma unroll
-    for (int s = 0; s < 4; ++s) ldsm4(w[s], from + r.at[s]);
+    for (int s = 0; s < 4; ++s) ldsm4(w[s], r.out + r.at[s]);
+    turn(r.out, r);
     fetch();
 #pragma unroll
-    for (int s = 0; s < 4; ++s)
+    for (int nb = 0; nb < NB; ++nb)
+      if (nb == 0 || nb < c.blocks)
 #pragma unroll
-      for (int nb = 0; nb < NB; ++nb) Num<T>::mma(acc[nb], w[s], b[s][nb].x, b[s][nb].y);
+        for (int s = 0; s < 4; ++s) {
+          Num<T>::mma(acc[nb], w[s], b[s][nb].x, b[s][nb].y);
+          if constexpr (TWO) Num<T>::mma(acc[nb], w[s], b[s][nb].z, b[s][nb].w);
+        }
     if (++c.stage == c.stages) {
       done(c, acc);
 #pragma unroll
@@ -343,6 +335,14 @@ NT_DEVICE void stream(const MoeTokensArgs& a, const void* smem, First first, Nex
         for (int e = 0; e < 4; ++e) acc[nb][e] = 0.f;
       c_more = next(c);
     }
+  };
+  Frag even[4][NB], odd[4][NB];
+  load(even);
+#pragma unroll 1
+  while (c_more) {
+    multiply(even, odd);
+    if (!c_more) break;
+    multiply(odd, even);
   }
   cp_wait<0>();
 }
@@ -356,7 +356,7 @@ __global__ void __launch_bounds__(THREADS, 2) fc_kernel(const MoeTokensArgs a, c
   wait_for_predecessor();
   dependents_may_start();
   make_lists(a, w, l);
-  const int tiles = (a.F + 15) / 16, shared_tiles = (a.Fs + 15) / 16, nb_x = (a.T + 7) / 8;
+  const int tiles = (a.F + 15) / 16, shared_tiles = (a.Fs + 15) / 16, groups = groups_of(a.F), shared_groups = groups_of(a.Fs);
   const int routed = l.routed * tiles, items = routed + (l.entries - l.routed) * shared_tiles, by = gridDim.x * WARPS;
   // (the first items go to different SMs)
   auto set = [&](Piece& p, int item) {
@@ -368,6 +368,7 @@ __global__ void __launch_bounds__(THREADS, 2) fc_kernel(const MoeTokensArgs a, c
     p.expert = l.expert[p.entry];
     p.inner = a.d;
     p.rows = min(16, (shared ? a.Fs : a.F) - p.tile * 16);
+    p.blocks = (__popcll(l.mask[p.expert]) - l.first[p.entry] + 7) >> 3;
     p.stage = 0;
     p.stages = (a.d + 63) / 64;
     return true;
@@ -375,8 +376,8 @@ __global__ void __launch_bounds__(THREADS, 2) fc_kernel(const MoeTokensArgs a, c
   auto item_at = [&](const Piece& p) {
     return p.entry >= l.routed ? routed + (p.entry - l.routed) * shared_tiles + p.tile : p.entry * tiles + p.tile;
   };
-  stream<T, NB>(
-      a, smem, [&](Piece& p) { return set(p, warp * gridDim.x + blockIdx.x); }, [&](Piece& p) { return set(p, item_at(p) + by); },
+  stream<T, NB, uint2>(
+      a, smem, (a.T + 7) / 8 * 32, [&](Piece& p) { return set(p, warp * gridDim.x + blockIdx.x); }, [&](Piece& p) { return set(p, item_at(p) + by); },
       [&](const Piece& p) -> const void* {
         const T* e = p.expert == a.E ? static_cast<const T*>(a.shared_fc) : static_cast<const T*>(a.w_fc) + static_cast<int64_t>(p.expert) * a.F * a.d;
         return e + static_cast<int64_t>(p.tile) * 16 * a.d;
@@ -385,10 +386,10 @@ __global__ void __launch_bounds__(THREADS, 2) fc_kernel(const MoeTokensArgs a, c
         const unsigned long long mask = l.mask[p.expert];
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
-          const int t = nth_token(mask, l.first[p.entry] + nb * 8 + (lane >> 2));
-          at[nb] = t < 0 ? nullptr : w.x + (t >> 3) * 32 + (t & 7) * 4 + (lane & 3);
+          // columns without a token may be anyone's: they are dropped
+          const int t = max(0, nth_token(mask, l.first[p.entry] + nb * 8 + (lane >> 2)));
+          at[nb] = w.x + (t >> 3) * 32 + (t & 7) * 4 + (lane & 3);
         }
-        return static_cast<int64_t>(nb_x) * 32;
       },
       [] {},
       [&](const Piece& p, const float (&acc)[NB][4]) {
@@ -396,11 +397,11 @@ __global__ void __launch_bounds__(THREADS, 2) fc_kernel(const MoeTokensArgs a, c
         // numbers of its type, so that nothing but the output is rounded.
         const bool shared = p.expert == a.E;
         const unsigned long long mask = l.mask[p.expert];
-        const int left = __popcll(mask) - l.first[p.entry], inner = shared ? shared_tiles : tiles;
-        uint2* h = w.h + (shared ? static_cast<int64_t>(w.pairs) * tiles * 2 : 0ll) * 32;
+        const int inner = shared ? shared_groups : groups;
+        uint4* h = w.h + (shared ? static_cast<int64_t>(w.pairs) * groups : 0ll) * 32;
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
-          if (nb * 8 >= left) break;
+          if (nb >= p.blocks) break;
           float v[4];
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
@@ -412,14 +413,15 @@ __global__ void __launch_bounds__(THREADS, 2) fc_kernel(const MoeTokensArgs a, c
               v[k] = t < 0 ? 0.f : c * (u * u);
             }
           }
-          uint2* to = h + ((static_cast<int64_t>(l.block[p.entry]) + nb) * inner + p.tile) * 64 + lane;
           const uint32_t hi0 = Num<T>::pack(v[0], v[1]), hi1 = Num<T>::pack(v[2], v[3]);
           const float2 f0 = Num<T>::unpack(hi0), f1 = Num<T>::unpack(hi1);
           // (of an infinite value the rest is NaN, and so would the sum be)
           const uint32_t lo0 = Num<T>::pack(isinf(f0.x) ? 0.f : v[0] - f0.x, isinf(f0.y) ? 0.f : v[1] - f0.y);
           const uint32_t lo1 = Num<T>::pack(isinf(f1.x) ? 0.f : v[2] - f1.x, isinf(f1.y) ? 0.f : v[3] - f1.y);
-          to[0] = make_uint2(transpose8x8(hi0), transpose8x8(hi1));
-          to[32] = make_uint2(transpose8x8(lo0), transpose8x8(lo1));
+          uint4* to = h + ((static_cast<int64_t>(l.block[p.entry]) + nb) * inner + p.tile) * 32 + lane;
+          *to = make_uint4(transpose8x8(hi0), transpose8x8(hi1), transpose8x8(lo0), transpose8x8(lo1));
+          if (p.tile == (shared ? shared_tiles : tiles) - 1)  // the groups behind the last
+            for (int g = p.tile + 1; g < inner; ++g) *(to += 32) = make_uint4(0, 0, 0, 0);
         }
       });
 }
@@ -428,11 +430,11 @@ template <class T, int NB>
 __global__ void __launch_bounds__(THREADS, 2) proj_kernel(const MoeTokensArgs a, const Workspace w, const int parts) {
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ Lists l;
-  __shared__ float sums[WARPS][MOST][17];  // a warp's, of the tile's 16 channels for each token
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, part = blockIdx.x % parts, tile = blockIdx.x / parts;
-  for (int i = tid; i < WARPS * MOST * 17; i += THREADS) (&sums[0][0][0])[i] = 0.f;
+  float* const sums = reinterpret_cast<float*>(smem + SMEM);  // [warp][token][17]: of the tile's 16 channels
+  for (int i = tid; i < WARPS * a.T * 17; i += THREADS) sums[i] = 0.f;
   make_lists(a, w, l);  // (the route kernel ended before the one before this began its work)
-  const int per = (a.F + 63) / 64, shared_per = (a.Fs + 63) / 64, tiles = (a.F + 15) / 16, shared_tiles = (a.Fs + 15) / 16;
+  const int per = (a.F + 63) / 64, shared_per = (a.Fs + 63) / 64, groups = groups_of(a.F), shared_groups = groups_of(a.Fs);
   // an equal run of the stages of all entries
   const int routed = l.routed * per, all = routed + (l.entries - l.routed) * shared_per;
   const int runs = parts * WARPS, run = part * WARPS + warp, few = all / runs, more = all % runs;
@@ -446,6 +448,7 @@ __global__ void __launch_bounds__(THREADS, 2) proj_kernel(const MoeTokensArgs a,
     p.expert = l.expert[p.entry];
     p.inner = shared ? a.Fs : a.F;
     p.rows = min(16, a.d - tile * 16);
+    p.blocks = (__popcll(l.mask[p.expert]) - l.first[p.entry] + 7) >> 3;
     p.stage = i - n * (shared ? shared_per : per);
     p.stages = min(shared ? shared_per : per, p.stage + last - at);
     return true;
@@ -453,26 +456,21 @@ __global__ void __launch_bounds__(THREADS, 2) proj_kernel(const MoeTokensArgs a,
   auto end_of = [&](const Piece& p) {  // the stage behind it, among all
     return p.entry >= l.routed ? routed + (p.entry - l.routed) * shared_per + p.stages : p.entry * per + p.stages;
   };
-  // the two numbers of a hidden value stand beside each other: blocks nb and NB + nb
-  stream<T, 2 * NB>(
-      a, smem, [&](Piece& p) { return set(p, first); }, [&](Piece& p) { return set(p, end_of(p)); },
+  stream<T, NB, uint4>(
+      a, smem, 32, [&](Piece& p) { return set(p, first); }, [&](Piece& p) { return set(p, end_of(p)); },
       [&](const Piece& p) -> const void* {
         const T* e = p.expert == a.E ? static_cast<const T*>(a.shared_proj) : static_cast<const T*>(a.w_proj) + static_cast<int64_t>(p.expert) * a.d * a.F;
         return e + static_cast<int64_t>(tile) * 16 * p.inner;
       },
-      [&](const Piece& p, const uint2* (&at)[2 * NB]) {
+      [&](const Piece& p, const uint4* (&at)[NB]) {
         const bool shared = p.expert == a.E;
-        const int left = __popcll(l.mask[p.expert]) - l.first[p.entry], inner = shared ? shared_tiles : tiles;
-        const uint2* h = w.h + (shared ? static_cast<int64_t>(w.pairs) * tiles * 2 : 0ll) * 32;
+        const int inner = shared ? shared_groups : groups;
+        const uint4* h = w.h + (shared ? static_cast<int64_t>(w.pairs) * groups : 0ll) * 32;
 #pragma unroll
-        for (int nb = 0; nb < NB; ++nb) {
-          at[nb] = nb * 8 < left ? h + (static_cast<int64_t>(l.block[p.entry]) + nb) * inner * 64 + lane : nullptr;
-          at[NB + nb] = at[nb] ? at[nb] + 32 : nullptr;
-        }
-        return static_cast<int64_t>(64);
+        for (int nb = 0; nb < NB; ++nb) at[nb] = h + ((static_cast<int64_t>(l.block[p.entry]) + nb) * inner + p.stage * 4) * 32 + lane;
       },
       [] { wait_for_predecessor(); },  // weights may come before, h may not
-      [&](const Piece& p, const float (&acc)[2 * NB][4]) {
+      [&](const Piece& p, const float (&acc)[NB][4]) {
         const unsigned long long mask = l.mask[p.expert];
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb)
@@ -480,32 +478,34 @@ __global__ void __launch_bounds__(THREADS, 2) proj_kernel(const MoeTokensArgs a,
           for (int e = 0; e < 2; ++e) {
             const int t = nth_token(mask, l.first[p.entry] + nb * 8 + (lane & 3) * 2 + e);
             if (t < 0) continue;
-            float* to = &sums[warp][t][lane >> 2];
-            to[0] += acc[nb][e] + acc[NB + nb][e];
-            to[8] += acc[nb][e + 2] + acc[NB + nb][e + 2];
+            float* to = sums + (warp * a.T + t) * 17 + (lane >> 2);
+            to[0] += acc[nb][e];
+            to[8] += acc[nb][e + 2];
           }
         __syncwarp();  // the next entry's lanes may hold this one's tokens elsewhere
       });
 
   // ---- the warps' sums, then the parts', in their order
   __syncthreads();
-  float(*whole)[17] = sums[0];
+  float* const whole = sums;
   for (int i = tid; i < a.T * 16; i += THREADS) {
+    const int at = (i >> 4) * 17 + (i & 15);
     float v = 0.f;
 #pragma unroll
-    for (int k = 0; k < WARPS; ++k) v += sums[k][i >> 4][i & 15];
-    whole[i >> 4][i & 15] = v;
+    for (int k = 0; k < WARPS; ++k) v += sums[k * a.T * 17 + at];
+    whole[at] = v;
   }
   if (parts > 1) cluster_sync();
   else __syncthreads();
   if (part == 0) {
     for (int i = tid; i < a.T * 8; i += THREADS) {  // a pair of channels of a token
       const int t = i >> 3, ch = (i & 7) * 2;
-      float2 v = make_float2(whole[t][ch], whole[t][ch + 1]);
+      const float* own = whole + t * 17 + ch;
+      float2 v = make_float2(own[0], own[1]);
       for (int c = 1; c < parts; ++c) {
         uint32_t remote;
         float2 u;
-        asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(smem_u32(&whole[t][ch])), "r"(c));
+        asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(smem_u32(own)), "r"(c));
         asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(u.x) : "r"(remote) : "memory");
         asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(u.y) : "r"(remote + 4) : "memory");
         v.x += u.x;
@@ -546,7 +546,7 @@ static int start(Kernel kern, int grid, int threads, size_t smem, int cluster, b
 template <class T, int NB>
 static int launch(const MoeTokensArgs& a, cudaStream_t s) {
   static std::atomic<uint64_t> fc_done{0}, proj_done{0};
-  if (smem_limit(fc_done, fc_kernel<T, NB>, SMEM) != cudaSuccess || smem_limit(proj_done, proj_kernel<T, NB>, SMEM) != cudaSuccess) return -1;
+  if (smem_limit(fc_done, fc_kernel<T, NB>, SMEM) != cudaSuccess || smem_limit(proj_done, proj_kernel<T, NB>, SMEM + WARPS * MOST * 17 * sizeof(float)) != cudaSuccess) return -1;
   Workspace w;
   layout(a, w);
   int ranks = 8;
@@ -555,7 +555,7 @@ static int launch(const MoeTokensArgs& a, cudaStream_t s) {
   if (start(route, a.T * ranks, ROUTE_THREADS, a.d * sizeof(float), ranks, false, s, a, w, ranks)) return -1;
   if (start(fc_kernel<T, NB>, 2 * a.sms, THREADS, SMEM, 1, true, s, a, w)) return -1;
   const int tiles = (a.d + 15) / 16, parts = std::max(1, std::min(8, 2 * a.sms / tiles));
-  return start(proj_kernel<T, NB>, tiles * parts, THREADS, SMEM, parts, true, s, a, w, parts);
+  return start(proj_kernel<T, NB>, tiles * parts, THREADS, SMEM + WARPS * a.T * 17 * sizeof(float), parts, true, s, a, w, parts);
 }
 }  // namespace moe_tokens
 }  // namespace nt
