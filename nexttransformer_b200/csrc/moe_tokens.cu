@@ -61,47 +61,69 @@ NT_DEVICE void dependents_may_start() { asm volatile("griddepcontrol.launch_depe
 NT_DEVICE void wait_for_predecessor() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 // ------------------------------------------------------------------------------------ route
-template <class T, int PER>  // experts a lane
-__global__ void __launch_bounds__(ROUTE_THREADS) route_kernel(const MoeTokensArgs a, const Workspace w, const int ranks) {
-  extern __shared__ __align__(16) float x[];
+// A cluster of ROUTE_RANKS CTAs has TOKENS tokens, a part of the experts each; the j-th CTA then chooses for the j-th token.  Several
+// tokens share a reading of the router: 64 tokens on 256 experts of width 1280 took 29 us with one token a cluster.
+constexpr int ROUTE_RANKS = 8;
+template <class T, int PER, int TOKENS>  // PER: experts a lane
+__global__ void __launch_bounds__(ROUTE_THREADS) route_kernel(const MoeTokensArgs a, const Workspace w) {
+  extern __shared__ __align__(16) float x[];  // [TOKENS, d]
   __shared__ float logits[EXPERTS];
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, t = blockIdx.x / ranks, rank = blockIdx.x % ranks;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, t0 = blockIdx.x / ROUTE_RANKS * TOKENS, rank = blockIdx.x % ROUTE_RANKS;
+  const int tokens = min(TOKENS, a.T - t0);
   dependents_may_start();
-  const T* src = static_cast<const T*>(a.x) + t * a.x_stride;
-  for (int i = tid * 8; i < a.d; i += ROUTE_THREADS * 8) {
-    const uint4 u = *reinterpret_cast<const uint4*>(src + i);
-    const uint32_t v[4] = {u.x, u.y, u.z, u.w};
+  // the router's rows are on their way while x comes
+  for (int e = rank * ROUTE_WARPS + warp; e < a.E; e += ROUTE_RANKS * ROUTE_WARPS)
+    for (int i = lane * 32; i < a.d; i += 1024) asm volatile("prefetch.global.L2 [%0];" ::"l"(a.router + static_cast<int64_t>(e) * a.d + i));
 #pragma unroll
-    for (int e = 0; e < 4; ++e) *reinterpret_cast<float2*>(x + i + 2 * e) = Num<T>::unpack(v[e]);
+  for (int j = 0; j < TOKENS; ++j) {
+    const T* src = static_cast<const T*>(a.x) + (t0 + min(j, tokens - 1)) * a.x_stride;
+    for (int i = tid * 8; i < a.d; i += ROUTE_THREADS * 8) {
+      const uint4 u = *reinterpret_cast<const uint4*>(src + i);
+      const uint32_t v[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) *reinterpret_cast<float2*>(x + j * a.d + i + 2 * e) = Num<T>::unpack(v[e]);
+    }
+    // x as an operand: lane 4 n + c of a 16 x 8 tile has token n's channels 2 c, 2 c + 1 and 2 c + 8, 2 c + 9
+    const int t = t0 + j, nb = (a.T + 7) / 8, groups = groups_of(a.d);
+    if (j < tokens)
+      for (int i = rank * ROUTE_THREADS + tid; i < groups * 4; i += ROUTE_RANKS * ROUTE_THREADS) {
+        const int g = i >> 2, at = g * 16 + (i & 3) * 2;
+        const uint32_t lo = at < a.d ? *reinterpret_cast<const uint32_t*>(src + at) : 0u;
+        const uint32_t hi = at + 8 < a.d ? *reinterpret_cast<const uint32_t*>(src + at + 8) : 0u;
+        w.x[(static_cast<int64_t>(g) * nb + t / 8) * 32 + (t % 8) * 4 + (i & 3)] = make_uint2(lo, hi);
+      }
   }
-  // x as an operand: lane 4 n + c of a 16 x 8 tile has token n's channels 2 c, 2 c + 1 and 2 c + 8, 2 c + 9
-  const int nb = (a.T + 7) / 8, groups = groups_of(a.d);
-  for (int i = rank * ROUTE_THREADS + tid; i < groups * 4; i += ranks * ROUTE_THREADS) {
-    const int g = i >> 2, at = g * 16 + (i & 3) * 2;
-    const uint32_t lo = at < a.d ? *reinterpret_cast<const uint32_t*>(src + at) : 0u, hi = at + 8 < a.d ? *reinterpret_cast<const uint32_t*>(src + at + 8) : 0u;
-    w.x[(static_cast<int64_t>(g) * nb + t / 8) * 32 + (t % 8) * 4 + (i & 3)] = make_uint2(lo, hi);
-  }
-  cluster_sync();  // x is there, and the first CTA, which gets the logits
-  for (int e = rank * ROUTE_WARPS + warp; e < a.E; e += ranks * ROUTE_WARPS) {
+  cluster_sync();  // x is there, and so are the CTAs that get the logits
+  for (int e = rank * ROUTE_WARPS + warp; e < a.E; e += ROUTE_RANKS * ROUTE_WARPS) {
     const float4* row = reinterpret_cast<const float4*>(a.router + static_cast<int64_t>(e) * a.d);
-    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);  // four chains of d / 128 products a lane
+    float4 sum[TOKENS];  // four chains of d / 128 products a lane
+#pragma unroll
+    for (int j = 0; j < TOKENS; ++j) sum[j] = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 8
     for (int i = lane; i < a.d / 4; i += 32) {
-      const float4 u = row[i], v = reinterpret_cast<const float4*>(x)[i];
-      sum.x = fmaf(u.x, v.x, sum.x);
-      sum.y = fmaf(u.y, v.y, sum.y);
-      sum.z = fmaf(u.z, v.z, sum.z);
-      sum.w = fmaf(u.w, v.w, sum.w);
+      const float4 u = row[i];
+#pragma unroll
+      for (int j = 0; j < TOKENS; ++j) {
+        const float4 v = reinterpret_cast<const float4*>(x + j * a.d)[i];
+        sum[j].x = fmaf(u.x, v.x, sum[j].x);
+        sum[j].y = fmaf(u.y, v.y, sum[j].y);
+        sum[j].z = fmaf(u.z, v.z, sum[j].z);
+        sum[j].w = fmaf(u.w, v.w, sum[j].w);
+      }
     }
-    const float l = warp_sum((sum.x + sum.y) + (sum.z + sum.w));
-    if (lane == 0) {
-      uint32_t to = smem_u32(logits + e), remote;
-      asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(remote) : "r"(to));
-      asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(remote), "f"(l) : "memory");
+#pragma unroll
+    for (int j = 0; j < TOKENS; ++j) {
+      const float l = warp_sum((sum[j].x + sum[j].y) + (sum[j].z + sum[j].w));
+      if (lane == 0) {
+        uint32_t remote;
+        asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(smem_u32(logits + e)), "r"(j));
+        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(remote), "f"(l) : "memory");
+      }
     }
   }
   cluster_sync();
-  if (rank != 0 || warp != 0) return;
+  if (rank >= tokens || warp != 0) return;
+  const int t = t0 + rank;
   float p[PER], score[PER], top = -INFINITY, sum = 0.f;
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
@@ -347,17 +369,19 @@ NT_DEVICE void stream(const MoeTokensArgs& a, const void* smem, const int step, 
   cp_wait<0>();
 }
 
-// NB blocks of 8 tokens an entry: 1 where there are no more than 8 tokens, else 2.
+// NB blocks of 8 tokens an entry: 1 where there are no more than 8 tokens, else 2.  Where there are fewer tiles than warps, `wide`
+// warps share one, a part of its stages each: one token on experts of 1024 x 2048 has 576 tiles for 2368 warps.
 template <class T, int NB>
-__global__ void __launch_bounds__(THREADS, 2) fc_kernel(const MoeTokensArgs a, const Workspace w) {
+__global__ void __launch_bounds__(THREADS, 2) fc_kernel(const MoeTokensArgs a, const Workspace w, const int wide) {
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ Lists l;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  __shared__ float4 parts[2][WARPS][NB][32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, group = warp / wide, part = warp % wide;
   wait_for_predecessor();
   dependents_may_start();
   make_lists(a, w, l);
   const int tiles = (a.F + 15) / 16, shared_tiles = (a.Fs + 15) / 16, groups = groups_of(a.F), shared_groups = groups_of(a.Fs);
-  const int routed = l.routed * tiles, items = routed + (l.entries - l.routed) * shared_tiles, by = gridDim.x * WARPS;
+  const int routed = l.routed * tiles, items = routed + (l.entries - l.routed) * shared_tiles, by = gridDim.x * (WARPS / wide);
   // (the first items go to different SMs)
   auto set = [&](Piece& p, int item) {
     if (item >= items) return false;
@@ -369,15 +393,17 @@ __global__ void __launch_bounds__(THREADS, 2) fc_kernel(const MoeTokensArgs a, c
     p.inner = a.d;
     p.rows = min(16, (shared ? a.Fs : a.F) - p.tile * 16);
     p.blocks = (__popcll(l.mask[p.expert]) - l.first[p.entry] + 7) >> 3;
-    p.stage = 0;
-    p.stages = (a.d + 63) / 64;
+    const int all = (a.d + 63) / 64;
+    p.stage = all * part / wide;
+    p.stages = all * (part + 1) / wide;
     return true;
   };
+  int turn_of_parts = 0;
   auto item_at = [&](const Piece& p) {
     return p.entry >= l.routed ? routed + (p.entry - l.routed) * shared_tiles + p.tile : p.entry * tiles + p.tile;
   };
   stream<T, NB, uint2>(
-      a, smem, (a.T + 7) / 8 * 32, [&](Piece& p) { return set(p, warp * gridDim.x + blockIdx.x); }, [&](Piece& p) { return set(p, item_at(p) + by); },
+      a, smem, (a.T + 7) / 8 * 32, [&](Piece& p) { return set(p, group * gridDim.x + blockIdx.x); }, [&](Piece& p) { return set(p, item_at(p) + by); },
       [&](const Piece& p) -> const void* {
         const T* e = p.expert == a.E ? static_cast<const T*>(a.shared_fc) : static_cast<const T*>(a.w_fc) + static_cast<int64_t>(p.expert) * a.F * a.d;
         return e + static_cast<int64_t>(p.tile) * 16 * a.d;
@@ -388,11 +414,25 @@ __global__ void __launch_bounds__(THREADS, 2) fc_kernel(const MoeTokensArgs a, c
         for (int nb = 0; nb < NB; ++nb) {
           // columns without a token may be anyone's: they are dropped
           const int t = max(0, nth_token(mask, l.first[p.entry] + nb * 8 + (lane >> 2)));
-          at[nb] = w.x + (t >> 3) * 32 + (t & 7) * 4 + (lane & 3);
+          at[nb] = w.x + (t >> 3) * 32 + (t & 7) * 4 + (lane & 3) + p.stage * 4 * ((a.T + 7) / 8 * 32);
         }
       },
       [] {},
-      [&](const Piece& p, const float (&acc)[NB][4]) {
+      [&](const Piece& p, float (&acc)[NB][4]) {
+        if (wide > 1) {  // the first warp adds up, while the others go on to the next tile and its other buffer
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb) parts[turn_of_parts][warp][nb][lane] = make_float4(acc[nb][0], acc[nb][1], acc[nb][2], acc[nb][3]);
+          named_bar_sync(1 + group, wide * 32);
+          if (part == 0)
+            for (int k = 1; k < wide; ++k)
+#pragma unroll
+              for (int nb = 0; nb < NB; ++nb) {
+                const float4 v = parts[turn_of_parts][warp + k][nb][lane];
+                acc[nb][0] += v.x; acc[nb][1] += v.y; acc[nb][2] += v.z; acc[nb][3] += v.w;
+              }
+          turn_of_parts ^= 1;
+          if (part) return;
+        }
         // h, in the order in which it is an operand: rows of the tile become the products' inner dimension.  It is held as two
         // numbers of its type, so that nothing but the output is rounded.
         const bool shared = p.expert == a.E;
@@ -543,18 +583,29 @@ static int start(Kernel kern, int grid, int threads, size_t smem, int cluster, b
   cfg.numAttrs = n;
   return cudaLaunchKernelEx(&cfg, kern, args...) == cudaSuccess ? 0 : -1;
 }
+template <class T, int TOKENS>
+static int route(const MoeTokensArgs& a, const Workspace& w, cudaStream_t s) {
+  const auto kern = a.E <= 64 ? route_kernel<T, 2, TOKENS> : a.E <= 256 ? route_kernel<T, 8, TOKENS> : route_kernel<T, EXPERTS / 32, TOKENS>;
+  return start(kern, (a.T + TOKENS - 1) / TOKENS * ROUTE_RANKS, ROUTE_THREADS, TOKENS * a.d * sizeof(float), ROUTE_RANKS, false, s, a, w);
+}
+template <class T>
+static int route_for(const MoeTokensArgs& a, const Workspace& w, cudaStream_t s) {
+  // as few tokens a cluster as keep the clusters on the SMs at once, and as 48 KB hold
+  if (a.T * ROUTE_RANKS <= a.sms || a.d * 16 > 48 * 1024) return route<T, 1>(a, w, s);
+  return route<T, 4>(a, w, s);
+}
 template <class T, int NB>
 static int launch(const MoeTokensArgs& a, cudaStream_t s) {
   static std::atomic<uint64_t> fc_done{0}, proj_done{0};
   if (smem_limit(fc_done, fc_kernel<T, NB>, SMEM) != cudaSuccess || smem_limit(proj_done, proj_kernel<T, NB>, SMEM + WARPS * MOST * 17 * sizeof(float)) != cudaSuccess) return -1;
   Workspace w;
   layout(a, w);
-  int ranks = 8;
-  while (ranks > 1 && a.T * ranks > 2 * a.sms) ranks /= 2;
-  const auto route = a.E <= 64 ? route_kernel<T, 2> : a.E <= 256 ? route_kernel<T, 8> : route_kernel<T, EXPERTS / 32>;
-  if (start(route, a.T * ranks, ROUTE_THREADS, a.d * sizeof(float), ranks, false, s, a, w, ranks)) return -1;
-  if (start(fc_kernel<T, NB>, 2 * a.sms, THREADS, SMEM, 1, true, s, a, w)) return -1;
-  const int tiles = (a.d + 15) / 16, parts = std::max(1, std::min(8, 2 * a.sms / tiles));
+  if (route_for<T>(a, w, s)) return -1;
+  const int64_t tiles_most = static_cast<int64_t>(std::min(a.E, a.T * a.k)) * blocks_of(a.F, 16) + static_cast<int64_t>(blocks_of(a.T, 16)) * blocks_of(a.Fs, 16);
+  int wide = 1;
+  while (wide < WARPS && tiles_most * wide * 2 <= 2 * a.sms * WARPS && wide * 2 <= blocks_of(a.d, 64)) wide *= 2;
+  if (start(fc_kernel<T, NB>, 2 * a.sms, THREADS, SMEM, 1, true, s, a, w, wide)) return -1;
+  const int tiles = blocks_of(a.d, 16), parts = std::max(1, std::min(8, 2 * a.sms / tiles));
   return start(proj_kernel<T, NB>, tiles * parts, THREADS, SMEM + WARPS * a.T * 17 * sizeof(float), parts, true, s, a, w, parts);
 }
 }  // namespace moe_tokens
