@@ -57,6 +57,10 @@ static size_t layout(const MoeTokensArgs& a, Workspace& w) {
   return at;
 }
 
+// L2 fetches 256 bytes at once: rows lie far apart, and the next stage wants the other half.
+NT_DEVICE void cp_async16_far(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global.L2::256B [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
 NT_DEVICE void dependents_may_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 NT_DEVICE void wait_for_predecessor() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
@@ -293,7 +297,7 @@ NT_DEVICE void stream(const MoeTokensArgs& a, const void* smem, const int step, 
       if (f.rows == 16 && (f.stage + 1) * 64 <= f.inner) {
         const char* p = f_at;
 #pragma unroll
-        for (int e = 0; e < 4; ++e, p += f_step) cp_async16(r.in + r.to[e & 1] + (e >> 1) * 1024, p);
+        for (int e = 0; e < 4; ++e, p += f_step) cp_async16_far(r.in + r.to[e & 1] + (e >> 1) * 1024, p);
       } else {  // what is not there becomes zero
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -323,7 +327,7 @@ NT_DEVICE void stream(const MoeTokensArgs& a, const void* smem, const int step, 
     for (int nb = 0; nb < NB; ++nb)
       if (nb == 0 || nb < o.blocks) {
 #pragma unroll
-        for (int s = 0; s < 4; ++s) b[s][nb] = __ldcg(at[nb] + s * step);
+        for (int s = 0; s < 4; ++s) b[s][nb] = TWO ? __ldcg(at[nb] + s * step) : at[nb][s * step];
         at[nb] += 4 * step;
       }
     if (++o.stage == o.stages) {
@@ -369,19 +373,24 @@ NT_DEVICE void stream(const MoeTokensArgs& a, const void* smem, const int step, 
   cp_wait<0>();
 }
 
-// NB blocks of 8 tokens an entry: 1 where there are no more than 8 tokens, else 2.  Where there are fewer tiles than warps, `wide`
-// warps share one, a part of its stages each: one token on experts of 1024 x 2048 has 576 tiles for 2368 warps.
+// NB blocks of 8 tokens an entry: 1 where there are no more than 8 tokens, else 2.  `wide`
+// warps share a tile, a part of its stages each, where the last round of tiles would leave more than a twelfth of the warps' time
+// unused: one token on experts of 1024 x 2048 has 576 tiles for 2368 warps, twelve tokens have about 3800.
 template <class T, int NB>
-__global__ void __launch_bounds__(THREADS, 2) fc_kernel(const MoeTokensArgs a, const Workspace w, const int wide) {
+__global__ void __launch_bounds__(THREADS, 2) fc_kernel(const MoeTokensArgs a, const Workspace w) {
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ Lists l;
   __shared__ float4 parts[2][WARPS][NB][32];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, group = warp / wide, part = warp % wide;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   wait_for_predecessor();
   dependents_may_start();
   make_lists(a, w, l);
   const int tiles = (a.F + 15) / 16, shared_tiles = (a.Fs + 15) / 16, groups = groups_of(a.F), shared_groups = groups_of(a.Fs);
-  const int routed = l.routed * tiles, items = routed + (l.entries - l.routed) * shared_tiles, by = gridDim.x * (WARPS / wide);
+  const int routed = l.routed * tiles, items = routed + (l.entries - l.routed) * shared_tiles;
+  const int stages = (a.d + 63) / 64, slots = gridDim.x * WARPS;
+  int wide = 1;
+  while (wide < WARPS && 2 * wide <= stages && (items * wide + slots - 1) / slots * slots * 12 > items * wide * 13) wide *= 2;
+  const int group = warp / wide, part = warp % wide, by = gridDim.x * (WARPS / wide);
   // (the first items go to different SMs)
   auto set = [&](Piece& p, int item) {
     if (item >= items) return false;
@@ -393,9 +402,8 @@ __global__ void __launch_bounds__(THREADS, 2) fc_kernel(const MoeTokensArgs a, c
     p.inner = a.d;
     p.rows = min(16, (shared ? a.Fs : a.F) - p.tile * 16);
     p.blocks = (__popcll(l.mask[p.expert]) - l.first[p.entry] + 7) >> 3;
-    const int all = (a.d + 63) / 64;
-    p.stage = all * part / wide;
-    p.stages = all * (part + 1) / wide;
+    p.stage = stages * part / wide;
+    p.stages = stages * (part + 1) / wide;
     return true;
   };
   int turn_of_parts = 0;
@@ -601,10 +609,7 @@ static int launch(const MoeTokensArgs& a, cudaStream_t s) {
   Workspace w;
   layout(a, w);
   if (route_for<T>(a, w, s)) return -1;
-  const int64_t tiles_most = static_cast<int64_t>(std::min(a.E, a.T * a.k)) * blocks_of(a.F, 16) + static_cast<int64_t>(blocks_of(a.T, 16)) * blocks_of(a.Fs, 16);
-  int wide = 1;
-  while (wide < WARPS && tiles_most * wide * 2 <= 2 * a.sms * WARPS && wide * 2 <= blocks_of(a.d, 64)) wide *= 2;
-  if (start(fc_kernel<T, NB>, 2 * a.sms, THREADS, SMEM, 1, true, s, a, w, wide)) return -1;
+  if (start(fc_kernel<T, NB>, 2 * a.sms, THREADS, SMEM, 1, true, s, a, w)) return -1;
   const int tiles = blocks_of(a.d, 16), parts = std::max(1, std::min(8, 2 * a.sms / tiles));
   return start(proj_kernel<T, NB>, tiles * parts, THREADS, SMEM + WARPS * a.T * 17 * sizeof(float), parts, true, s, a, w, parts);
 }
