@@ -78,15 +78,21 @@ __global__ void __launch_bounds__(ROUTE_THREADS) route_kernel(const MoeTokensArg
   // the router's rows are on their way while x comes
   for (int e = rank * ROUTE_WARPS + warp; e < a.E; e += ROUTE_RANKS * ROUTE_WARPS)
     for (int i = lane * 32; i < a.d; i += 1024) asm volatile("prefetch.global.L2 [%0];" ::"l"(a.router + static_cast<int64_t>(e) * a.d + i));
+  for (int i = tid * 8; i < a.d; i += ROUTE_THREADS * 8) {
+    uint4 u[TOKENS];
 #pragma unroll
-  for (int j = 0; j < TOKENS; ++j) {
-    const T* src = static_cast<const T*>(a.x) + (t0 + min(j, tokens - 1)) * a.x_stride;
-    for (int i = tid * 8; i < a.d; i += ROUTE_THREADS * 8) {
-      const uint4 u = *reinterpret_cast<const uint4*>(src + i);
-      const uint32_t v[4] = {u.x, u.y, u.z, u.w};
+    for (int j = 0; j < TOKENS; ++j)
+      u[j] = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.x) + (t0 + min(j, tokens - 1)) * a.x_stride + i);
+#pragma unroll
+    for (int j = 0; j < TOKENS; ++j) {
+      const uint32_t v[4] = {u[j].x, u[j].y, u[j].z, u[j].w};
 #pragma unroll
       for (int e = 0; e < 4; ++e) *reinterpret_cast<float2*>(x + j * a.d + i + 2 * e) = Num<T>::unpack(v[e]);
     }
+  }
+#pragma unroll
+  for (int j = 0; j < TOKENS; ++j) {
+    const T* src = static_cast<const T*>(a.x) + (t0 + min(j, tokens - 1)) * a.x_stride;
     // x as an operand: lane 4 n + c of a 16 x 8 tile has token n's channels 2 c, 2 c + 1 and 2 c + 8, 2 c + 9
     const int t = t0 + j, nb = (a.T + 7) / 8, groups = groups_of(a.d);
     if (j < tokens)
@@ -98,32 +104,44 @@ __global__ void __launch_bounds__(ROUTE_THREADS) route_kernel(const MoeTokensArg
       }
   }
   cluster_sync();  // x is there, and so are the CTAs that get the logits
-  for (int e = rank * ROUTE_WARPS + warp; e < a.E; e += ROUTE_RANKS * ROUTE_WARPS) {
-    const float4* row = reinterpret_cast<const float4*>(a.router + static_cast<int64_t>(e) * a.d);
-    float4 sum[TOKENS];  // four chains of d / 128 products a lane
+  constexpr int ROWS = 2, BY = ROUTE_RANKS * ROUTE_WARPS;  // experts at once
+  for (int e0 = rank * ROUTE_WARPS + warp; e0 < a.E; e0 += ROWS * BY) {
+    float4 sum[ROWS][TOKENS];  // four chains of d / 128 products a lane
+    const float4* row[ROWS];
 #pragma unroll
-    for (int j = 0; j < TOKENS; ++j) sum[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int k = 0; k < ROWS; ++k) {
+      row[k] = reinterpret_cast<const float4*>(a.router + static_cast<int64_t>(min(e0 + k * BY, a.E - 1)) * a.d);
+#pragma unroll
+      for (int j = 0; j < TOKENS; ++j) sum[k][j] = make_float4(0.f, 0.f, 0.f, 0.f);
+    }
 #pragma unroll 8
     for (int i = lane; i < a.d / 4; i += 32) {
-      const float4 u = row[i];
+      float4 u[ROWS];
+#pragma unroll
+      for (int k = 0; k < ROWS; ++k) u[k] = row[k][i];
 #pragma unroll
       for (int j = 0; j < TOKENS; ++j) {
         const float4 v = reinterpret_cast<const float4*>(x + j * a.d)[i];
-        sum[j].x = fmaf(u.x, v.x, sum[j].x);
-        sum[j].y = fmaf(u.y, v.y, sum[j].y);
-        sum[j].z = fmaf(u.z, v.z, sum[j].z);
-        sum[j].w = fmaf(u.w, v.w, sum[j].w);
+#pragma unroll
+        for (int k = 0; k < ROWS; ++k) {
+          sum[k][j].x = fmaf(u[k].x, v.x, sum[k][j].x);
+          sum[k][j].y = fmaf(u[k].y, v.y, sum[k][j].y);
+          sum[k][j].z = fmaf(u[k].z, v.z, sum[k][j].z);
+          sum[k][j].w = fmaf(u[k].w, v.w, sum[k][j].w);
+        }
       }
     }
 #pragma unroll
-    for (int j = 0; j < TOKENS; ++j) {
-      const float l = warp_sum((sum[j].x + sum[j].y) + (sum[j].z + sum[j].w));
-      if (lane == 0) {
-        uint32_t remote;
-        asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(smem_u32(logits + e)), "r"(j));
-        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(remote), "f"(l) : "memory");
+    for (int k = 0; k < ROWS; ++k)
+#pragma unroll
+      for (int j = 0; j < TOKENS; ++j) {
+        const float v = warp_sum((sum[k][j].x + sum[k][j].y) + (sum[k][j].z + sum[k][j].w));
+        if (lane == 0 && e0 + k * BY < a.E) {
+          uint32_t remote;
+          asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(smem_u32(logits + e0 + k * BY)), "r"(j));
+          asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(remote), "f"(v) : "memory");
+        }
       }
-    }
   }
   cluster_sync();
   if (rank >= tokens || warp != 0) return;
@@ -189,6 +207,7 @@ struct Lists {
   unsigned long long mask[EXPERTS + 1];  // an expert's tokens; [E]: the shared expert's, all
   uint16_t expert[ENTRIES], block[ENTRIES];  // an entry's expert, and its first block of 8 tokens in h
   uint8_t first[ENTRIES];                // the first of its tokens, counted among the expert's
+  uint8_t blocks[ENTRIES];               // of 8 of its tokens: 1 or 2
   int routed, entries;
 };
 NT_DEVICE void make_lists(const MoeTokensArgs& a, const Workspace& w, Lists& l) {
@@ -213,6 +232,7 @@ NT_DEVICE void make_lists(const MoeTokensArgs& a, const Workspace& w, Lists& l) 
         l.expert[at] = static_cast<uint16_t>(e);
         l.block[at] = static_cast<uint16_t>(blocks + ((upto - own) >> 16) + 2 * i);
         l.first[at] = static_cast<uint8_t>(16 * i);
+        l.blocks[at] = static_cast<uint8_t>(tokens - 16 * i > 8 ? 2 : 1);
       }
       const int all = __shfl_sync(0xffffffffu, upto, 31);
       n += all & 0xffff;
@@ -223,6 +243,7 @@ NT_DEVICE void make_lists(const MoeTokensArgs& a, const Workspace& w, Lists& l) 
       l.expert[n + lane] = static_cast<uint16_t>(a.E);
       l.block[n + lane] = static_cast<uint16_t>(2 * lane);
       l.first[n + lane] = static_cast<uint8_t>(16 * lane);
+      l.blocks[n + lane] = static_cast<uint8_t>(a.T - 16 * lane > 8 ? 2 : 1);
     }
     if (lane == 0) {
       l.mask[a.E] = a.T == 64 ? ~0ull : (1ull << a.T) - 1;
@@ -266,6 +287,7 @@ struct Piece {
   int inner, rows;    // elements of a weight row; rows of the tile (16, or fewer at the end)
   int blocks;         // of 8 tokens
   int stage, stages;  // the next one; the first behind the piece
+  int behind;         // what comes after it: an item, or a stage of all
 };
 
 // Goes through a warp's pieces: weights come `STAGES - 1` stages ahead, the other operand one.
@@ -401,17 +423,15 @@ __global__ void __launch_bounds__(THREADS, 2) fc_kernel(const MoeTokensArgs a, c
     p.expert = l.expert[p.entry];
     p.inner = a.d;
     p.rows = min(16, (shared ? a.Fs : a.F) - p.tile * 16);
-    p.blocks = (__popcll(l.mask[p.expert]) - l.first[p.entry] + 7) >> 3;
+    p.blocks = l.blocks[p.entry];
     p.stage = stages * part / wide;
     p.stages = stages * (part + 1) / wide;
+    p.behind = item + by;
     return true;
   };
   int turn_of_parts = 0;
-  auto item_at = [&](const Piece& p) {
-    return p.entry >= l.routed ? routed + (p.entry - l.routed) * shared_tiles + p.tile : p.entry * tiles + p.tile;
-  };
   stream<T, NB, uint2>(
-      a, smem, (a.T + 7) / 8 * 32, [&](Piece& p) { return set(p, group * gridDim.x + blockIdx.x); }, [&](Piece& p) { return set(p, item_at(p) + by); },
+      a, smem, (a.T + 7) / 8 * 32, [&](Piece& p) { return set(p, group * gridDim.x + blockIdx.x); }, [&](Piece& p) { return set(p, p.behind); },
       [&](const Piece& p) -> const void* {
         const T* e = p.expert == a.E ? static_cast<const T*>(a.shared_fc) : static_cast<const T*>(a.w_fc) + static_cast<int64_t>(p.expert) * a.F * a.d;
         return e + static_cast<int64_t>(p.tile) * 16 * a.d;
@@ -487,25 +507,34 @@ __global__ void __launch_bounds__(THREADS, 2) proj_kernel(const MoeTokensArgs a,
   const int routed = l.routed * per, all = routed + (l.entries - l.routed) * shared_per;
   const int runs = parts * WARPS, run = part * WARPS + warp, few = all / runs, more = all % runs;
   const int first = run * few + min(run, more), last = first + few + (run < more ? 1 : 0);
-  auto set = [&](Piece& p, int at) {
-    if (at >= last) return false;
-    const bool shared = at >= routed;
-    const int i = shared ? at - routed : at, n = quotient(i, shared ? shared_per : per);
-    p.entry = (shared ? l.routed : 0) + n;
+  auto enter = [&](Piece& p, int at) {  // at stage p.stage of p.entry, which is stage `at` of all
+    const bool shared = p.entry >= l.routed;
     p.tile = tile;
     p.expert = l.expert[p.entry];
     p.inner = shared ? a.Fs : a.F;
     p.rows = min(16, a.d - tile * 16);
-    p.blocks = (__popcll(l.mask[p.expert]) - l.first[p.entry] + 7) >> 3;
-    p.stage = i - n * (shared ? shared_per : per);
+    p.blocks = l.blocks[p.entry];
     p.stages = min(shared ? shared_per : per, p.stage + last - at);
+    p.behind = at + p.stages - p.stage;
+  };
+  auto set = [&](Piece& p) {
+    if (first >= last) return false;
+    const bool shared = first >= routed;
+    const int i = shared ? first - routed : first, n = quotient(i, shared ? shared_per : per);
+    p.entry = (shared ? l.routed : 0) + n;
+    p.stage = i - n * (shared ? shared_per : per);
+    enter(p, first);
     return true;
   };
-  auto end_of = [&](const Piece& p) {  // the stage behind it, among all
-    return p.entry >= l.routed ? routed + (p.entry - l.routed) * shared_per + p.stages : p.entry * per + p.stages;
+  auto next = [&](Piece& p) {
+    if (p.behind >= last) return false;
+    ++p.entry;
+    p.stage = 0;
+    enter(p, p.behind);
+    return true;
   };
   stream<T, NB, uint4>(
-      a, smem, 32, [&](Piece& p) { return set(p, first); }, [&](Piece& p) { return set(p, end_of(p)); },
+      a, smem, 32, set, next,
       [&](const Piece& p) -> const void* {
         const T* e = p.expert == a.E ? static_cast<const T*>(a.shared_proj) : static_cast<const T*>(a.w_proj) + static_cast<int64_t>(p.expert) * a.d * a.F;
         return e + static_cast<int64_t>(tile) * 16 * p.inner;
