@@ -9,16 +9,19 @@ shell decode by re-running the full prefix, as the reference's ``generate`` does
 models and delta-rule hybrids (DeltaNet, GDN, KDA layers between the shell's attention) alike: keys and values
 lie in pages that rows take and give back (``ops.paged``), linear layers carry their convolution inputs and
 recurrent state (``ops.delta_recurrent``), and next-token logits pass ``ops.logits.adjust_logits`` before they
-are sampled.
+are sampled.  The cache may be held in 8 bits, the experts of a mixture-of-experts model may be laid out for a few tokens
+(``serve_experts``, ``ops.moe.moe_tokens``), and ``ops.sampling.sample_logits`` draws with top-p and min-p.
 """
 import torch
 import torch.nn.functional as F
 
 from nexttransformer_b200.models.linear import LinearMixer
+from nexttransformer_b200.models.moe import MoEFFN
 from nexttransformer_b200.models.shell import Block, CausalSelfAttention, apply_rotary_emb, norm
 from nexttransformer_b200.ops._ext import check_errors
 from nexttransformer_b200.ops.logits import adjust_logits
-from nexttransformer_b200.ops.paged import paged_append, paged_attention
+from nexttransformer_b200.ops.paged import BLOCK, paged_append, paged_attention
+from nexttransformer_b200.ops.sampling import sample_logits
 
 
 class KVCache:
@@ -126,21 +129,30 @@ class PagedCache:
 
     Attention layers share one pool of ``pages`` pages of ``page`` tokens (by default enough for every row to
     reach ``max_len``); ``reserve`` gives a row the pages for its next tokens, ``release`` takes them back and
-    clears the row.
+    clears the row.  ``dtype`` is what keys and values are held in: the model's type, or ``torch.float8_e4m3fn`` with a scale
+    for each 16 tokens and KV head (half the memory, and half of what attention reads).
     """
 
-    def __init__(self, model, rows, max_len, page=64, pages=None):
+    def __init__(self, model, rows, max_len, page=64, pages=None, dtype=None):
         if not supports_paged(model):
             raise ValueError("this model has layers that the paged decoder does not serve")
-        cfg, device, dtype = model.shell, model.get_device(), model.cos.dtype
+        cfg, device = model.shell, model.get_device()
+        held, dtype = model.cos.dtype if dtype is None else dtype, model.cos.dtype
+        if held not in (dtype, torch.float8_e4m3fn):
+            raise ValueError("the cache is held in the model's type or in float8_e4m3fn")
         self.rows, self.page, self.columns = rows, page, -(-max_len // page)
         pages = rows * self.columns if pages is None else pages
         mixers = [b.attn for b in model.transformer.h]
         attention = [i for i, a in enumerate(mixers) if type(a) is CausalSelfAttention]
         linear = [i for i, a in enumerate(mixers) if type(a) is LinearMixer]
         shape = (len(attention), pages, cfg.n_kv_head, page, cfg.head_dim)
-        keys, values = torch.zeros(shape, device=device, dtype=dtype), torch.zeros(shape, device=device, dtype=dtype)
+        keys, values = torch.zeros(shape, device=device, dtype=held), torch.zeros(shape, device=device, dtype=held)
         self.pages = {i: (keys[n], values[n]) for n, i in enumerate(attention)}
+        self.scales = {i: {} for i in attention}
+        if held == torch.float8_e4m3fn:
+            shape = (2, *shape[:3], -(-page // BLOCK))
+            k_scale, v_scale = torch.zeros(shape, device=device)
+            self.scales = {i: dict(k_scale=k_scale[n], v_scale=v_scale[n]) for n, i in enumerate(attention)}
         self.linear = {}
         for i in linear:
             c = mixers[i].config
@@ -184,6 +196,14 @@ class PagedCache:
         for conv, state in self.linear.values():
             conv[row] = 0
             state[row] = 0
+
+
+def serve_experts(model):
+    """Lay the experts of a mixture-of-experts model out for decoding (``MoEFFN.serve``), once its weights are what is to be
+    served; ``decode_paged`` then sends calls of up to 64 tokens through ``ops.moe.moe_tokens``.  Other layers are left alone."""
+    for b in model.transformer.h:
+        if isinstance(b.mlp, MoEFFN):
+            b.mlp.serve(model.cos.dtype)
 
 
 @torch.no_grad()
@@ -232,20 +252,35 @@ def decode_paged(model, idx, cache, counts=None):
                 gate = a.ve_gate(h[..., :a.ve_gate_channels])
                 ve = ve.view(B, t, a.n_kv_head, a.head_dim)
             q = paged_append(q, k, v, *cache.pages[i], cache.table, cache.start, count, cos=cos, sin=sin, qk_scale=1.2,
-                             ve=ve if gate is not None else None, ve_gate=gate)
-            y = paged_attention(q, *cache.pages[i], cache.table, cache.start, count, window=model.layer_window(i))
+                             ve=ve if gate is not None else None, ve_gate=gate, **cache.scales[i])
+            y = paged_attention(q, *cache.pages[i], cache.table, cache.start, count, window=model.layer_window(i), **cache.scales[i])
             y = a.c_proj(y.view(B, t, -1))
         x = x + y
-        x = x + blk.mlp(norm(x))
+        x = x + (blk.mlp.step if isinstance(blk.mlp, MoEFFN) else blk.mlp)(norm(x))
         if i == n // 2:
             backout = x
     cache.advance(counts, count)
     return model.readout(x.gather(1, last), backout.gather(1, last) if backout is not None else None)[:, -1]
 
 
+def _drawn_by_softmax(logits, temperature, top_k, g):
+    """Next tokens ``[B, 1]`` by ``torch.multinomial``, and which rows permit no token or hold a NaN."""
+    if top_k:
+        v, _ = torch.topk(logits, min(top_k, logits.size(-1)))
+        logits = logits.masked_fill(logits < v[:, [-1]], -float("inf"))
+    # a row whose largest logit is not finite (over a small temperature, too) has a softmax of NaN, which sampling on
+    # CUDA answers with a device assert: its largest logits share the choice; rows that have none are told apart below
+    top = logits.amax(-1, keepdim=True)
+    scaled = logits / temperature if temperature > 0 else logits
+    scaled = torch.where(scaled.amax(-1, keepdim=True).isfinite(), scaled,
+                         torch.where(top.isnan() | (logits == top), 0.0, -torch.inf))
+    nxt = torch.multinomial(F.softmax(scaled, -1), 1, generator=g) if temperature > 0 else scaled.argmax(-1, keepdim=True)
+    return nxt, top == -torch.inf, top.isnan()
+
+
 @torch.no_grad()
 def generate_batch(model, prompts, max_tokens, temperature=1.0, top_k=None, seed=42, stop=(), repetition=None,
-                   presence=None, frequency=None, bias=None, allowed=None, page=64):
+                   presence=None, frequency=None, bias=None, allowed=None, page=64, top_p=None, min_p=None, cache_dtype=None):
     """Sample up to ``max_tokens`` tokens after each of ``prompts`` (lists of ints); a list of lists comes back.
 
     A row ends behind a token of ``stop``.  ``repetition``, ``presence`` and ``frequency`` are numbers, ``bias`` a
@@ -254,13 +289,24 @@ def generate_batch(model, prompts, max_tokens, temperature=1.0, top_k=None, seed
     ``ops.logits.adjust_logits``).  A row that it allows nothing ends there; rows that have ended may have any mask.  A
     bias of inf settles the choice; a NaN among a row's logits raises, as does at the end whatever the kernels recorded
     (``ops._ext.check_errors``).
+
+    With ``top_p`` or ``min_p``, or where ``temperature`` or ``top_k`` is a list with one value for each prompt (as all four may
+    be), tokens are drawn by ``ops.sampling.sample_logits`` from numbers of the seed's generator.  ``cache_dtype`` is the cache's
+    (``PagedCache``).
     """
     if not prompts or any(not p for p in prompts):
         raise ValueError("every prompt needs at least one token")
     dev, B = model.get_device(), len(prompts)
     lengths = [len(p) for p in prompts]
-    cache = PagedCache(model, B, max(lengths) + max_tokens, page)
-    g = torch.Generator(device=dev).manual_seed(seed) if temperature > 0 else None
+    filters = dict(temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
+    drawn = top_p is not None or min_p is not None or any(isinstance(v, (list, tuple)) for v in filters.values())
+    for name, v in filters.items():
+        if isinstance(v, (list, tuple)):
+            if len(v) != B:
+                raise ValueError(f"{name}: one value for each prompt")
+            filters[name] = torch.tensor(v, dtype=torch.int32 if name == "top_k" else torch.float32, device=dev)
+    cache = PagedCache(model, B, max(lengths) + max_tokens, page, dtype=cache_dtype)
+    g = torch.Generator(device=dev).manual_seed(seed) if drawn or temperature > 0 else None
     history = torch.zeros(B, max(lengths) + max_tokens, dtype=torch.int32)
     for row, p in enumerate(prompts):
         history[row, :len(p)] = torch.tensor(p, dtype=torch.int32)
@@ -279,17 +325,12 @@ def generate_batch(model, prompts, max_tokens, temperature=1.0, top_k=None, seed
     for step in range(max_tokens):
         logits = adjust_logits(logits, tokens=history, length=length, prompt=prompt, **penalties,
                                allowed=None if allowed is None else allowed(answers).to(dev))
-        if top_k:
-            v, _ = torch.topk(logits, min(top_k, logits.size(-1)))
-            logits = logits.masked_fill(logits < v[:, [-1]], -float("inf"))
-        # a row whose largest logit is not finite (over a small temperature, too) has a softmax of NaN, which sampling on
-        # CUDA answers with a device assert: its largest logits share the choice; rows that have none are told apart below
-        top = logits.amax(-1, keepdim=True)
-        scaled = logits / temperature if temperature > 0 else logits
-        scaled = torch.where(scaled.amax(-1, keepdim=True).isfinite(), scaled,
-                             torch.where(top.isnan() | (logits == top), 0.0, -torch.inf))
-        nxt = torch.multinomial(F.softmax(scaled, -1), 1, generator=g) if temperature > 0 else scaled.argmax(-1, keepdim=True)
-        for row, (token, nothing, broken) in enumerate(torch.cat((nxt, top == -torch.inf, top.isnan()), 1).tolist()):
+        if drawn:
+            token, _ = sample_logits(logits, torch.rand(B, generator=g, device=dev), **filters)
+            nxt, nothing, broken = token.clamp(min=0)[:, None], token[:, None] == -1, token[:, None] == -2
+        else:
+            nxt, nothing, broken = _drawn_by_softmax(logits, temperature, top_k, g)
+        for row, (token, nothing, broken) in enumerate(torch.cat((nxt, nothing, broken), 1).tolist()):
             if live[row] and broken:
                 raise RuntimeError(f"NaN among the logits of row {row}")
             if live[row] and not nothing:

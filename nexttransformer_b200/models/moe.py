@@ -58,6 +58,7 @@ class MoEFFN(nn.Module):
         # CUDA routing through the fused kernels (ops.moe.fused_route); False: the torch ops below
         self.fused_route = True
         self._plan = None
+        self._served = None        # weights laid out for ``step`` by ``serve``
 
     # -------------------------------------------------------------- experts held by this rank
     def local_experts(self):
@@ -149,6 +150,33 @@ class MoEFFN(nn.Module):
             start += n
         y = torch.cat(outs) if outs else xs.new_zeros(0, rows.shape[-1])
         return torch.zeros_like(rows).index_add(0, tokens[:y.shape[0]], y)
+
+    # -------------------------------------------------------------- decoding
+    @torch.no_grad()
+    def serve(self, dtype):
+        """Lay the weights out in ``dtype`` for ``step``: once, before decoding, and again after they have changed.  A layer with
+        kernel state on CUDA in bf16 shares the routed experts' stacks, which the optimizer keeps; everything else is a copy."""
+        if self.ep_size > 1:
+            raise ValueError("experts of other ranks are not served here")
+        experts = self.local_experts()
+        stacked = self._w_fc is not None and dtype == torch.bfloat16
+        self._served = dict(
+            router=self.router.weight.detach().float().contiguous().clone(),
+            w_fc=self._w_fc if stacked else torch.stack([e.c_fc.weight.detach().to(dtype) for e in experts]),
+            w_proj=self._w_proj if stacked else torch.stack([e.c_proj.weight.detach().to(dtype) for e in experts]),
+            shared_fc=None if self.shared is None else self.shared.c_fc.weight.detach().to(dtype, copy=True).contiguous(),
+            shared_proj=None if self.shared is None else self.shared.c_proj.weight.detach().to(dtype, copy=True).contiguous())
+
+    def step(self, x):
+        """``forward`` without gradients and load statistics for a few tokens: ``ops.moe.moe_tokens`` on the weights that ``serve``
+        laid out.  More tokens than that takes, other types than they have, and a layer that was not laid out go through ``forward``."""
+        from nexttransformer_b200.ops.moe import TOKENS_MOST, moe_tokens
+        rows = x.reshape(-1, x.shape[-1])
+        s = self._served
+        if s is None or rows.shape[0] > TOKENS_MOST or s["w_fc"].dtype != x.dtype or s["w_fc"].device != x.device:
+            return self(x)
+        return moe_tokens(rows, s["router"], s["w_fc"], s["w_proj"], self.top_k, bias=self.expert_bias, shared_fc=s["shared_fc"],
+                          shared_proj=s["shared_proj"]).reshape_as(x)
 
     @torch.no_grad()
     def update_bias(self):
