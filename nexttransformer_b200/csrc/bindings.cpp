@@ -1257,6 +1257,7 @@ std::vector<int64_t> read_errors() {
 }
 
 // ------------------------------------------------------------------ serving
+// (Numbers go into messages as text: a stream of the C++ library that builds this and the one that loads it may differ.)
 void inference_only(std::initializer_list<const Tensor*> tensors, std::initializer_list<const OptT*> optional = {}) {
   if (!at::GradMode::is_enabled()) return;
   auto check = [](const Tensor& t) {
@@ -1582,7 +1583,7 @@ std::vector<Tensor> sample_logits(const Tensor& logits, const Tensor& uniform, c
   TORCH_CHECK(logits.dim() == 2 && (logits.stride(1) == 1 || logits.size(1) == 1), "logits must be [B, V] with contiguous rows");
   SampleArgs a;
   const int64_t B = logits.size(0), V = logits.size(1);
-  TORCH_CHECK(V >= 1 && V <= nt_sample_most(), "sample_logits takes vocabularies of 1 to ", nt_sample_most(), " tokens");
+  TORCH_CHECK(V >= 1 && V <= nt_sample_most(), "sample_logits takes vocabularies of 1 to ", std::to_string(nt_sample_most()), " tokens");
   TORCH_CHECK(B <= INT32_MAX / 8, "sample_logits: too many rows");
   a.B = static_cast<int>(B);
   a.V = static_cast<int>(V);
@@ -1624,9 +1625,9 @@ Tensor moe_tokens(const Tensor& x, const Tensor& router, const Tensor& w_fc, con
   inference_only({&x, &router, &w_fc, &w_proj}, {&bias, &shared_fc, &shared_proj});
   const auto type = x.scalar_type();
   TORCH_CHECK(type == at::kBFloat16 || type == at::kHalf, "moe_tokens takes bf16 or fp16");
-  TORCH_CHECK(x.dim() == 2 && x.size(0) <= NT_MOE_TOKENS_MOST, "x must be [T, d] with at most ", NT_MOE_TOKENS_MOST, " tokens");
+  TORCH_CHECK(x.dim() == 2 && x.size(0) <= NT_MOE_TOKENS_MOST, "x must be [T, d] with at most ", std::to_string(NT_MOE_TOKENS_MOST), " tokens");
   const int64_t T = x.size(0), d = x.size(1);
-  TORCH_CHECK(d >= 8 && d % 8 == 0 && d <= NT_MOE_TOKENS_WIDTH, "the width must be a multiple of 8, at most ", NT_MOE_TOKENS_WIDTH);
+  TORCH_CHECK(d >= 8 && d % 8 == 0 && d <= NT_MOE_TOKENS_WIDTH, "the width must be a multiple of 8, at most ", std::to_string(NT_MOE_TOKENS_WIDTH));
   TORCH_CHECK((x.stride(1) == 1) && (T <= 1 || x.stride(0) % 8 == 0), "x must have contiguous rows on 16-byte boundaries");
   const auto aligned = [](const Tensor& t, const char* name) {
     TORCH_CHECK(reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0, name, " must be 16-byte aligned");
@@ -1634,10 +1635,10 @@ Tensor moe_tokens(const Tensor& x, const Tensor& router, const Tensor& w_fc, con
   aligned(x, "x");
   TORCH_CHECK(router.device() == x.device() && router.scalar_type() == at::kFloat && router.is_contiguous() && router.dim() == 2 &&
                   router.size(1) == d && router.size(0) >= 1 && router.size(0) <= NT_MOE_TOKENS_EXPERTS,
-              "router must be contiguous fp32 [E, d] on the device of x, with 1 to ", NT_MOE_TOKENS_EXPERTS, " experts");
+              "router must be contiguous fp32 [E, d] on the device of x, with 1 to ", std::to_string(NT_MOE_TOKENS_EXPERTS), " experts");
   aligned(router, "router");
   const int64_t E = router.size(0);
-  TORCH_CHECK(top_k >= 1 && top_k <= E && top_k <= NT_MOE_TOKENS_CHOICES, "top_k must lie between 1 and the experts, at most ", NT_MOE_TOKENS_CHOICES);
+  TORCH_CHECK(top_k >= 1 && top_k <= E && top_k <= NT_MOE_TOKENS_CHOICES, "top_k must lie between 1 and the experts, at most ", std::to_string(NT_MOE_TOKENS_CHOICES));
   const auto weight = [&](const Tensor& t, const char* name) {
     TORCH_CHECK(t.device() == x.device() && t.scalar_type() == type && t.is_contiguous(), name, " must be contiguous, of x's type and device");
     aligned(t, name);

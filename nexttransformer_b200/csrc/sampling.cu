@@ -465,6 +465,11 @@ struct Filters {
   double least;    // min-p
   float number;    // u
 };
+// min-p; the largest logits pass whatever their computed weight is
+template <class R>
+NT_DEVICE bool passes(const R& r, const Filters& f, float x) {
+  return !(f.least > 0.0) || x == r.top || (f.least < 1.0 && power(r, x, 0) >= f.least);
+}
 
 // The entry of the list at which the sum (of weights, or of ones) over the order reaches `target`.  `chosen`, `done`: its bin, and the
 // sum before that.  A thread has EACH entries; those up to `last` count.  Entries are ordered as their numbers are.
@@ -556,7 +561,7 @@ NT_DEVICE bool draw_from_few(const SampleArgs& a, const R& r, Shared& s, int& ro
   for (int e = 0; e < EACH; ++e) {
     const float x = value_in(entry[e]);
     index[e] = static_cast<uint32_t>(entry[e]);
-    if (entry[e] > last || (f.least > 0.0 && !(power(r, x, 0) >= f.least))) w[e] = 0;
+    if (entry[e] > last || !passes(r, f, x)) w[e] = 0;
     sum += w[e];
   }
   block_scan(sum, s, total);
@@ -725,7 +730,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const SampleArgs a, 
     const float x = r[i];
     if (!all && !within(kept, x, r.first + i)) return 0ull;
     if (greedy) return 1ull;
-    if (f.least > 0.0 && !(power(r, x, 0) >= f.least)) return 0ull;
+    if (!passes(r, f, x)) return 0ull;
     return weight_of(r, x);
   };
 

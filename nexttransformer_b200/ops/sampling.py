@@ -73,7 +73,7 @@ def _plain(logits, uniform, temperature, top_k, top_p, min_p):
             mass = w.cumsum(0)
             keep &= mass - w < p[b] * mass[-1]
         if m[b] > 0:
-            keep &= w >= min(m[b], 1.0)
+            keep &= (w >= m[b]) if m[b] < 1 else (x == top)[order]
         keep[0] = True
         kept = torch.zeros(V, dtype=torch.float64).index_add_(0, order, w * keep)
         mass = kept.cumsum(0)
