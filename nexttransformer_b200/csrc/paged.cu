@@ -474,7 +474,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
     attn_kernel(const PagedAttnArgs a, const Geometry g, float* ws, unsigned* counters) {
   using S = Shape<C, D, NQ>;
   using M = std::conditional_t<S::F8, __half, T>;  // what the products multiply
-  constexpr bool F8 = S::F8;
+  constexpr bool F8 = S::F8, TWO = !F8 || std::is_same_v<T, M>;  // probabilities as two numbers, see below
   constexpr int NR = S::NR, LINE = S::LINE, CHUNKS = LINE / 16;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ int pre[MAX_ITEMS + 1];  // tiles of a KV head before each item
@@ -834,6 +834,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
         // calls).  fp16 ends at 2^-24, where the second number of a probability below 2^-14 is lost, so its reference m lies
         // RAISE below the maximum that it follows: probabilities reach 2^(RAISE + LAZY) = 2^15, the type's top, in products and
         // totals alike, and what is then lost is 2^-32 of the largest a key.
+        // 8 bits: one fp16 number (11 bits) is enough where the output has bf16's 8; fp16 queries keep both.
         uint32_t pf[NQ][2], pl[NQ][2];
         if (F8 && scales.y > v_top) {  // (the same for the whole warp)
           const float f = v_top / scales.y;
@@ -861,9 +862,11 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
               s[nq][2 * e + 1] *= weight;
             }
             const uint32_t high = Num<M>::pack(s[nq][2 * e], s[nq][2 * e + 1]);
-            const float2 h = Num<M>::unpack(high);
             pf[nq][e] = transpose8x8(high);
-            pl[nq][e] = transpose8x8(Num<M>::pack(s[nq][2 * e] - h.x, s[nq][2 * e + 1] - h.y));
+            if constexpr (TWO) {
+              const float2 h = Num<M>::unpack(high);
+              pl[nq][e] = transpose8x8(Num<M>::pack(s[nq][2 * e] - h.x, s[nq][2 * e + 1] - h.y));
+            }
           }
         }
         if constexpr (F8) {
@@ -877,8 +880,9 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
               const uint32_t vf[4] = {widen_low(x), widen_high(x), widen_low(y), widen_high(y)};
 #pragma unroll
               for (int nq = 0; nq < NQ; ++nq) Num<M>::mma(o[nq][d + e], vf, pf[nq][0], pf[nq][1]);
+              if constexpr (TWO)
 #pragma unroll
-              for (int nq = 0; nq < NQ; ++nq) Num<M>::mma(o[nq][d + e], vf, pl[nq][0], pl[nq][1]);
+                for (int nq = 0; nq < NQ; ++nq) Num<M>::mma(o[nq][d + e], vf, pl[nq][0], pl[nq][1]);
             }
           }
         } else {
