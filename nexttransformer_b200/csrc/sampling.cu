@@ -598,6 +598,111 @@ NT_DEVICE bool draw_from_few(const SampleArgs& a, const R& r, Shared& s, int& ro
   return true;
 }
 
+struct Sums {        // of the kept mass
+  u64 total, prior, own;  // of the row, of the CTAs before this one, of this one
+};
+// The runs of indices that warps sum up: warp w of a CTA has [w run, (w + 1) run).
+template <class R>
+NT_DEVICE int run_of(const R& r) { return (r.n + WARPS - 1) / WARPS; }
+
+// Where many are kept up to bin `chosen`: one pass sums the masses of the bins before it (into s.own, a warp's run each) and lists that
+// bin's elements, which are few as a rule; ranked, they give the border and their part of the masses.  False: the bin's are many.
+template <class R>
+NT_DEVICE bool sum_up_to(const R& r, Shared& s, int& round, const Border& outer, int chosen, u64 target, u64 done, const Filters& f, Border& border,
+                         Sums& sums) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, run = run_of(r), from = min(r.n, warp * run), to = min(r.n, from + run);
+  if (tid == 0) s.listed = 0;
+  __syncthreads();
+  const bool any = outer.key == 0;
+  const float end = static_cast<float>(chosen) + 8388608.f;
+  u64 mass = 0;
+  for (int i0 = from; i0 < to; i0 += 1024) {  // a thread looks at 32 before it computes any weight: most are not kept
+    unsigned below = 0, at = 0;
+#pragma unroll 1
+    for (int e = 0; e < 32 && i0 + 32 * e < to; e += 8) {
+      float x[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const int i = i0 + 32 * (e + k) + lane;
+        x[k] = i < to ? r[i] : -INFINITY;
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const float v = bin_sum(r, x[k]);
+        if (v <= end && (any || within(outer, x[k], r.first + i0 + 32 * (e + k) + lane))) (v == end ? at : below) |= 1u << (e + k);
+      }
+    }
+    while (__any_sync(0xffffffffu, below)) {
+      if (below) {
+        const float x = r[i0 + 32 * (__ffs(below) - 1) + lane];
+        if (passes(r, f, x)) mass += weight_of(r, x);
+        below &= below - 1;
+      }
+    }
+    if (!__any_sync(0xffffffffu, at)) continue;
+    const uint32_t upto = warp_scan(static_cast<uint32_t>(__popc(at)), lane);
+    uint32_t place = 0;
+    if (lane == 31) place = atomicAdd(&s.listed, upto);
+    place = __shfl_sync(0xffffffffu, place, 31) + upto - __popc(at);
+    for (; at; at &= at - 1, ++place) {
+      const int i = i0 + 32 * (__ffs(at) - 1) + lane;
+      if (place < FEW) s.list[place] = entry_of(key_of(r[i]), r.first + i);
+    }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) mass += __shfl_xor_sync(0xffffffffu, mass, o);
+  if (lane == 0) s.own[warp] = mass;
+  __syncthreads();
+  if (tid == 0) {
+    Note& n = s.note[round & 1];
+    n.count = s.listed;
+    n.mass = 0;
+    for (int w = 0; w < WARPS; ++w) n.mass += s.own[w];
+  }
+  cluster_sync();
+  const Note* theirs = peer(&s.note[round & 1], min(lane, r.ranks - 1));
+  const uint32_t counts = lane < r.ranks ? theirs->count : 0u;  // lane c: CTA c's
+  u64 masses = lane < r.ranks ? theirs->mass : 0ull;
+  ++round;
+  if (__reduce_add_sync(0xffffffffu, counts) > CAP) return false;
+  uint32_t many = 0;
+  for (int c = 0; c < r.ranks; ++c) {
+    const uint32_t n = __shfl_sync(0xffffffffu, counts, c);
+    for (uint32_t i = tid; i < n; i += THREADS) {
+      const u64 v = peer(s.list, c)[i];
+      s.sorted[many + i] = v;
+      s.sorted[CAP + many + i] = weight_of(r, value_in(v));
+    }
+    many += n;
+  }
+  __syncthreads();
+  const u64 last = ranked(s.sorted, s.sorted + CAP, static_cast<int>(many), target, done, s);
+  border = {~static_cast<uint32_t>(last >> 32), static_cast<int>(static_cast<uint32_t>(last))};
+  // what the bin adds: to every CTA's mass (each knows them all), and to this CTA's runs
+  uint32_t at = 0;
+  for (int c = 0; c < r.ranks; ++c) {
+    const uint32_t n = __shfl_sync(0xffffffffu, counts, c);
+    u64 more = 0;
+    for (uint32_t i = lane; i < n; i += 32) {
+      const u64 v = s.sorted[at + i];
+      if (v > last || !passes(r, f, value_in(v))) continue;
+      const u64 w = s.sorted[CAP + at + i];
+      more += w;
+      if (c == r.rank && warp == 0) add_to(&s.own[(static_cast<int>(static_cast<uint32_t>(v)) - r.first) / run], w);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) more += __shfl_xor_sync(0xffffffffu, more, o);
+    if (lane == c) masses += more;
+    at += n;
+  }
+  const u64 upto = warp_scan(masses, lane);
+  sums.total = __shfl_sync(0xffffffffu, upto, 31);
+  sums.own = __shfl_sync(0xffffffffu, masses, r.rank);
+  sums.prior = __shfl_sync(0xffffffffu, upto, r.rank) - sums.own;
+  __syncthreads();
+  return true;
+}
+
 template <class T, bool HELD, bool VECTORS>
 __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const SampleArgs a, const int segment, const int ranks) {
   extern __shared__ __align__(16) float values[];
@@ -706,6 +811,8 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const SampleArgs a, 
                      min_p > 0.f ? fmin(static_cast<double>(min_p), 1.0) : 0.0, u > 0.f ? fminf(u, 0.99999994f) : 0.f};
 
   // ---- the order's kept part
+  bool summed = false;
+  Sums sums;
   Border kept = {0u, 0x7fffffff};
   if (greedy) {
     kept.key = key_of(top);  // its first index is found below
@@ -721,8 +828,12 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const SampleArgs a, 
     if (f.share < 1.f) {
       target = 0;
       const int chosen = first_crossing<true>(r, s, round, kept, target, f.share, before);
-      if (draw_from_few<true>(a, r, s, round, kept, chosen, target, before, f, b)) return;
-      kept = find_border<true>(r, s, round, kept, target, chosen, before);
+      // The mass over the weight of the bin's lower end bounds their number; real rows have an eighth of that, or less
+      const bool few = target >> 3 <= static_cast<u64>(FEW) * weight_of(r, top - static_cast<float>(chosen + 1) / r.per_bin);
+      if (few && draw_from_few<true>(a, r, s, round, kept, chosen, target, before, f, b)) return;
+      Border cut;
+      summed = sum_up_to(r, s, round, kept, chosen, target, before, f, cut, sums);
+      kept = summed ? cut : find_border<true>(r, s, round, kept, target, chosen, before);
     }
   }
   const bool all = kept.key == 0;
@@ -735,22 +846,26 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const SampleArgs a, 
   };
 
   // ---- the draw: masses of the warps' runs of indices, the run that u falls into, the thread, the token
-  const int run = (r.n + WARPS - 1) / WARPS, from = min(r.n, warp * run), to = min(r.n, from + run);
-  u64 mine = 0;
-  for (int i = from + lane; i < to; i += 32) mine += mass_of(i);
+  const int run = run_of(r), from = min(r.n, warp * run), to = min(r.n, from + run);
+  if (!summed) {
+    u64 mine = 0;
+    for (int i = from + lane; i < to; i += 32) mine += mass_of(i);
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
-  if (lane == 0) s.own[warp] = mine;
-  __syncthreads();
-  if (tid == 0) {
-    u64 sum = 0;
-    for (int w = 0; w < WARPS; ++w) sum += s.own[w];
-    s.note[round & 1].mass = sum;
+    for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+    if (lane == 0) s.own[warp] = mine;
+    __syncthreads();
+    if (tid == 0) {
+      u64 sum = 0;
+      for (int w = 0; w < WARPS; ++w) sum += s.own[w];
+      s.note[round & 1].mass = sum;
+    }
+    cluster_sync();
+    const u64 theirs = lane < ranks ? peer(&s.note[round & 1], lane)->mass : 0ull, upto = warp_scan(theirs, lane);  // lane c: CTA c's
+    sums.total = __shfl_sync(0xffffffffu, upto, 31);
+    sums.own = __shfl_sync(0xffffffffu, theirs, r.rank);
+    sums.prior = __shfl_sync(0xffffffffu, upto, r.rank) - sums.own;
   }
-  cluster_sync();
-  const u64 theirs = lane < ranks ? peer(&s.note[round & 1], lane)->mass : 0ull, upto = warp_scan(theirs, lane);  // lane c: CTA c's
-  const u64 total = __shfl_sync(0xffffffffu, upto, 31), own = __shfl_sync(0xffffffffu, theirs, r.rank);
-  const u64 prior = __shfl_sync(0xffffffffu, upto, r.rank) - own;
+  const u64 total = sums.total, prior = sums.prior, own = sums.own;
   const u64 aim = greedy ? 0 : min(share_of(f.number, total, false), total - 1);
   if (prior <= aim && aim < prior + own) {
     int w = 0;
