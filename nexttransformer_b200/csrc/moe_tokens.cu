@@ -21,9 +21,8 @@ namespace nt {
 namespace moe_tokens {
 
 constexpr int ROUTE_WARPS = 8, ROUTE_THREADS = ROUTE_WARPS * 32;
-constexpr int WARPS = 8, THREADS = WARPS * 32;
-constexpr int STAGE = 2048, STAGES = 4, RING = STAGE * STAGES;  // 8 KB a warp, 16 warps an SM
-constexpr int SMEM = WARPS * RING;
+constexpr int WARPS = 4, THREADS = WARPS * 32, RESIDENT = 3;  // of the products: three CTAs an SM
+constexpr int TILE = 16 * 128;  // bytes of 16 rows of 64 elements
 constexpr int MOST = NT_MOE_TOKENS_MOST, EXPERTS = NT_MOE_TOKENS_EXPERTS, CHOICES = NT_MOE_TOKENS_CHOICES;
 // Hidden values are held in the weights' type.  fp16 ends at 65504, which a square passes where its root is 256: they
 // are held as 2^-6 of themselves there (up to 4.2e6), and the sums are raised again.
@@ -57,10 +56,6 @@ static size_t layout(const MoeTokensArgs& a, Workspace& w) {
   return at;
 }
 
-// L2 fetches 256 bytes at once: rows lie far apart, and the next stage wants the other half.
-NT_DEVICE void cp_async16_far(uint32_t dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global.L2::256B [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-}
 NT_DEVICE void dependents_may_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 NT_DEVICE void wait_for_predecessor() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
@@ -260,16 +255,17 @@ NT_DEVICE int nth_token(unsigned long long m, int n) {
   return m ? __ffsll(static_cast<long long>(m)) - 1 : -1;
 }
 
-// A warp's ring: 16 rows of 64 elements a stage, chunk c of row r at c ^ (r & 7).
+// A warp's ring: STAGES stages of 16 MT rows of 64 elements, chunk c (16 bytes) of row r at c ^ (r & 7).
 struct Ring {
   uint32_t base, in, out;  // addresses of the ring, of the stage that is filled next and of the one that is read next
-  uint32_t to[2];          // this lane's place in a stage for rows r and r + 4 (r < 4); 1024 further on for r + 8 and r + 12
-  uint32_t at[4];          // this lane's matrix row of the four 16-column tiles
+  uint32_t to[2];          // this lane's place in a stage for rows r and r + 4 (r < 4); 1024 further on for each 8 rows
+  uint32_t at[4];          // this lane's matrix row of the four 16-column tiles; 2048 further on for each 16 rows
 };
+template <int BYTES>
 NT_DEVICE Ring make_ring(const void* smem) {
   Ring r;
   const int lane = threadIdx.x & 31, row = lane >> 3, chunk = lane & 7;
-  r.base = r.in = r.out = smem_u32(smem) + (threadIdx.x >> 5) * RING;
+  r.base = r.in = r.out = smem_u32(smem) + (threadIdx.x >> 5) * BYTES;
   r.to[0] = row * 128 + ((chunk ^ row) << 4);
   r.to[1] = (row + 4) * 128 + ((chunk ^ (row + 4)) << 4);
 #pragma unroll
@@ -279,13 +275,12 @@ NT_DEVICE Ring make_ring(const void* smem) {
   }
   return r;
 }
-NT_DEVICE void turn(uint32_t& stage, const Ring& r) { stage = stage == r.base + (STAGES - 1) * STAGE ? r.base : stage + STAGE; }
 
 // A row tile of an entry: what a warp goes through, a stage of 64 inner elements after the other.
 struct Piece {
   int entry, expert, tile;
-  int inner, rows;    // elements of a weight row; rows of the tile (16, or fewer at the end)
-  int blocks;         // of 8 tokens
+  int inner, rows;    // elements of a weight row; rows of the tile (16 MT, or fewer at the end)
+  unsigned blocks;    // bit b: it has tokens in its b-th block of 8
   int stage, stages;  // the next one; the first behind the piece
   int behind;         // what comes after it: an item, or a stage of all
 };
@@ -293,15 +288,18 @@ struct Piece {
 // Goes through a warp's pieces: weights come `STAGES - 1` stages ahead, the other operand one.
 //   first(piece) / next(piece) set a piece and say whether there is one (the copies, the operand and the products each go through them);
 //   base(piece): the tile's first weight; operand(piece, pointers): this lane's part of the 16 x 8 tile of the piece's next stage, of
-//   each block of 8 tokens, `step` apart from tile to tile (a Frag of 16 bytes holds two numbers for each value); ready(): what has to
-//   be waited for before the operand is read; done(piece, sums): a piece's products are complete.
-// With 8 warps an SM and 187 instructions a stage the first product took 60 us for 12 tokens (3.7 TB/s): a warp's instructions wait
-// for each other, so there are 16 warps, and what a stage needs is counted on.
-template <class T, int NB, class Frag, class First, class Next, class Base, class Operand, class Ready, class Done>
-NT_DEVICE void stream(const MoeTokensArgs& a, const void* smem, const int step, First first, Next next, Base base, Operand operand, Ready ready,
-                      Done done) {
+//   each block of 8 tokens (null: zeros), `step` apart from tile to tile (a Frag of 16 bytes holds two numbers for each value);
+//   ready(): what has to be waited for before the operand is read; done(piece, sums): a piece's products are complete.  KEEP: the sums
+//   run on through all pieces, and done is not called.
+// MT tiles of 16 rows share an operand's reading and the way through the loop: a warp's instructions wait for each other, and with 8
+// warps an SM, 16 rows and 187 instructions a stage the first product took 60 us for 12 tokens, with 16 warps and 137 it took 44.
+template <class T, int MT, int NB, int STAGES, class Frag, bool KEEP, class First, class Next, class Base, class Operand, class Ready, class Done>
+NT_DEVICE void stream(const MoeTokensArgs& a, const void* smem, const int step, float (&acc)[MT][NB][4], First first, Next next, Base base,
+                      Operand operand, Ready ready, Done done) {
   constexpr bool TWO = sizeof(Frag) == 16;
-  Ring r = make_ring(smem);
+  constexpr int STAGE = MT * TILE;
+  Ring r = make_ring<STAGES * STAGE>(smem);
+  auto turn = [&](uint32_t& stage) { stage = stage == r.base + (STAGES - 1) * STAGE ? r.base : stage + STAGE; };
   const int lane = threadIdx.x & 31, row = lane >> 3, chunk = lane & 7;
   Piece f, o, c;  // where the copies, the operand and the products stand
   bool f_more = first(f);
@@ -315,19 +313,19 @@ NT_DEVICE void stream(const MoeTokensArgs& a, const void* smem, const int step, 
   enter();
   auto fetch = [&]() {
     if (f_more) {
-      const bool inside = f.stage * 64 + chunk * 8 < f.inner;
-      if (f.rows == 16 && (f.stage + 1) * 64 <= f.inner) {
+      if (f.rows == 16 * MT && (f.stage + 1) * 64 <= f.inner) {
         const char* p = f_at;
 #pragma unroll
-        for (int e = 0; e < 4; ++e, p += f_step) cp_async16_far(r.in + r.to[e & 1] + (e >> 1) * 1024, p);
+        for (int e = 0; e < 4 * MT; ++e, p += f_step) cp_async16(r.in + r.to[e & 1] + (e >> 1) * 1024, p);
       } else {  // what is not there becomes zero
+        const bool inside = f.stage * 64 + chunk * 8 < f.inner;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
+        for (int e = 0; e < 4 * MT; ++e) {
           const bool valid = inside && row + 4 * e < f.rows;
           cp_async16_or_zero(r.in + r.to[e & 1] + (e >> 1) * 1024, valid ? f_at + e * f_step : static_cast<const char*>(a.x), valid);
         }
       }
-      turn(r.in, r);
+      turn(r.in);
       f_at += 128;
       if (++f.stage == f.stages) {
         f_more = next(f);
@@ -347,40 +345,57 @@ NT_DEVICE void stream(const MoeTokensArgs& a, const void* smem, const int step, 
     if (!o_more) return;
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb)
-      if (nb == 0 || nb < o.blocks) {
+      if ((o.blocks >> nb) & 1u) {
 #pragma unroll
-        for (int s = 0; s < 4; ++s) b[s][nb] = TWO ? __ldcg(at[nb] + s * step) : at[nb][s * step];
-        at[nb] += 4 * step;
+        for (int s = 0; s < 4; ++s) {
+          b[s][nb] = Frag{};
+          if (!KEEP || at[nb]) b[s][nb] = TWO ? __ldcg(at[nb] + s * step) : at[nb][s * step];
+        }
+        if (!KEEP || at[nb]) at[nb] += 4 * step;
       }
     if (++o.stage == o.stages) {
       o_more = next(o);
       if (o_more) operand(o, at);
     }
   };
-  float acc[NB][4] = {};
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[m][nb][e] = 0.f;
   auto multiply = [&](const Frag (&b)[4][NB], Frag (&ahead)[4][NB]) {
     load(ahead);
     cp_wait<STAGES - 2>();
     __syncwarp();  // this stage has landed for every lane, and the stage before it is read by none
-    uint32_t w[4][4];
 #pragma unroll
-    for (int s = 0; s < 4; ++s) ldsm4(w[s], r.out + r.at[s]);
-    turn(r.out, r);
-    fetch();
+    for (int m = 0; m < MT; ++m) {
+      uint32_t w[4][4];
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb)
-      if (nb == 0 || nb < c.blocks)
-#pragma unroll
-        for (int s = 0; s < 4; ++s) {
-          Num<T>::mma(acc[nb], w[s], b[s][nb].x, b[s][nb].y);
-          if constexpr (TWO) Num<T>::mma(acc[nb], w[s], b[s][nb].z, b[s][nb].w);
-        }
-    if (++c.stage == c.stages) {
-      done(c, acc);
+      for (int s = 0; s < 4; ++s) ldsm4(w[s], r.out + r.at[s] + m * TILE);
+      if (m == MT - 1) {
+        turn(r.out);
+        fetch();
+      }
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb)
+        if ((c.blocks >> nb) & 1u)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) acc[nb][e] = 0.f;
+          for (int s = 0; s < 4; ++s) {
+            Num<T>::mma(acc[m][nb], w[s], b[s][nb].x, b[s][nb].y);
+            if constexpr (TWO) Num<T>::mma(acc[m][nb], w[s], b[s][nb].z, b[s][nb].w);
+          }
+    }
+    if (++c.stage == c.stages) {
+      if constexpr (!KEEP) {
+        done(c, acc);
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[m][nb][e] = 0.f;
+      }
       c_more = next(c);
     }
   };
@@ -396,22 +411,27 @@ NT_DEVICE void stream(const MoeTokensArgs& a, const void* smem, const int step, 
 }
 
 // NB blocks of 8 tokens an entry: 1 where there are no more than 8 tokens, else 2.  `wide`
-// warps share a tile, a part of its stages each, where the last round of tiles would leave more than a twelfth of the warps' time
-// unused: one token on experts of 1024 x 2048 has 576 tiles for 2368 warps, twelve tokens have about 3800.
+// warps share a tile, a part of its stages each, where tiles are few or their last round would leave many warps without one: one token
+// on experts of 1024 x 2048 has 288 tiles for 1776 warps.
+constexpr int FC_MT = 2, FC_STAGES = 3;
 template <class T, int NB>
-__global__ void __launch_bounds__(THREADS, 2) fc_kernel(const MoeTokensArgs a, const Workspace w) {
+__global__ void __launch_bounds__(THREADS, RESIDENT) fc_kernel(const MoeTokensArgs a, const Workspace w) {
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ Lists l;
-  __shared__ float4 parts[2][WARPS][NB][32];
+  __shared__ float4 parts[WARPS][FC_MT][NB][32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   wait_for_predecessor();
   dependents_may_start();
   make_lists(a, w, l);
-  const int tiles = (a.F + 15) / 16, shared_tiles = (a.Fs + 15) / 16, groups = groups_of(a.F), shared_groups = groups_of(a.Fs);
+  constexpr int ROWS = 16 * FC_MT;
+  const int tiles = (a.F + ROWS - 1) / ROWS, shared_tiles = (a.Fs + ROWS - 1) / ROWS, groups = groups_of(a.F), shared_groups = groups_of(a.Fs);
   const int routed = l.routed * tiles, items = routed + (l.entries - l.routed) * shared_tiles;
   const int stages = (a.d + 63) / 64, slots = gridDim.x * WARPS;
+  // rounds of tiles times what a warp does for one: its part of the stages, and about three stages' time for beginning and ending it
+  auto cost = [&](int n) { return static_cast<float>((items * n + slots - 1) / slots) * (static_cast<float>(stages) / n + 3.f); };
   int wide = 1;
-  while (wide < WARPS && 2 * wide <= stages && (items * wide + slots - 1) / slots * slots * 12 > items * wide * 13) wide *= 2;
+  for (int n = 2; n <= WARPS && n <= stages; n *= 2)
+    if (cost(n) < cost(wide)) wide = n;
   const int group = warp / wide, part = warp % wide, by = gridDim.x * (WARPS / wide);
   // (the first items go to different SMs)
   auto set = [&](Piece& p, int item) {
@@ -422,19 +442,19 @@ __global__ void __launch_bounds__(THREADS, 2) fc_kernel(const MoeTokensArgs a, c
     p.tile = i - n * per;
     p.expert = l.expert[p.entry];
     p.inner = a.d;
-    p.rows = min(16, (shared ? a.Fs : a.F) - p.tile * 16);
-    p.blocks = l.blocks[p.entry];
+    p.rows = min(ROWS, (shared ? a.Fs : a.F) - p.tile * ROWS);
+    p.blocks = (1u << l.blocks[p.entry]) - 1u;
     p.stage = stages * part / wide;
     p.stages = stages * (part + 1) / wide;
     p.behind = item + by;
     return true;
   };
-  int turn_of_parts = 0;
-  stream<T, NB, uint2>(
-      a, smem, (a.T + 7) / 8 * 32, [&](Piece& p) { return set(p, group * gridDim.x + blockIdx.x); }, [&](Piece& p) { return set(p, p.behind); },
+  float sums[FC_MT][NB][4];
+  stream<T, FC_MT, NB, FC_STAGES, uint2, false>(
+      a, smem, (a.T + 7) / 8 * 32, sums, [&](Piece& p) { return set(p, group * gridDim.x + blockIdx.x); }, [&](Piece& p) { return set(p, p.behind); },
       [&](const Piece& p) -> const void* {
         const T* e = p.expert == a.E ? static_cast<const T*>(a.shared_fc) : static_cast<const T*>(a.w_fc) + static_cast<int64_t>(p.expert) * a.F * a.d;
-        return e + static_cast<int64_t>(p.tile) * 16 * a.d;
+        return e + static_cast<int64_t>(p.tile) * ROWS * a.d;
       },
       [&](const Piece& p, const uint2* (&at)[NB]) {
         const unsigned long long mask = l.mask[p.expert];
@@ -446,19 +466,23 @@ __global__ void __launch_bounds__(THREADS, 2) fc_kernel(const MoeTokensArgs a, c
         }
       },
       [] {},
-      [&](const Piece& p, float (&acc)[NB][4]) {
-        if (wide > 1) {  // the first warp adds up, while the others go on to the next tile and its other buffer
+      [&](const Piece& p, float (&acc)[FC_MT][NB][4]) {
+        if (wide > 1) {  // the first warp adds up
 #pragma unroll
-          for (int nb = 0; nb < NB; ++nb) parts[turn_of_parts][warp][nb][lane] = make_float4(acc[nb][0], acc[nb][1], acc[nb][2], acc[nb][3]);
+          for (int m = 0; m < FC_MT; ++m)
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) parts[warp][m][nb][lane] = make_float4(acc[m][nb][0], acc[m][nb][1], acc[m][nb][2], acc[m][nb][3]);
           named_bar_sync(1 + group, wide * 32);
           if (part == 0)
             for (int k = 1; k < wide; ++k)
 #pragma unroll
-              for (int nb = 0; nb < NB; ++nb) {
-                const float4 v = parts[turn_of_parts][warp + k][nb][lane];
-                acc[nb][0] += v.x; acc[nb][1] += v.y; acc[nb][2] += v.z; acc[nb][3] += v.w;
-              }
-          turn_of_parts ^= 1;
+              for (int m = 0; m < FC_MT; ++m)
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb) {
+                  const float4 v = parts[warp + k][m][nb][lane];
+                  acc[m][nb][0] += v.x; acc[m][nb][1] += v.y; acc[m][nb][2] += v.z; acc[m][nb][3] += v.w;
+                }
+          named_bar_sync(1 + group, wide * 32);
           if (part) return;
         }
         // h, in the order in which it is an operand: rows of the tile become the products' inner dimension.  It is held as two
@@ -469,38 +493,47 @@ __global__ void __launch_bounds__(THREADS, 2) fc_kernel(const MoeTokensArgs a, c
         uint4* h = w.h + (shared ? static_cast<int64_t>(w.pairs) * groups : 0ll) * 32;
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
-          if (nb >= p.blocks) break;
-          float v[4];
+          if (!((p.blocks >> nb) & 1u)) break;
+          int t[2];
+          float share[2];
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            const int t = nth_token(mask, l.first[p.entry] + nb * 8 + (lane & 3) * 2 + e);
-            const float c = t < 0 ? 0.f : shared ? LOWER<T> : LOWER<T> * __ldcg(w.share + static_cast<int64_t>(t) * a.E + p.expert);
-#pragma unroll
-            for (int k = e; k < 4; k += 2) {
-              const float u = acc[nb][k] < 0.f ? 0.f : acc[nb][k];  // a NaN stays one
-              v[k] = t < 0 ? 0.f : c * (u * u);
-            }
+            t[e] = nth_token(mask, l.first[p.entry] + nb * 8 + (lane & 3) * 2 + e);
+            share[e] = t[e] < 0 ? 0.f : shared ? LOWER<T> : LOWER<T> * __ldcg(w.share + static_cast<int64_t>(t[e]) * a.E + p.expert);
           }
-          const uint32_t hi0 = Num<T>::pack(v[0], v[1]), hi1 = Num<T>::pack(v[2], v[3]);
-          const float2 f0 = Num<T>::unpack(hi0), f1 = Num<T>::unpack(hi1);
-          // (of an infinite value the rest is NaN, and so would the sum be)
-          const uint32_t lo0 = Num<T>::pack(isinf(f0.x) ? 0.f : v[0] - f0.x, isinf(f0.y) ? 0.f : v[1] - f0.y);
-          const uint32_t lo1 = Num<T>::pack(isinf(f1.x) ? 0.f : v[2] - f1.x, isinf(f1.y) ? 0.f : v[3] - f1.y);
-          uint4* to = h + ((static_cast<int64_t>(l.block[p.entry]) + nb) * inner + p.tile) * 32 + lane;
-          *to = make_uint4(transpose8x8(hi0), transpose8x8(hi1), transpose8x8(lo0), transpose8x8(lo1));
+          uint4* to = h + ((static_cast<int64_t>(l.block[p.entry]) + nb) * inner + p.tile * FC_MT) * 32 + lane;
+#pragma unroll
+          for (int m = 0; m < FC_MT; ++m, to += 32) {
+            float v[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const float u = acc[m][nb][k] < 0.f ? 0.f : acc[m][nb][k];  // a NaN stays one
+              v[k] = t[k & 1] < 0 ? 0.f : share[k & 1] * (u * u);
+            }
+            const uint32_t hi0 = Num<T>::pack(v[0], v[1]), hi1 = Num<T>::pack(v[2], v[3]);
+            const float2 f0 = Num<T>::unpack(hi0), f1 = Num<T>::unpack(hi1);
+            // (of an infinite value the rest is NaN, and so would the sum be)
+            const uint32_t lo0 = Num<T>::pack(isinf(f0.x) ? 0.f : v[0] - f0.x, isinf(f0.y) ? 0.f : v[1] - f0.y);
+            const uint32_t lo1 = Num<T>::pack(isinf(f1.x) ? 0.f : v[2] - f1.x, isinf(f1.y) ? 0.f : v[3] - f1.y);
+            *to = make_uint4(transpose8x8(hi0), transpose8x8(hi1), transpose8x8(lo0), transpose8x8(lo1));
+          }
           if (p.tile == (shared ? shared_tiles : tiles) - 1)  // the groups behind the last
-            for (int g = p.tile + 1; g < inner; ++g) *(to += 32) = make_uint4(0, 0, 0, 0);
+            for (int g = (p.tile + 1) * FC_MT; g < inner; ++g, to += 32) *to = make_uint4(0, 0, 0, 0);
         }
       });
 }
 
-template <class T, int NB>
-__global__ void __launch_bounds__(THREADS, 2) proj_kernel(const MoeTokensArgs a, const Workspace w, const int parts) {
+// Up to 16 tokens are the columns of every entry, and the sums stay in registers (KEEP); of more, an entry's own are, and its sums are added
+// to the tokens' in shared memory.
+template <class T, int MT, int NB, int STAGES, bool KEEP>
+__global__ void __launch_bounds__(THREADS, RESIDENT) proj_kernel(const MoeTokensArgs a, const Workspace w, const int parts) {
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ Lists l;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, part = blockIdx.x % parts, tile = blockIdx.x / parts;
-  float* const sums = reinterpret_cast<float*>(smem + SMEM);  // [warp][token][17]: of the tile's 16 channels
-  for (int i = tid; i < WARPS * a.T * 17; i += THREADS) sums[i] = 0.f;
+  constexpr int ROWS = 16 * MT, PITCH = ROWS + 1;
+  float* const sums = reinterpret_cast<float*>(smem + (KEEP ? 0 : WARPS * STAGES * MT * TILE));  // [warp][token][PITCH]
+  if (!KEEP)
+    for (int i = tid; i < WARPS * a.T * PITCH; i += THREADS) sums[i] = 0.f;
   make_lists(a, w, l);  // (the route kernel ended before the one before this began its work)
   const int per = (a.F + 63) / 64, shared_per = (a.Fs + 63) / 64, groups = groups_of(a.F), shared_groups = groups_of(a.Fs);
   // an equal run of the stages of all entries
@@ -512,8 +545,13 @@ __global__ void __launch_bounds__(THREADS, 2) proj_kernel(const MoeTokensArgs a,
     p.tile = tile;
     p.expert = l.expert[p.entry];
     p.inner = shared ? a.Fs : a.F;
-    p.rows = min(16, a.d - tile * 16);
-    p.blocks = l.blocks[p.entry];
+    p.rows = min(ROWS, a.d - tile * ROWS);
+    if (KEEP) {
+      const unsigned mask = static_cast<unsigned>(l.mask[p.expert]);
+      p.blocks = (mask & 0xffu ? 1u : 0u) | (mask >> 8 ? 2u : 0u);
+    } else {
+      p.blocks = (1u << l.blocks[p.entry]) - 1u;
+    }
     p.stages = min(shared ? shared_per : per, p.stage + last - at);
     p.behind = at + p.stages - p.stage;
   };
@@ -533,21 +571,32 @@ __global__ void __launch_bounds__(THREADS, 2) proj_kernel(const MoeTokensArgs a,
     enter(p, p.behind);
     return true;
   };
-  stream<T, NB, uint4>(
-      a, smem, 32, set, next,
+  float acc[MT][NB][4];
+  stream<T, MT, NB, STAGES, uint4, KEEP>(
+      a, smem, 32, acc, set, next,
       [&](const Piece& p) -> const void* {
         const T* e = p.expert == a.E ? static_cast<const T*>(a.shared_proj) : static_cast<const T*>(a.w_proj) + static_cast<int64_t>(p.expert) * a.d * a.F;
-        return e + static_cast<int64_t>(tile) * 16 * p.inner;
+        return e + static_cast<int64_t>(tile) * ROWS * p.inner;
       },
       [&](const Piece& p, const uint4* (&at)[NB]) {
         const bool shared = p.expert == a.E;
         const int inner = shared ? shared_groups : groups;
         const uint4* h = w.h + (shared ? static_cast<int64_t>(w.pairs) * groups : 0ll) * 32;
+        const unsigned mask = static_cast<unsigned>(l.mask[p.expert]);
 #pragma unroll
-        for (int nb = 0; nb < NB; ++nb) at[nb] = h + ((static_cast<int64_t>(l.block[p.entry]) + nb) * inner + p.stage * 4) * 32 + lane;
+        for (int nb = 0; nb < NB; ++nb) {
+          if (KEEP) {  // column t is token t, which is the expert's `place`-th
+            const int t = nb * 8 + (lane >> 2), place = __popc(mask & ((1u << t) - 1u));
+            at[nb] = (mask >> t) & 1u
+                         ? h + ((static_cast<int64_t>(l.block[p.entry]) + (place >> 3)) * inner + p.stage * 4) * 32 + (place & 7) * 4 + (lane & 3)
+                         : nullptr;
+          } else {
+            at[nb] = h + ((static_cast<int64_t>(l.block[p.entry]) + nb) * inner + p.stage * 4) * 32 + lane;
+          }
+        }
       },
       [] { wait_for_predecessor(); },  // weights may come before, h may not
-      [&](const Piece& p, const float (&acc)[NB][4]) {
+      [&](const Piece& p, const float (&own)[MT][NB][4]) {
         const unsigned long long mask = l.mask[p.expert];
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb)
@@ -555,29 +604,48 @@ __global__ void __launch_bounds__(THREADS, 2) proj_kernel(const MoeTokensArgs a,
           for (int e = 0; e < 2; ++e) {
             const int t = nth_token(mask, l.first[p.entry] + nb * 8 + (lane & 3) * 2 + e);
             if (t < 0) continue;
-            float* to = sums + (warp * a.T + t) * 17 + (lane >> 2);
-            to[0] += acc[nb][e];
-            to[8] += acc[nb][e + 2];
+            float* to = sums + (warp * a.T + t) * PITCH + (lane >> 2);
+#pragma unroll
+            for (int m = 0; m < MT; ++m) {
+              to[16 * m] += own[m][nb][e];
+              to[16 * m + 8] += own[m][nb][e + 2];
+            }
           }
         __syncwarp();  // the next entry's lanes may hold this one's tokens elsewhere
       });
+  if (KEEP) {
+    __syncthreads();  // the rings are done with
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int t = nb * 8 + (lane & 3) * 2 + e;
+        if (t >= a.T) continue;
+        float* to = sums + (warp * a.T + t) * PITCH + (lane >> 2);
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          to[16 * m] = acc[m][nb][e];
+          to[16 * m + 8] = acc[m][nb][e + 2];
+        }
+      }
+  }
 
   // ---- the warps' sums, then the parts', in their order
   __syncthreads();
   float* const whole = sums;
-  for (int i = tid; i < a.T * 16; i += THREADS) {
-    const int at = (i >> 4) * 17 + (i & 15);
+  for (int i = tid; i < a.T * ROWS; i += THREADS) {
+    const int at = i / ROWS * PITCH + i % ROWS;
     float v = 0.f;
 #pragma unroll
-    for (int k = 0; k < WARPS; ++k) v += sums[k * a.T * 17 + at];
+    for (int k = 0; k < WARPS; ++k) v += sums[k * a.T * PITCH + at];
     whole[at] = v;
   }
   if (parts > 1) cluster_sync();
   else __syncthreads();
   if (part == 0) {
-    for (int i = tid; i < a.T * 8; i += THREADS) {  // a pair of channels of a token
-      const int t = i >> 3, ch = (i & 7) * 2;
-      const float* own = whole + t * 17 + ch;
+    for (int i = tid; i < a.T * ROWS / 2; i += THREADS) {  // a pair of channels of a token
+      const int t = i / (ROWS / 2), ch = i % (ROWS / 2) * 2;
+      const float* own = whole + t * PITCH + ch;
       float2 v = make_float2(own[0], own[1]);
       for (int c = 1; c < parts; ++c) {
         uint32_t remote;
@@ -589,8 +657,8 @@ __global__ void __launch_bounds__(THREADS, 2) proj_kernel(const MoeTokensArgs a,
         v.y += u.y;
       }
       const float f = 1.f / LOWER<T>;
-      if (tile * 16 + ch < a.d)  // (d is even)
-        *reinterpret_cast<uint32_t*>(static_cast<T*>(a.y) + static_cast<int64_t>(t) * a.d + tile * 16 + ch) = Num<T>::pack(v.x * f, v.y * f);
+      if (tile * ROWS + ch < a.d)  // (d is even)
+        *reinterpret_cast<uint32_t*>(static_cast<T*>(a.y) + static_cast<int64_t>(t) * a.d + tile * ROWS + ch) = Num<T>::pack(v.x * f, v.y * f);
     }
   }
   if (parts > 1) cluster_sync();  // nobody leaves while its sums are read
@@ -631,17 +699,49 @@ static int route_for(const MoeTokensArgs& a, const Workspace& w, cudaStream_t s)
   if (a.T * ROUTE_RANKS <= a.sms || a.d * 16 > 48 * 1024) return route<T, 1>(a, w, s);
   return route<T, 4>(a, w, s);
 }
+// Clusters of more than 8 CTAs have to be allowed for a kernel, on each device once.
+template <class Kernel>
+static cudaError_t larger_clusters(std::atomic<uint64_t>& done, Kernel kern) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) dev = 0;
+  const uint64_t bit = dev < 64 ? (uint64_t(1) << dev) : 0;
+  if (bit && (done.load(std::memory_order_acquire) & bit)) return cudaSuccess;
+  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  if (e == cudaSuccess && bit) done.fetch_or(bit, std::memory_order_acq_rel);
+  return e;
+}
+template <class T, int MT, int NB, int STAGES, bool KEEP>
+static int project(const MoeTokensArgs& a, const Workspace& w, cudaStream_t s) {
+  static std::atomic<uint64_t> done{0}, wide_done{0};
+  constexpr int RINGS = WARPS * STAGES * MT * TILE, SUM = WARPS * (16 * MT + 1) * static_cast<int>(sizeof(float));  // of a token
+  static_assert(!KEEP || 16 * SUM <= RINGS, "sums lie in the rings");
+  const auto kern = proj_kernel<T, MT, NB, STAGES, KEEP>;
+  if (smem_limit(done, kern, RINGS + (KEEP ? 0 : MOST * SUM)) != cudaSuccess || larger_clusters(wide_done, kern) != cudaSuccess) return -1;
+  // Parts of the sum as a cluster, as many as are resident at once; more than 8 where a warp still gets a dozen stages (few tiles of
+  // wide experts: 6 tokens, 216 / 3424: 60 us with 8, 44 with 16; but 28 tokens, 424 / 216: 38 and 47).
+  const int64_t stages = static_cast<int64_t>(std::min(a.E, a.T * a.k)) * blocks_of(a.F, 64) + blocks_of(a.Fs, 64);
+  const int tiles = blocks_of(a.d, 16 * MT), most = stages >= 12 * WARPS * 16 ? 16 : 8, places = RESIDENT * a.sms;
+  // Clusters that are placed beside the last CTAs of the kernel before leave gaps, so they take 13 of 15 places, or wait for its end where
+  // the rest is worth it (80 clusters for 444 places, 64 tokens: 122 us with 4 CTAs each, 158 with 5, and 113 if these wait).
+  const int spare = std::max(1, std::min(most, places * 13 / 15 / tiles)), full = std::max(1, std::min(most, places / tiles));
+  const bool early = full * 4 < spare * 5;
+  const int parts = early ? spare : full;
+  return start(kern, tiles * parts, THREADS, RINGS + (KEEP ? 0 : a.T * SUM), parts, early, s, a, w, parts);
+}
 template <class T, int NB>
 static int launch(const MoeTokensArgs& a, cudaStream_t s) {
-  static std::atomic<uint64_t> fc_done{0}, proj_done{0};
-  if (smem_limit(fc_done, fc_kernel<T, NB>, SMEM) != cudaSuccess || smem_limit(proj_done, proj_kernel<T, NB>, SMEM + WARPS * MOST * 17 * sizeof(float)) != cudaSuccess) return -1;
+  static std::atomic<uint64_t> done{0};
+  constexpr int RINGS = WARPS * FC_STAGES * FC_MT * TILE;
+  if (smem_limit(done, fc_kernel<T, NB>, RINGS) != cudaSuccess) return -1;
   Workspace w;
   layout(a, w);
   if (route_for<T>(a, w, s)) return -1;
-  if (start(fc_kernel<T, NB>, 2 * a.sms, THREADS, SMEM, 1, true, s, a, w)) return -1;
-  const int tiles = blocks_of(a.d, 16), parts = std::max(1, std::min(8, 2 * a.sms / tiles));
-  return start(proj_kernel<T, NB>, tiles * parts, THREADS, SMEM + WARPS * a.T * 17 * sizeof(float), parts, true, s, a, w, parts);
+  if (start(fc_kernel<T, NB>, RESIDENT * a.sms, THREADS, RINGS, 1, true, s, a, w)) return -1;
+  if (a.T > 16) return project<T, 1, 2, 5, false>(a, w, s);
+  // narrow layers have too few tiles of 32 rows for the SMs
+  return blocks_of(a.d, 32) * 8 * 3 >= RESIDENT * a.sms * 2 ? project<T, 2, NB, 3, true>(a, w, s) : project<T, 1, NB, 5, true>(a, w, s);
 }
+
 }  // namespace moe_tokens
 }  // namespace nt
 
