@@ -1341,6 +1341,8 @@ Tensor paged_append(const Tensor& q, const Tensor& k, const Tensor& v, const Ten
   inference_only({&q, &k, &v, &k_pages, &v_pages, &cos, &sin}, {&ve, &ve_gate, &k_scale, &v_scale});
   PagedAppendArgs a;
   a.cache = paged_cache(q, k_pages, v_pages, table, k_scale, v_scale);
+  for (int i = 0; i < 3 && a.cache.k_scale; ++i)
+    TORCH_CHECK(k_scale->size(i) <= 1 || (k_scale->stride(i) > 0 && v_scale->stride(i) > 0), "blocks may not share a scale in memory");
   a.B = static_cast<int>(q.size(0));
   a.t = static_cast<int>(q.size(1));
   a.H = static_cast<int>(q.size(2));

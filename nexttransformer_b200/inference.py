@@ -140,6 +140,8 @@ class PagedCache:
         held, dtype = model.cos.dtype if dtype is None else dtype, model.cos.dtype
         if held not in (dtype, torch.float8_e4m3fn):
             raise ValueError("the cache is held in the model's type or in float8_e4m3fn")
+        if held == torch.float8_e4m3fn and page % BLOCK:
+            raise ValueError(f"a float8_e4m3fn cache has pages of a multiple of {BLOCK} tokens")
         self.rows, self.page, self.columns = rows, page, -(-max_len // page)
         pages = rows * self.columns if pages is None else pages
         mixers = [b.attn for b in model.transformer.h]
@@ -150,7 +152,7 @@ class PagedCache:
         self.pages = {i: (keys[n], values[n]) for n, i in enumerate(attention)}
         self.scales = {i: {} for i in attention}
         if held == torch.float8_e4m3fn:
-            shape = (2, *shape[:3], -(-page // BLOCK))
+            shape = (2, *shape[:3], page // BLOCK)
             k_scale, v_scale = torch.zeros(shape, device=device)
             self.scales = {i: dict(k_scale=k_scale[n], v_scale=v_scale[n]) for n, i in enumerate(attention)}
         self.linear = {}

@@ -154,18 +154,22 @@ class MoEFFN(nn.Module):
     # -------------------------------------------------------------- decoding
     @torch.no_grad()
     def serve(self, dtype):
-        """Lay the weights out in ``dtype`` for ``step``: once, before decoding, and again after they have changed.  A layer with
-        kernel state on CUDA in bf16 shares the routed experts' stacks, which the optimizer keeps; everything else is a copy."""
+        """Lay the weights out in ``dtype`` for ``step``, once before decoding.  A bf16 layer all of whose weights the kernel state keeps
+        uses those, and follows updates as ``forward`` does; otherwise all are copies, to be laid out again after a change."""
         if self.ep_size > 1:
             raise ValueError("experts of other ranks are not served here")
-        experts = self.local_experts()
-        stacked = self._w_fc is not None and dtype == torch.bfloat16
-        self._served = dict(
-            router=self.router.weight.detach().float().contiguous().clone(),
-            w_fc=self._w_fc if stacked else torch.stack([e.c_fc.weight.detach().to(dtype) for e in experts]),
-            w_proj=self._w_proj if stacked else torch.stack([e.c_proj.weight.detach().to(dtype) for e in experts]),
-            shared_fc=None if self.shared is None else self.shared.c_fc.weight.detach().to(dtype, copy=True).contiguous(),
-            shared_proj=None if self.shared is None else self.shared.c_proj.weight.detach().to(dtype, copy=True).contiguous())
+        experts, router = self.local_experts(), self.router.weight.detach()
+        shared = () if self.shared is None else (self.shared.c_fc, self.shared.c_proj)
+        if (self._w_fc is not None and dtype == torch.bfloat16 and router.dtype == torch.float32 and router.is_contiguous()
+                and all(getattr(lin, "_w", None) is not None for lin in shared)):
+            stacks, rows, bias = (self._w_fc, self._w_proj), [lin._w for lin in shared], self.expert_bias
+        else:
+            stacks = [torch.stack([lin.weight.detach().to(dtype) for lin in lins])
+                      for lins in ([e.c_fc for e in experts], [e.c_proj for e in experts])]
+            rows = [lin.weight.detach().to(dtype, copy=True).contiguous() for lin in shared]
+            router, bias = router.float().contiguous().clone(), self.expert_bias.clone()
+        self._served = dict(router=router, w_fc=stacks[0], w_proj=stacks[1], bias=bias,
+                            shared_fc=rows[0] if rows else None, shared_proj=rows[1] if rows else None)
 
     def step(self, x):
         """``forward`` without gradients and load statistics for a few tokens: ``ops.moe.moe_tokens`` on the weights that ``serve``
@@ -175,7 +179,7 @@ class MoEFFN(nn.Module):
         s = self._served
         if s is None or rows.shape[0] > TOKENS_MOST or s["w_fc"].dtype != x.dtype or s["w_fc"].device != x.device:
             return self(x)
-        return moe_tokens(rows, s["router"], s["w_fc"], s["w_proj"], self.top_k, bias=self.expert_bias, shared_fc=s["shared_fc"],
+        return moe_tokens(rows, s["router"], s["w_fc"], s["w_proj"], self.top_k, bias=s["bias"], shared_fc=s["shared_fc"],
                           shared_proj=s["shared_proj"]).reshape_as(x)
 
     @torch.no_grad()

@@ -112,6 +112,9 @@ def test_refusals_of_the_8_bit_cache():
     refused(k_pages, v_pages.float(), k_scale, v_scale)
     refused(k_pages, v_pages, k_scale[:1], v_scale)
     refused(k_pages, v_pages, k_scale.double(), v_scale)
+    with pytest.raises(RuntimeError, match="share a scale"):
+        paged_append(q, q[:, :, :2], q[:, :, :2], k_pages, v_pages, table, start, cos=torch.ones(4, 8), sin=torch.ones(4, 8),
+                     k_scale=k_scale, v_scale=v_scale[:1].expand(2, 2, 1))
     with torch.enable_grad(), pytest.raises(RuntimeError, match="no backward"):
         paged_attention(q, k_pages, v_pages, table, start, k_scale=k_scale.clone().requires_grad_(), v_scale=v_scale)
 
@@ -216,6 +219,25 @@ def test_plain_experts_refusals_and_ties():
         moe_tokens(x.clone().requires_grad_(), router, w_fc, w_proj, 2)
 
 
+def test_laid_out_experts_change_together():
+    """What was laid out stays of one state of the weights until it is laid out again."""
+    from nexttransformer_b200.models.moe import MoEFFN
+    torch.manual_seed(3)
+    layer, x = MoEFFN(32, 8, 3, 24, shared=1).eval(), torch.randn(5, 32)
+    with torch.no_grad():
+        for p in layer.parameters():
+            p.normal_(0, 0.3)
+        before = layer(x)
+        layer.serve(torch.float32)
+        for p in (*layer.parameters(), layer.expert_bias):
+            p.normal_(0, 0.3)
+        after = layer(x)
+        assert not torch.allclose(before, after, rtol=1e-2)
+        assert torch.allclose(layer.step(x), before, rtol=1e-5, atol=1e-5 * before.abs().max().item())
+        layer.serve(torch.float32)
+        assert torch.allclose(layer.step(x), after, rtol=1e-5, atol=1e-5 * after.abs().max().item())
+
+
 # ------------------------------------------------------------------------------------------ the engine
 def test_decode_with_laid_out_experts():
     """Ragged prompts and pausing rows against the same without: the same layer, so the same logits but for the sums' order."""
@@ -257,6 +279,8 @@ def test_decode_over_an_8_bit_cache():
     cache.release(0)
     decode_paged(m, ids[:, :3], cache, [3, 0])
     assert cache.lengths == [3, 4]
+    with pytest.raises(ValueError, match="multiple of 16"):
+        PagedCache(m, 1, 32, page=24, dtype=F8)
     with pytest.raises(ValueError, match="float8_e4m3fn"):
         PagedCache(m, 2, 32, dtype=torch.float16)
 

@@ -324,6 +324,9 @@ def test_8_bit_refusals_and_device_checks():
         append(t, table, 21, "behind the rotary table")
     for x, y in zip((k, v, ks, vs), before):
         assert torch.equal(x.view(torch.uint8), y.view(torch.uint8))
+    x = torch.randn(1, 1, 8, 64, device=DEV).bfloat16()
+    with pytest.raises(RuntimeError, match="share a scale"):
+        paged_append(x[:, :, :4], x[:, :, 4:6], x[:, :, 6:], k, v, table, start, cos=cos, sin=sin, k_scale=ks, v_scale=vs[:1].expand_as(vs))
     with pytest.raises(RuntimeError, match="no backward"):
         paged_attention(**dict(good, k_scale=ks.clone().requires_grad_()))
 
@@ -630,3 +633,28 @@ def test_generation_with_all_four():
     prompts = [[1, 2, 3], [4], list(range(20))]
     answers = [generate_batch(m, prompts, 12, top_p=0.9, min_p=0.01, temperature=[0.5, 1.0, 0.0], cache_dtype=F8) for _ in range(2)]
     assert answers[0] == answers[1] and all(len(a) == 12 for a in answers[0])
+
+
+def test_laid_out_experts_follow_the_kernel_state():
+    """Where the kernel state keeps all of a layer's bf16 weights, one update reaches all of what ``step`` reads."""
+    from dataclasses import replace
+    from nexttransformer_b200.inference import serve_experts
+    from nexttransformer_b200.models import build_model
+    from nexttransformer_b200.models.config import debug_config
+    from nexttransformer_b200.models.moe import MoEFFN
+    c = replace(debug_config("moe"), width=256, heads=4, kv_heads=2, moe_ffn=128)
+    m = build_model(c, DEV, seed=2).eval()
+    m.fused_state()
+    layer = next(b.mlp for b in m.transformer.h if isinstance(b.mlp, MoEFFN))
+    serve_experts(m)
+    assert layer._w_fc is not None and layer._served["w_fc"] is layer._w_fc
+    x = torch.randn(9, 256, device=DEV).to(m.cos.dtype)
+    results = []
+    with torch.no_grad():
+        for _ in range(2):
+            for p in (*layer.parameters(), layer.expert_bias):
+                p.normal_(0, 0.05)
+            m.refresh_shadows()
+            results.append((layer.step(x).double(), layer(x).double()))
+    for got, ref in results:    # the layer's own roundings, as above
+        assert (got - ref).norm() <= 4 * U[torch.bfloat16] * ref.norm()
