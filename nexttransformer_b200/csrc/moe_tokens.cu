@@ -5,13 +5,22 @@
 //
 // Three kernels, each started while the one before it ends:
 //   route  a cluster of CTAs a token: logits in fp32, the choice, and x in the order of a matrix operand
-//   fc     h = c relu(W1 x)^2, a warp for 16 rows of an expert's W1
-//   proj   y, a CTA (or a cluster, by parts of the sum) for 16 rows of every expert's W2, added up in registers
+//   fc     h = c relu(W1 x)^2, a warp (or a few) for 32 rows of an expert's W1
+//   proj   y, a cluster for 32 (or 16) rows of every expert's W2, by parts of the sum
 //
 // With few tokens an expert meets one or two of them, so weights are the 16-row side of a 16 x 8 x 16 matrix instruction and
 // tokens the narrow side; 2 to 16 operations a byte are far below the ratio at which tensor memory would matter.  The work is to
-// keep loads in flight: each warp owns a ring of 2 KB stages (16 rows of 128 bytes) that asynchronous copies fill across the
-// borders of tiles and experts, and waits for nobody else until its sums are done.
+// keep loads in flight: each warp owns a ring of stages (16 or 32 rows of 128 bytes) that asynchronous copies fill across the
+// borders of tiles and experts, and waits for nobody else until its sums are done.  An expert's tokens stand beside each other in
+// the operands (gathered where they are read), so an expert costs a block of 8 columns whoever wants it.
+//
+// 12 tokens, d 2048, 64 experts of 1024, 8 a token and a shared one: 93 us for 438 MB (68 at 6.46 TB/s): fc and proj stream at 5 to 5.8 TB/s once
+// they run, the rest is three launches' ways to their first tile.  One token: 28.7 us for 76 MB (11.8), those ways alone.
+// 64 tokens, 256 experts of 320: 100 us for 368 MB (57), where proj's pieces are five stages long and a third of its 190 instructions a
+// stage begin and end them (19.7 million instructions and 113 us with tokens found in masks, a third walk through the pieces and one sum).
+// Tried and not kept: stages of 128 columns (12 tokens 97 -> 128 us), fc with 16 rows at three CTAs an SM (93 -> 106), L2 prefetches of 256 bytes
+// (1 %), x kept out of shared memory in route (28.7 -> 29.9), weights fetched into L2 while route runs (0 to 2 %) or while fc ends (64 tokens: +10 %),
+// 32 rows and two CTAs an SM for proj of more than 16 tokens (104 -> 112).
 #include "moe_tokens.h"
 #include "warp_mma.cuh"
 
@@ -61,7 +70,8 @@ NT_DEVICE void wait_for_predecessor() { asm volatile("griddepcontrol.wait;" ::: 
 
 // ------------------------------------------------------------------------------------ route
 // A cluster of ROUTE_RANKS CTAs has TOKENS tokens, a part of the experts each; the j-th CTA then chooses for the j-th token.  Several
-// tokens share a reading of the router: 64 tokens on 256 experts of width 1280 took 29 us with one token a cluster.
+// tokens share a reading of the router: 64 tokens on 256 experts of width 1280
+// took 29 us with one token a cluster and 19 with four; the whole layer takes 104 us with four and 100 with two (16 warps a CTA: no less).
 constexpr int ROUTE_RANKS = 8;
 template <class T, int PER, int TOKENS>  // PER: experts a lane
 __global__ void __launch_bounds__(ROUTE_THREADS) route_kernel(const MoeTokensArgs a, const Workspace w) {
@@ -204,7 +214,9 @@ struct Lists {
   uint8_t first[ENTRIES];                // the first of its tokens, counted among the expert's
   uint8_t blocks[ENTRIES];               // of 8 of its tokens: 1 or 2
   int routed, entries;
+  uint4 tokens[ENTRIES];                 // its tokens, a byte each, and -1
 };
+template <bool TOKENS>
 NT_DEVICE void make_lists(const MoeTokensArgs& a, const Workspace& w, Lists& l) {
   const int tid = threadIdx.x, lane = tid & 31;
   for (int e = tid; e <= a.E; e += THREADS) l.mask[e] = 0;
@@ -247,13 +259,23 @@ NT_DEVICE void make_lists(const MoeTokensArgs& a, const Workspace& w, Lists& l) 
     }
   }
   __syncthreads();
+  if constexpr (TOKENS) {
+    for (int i = tid; i < l.entries; i += THREADS) {
+      unsigned long long m = l.mask[l.expert[i]];
+      for (int skip = l.first[i]; skip; --skip) m &= m - 1;
+      uint32_t u[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        u[j / 4] |= static_cast<uint32_t>((__ffsll(static_cast<long long>(m)) - 1) & 0xff) << (j % 4 * 8);
+        m &= m - 1;
+      }
+      l.tokens[i] = make_uint4(u[0], u[1], u[2], u[3]);
+    }
+    __syncthreads();
+  }
 }
-// The n-th token (from 0) of a mask, or -1.
-NT_DEVICE int nth_token(unsigned long long m, int n) {
-  if ((m & (m + 1)) == 0) return n < __popcll(m) ? n : -1;  // all of the first
-  for (int i = 0; i < n && m; ++i) m &= m - 1;
-  return m ? __ffsll(static_cast<long long>(m)) - 1 : -1;
-}
+// The n-th token (from 0) of an entry, or -1.
+NT_DEVICE int nth_token(const Lists& l, int entry, int n) { return reinterpret_cast<const int8_t*>(l.tokens + entry)[n]; }
 
 // A warp's ring: STAGES stages of 16 MT rows of 64 elements, chunk c (16 bytes) of row r at c ^ (r & 7).
 struct Ring {
@@ -285,6 +307,12 @@ struct Piece {
   int behind;         // what comes after it: an item, or a stage of all
 };
 
+struct Brief {  // what the products need of a piece
+  int entry, expert, tile;
+  unsigned blocks;
+  bool last, more;  // this stage is the piece's last; there is one
+};
+
 // Goes through a warp's pieces: weights come `STAGES - 1` stages ahead, the other operand one.
 //   first(piece) / next(piece) set a piece and say whether there is one (the copies, the operand and the products each go through them);
 //   base(piece): the tile's first weight; operand(piece, pointers): this lane's part of the 16 x 8 tile of the piece's next stage, of
@@ -301,7 +329,8 @@ NT_DEVICE void stream(const MoeTokensArgs& a, const void* smem, const int step, 
   Ring r = make_ring<STAGES * STAGE>(smem);
   auto turn = [&](uint32_t& stage) { stage = stage == r.base + (STAGES - 1) * STAGE ? r.base : stage + STAGE; };
   const int lane = threadIdx.x & 31, row = lane >> 3, chunk = lane & 7;
-  Piece f, o, c;  // where the copies, the operand and the products stand
+  Piece f, o;  // where the copies and the operand stand
+  Brief c, n;  // the piece of the stage that is multiplied, and of the next one
   bool f_more = first(f);
   const char* f_at = nullptr;
   int64_t f_step = 0;  // four rows
@@ -338,11 +367,17 @@ NT_DEVICE void stream(const MoeTokensArgs& a, const void* smem, const int step, 
   for (int i = 0; i < STAGES - 1; ++i) fetch();
   ready();
 
-  bool o_more = first(o), c_more = first(c);
+  bool o_more = first(o);
   const Frag* at[NB];
   if (o_more) operand(o, at);
   auto load = [&](Frag (&b)[4][NB]) {
+    n.more = o_more;
     if (!o_more) return;
+    n.entry = o.entry;
+    n.expert = o.expert;
+    n.tile = o.tile;
+    n.blocks = o.blocks;
+    n.last = o.stage + 1 == o.stages;
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb)
       if ((o.blocks >> nb) & 1u) {
@@ -364,7 +399,24 @@ NT_DEVICE void stream(const MoeTokensArgs& a, const void* smem, const int step, 
     for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
       for (int e = 0; e < 4; ++e) acc[m][nb][e] = 0.f;
+  // second numbers add up beside the first, where registers allow it: products on one sum wait for each other
+  constexpr bool APART = TWO && MT * NB <= 2;
+  float low[MT][NB][4] = {};
+  auto together = [&]() {
+    if constexpr (APART) {
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            acc[m][nb][e] += low[m][nb][e];
+            low[m][nb][e] = 0.f;
+          }
+    }
+  };
   auto multiply = [&](const Frag (&b)[4][NB], Frag (&ahead)[4][NB]) {
+    c = n;
     load(ahead);
     cp_wait<STAGES - 2>();
     __syncwarp();  // this stage has landed for every lane, and the stage before it is read by none
@@ -383,11 +435,12 @@ NT_DEVICE void stream(const MoeTokensArgs& a, const void* smem, const int step, 
 #pragma unroll
           for (int s = 0; s < 4; ++s) {
             Num<T>::mma(acc[m][nb], w[s], b[s][nb].x, b[s][nb].y);
-            if constexpr (TWO) Num<T>::mma(acc[m][nb], w[s], b[s][nb].z, b[s][nb].w);
+            if constexpr (TWO) Num<T>::mma(APART ? low[m][nb] : acc[m][nb], w[s], b[s][nb].z, b[s][nb].w);
           }
     }
-    if (++c.stage == c.stages) {
-      if constexpr (!KEEP) {
+    if constexpr (!KEEP)
+      if (c.last) {
+        together();
         done(c, acc);
 #pragma unroll
         for (int m = 0; m < MT; ++m)
@@ -396,17 +449,16 @@ NT_DEVICE void stream(const MoeTokensArgs& a, const void* smem, const int step, 
 #pragma unroll
             for (int e = 0; e < 4; ++e) acc[m][nb][e] = 0.f;
       }
-      c_more = next(c);
-    }
   };
   Frag even[4][NB], odd[4][NB];
   load(even);
 #pragma unroll 1
-  while (c_more) {
+  while (n.more) {
     multiply(even, odd);
-    if (!c_more) break;
+    if (!n.more) break;
     multiply(odd, even);
   }
+  if constexpr (KEEP) together();
   cp_wait<0>();
 }
 
@@ -422,7 +474,7 @@ __global__ void __launch_bounds__(THREADS, RESIDENT) fc_kernel(const MoeTokensAr
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   wait_for_predecessor();
   dependents_may_start();
-  make_lists(a, w, l);
+  make_lists<true>(a, w, l);
   constexpr int ROWS = 16 * FC_MT;
   const int tiles = (a.F + ROWS - 1) / ROWS, shared_tiles = (a.Fs + ROWS - 1) / ROWS, groups = groups_of(a.F), shared_groups = groups_of(a.Fs);
   const int routed = l.routed * tiles, items = routed + (l.entries - l.routed) * shared_tiles;
@@ -457,16 +509,15 @@ __global__ void __launch_bounds__(THREADS, RESIDENT) fc_kernel(const MoeTokensAr
         return e + static_cast<int64_t>(p.tile) * ROWS * a.d;
       },
       [&](const Piece& p, const uint2* (&at)[NB]) {
-        const unsigned long long mask = l.mask[p.expert];
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
           // columns without a token may be anyone's: they are dropped
-          const int t = max(0, nth_token(mask, l.first[p.entry] + nb * 8 + (lane >> 2)));
+          const int t = max(0, nth_token(l, p.entry, nb * 8 + (lane >> 2)));
           at[nb] = w.x + (t >> 3) * 32 + (t & 7) * 4 + (lane & 3) + p.stage * 4 * ((a.T + 7) / 8 * 32);
         }
       },
       [] {},
-      [&](const Piece& p, float (&acc)[FC_MT][NB][4]) {
+      [&](const Brief& p, float (&acc)[FC_MT][NB][4]) {
         if (wide > 1) {  // the first warp adds up
 #pragma unroll
           for (int m = 0; m < FC_MT; ++m)
@@ -488,7 +539,6 @@ __global__ void __launch_bounds__(THREADS, RESIDENT) fc_kernel(const MoeTokensAr
         // h, in the order in which it is an operand: rows of the tile become the products' inner dimension.  It is held as two
         // numbers of its type, so that nothing but the output is rounded.
         const bool shared = p.expert == a.E;
-        const unsigned long long mask = l.mask[p.expert];
         const int inner = shared ? shared_groups : groups;
         uint4* h = w.h + (shared ? static_cast<int64_t>(w.pairs) * groups : 0ll) * 32;
 #pragma unroll
@@ -498,7 +548,7 @@ __global__ void __launch_bounds__(THREADS, RESIDENT) fc_kernel(const MoeTokensAr
           float share[2];
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            t[e] = nth_token(mask, l.first[p.entry] + nb * 8 + (lane & 3) * 2 + e);
+            t[e] = nth_token(l, p.entry, nb * 8 + (lane & 3) * 2 + e);
             share[e] = t[e] < 0 ? 0.f : shared ? LOWER<T> : LOWER<T> * __ldcg(w.share + static_cast<int64_t>(t[e]) * a.E + p.expert);
           }
           uint4* to = h + ((static_cast<int64_t>(l.block[p.entry]) + nb) * inner + p.tile * FC_MT) * 32 + lane;
@@ -534,7 +584,7 @@ __global__ void __launch_bounds__(THREADS, RESIDENT) proj_kernel(const MoeTokens
   float* const sums = reinterpret_cast<float*>(smem + (KEEP ? 0 : WARPS * STAGES * MT * TILE));  // [warp][token][PITCH]
   if (!KEEP)
     for (int i = tid; i < WARPS * a.T * PITCH; i += THREADS) sums[i] = 0.f;
-  make_lists(a, w, l);  // (the route kernel ended before the one before this began its work)
+  make_lists<!KEEP>(a, w, l);  // (the route kernel ended before the one before this began its work)
   const int per = (a.F + 63) / 64, shared_per = (a.Fs + 63) / 64, groups = groups_of(a.F), shared_groups = groups_of(a.Fs);
   // an equal run of the stages of all entries
   const int routed = l.routed * per, all = routed + (l.entries - l.routed) * shared_per;
@@ -596,13 +646,13 @@ __global__ void __launch_bounds__(THREADS, RESIDENT) proj_kernel(const MoeTokens
         }
       },
       [] { wait_for_predecessor(); },  // weights may come before, h may not
-      [&](const Piece& p, const float (&own)[MT][NB][4]) {
-        const unsigned long long mask = l.mask[p.expert];
+      [&](const Brief& p, const float (&own)[MT][NB][4]) {
 #pragma unroll
-        for (int nb = 0; nb < NB; ++nb)
+        for (int nb = 0; nb < NB; ++nb) {
+          if (!((p.blocks >> nb) & 1u)) break;
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            const int t = nth_token(mask, l.first[p.entry] + nb * 8 + (lane & 3) * 2 + e);
+            const int t = nth_token(l, p.entry, nb * 8 + (lane & 3) * 2 + e);
             if (t < 0) continue;
             float* to = sums + (warp * a.T + t) * PITCH + (lane >> 2);
 #pragma unroll
@@ -611,6 +661,7 @@ __global__ void __launch_bounds__(THREADS, RESIDENT) proj_kernel(const MoeTokens
               to[16 * m + 8] += own[m][nb][e + 2];
             }
           }
+        }
         __syncwarp();  // the next entry's lanes may hold this one's tokens elsewhere
       });
   if (KEEP) {
@@ -696,8 +747,8 @@ static int route(const MoeTokensArgs& a, const Workspace& w, cudaStream_t s) {
 template <class T>
 static int route_for(const MoeTokensArgs& a, const Workspace& w, cudaStream_t s) {
   // as few tokens a cluster as keep the clusters on the SMs at once, and as 48 KB hold
-  if (a.T * ROUTE_RANKS <= a.sms || a.d * 16 > 48 * 1024) return route<T, 1>(a, w, s);
-  return route<T, 4>(a, w, s);
+  if (a.T * ROUTE_RANKS <= a.sms || a.d * 8 > 48 * 1024) return route<T, 1>(a, w, s);
+  return route<T, 2>(a, w, s);
 }
 // Clusters of more than 8 CTAs have to be allowed for a kernel, on each device once.
 template <class Kernel>
