@@ -8,10 +8,17 @@
 // the split of a row change nothing, and a token differs from the one that real numbers give only when u lies within
 // about V 2^-S of a border.
 //
-// A row lies in the shared memory of a cluster of CTAs and is read from memory once.  A selection's border (the k-th, or the
-// one at which p is reached) is found by a histogram of 2048 bins of T / 32 below the maximum, whose bins the CTAs add up
-// through distributed shared memory; the few logits of the border's bin are then ranked among each other.  Where
-// they are many, further histograms split the bin by the numbers' bits, and equal logits by their indices.
+// A row lies in the shared memory of a cluster of CTAs and is read from memory once (longer ones are read again, from L2).  A
+// selection's border (the k-th, or the one at which p is reached) is found by a histogram of 2048 bins of T / 32 below the
+// maximum, whose bins the CTAs add up through distributed shared memory.  What can be kept, where it is few, goes to one CTA, which
+// ranks the border's bin and draws; where it is many, the masses before the border's bin are summed by runs of indices.  A bin of
+// more than 1024 is split by the numbers' bits, and equal logits by their indices.
+//
+// Bound by latency and by 64-bit arithmetic: 1 x 32768, top-k and top-p: 14 us, of which (clock stamps) loads take 0.5, the maximum 1.3, the
+// histogram 1.1, its crossing and the list 3.4, the gathering 1.8, the two borders 3.1, the draw 2.4.  224 x 65536 with a setting for each row: 80 us
+// for 59 MB (9 at the copy rate): two CTAs an SM, so three to four rounds, each CTA 17 us (top-k) to 40 (top-p alone), with 8 or 9
+// for each pass that takes the exp of every logit in 64 bits.
+// Tried and not kept: a sort of the kept ones (5 us and more), every CTA reading all bins' masses of all (15 us instead of 4).
 #include "sampling.h"
 #include "common.cuh"
 
