@@ -658,3 +658,61 @@ def test_laid_out_experts_follow_the_kernel_state():
             results.append((layer.step(x).double(), layer(x).double()))
     for got, ref in results:    # the layer's own roundings, as above
         assert (got - ref).norm() <= 4 * U[torch.bfloat16] * ref.norm()
+
+
+def test_8_bit_cache_captured_and_on_two_streams():
+    """A step (append and attention) captured once and replayed over several positions, across a block's border, beside the same on another
+    stream: both equal eager steps bit for bit."""
+    from nexttransformer_b200.ops._ext import check_errors
+    from nexttransformer_b200.ops.paged import paged_append, paged_attention
+    B, H, Hk, D = 5, 8, 2, 128
+    lengths = [13, 0, 31, 200, 64]
+    cos, sin = torch.ones(300, D // 2, device=DEV).bfloat16(), torch.zeros(300, D // 2, device=DEV).bfloat16()
+    torch.manual_seed(9)
+    news = [torch.randn(B, 1, H + 2 * Hk, D, device=DEV).bfloat16() for _ in range(6)]
+
+    def state():
+        k, v, ks, vs, table = make_cache8([n + 8 for n in lengths], Hk, 32, D)
+        return dict(k=k, v=v, ks=ks, vs=vs, table=table, x=torch.zeros_like(news[0]), start=torch.tensor(lengths, device=DEV, dtype=torch.int32))
+
+    def step(s):
+        x = s["x"]
+        q = paged_append(x[:, :, :H], x[:, :, H:H + Hk], x[:, :, H + Hk:], s["k"], s["v"], s["table"], s["start"], cos=cos, sin=sin, qk_scale=1.2,
+                         k_scale=s["ks"], v_scale=s["vs"])
+        y = paged_attention(q, s["k"], s["v"], s["table"], s["start"], k_scale=s["ks"], v_scale=s["vs"])
+        s["start"] += 1
+        return y
+
+    first = state()
+    states = [first] + [{n: t.clone() for n, t in first.items()} for _ in range(2)]
+    eager = []
+    for x in news:
+        states[0]["x"].copy_(x)
+        eager.append(step(states[0]).clone())
+    streams, graphs, outs = [torch.cuda.Stream() for _ in range(2)], [], []
+    torch.cuda.synchronize()
+    for s, stream in zip(states[1:], streams):
+        keep = {n: t.clone() for n, t in s.items()}
+        with torch.cuda.stream(stream):
+            step(s)                                     # once before capture
+            for n, t in keep.items():
+                s[n].copy_(t)
+        stream.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            outs.append(step(s))
+        graphs.append(graph)
+    got = [[], []]
+    for x in news:
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                states[1 + i]["x"].copy_(x)
+                graphs[i].replay()
+                got[i].append(outs[i].clone())
+    torch.cuda.synchronize()
+    for i in range(2):
+        for a, b in zip(got[i], eager):
+            assert torch.equal(a, b)
+        for n in ("k", "v", "ks", "vs"):
+            assert torch.equal(states[1 + i][n].view(torch.uint8), states[0][n].view(torch.uint8))
+    check_errors()
