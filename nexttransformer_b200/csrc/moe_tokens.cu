@@ -746,8 +746,8 @@ static int route(const MoeTokensArgs& a, const Workspace& w, cudaStream_t s) {
 }
 template <class T>
 static int route_for(const MoeTokensArgs& a, const Workspace& w, cudaStream_t s) {
-  // as few tokens a cluster as keep the clusters on the SMs at once, and as 48 KB hold
-  if (a.T * ROUTE_RANKS <= a.sms || a.d * 8 > 48 * 1024) return route<T, 1>(a, w, s);
+  // as few tokens a cluster as keep the clusters on the SMs at once, and as 48 KB hold beside the logits
+  if (a.T * ROUTE_RANKS <= a.sms || a.d * 8 > 48 * 1024 - static_cast<int>(sizeof(float)) * EXPERTS) return route<T, 1>(a, w, s);
   return route<T, 2>(a, w, s);
 }
 // Clusters of more than 8 CTAs have to be allowed for a kernel, on each device once.

@@ -471,7 +471,7 @@ def check_experts(got, ref, size, dtype, steps):
 @pytest.mark.parametrize("T,d,F,E,k,shared", [
     (1, 256, 128, 8, 2, 128), (1, 8, 8, 1, 1, 0), (2, 2048, 264, 64, 8, 264), (3, 72, 200, 5, 5, 8), (8, 640, 136, 33, 4, 0),
     (9, 640, 136, 32, 4, 136), (17, 128, 64, 4, 1, 64), (33, 136, 72, 3, 2, 0), (64, 320, 80, 256, 8, 80), (64, 64, 24, 2, 2, 4000),
-    (5, 8192, 16, 512, 16, 0), (64, 1280, 320, 4, 2, 320), (12, 512, 1024, 16, 16, 1024)])
+    (5, 8192, 16, 512, 16, 0), (20, 5888, 24, 6, 2, 8), (31, 5896, 8, 6, 2, 0), (64, 6144, 16, 5, 1, 0), (64, 8192, 8, 300, 2, 8), (64, 1280, 320, 4, 2, 320), (12, 512, 1024, 16, 16, 1024)])
 def test_experts_of_a_few_tokens(T, d, F, E, k, shared, dtype):
     from nexttransformer_b200.ops.moe import moe_tokens
     a = make_experts(T, d, F, E, shared, dtype, seed=T * 1000 + d)
