@@ -4,7 +4,7 @@
 //   y = sum over the chosen of c W2 relu(W1 x)^2 + W2' relu(W1' x)^2 (the shared expert)
 //
 // Three kernels, each started while the one before it ends:
-//   route  a cluster of CTAs a token: logits in fp32, the choice, and x in the order of a matrix operand
+//   route  a cluster of 8 CTAs for one or two tokens: logits in fp32, the choice, and x in the order of a matrix operand
 //   fc     h = c relu(W1 x)^2, a warp (or a few) for 32 rows of an expert's W1
 //   proj   y, a cluster for 32 (or 16) rows of every expert's W2, by parts of the sum
 //
@@ -14,8 +14,8 @@
 // borders of tiles and experts, and waits for nobody else until its sums are done.  An expert's tokens stand beside each other in
 // the operands (gathered where they are read), so an expert costs a block of 8 columns whoever wants it.
 //
-// 12 tokens, d 2048, 64 experts of 1024, 8 a token and a shared one: 93 us for 438 MB (68 at 6.46 TB/s): fc and proj stream at 5 to 5.8 TB/s once
-// they run, the rest is three launches' ways to their first tile.  One token: 28.7 us for 76 MB (11.8), those ways alone.
+// 12 tokens, d 2048, 64 experts of 1024, 8 a token and a shared one: 91 to 93 us for 438 MB (68 at 6.46 TB/s): fc and proj stream at about 5 TB/s once
+// they run, the rest is three launches' ways to their first tile.  One token: 29 us for 76 MB (11.8), those ways alone.
 // 64 tokens, 256 experts of 320: 100 us for 368 MB (57), where proj's pieces are five stages long and a third of its 190 instructions a
 // stage begin and end them (19.7 million instructions and 113 us with tokens found in masks, a third walk through the pieces and one sum).
 // Tried and not kept: stages of 128 columns (12 tokens 97 -> 128 us), fc with 16 rows at three CTAs an SM (93 -> 106), L2 prefetches of 256 bytes
