@@ -215,7 +215,8 @@ NT_DEVICE void add_to_bin(const R& r, Shared& s, int bin, float x) {
 // The bin in which the sum over the cluster's bins (`alone`: this CTA's) reaches the target, or -1; `before`: the sum over those
 // before it.  A target of 0 is set to `share` of the whole first.  Counts of up to four
 // CTAs are read by all of them; else each adds up its part of the bins and tells the others (all masses of eight CTAs read by all took 15 us
-// instead of 4).
+// instead of 4).  Where all read all, others may still be at this CTA's bins when it returns: `s.count` and what shares its memory may be
+// written again only behind a cluster barrier.
 template <bool MASS, class R>
 NT_DEVICE int crossing(const R& r, Shared& s, int& round, u64& target, float share, u64& before, bool alone = false) {
   constexpr int MOST = BINS / THREADS;
@@ -830,6 +831,8 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const SampleArgs a, 
       if (chosen >= 0) {  // (else the k-th has no weight)
         if (draw_from_few<false>(a, r, s, round, kept, chosen, target, before, f, b)) return;
         kept = find_border<false>(r, s, round, kept, target, chosen, before);
+      } else {
+        cluster_sync();  // the bins are read by all, and may be cleared
       }
     }
     if (f.share < 1.f) {
