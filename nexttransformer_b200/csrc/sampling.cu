@@ -103,7 +103,7 @@ struct Row {
   float top;         // the row's largest
   float none;        // smaller ones have no weight
   bool infinite;     // the largest are inf: they count as 0, the others as -inf
-  double factor, offset;  // 64 log2(e) / T, and -top times it
+  double factor, peak;  // 64 log2(e) / T; top
   const double* table;
   float per_bin;     // bins a logit's distance from the top
   int shift;         // S
@@ -133,7 +133,7 @@ struct Row {
 template <class R>
 NT_DEVICE double power(const R& r, float x, int shift) {
   constexpr double LN = 0.69314718055994530942 / TABLE, MAGIC = 6755399441055744.0;  // 1.5 2^52: adding it rounds to a whole number
-  const double t = fma(static_cast<double>(fmaxf(x, r.none)), r.factor, r.offset);
+  const double t = (static_cast<double>(fmaxf(x, r.none)) - r.peak) * r.factor;  // 0 for the top whatever T is: of two products a rest would stay
   const double whole = t + MAGIC, z = t - (whole - MAGIC);
   double p = LN * LN * LN * LN / 24;
   p = fma(p, z, LN * LN * LN / 6);
@@ -142,7 +142,7 @@ NT_DEVICE double power(const R& r, float x, int shift) {
   p = fma(p, z, 1.0);
   const int n = __double2loint(whole);
   p *= r.table[n & (TABLE - 1)];
-  // p 2^e; never below 2^-102, so that only the exponent's bits change
+  // p 2^e; never below 2^-140 (48 T may be rounded to twice that), so that only the exponent's bits change
   const double v = __hiloint2double(__double2hiint(p) + (((n >> 6) + shift) << 20), __double2loint(p));
   return x < r.none ? 0.0 : v;
 }
@@ -809,7 +809,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const SampleArgs a, 
   const bool greedy = !(heat > 0.f);
   r.top = top;
   r.factor = greedy ? 0.0 : TABLE * 1.4426950408889634074 / static_cast<double>(heat);
-  r.offset = -r.factor * static_cast<double>(top);
+  r.peak = top;
   r.table = s.table;
   r.none = fmaxf(top - 48.f * heat, -3.4028235e38f);  // 2^-69
   r.per_bin = fminf(32.f / heat, 3e38f);

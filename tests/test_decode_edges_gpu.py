@@ -29,3 +29,44 @@ def test_sampling_with_fewer_permitted_tokens_than_top_k(B, V, allowed):
     x[::3, 1:] = -math.inf
     some = torch.where(torch.arange(B, device=DEV) % 2 == 0, k, max(1, allowed // 2)).int()
     both(x, u, top_k=some, top_p=0.8)
+
+
+# what a call may ask for: drawn by one CTA from a few, by sums up to a border, and from a whole row
+WAYS = [dict(), dict(top_k=17), dict(top_p=0.37), dict(top_k=7000, top_p=0.9), dict(min_p=0.02), dict(top_k=40, top_p=0.5, min_p=0.3)]
+
+
+@pytest.mark.parametrize("V,dtype", [(700, torch.bfloat16), (32768, torch.float32), (32768, torch.bfloat16), (131072, torch.float32)])
+def test_sampling_at_low_temperatures(V, dtype):
+    """The largest logit's weight is 1 whatever top / T is: one largest, and many that share the choice."""
+    torch.manual_seed(V)
+    single = torch.randn(6, V, device=DEV) * 4 + torch.tensor([15.0, -20.0, 3.0, 0.0, 31.0, 14.3], device=DEV)[:, None]
+    many = torch.where(torch.rand(6, V, device=DEV) < 0.4, 14.3, single.clamp(max=10.0))
+    u = torch.rand(6, device=DEV)
+    for x in (single, many):
+        for T in (1e-9, 1e-12, 1e-14, 1e-15, 1e-16, 1e-17, 1e-18, 1e-20, 1e-24, 1e-38, 1e-44):
+            for kw in WAYS:
+                both(x.to(dtype), u, temperature=T, **kw)
+    T = torch.tensor([1e-9, 1e-16, 1e-17, 1e-20, 0.7, 1e-24], device=DEV)
+    for kw in WAYS:
+        both(single.to(dtype), u, temperature=T, **kw)
+
+
+@pytest.mark.parametrize("V,dtype", [(700, torch.float32), (700, torch.bfloat16), (32768, torch.float32), (131072, torch.bfloat16)])
+def test_sampling_of_large_logits(V, dtype):
+    """Logits as a bias of 1e18 leaves them, and rows that are large altogether."""
+    torch.manual_seed(V + 1)
+    rows = torch.randn(4, V, device=DEV)
+    u = torch.rand(4, device=DEV)
+    for size in (1e9, 6e15, 1e17, 1e19, 1e30, 3e38):
+        for sign in (1, -1):
+            one, equal, some = rows.clone(), torch.full_like(rows, sign * size), rows.clone()
+            one[:, V // 3] = size if sign > 0 else one[:, V // 3]
+            if sign < 0:
+                one = one - size                     # most of them equal, by rounding
+            some[:, 5::7] = sign * size              # a seventh of the row above, or below, the rest
+            for x in (one, equal, some):
+                for T in (0.3, 1.0):
+                    for kw in WAYS:
+                        both(x.to(dtype), u, temperature=T, **kw)
+        both((rows * min(size, 1e37)).to(dtype), u, temperature=min(size, 1e37) / 2, top_p=0.9)
+        both((rows * min(size, 1e37)).to(dtype), u, temperature=min(size, 1e37) / 2, top_k=50)
