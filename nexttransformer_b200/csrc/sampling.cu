@@ -105,7 +105,7 @@ struct Row {
   bool infinite;     // the largest are inf: they count as 0, the others as -inf
   double factor, peak;  // 64 log2(e) / T; top
   const double* table;
-  float per_bin;     // bins a logit's distance from the top
+  float half_top, per_bin;  // half the largest; bins for half a logit's distance from it
   int shift;         // S
 
   NT_DEVICE float operator[](int i) const {
@@ -152,9 +152,10 @@ NT_DEVICE u64 weight_of(const R& r, float x) {
   return static_cast<u64>(__double_as_longlong(v)) & 0xfffffffffffffull;
 }
 // Bins keep the order of the logits; the last, from 64 T on, has no weight (-inf and NaN, of inf 0, go there).  Adding 2^23 rounds
-// to a whole number, which is the sum's lower bits: a conversion would take an instruction of a quarter of the rate.
+// to a whole number, which is the sum's lower bits: a conversion would take an instruction of a quarter of the rate.  (Half the distance: the
+// whole passes fp32's range where logits of 3e38 stand on both sides of 0.)
 template <class R>
-NT_DEVICE float bin_sum(const R& r, float x) { return fminf((r.top - x) * r.per_bin, static_cast<float>(BINS - 1)) + 8388608.f; }
+NT_DEVICE float bin_sum(const R& r, float x) { return fminf(fmaf(x, -0.5f, r.half_top) * r.per_bin, static_cast<float>(BINS - 1)) + 8388608.f; }
 template <class R>
 NT_DEVICE int bin_of(const R& r, float x) { return __float_as_int(bin_sum(r, x)) & (BINS - 1); }
 NT_DEVICE bool within(const Border& b, float x, int index) {
@@ -812,7 +813,8 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const SampleArgs a, 
   r.peak = top;
   r.table = s.table;
   r.none = fmaxf(top - 48.f * heat, -3.4028235e38f);  // 2^-69
-  r.per_bin = fminf(32.f / heat, 3e38f);
+  r.half_top = 0.5f * top;
+  r.per_bin = fminf(64.f / heat, 3e38f);
   r.shift = min(50, 30 + __clz(a.V));  // V 2^S <= 2^62
 
   const Filters f = {top_k > 0 && top_k < a.V ? top_k : 0x7fffffff, top_p < 1.f ? top_p : 1.f,
@@ -839,7 +841,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const SampleArgs a, 
       target = 0;
       const int chosen = first_crossing<true>(r, s, round, kept, target, f.share, before);
       // The mass over the weight of the bin's lower end bounds their number; real rows have an eighth of that, or less
-      const bool few = target >> 3 <= static_cast<u64>(FEW) * weight_of(r, top - static_cast<float>(chosen + 1) / r.per_bin);
+      const bool few = target >> 3 <= static_cast<u64>(FEW) * weight_of(r, top - static_cast<float>(2 * chosen + 2) / r.per_bin);
       if (few && draw_from_few<true>(a, r, s, round, kept, chosen, target, before, f, b)) return;
       Border cut;
       summed = sum_up_to(r, s, round, kept, chosen, target, before, f, cut, sums);

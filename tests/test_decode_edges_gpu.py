@@ -70,3 +70,14 @@ def test_sampling_of_large_logits(V, dtype):
                         both(x.to(dtype), u, temperature=T, **kw)
         both((rows * min(size, 1e37)).to(dtype), u, temperature=min(size, 1e37) / 2, top_p=0.9)
         both((rows * min(size, 1e37)).to(dtype), u, temperature=min(size, 1e37) / 2, top_k=50)
+
+
+@pytest.mark.parametrize("V,dtype", [(50, torch.float32), (700, torch.bfloat16), (32768, torch.float32)])
+def test_sampling_where_logits_lie_further_apart_than_fp32_reaches(V, dtype):
+    torch.manual_seed(V + 2)
+    x = ((torch.rand(4, V, device=DEV) * 2 - 1) * 3.3e38).to(dtype)
+    x[:, 0], x[:, -1] = 3.3e38, -3.3e38
+    u = torch.rand(4, device=DEV)
+    for T in (1e36, 1e37, 1e38, 3e38, math.inf):
+        for kw in (*WAYS, dict(top_k=V - 1), dict(top_p=0.999)):
+            both(x, u, temperature=T, **kw)
