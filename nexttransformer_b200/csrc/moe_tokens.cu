@@ -33,10 +33,15 @@ constexpr int ROUTE_WARPS = 8, ROUTE_THREADS = ROUTE_WARPS * 32;
 constexpr int WARPS = 4, THREADS = WARPS * 32, RESIDENT = 3;  // of the products: three CTAs an SM
 constexpr int TILE = 16 * 128;  // bytes of 16 rows of 64 elements
 constexpr int MOST = NT_MOE_TOKENS_MOST, EXPERTS = NT_MOE_TOKENS_EXPERTS, CHOICES = NT_MOE_TOKENS_CHOICES;
-// Hidden values are held in the weights' type.  fp16 ends at 65504, which a square passes where its root is 256: they
-// are held as 2^-6 of themselves there (up to 4.2e6), and the sums are raised again.
+// Hidden values are held in the weights' type, as two numbers: the value rounded, and what that left.  fp16 ends at 65504, which a
+// square passes where its root is 256: they are held as 2^-6 of themselves there (up to 4.2e6), and the sums are raised again.  Its smallest step, 2^-24,
+// would then leave 2^-19 of any value out, however small, where outputs are rounded by as little as 2^-25.  So the second number
+// is 2^11 times what is left (at most 16, half a unit of the largest, so 2^15), and has sums of its own: a hidden value is off by 2^-22 of itself or
+// 2^-30, and a row of W2 would need a norm of 32 before that showed in an output.
 template <class T> constexpr float LOWER = 1.f;
 template <> constexpr float LOWER<__half> = 1.f / 64;
+template <class T> constexpr float FINER = 1.f;
+template <> constexpr float FINER<__half> = 2048.f;
 
 struct Workspace {
   int* choice;    // [T, k]
@@ -399,8 +404,8 @@ NT_DEVICE void stream(const MoeTokensArgs& a, const void* smem, const int step, 
     for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
       for (int e = 0; e < 4; ++e) acc[m][nb][e] = 0.f;
-  // second numbers add up beside the first, where registers allow it: products on one sum wait for each other
-  constexpr bool APART = TWO && MT * NB <= 2;
+  // second numbers add up beside the first, where registers allow it (products on one sum wait for each other) or they are finer
+  constexpr bool APART = TWO && (MT * NB <= 2 || FINER<T> != 1.f);
   float low[MT][NB][4] = {};
   auto together = [&]() {
     if constexpr (APART) {
@@ -410,7 +415,7 @@ NT_DEVICE void stream(const MoeTokensArgs& a, const void* smem, const int step, 
         for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            acc[m][nb][e] += low[m][nb][e];
+            acc[m][nb][e] += low[m][nb][e] * (1.f / FINER<T>);
             low[m][nb][e] = 0.f;
           }
     }
@@ -537,7 +542,7 @@ __global__ void __launch_bounds__(THREADS, RESIDENT) fc_kernel(const MoeTokensAr
           if (part) return;
         }
         // h, in the order in which it is an operand: rows of the tile become the products' inner dimension.  It is held as two
-        // numbers of its type, so that nothing but the output is rounded.
+        // numbers of its type, so that little but the output's rounding shows.
         const bool shared = p.expert == a.E;
         const int inner = shared ? shared_groups : groups;
         uint4* h = w.h + (shared ? static_cast<int64_t>(w.pairs) * groups : 0ll) * 32;
@@ -563,8 +568,8 @@ __global__ void __launch_bounds__(THREADS, RESIDENT) fc_kernel(const MoeTokensAr
             const uint32_t hi0 = Num<T>::pack(v[0], v[1]), hi1 = Num<T>::pack(v[2], v[3]);
             const float2 f0 = Num<T>::unpack(hi0), f1 = Num<T>::unpack(hi1);
             // (of an infinite value the rest is NaN, and so would the sum be)
-            const uint32_t lo0 = Num<T>::pack(isinf(f0.x) ? 0.f : v[0] - f0.x, isinf(f0.y) ? 0.f : v[1] - f0.y);
-            const uint32_t lo1 = Num<T>::pack(isinf(f1.x) ? 0.f : v[2] - f1.x, isinf(f1.y) ? 0.f : v[3] - f1.y);
+            auto rest = [](float value, float held) { return isinf(held) ? 0.f : (value - held) * FINER<T>; };
+            const uint32_t lo0 = Num<T>::pack(rest(v[0], f0.x), rest(v[1], f0.y)), lo1 = Num<T>::pack(rest(v[2], f1.x), rest(v[3], f1.y));
             *to = make_uint4(transpose8x8(hi0), transpose8x8(hi1), transpose8x8(lo0), transpose8x8(lo1));
           }
           if (p.tile == (shared ? shared_tiles : tiles) - 1)  // the groups behind the last

@@ -4,7 +4,7 @@ import math
 import pytest
 import torch
 
-from tests.test_decode_ops_gpu import both
+from tests.test_decode_ops_gpu import both, check_experts, experts, make_experts
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -81,3 +81,36 @@ def test_sampling_where_logits_lie_further_apart_than_fp32_reaches(V, dtype):
     for T in (1e36, 1e37, 1e38, 3e38, math.inf):
         for kw in (*WAYS, dict(top_k=V - 1), dict(top_p=0.999)):
             both(x, u, temperature=T, **kw)
+
+
+# ------------------------------------------------------------------------------------------ experts
+@pytest.mark.parametrize("scale", [1.0, 0.1, 0.03, 0.01, 0.001])
+@pytest.mark.parametrize("T,d,F,E,k,shared", [
+    (1, 256, 64, 16, 8, 64), (5, 2048, 128, 32, 8, 0), (12, 2048, 64, 16, 16, 64), (13, 136, 72, 16, 8, 0), (16, 64, 24, 3, 2, 1000),
+    (20, 320, 80, 32, 8, 80), (64, 128, 64, 16, 10, 64)])
+def test_fp16_experts_of_small_tokens(T, d, F, E, k, shared, scale):
+    """Small tokens have small hidden values, whose squares must not fall between fp16's steps.
+
+    As `check_experts`: a hidden value is 2^-22 of itself off, or 2^-30 where that is more.  The latter, over the products of an output (a
+    row of W2 has a norm of sqrt(k) or sqrt(k + 1) here, at most 4.2, and the errors have independent signs), is 2^-30 * 4.2 * 6 at the outside, less than
+    the 2^-25 that the output's smallest half step leaves of the 2^-24 there."""
+    from nexttransformer_b200.ops.moe import moe_tokens
+    a = make_experts(T, d, F, E, shared, torch.float16, seed=T * 100 + d, scale=scale)
+    got = moe_tokens(top_k=k, **a)
+    ref, size = experts(a["x"], a["router"], a["w_fc"], a["w_proj"], k, a["bias"], a.get("shared_fc"), a.get("shared_proj"))
+    check_experts(got, ref, size, torch.float16, d / 4 + (k * F + shared) / 16)
+    assert torch.equal(got, moe_tokens(top_k=k, **a))
+
+
+def test_fp16_experts_of_large_and_small_hidden_values():
+    """The same layer for tokens of 1e-2 to 3e2 beside each other: hidden values of 1e-6 to 1e5."""
+    from nexttransformer_b200.ops.moe import moe_tokens
+    for T in (6, 15, 30):
+        a = make_experts(T, 256, 64, 16, 64, torch.float16, seed=T)
+        size_of = torch.logspace(-2, 2.5, T, device=DEV)
+        a["x"] = (a["x"].float() * size_of[:, None]).half()
+        a["router"] /= 300
+        for n in ("w_proj", "shared_proj"):
+            a[n] = a[n] * 2.0 ** -6
+        ref, size = experts(a["x"], a["router"], a["w_fc"], a["w_proj"], 4, a["bias"], a["shared_fc"], a["shared_proj"])
+        check_experts(moe_tokens(top_k=4, **a), ref, size, torch.float16, 64 + 20)
