@@ -321,14 +321,14 @@ struct Brief {  // what the products need of a piece
 // Goes through a warp's pieces: weights come `STAGES - 1` stages ahead, the other operand one.
 //   first(piece) / next(piece) set a piece and say whether there is one (the copies, the operand and the products each go through them);
 //   base(piece): the tile's first weight; operand(piece, pointers): this lane's part of the 16 x 8 tile of the piece's next stage, of
-//   each block of 8 tokens (null: zeros), `step` apart from tile to tile (a Frag of 16 bytes holds two numbers for each value);
-//   ready(): what has to be waited for before the operand is read; done(piece, sums): a piece's products are complete.  KEEP: the sums
-//   run on through all pieces, and done is not called.
+//   each block of 8 tokens (KEEP: null for zeros), `step` apart from tile to tile (a Frag of 16 bytes holds two numbers for each value);
+//   ready(): what has to be waited for before the operand is read; done(piece, sums): a piece's products are complete.
 // MT tiles of 16 rows share an operand's reading and the way through the loop: a warp's instructions wait for each other, and with 8
 // warps an SM, 16 rows and 187 instructions a stage the first product took 60 us for 12 tokens, with 16 warps and 137 it took 44.
 template <class T, int MT, int NB, int STAGES, class Frag, bool KEEP, class First, class Next, class Base, class Operand, class Ready, class Done>
-NT_DEVICE void stream(const MoeTokensArgs& a, const void* smem, const int step, float (&acc)[MT][NB][4], First first, Next next, Base base,
-                      Operand operand, Ready ready, Done done) {
+NT_DEVICE void stream(const MoeTokensArgs& a, const void* smem, const int step, First first, Next next, Base base, Operand operand, Ready ready,
+                      Done done) {
+  float acc[MT][NB][4];
   constexpr bool TWO = sizeof(Frag) == 16;
   constexpr int STAGE = MT * TILE;
   Ring r = make_ring<STAGES * STAGE>(smem);
@@ -443,17 +443,16 @@ NT_DEVICE void stream(const MoeTokensArgs& a, const void* smem, const int step, 
             if constexpr (TWO) Num<T>::mma(APART ? low[m][nb] : acc[m][nb], w[s], b[s][nb].z, b[s][nb].w);
           }
     }
-    if constexpr (!KEEP)
-      if (c.last) {
-        together();
-        done(c, acc);
+    if (c.last) {
+      together();
+      done(c, acc);
 #pragma unroll
-        for (int m = 0; m < MT; ++m)
+      for (int m = 0; m < MT; ++m)
 #pragma unroll
-          for (int nb = 0; nb < NB; ++nb)
+        for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) acc[m][nb][e] = 0.f;
-      }
+          for (int e = 0; e < 4; ++e) acc[m][nb][e] = 0.f;
+    }
   };
   Frag even[4][NB], odd[4][NB];
   load(even);
@@ -463,7 +462,6 @@ NT_DEVICE void stream(const MoeTokensArgs& a, const void* smem, const int step, 
     if (!n.more) break;
     multiply(odd, even);
   }
-  if constexpr (KEEP) together();
   cp_wait<0>();
 }
 
@@ -506,9 +504,8 @@ __global__ void __launch_bounds__(THREADS, RESIDENT) fc_kernel(const MoeTokensAr
     p.behind = item + by;
     return true;
   };
-  float sums[FC_MT][NB][4];
   stream<T, FC_MT, NB, FC_STAGES, uint2, false>(
-      a, smem, (a.T + 7) / 8 * 32, sums, [&](Piece& p) { return set(p, group * gridDim.x + blockIdx.x); }, [&](Piece& p) { return set(p, p.behind); },
+      a, smem, (a.T + 7) / 8 * 32, [&](Piece& p) { return set(p, group * gridDim.x + blockIdx.x); }, [&](Piece& p) { return set(p, p.behind); },
       [&](const Piece& p) -> const void* {
         const T* e = p.expert == a.E ? static_cast<const T*>(a.shared_fc) : static_cast<const T*>(a.w_fc) + static_cast<int64_t>(p.expert) * a.F * a.d;
         return e + static_cast<int64_t>(p.tile) * ROWS * a.d;
@@ -578,8 +575,8 @@ __global__ void __launch_bounds__(THREADS, RESIDENT) fc_kernel(const MoeTokensAr
       });
 }
 
-// Up to 16 tokens are the columns of every entry, and the sums stay in registers (KEEP); of more, an entry's own are, and its sums are added
-// to the tokens' in shared memory.
+// Up to 16 tokens are the columns of every entry, and the sums stay in registers (KEEP; a piece's are added to those of the tokens that
+// it is for); of more, an entry's own are, and its sums are added to the tokens' in shared memory.
 template <class T, int MT, int NB, int STAGES, bool KEEP>
 __global__ void __launch_bounds__(THREADS, RESIDENT) proj_kernel(const MoeTokensArgs a, const Workspace w, const int parts) {
   extern __shared__ __align__(128) uint8_t smem[];
@@ -626,9 +623,9 @@ __global__ void __launch_bounds__(THREADS, RESIDENT) proj_kernel(const MoeTokens
     enter(p, p.behind);
     return true;
   };
-  float acc[MT][NB][4];
+  float kept[MT][NB][4] = {};
   stream<T, MT, NB, STAGES, uint4, KEEP>(
-      a, smem, 32, acc, set, next,
+      a, smem, 32, set, next,
       [&](const Piece& p) -> const void* {
         const T* e = p.expert == a.E ? static_cast<const T*>(a.shared_proj) : static_cast<const T*>(a.w_proj) + static_cast<int64_t>(p.expert) * a.d * a.F;
         return e + static_cast<int64_t>(tile) * ROWS * p.inner;
@@ -652,6 +649,21 @@ __global__ void __launch_bounds__(THREADS, RESIDENT) proj_kernel(const MoeTokens
       },
       [] { wait_for_predecessor(); },  // weights may come before, h may not
       [&](const Brief& p, const float (&own)[MT][NB][4]) {
+        if constexpr (KEEP) {
+          // A token has the sums of its own experts alone: another's weights times its zeros need not be 0 (infinities)
+          const unsigned mask = static_cast<unsigned>(l.mask[p.expert]) >> ((lane & 3) * 2);
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+              if ((mask >> (nb * 8 + e)) & 1u)
+#pragma unroll
+                for (int m = 0; m < MT; ++m) {
+                  kept[m][nb][e] += own[m][nb][e];
+                  kept[m][nb][e + 2] += own[m][nb][e + 2];
+                }
+          return;
+        }
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
           if (!((p.blocks >> nb) & 1u)) break;
@@ -680,8 +692,8 @@ __global__ void __launch_bounds__(THREADS, RESIDENT) proj_kernel(const MoeTokens
         float* to = sums + (warp * a.T + t) * PITCH + (lane >> 2);
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
-          to[16 * m] = acc[m][nb][e];
-          to[16 * m + 8] = acc[m][nb][e + 2];
+          to[16 * m] = kept[m][nb][e];
+          to[16 * m + 8] = kept[m][nb][e + 2];
         }
       }
   }

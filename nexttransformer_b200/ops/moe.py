@@ -173,7 +173,8 @@ def moe_tokens(x, router, w_fc, w_proj, top_k, *, bias=None, shared_fc=None, sha
     ``w_proj[e] relu(w_fc[e] x)^2`` with ``w_fc [E, F, d]`` and ``w_proj [E, d, F]`` in the type of x; the shared expert
     ``shared_fc [Fs, d]``, ``shared_proj [d, Fs]`` is added for every token.  Widths are multiples of 8; d up to 8192, E up to 512,
     top_k up to 16.  Logits and sums are fp32; a hidden value, times its share, is held as two numbers of the type of x: bf16 2^-16 of
-    it off, fp16 2^-22 of it or 2^-30, and at most 4e6 in fp16.  A token with a NaN gives NaN and leaves the others alone.
+    it off, fp16 2^-22 of it or 2^-30, and at most 4e6 in fp16.  A token with a NaN gives NaN and leaves the others
+    alone, and an expert's weights that are not finite reach only the tokens that chose it.
 
     Only the chosen experts' weights are read, each once (``csrc/moe_tokens.cu``).  It has no backward: training takes
     ``fused_route`` and ``grouped_experts``.

@@ -114,3 +114,30 @@ def test_fp16_experts_of_large_and_small_hidden_values():
             a[n] = a[n] * 2.0 ** -6
         ref, size = experts(a["x"], a["router"], a["w_fc"], a["w_proj"], 4, a["bias"], a["shared_fc"], a["shared_proj"])
         check_experts(moe_tokens(top_k=4, **a), ref, size, torch.float16, 64 + 20)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("T,d,F", [(1, 64, 64), (6, 2048, 72), (7, 136, 200), (12, 2048, 64), (16, 72, 136), (20, 136, 72), (64, 64, 24)])
+def test_weights_that_are_not_finite_reach_the_tokens_that_chose_them(T, d, F, dtype):
+    from nexttransformer_b200.ops.moe import moe_tokens
+    a = make_experts(T, d, F, 12, 64, dtype, seed=T)
+    a["bias"][7] = -5.0                                                   # nobody's
+    clean = moe_tokens(top_k=2, **a)
+    assert torch.isfinite(clean).all()
+    score = torch.softmax(a["x"].double() @ a["router"].double().T, -1) + a["bias"].double()
+    choice = score.topk(2).indices
+    for e in (7, int(choice[0, 0]), int(choice[-1, 1])):
+        hit = (choice == e).any(-1)
+        for bad in (math.inf, -math.inf, math.nan):
+            b = dict(a, w_proj=a["w_proj"].clone(), w_fc=a["w_fc"])
+            b["w_proj"][e, 9, F // 2] = bad                               # one channel of y
+            got = moe_tokens(top_k=2, **b)
+            assert torch.equal(got[~hit], clean[~hit]) and not got[hit, 9].isfinite().any()
+            got[:, 9] = clean[:, 9]
+            assert torch.equal(got, clean)
+            b = dict(a, w_fc=a["w_fc"].clone())
+            b["w_fc"][e, F - 1, d // 2] = bad                             # one hidden value
+            got = moe_tokens(top_k=2, **b)
+            assert torch.equal(got[~hit], clean[~hit])
+            if math.isnan(bad):
+                assert got[hit].isnan().all()
