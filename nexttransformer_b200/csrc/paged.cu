@@ -248,8 +248,8 @@ static int launch_append(const PagedAppendArgs& a, cudaStream_t s) {
 // prompts of 2048 tokens.  Neither was kept.
 //
 // Pages in 8 bits: codes become fp16 in registers, which holds them exactly, and so do queries (bf16 ones after a power of two a row).  A
-// tile is a block, so its keys' scale goes into the scores' factor and its values' into the probabilities, relative to the largest scale so
-// far, like the maximum.  A line's bytes suit the products as they lie: a lane's four neighbouring channels of a key are its share of a
+// tile is a block, so its keys' scale goes into the scores' factor and its values' into the probabilities, relative to a unit that follows
+// them, like the maximum.  A line's bytes suit the products as they lie: a lane's four neighbouring channels of a key are its share of a
 // 16-column step, for keys and queries alike, and two keys' pairs of channels from a transposing load are two rows of V^T.
 // 16 rows of 32768 keys, 10 / 5 heads of 128: 122 us, 5.5 TB/s (209 in 16 bits): a tile is 324 instructions, and two warps
 // a scheduler wait for their own (4.6 cycles each).  64 rows of 512 to 8192 keys, 16 / 1 heads: 27.0 us, 24 x 4 tokens with a window of 1023: 23.5,
@@ -683,7 +683,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
       const int n = min(left, c.it.tiles - c.j), j0 = c.j;
       uint32_t qf[NQ][D / 16][2];
       float to_log[NQ][2];            // 8 bits: the factor of this lane's two queries' products
-      float v_top = 0.f, v_less = 0.f;  // 8 bits: the largest scale of values so far, to which sums are relative, and its inverse
+      float v_unit = 0.f, v_less = 0.f, v_most = 0.f;  // 8 bits: what sums are in units of, its inverse, and the largest it was
       int last[NQ][2], oldest[NQ][2];  // newest and oldest key that this lane's two queries see
 #pragma unroll
       for (int nq = 0; nq < NQ; ++nq) {
@@ -845,10 +845,16 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
         // totals alike, and what is then lost is 2^-32 of the largest a key.
         // 8 bits: one fp16 number (11 bits) is enough where the output has bf16's 8; fp16 queries keep both.
         uint32_t pf[NQ][2], pl[NQ][2];
-        if (F8 && scales.y > v_top) {  // (the same for the whole warp)
-          const float f = v_top / scales.y;
-          v_top = scales.y;
-          v_less = 1.f / scales.y;
+        // Values' scales go into the probabilities relative to a unit, the power of two at or above the scale of a tile.  It stays while
+        // scales are no larger, and no smaller than 2^-7 of it: a probability is held in full down to 2^-14 of the largest then, and what is lost below
+        // is 2^-25 of the tile's own values.  Else it follows the tile (a block of values 2^20 times the others', which these queries may not
+        // even see, would leave nothing of theirs), down to 2^-64 of the largest, so that sums stay in range.
+        if (F8 && (scales.y > v_unit || scales.y * 128.f < v_unit) && scales.y > 0.f) {  // (the same for the whole warp)
+          const float up = __uint_as_float(min((__float_as_uint(scales.y) + 0x7fffffu) & 0xff800000u, 0x7f000000u));
+          v_most = fmaxf(v_most, up);
+          const float unit = fmaxf(up, v_most * 0x1p-64f), f = v_unit / unit;  // (a power of two, so that nothing is rounded)
+          v_unit = unit;
+          v_less = 1.f / unit;
 #pragma unroll
           for (int nq = 0; nq < NQ; ++nq)
 #pragma unroll
@@ -912,7 +918,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
 #pragma unroll
           for (int d = 0; d < D / 16; ++d)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) o[nq][d][e] *= v_top;
+            for (int e = 0; e < 4; ++e) o[nq][d][e] *= v_unit;
 
       // ---- the piece's end; rows that are no tokens have no keys
 #pragma unroll

@@ -4,7 +4,8 @@ import math
 import pytest
 import torch
 
-from tests.test_decode_ops_gpu import both, check_experts, experts, make_experts
+from tests.test_decode_ops_gpu import F8, both, check_experts, experts, make_experts, stands_for
+from tests.test_serving_gpu import U
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -141,3 +142,86 @@ def test_weights_that_are_not_finite_reach_the_tokens_that_chose_them(T, d, F, d
             assert torch.equal(got[~hit], clean[~hit])
             if math.isnan(bad):
                 assert got[hit].isnan().all()
+
+
+# ------------------------------------------------------------------------------------------ attention in 8 bits
+def check_keys(got, q, k, v, table, start, window=-1):
+    """Attention in 64 bits over what the codes stand for, with a bound for each output from the keys that its query sees.
+
+    The output is rounded once (u |out|).  A score, a sum of D products in fp32, is 2^-22 of its terms' sum off, which moves a probability
+    p by twice that.  p is held as one fp16 number beside bf16 queries (2^-11 of it at most, half a step), two beside fp16 ones (2^-22), and below 2^-14 of the
+    largest as a multiple of 2^-24 after a factor of 2^7 * 2^-8 at the least (a tile's scale may be 2^-7 of the unit, itself rounded up to
+    a power of two): 2^-25 / 2^-1 of the largest probability, which is at most 1, 2^-24, and never more than p itself.  Where a tile's scale is the
+    largest, the factor is 2^6 at the least, and it is 2^-31.  fp32 sums of n terms: n * 2^-24 of their size."""
+    B, t, H, D = q.shape
+    Hk, page = k.shape[1:3]
+    group = H // Hk
+    for b in range(B):
+        for i in range(t):
+            pos = start[b] + i
+            key = torch.arange(max(0, pos - window) if window >= 0 else 0, pos + 1, device=DEV)
+            at = table[b].long()[key // page], slice(None), key % page
+            K, V = k[at], v[at].abs()
+            qq = q[b, i].double().view(Hk, group, D)
+            s = torch.einsum("hgd,khd->hgk", qq, K) * D ** -0.5
+            terms = torch.einsum("hgd,khd->hgk", qq.abs(), K.abs()) * D ** -0.5
+            p = torch.softmax(s, -1)
+            ref = torch.einsum("hgk,khd->hgd", p, v[at])
+            largest = V.amax(-1) >= V.amax((0, 2)) / 256                                   # [key, head]
+            lost = torch.where(largest.T[:, None], 2.0 ** -31, 2.0 ** -24)
+            each = p * (2 * terms.amax(-1, keepdim=True) * 2.0 ** -22 + (1.01 * 2.0 ** -11 if got.dtype == torch.bfloat16 else 2.0 ** -21) + len(key) * 2.0 ** -24)
+            slack = torch.einsum("hgk,khd->hgd", each + torch.minimum(p, lost), V)
+            err = (got[b, i].double().view(Hk, group, D) - ref).abs()
+            assert torch.isfinite(got[b, i].float()).all()
+            assert (err <= 1.02 * U[got.dtype] * ref.abs() + slack + 2.0 ** -25).all(), ((err - U[got.dtype] * ref.abs()) / slack).max().item()
+
+
+def make_far_apart(rows, Hk, D, page, seed):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    columns = -(-max(rows) // page)
+    P = len(rows) * columns
+    table = torch.randperm(P, generator=g, device=DEV).int().view(len(rows), columns)
+    k, v = ((torch.randn(P, Hk, page, D, generator=g, device=DEV) * 80).clamp(-448, 448).to(F8) for _ in "kv")
+    ks, vs = (torch.full((P, Hk, page // 16), 2.0 ** -7, device=DEV) for _ in "kv")
+    return k, v, ks, vs, table
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("larger", [12, 20, 30, 100])
+@pytest.mark.parametrize("H,Hk,D,first,t", [(4, 2, 64, 30, 4), (8, 1, 128, 700, 12), (2, 2, 128, 9, 40)])
+def test_attention_in_8_bits_before_a_block_of_larger_values(H, Hk, D, first, t, larger, dtype):
+    """Queries that a later block of the same call is hidden from: its values are 2^12 to 2^100 times theirs."""
+    from nexttransformer_b200.ops.paged import paged_attention
+    k, v, ks, vs, table = make_far_apart([first + t] * 2, Hk, D, 16, seed=first)
+    last = (first + t - 1) // 16
+    vs[table[:, last].long()] *= 2.0 ** larger
+    q = torch.randn(2, t, H, D, device=DEV).to(dtype)
+    start = torch.full((2,), first, device=DEV, dtype=torch.int32)
+    got = paged_attention(q, k, v, table, start, k_scale=ks, v_scale=vs)
+    seen = last * 16 - first                           # queries that do not see it
+    assert 0 < seen < t
+    check_keys(got[:, :seen], q[:, :seen], stands_for(k, ks), stands_for(v, vs), table, [first] * 2)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("keys,larger,window", [(40, 20, -1), (700, 24, -1), (3000, 16, -1), (9000, 20, -1), (600, 30, 100)])
+def test_attention_in_8_bits_beside_blocks_of_larger_values(keys, larger, window, dtype):
+    """Blocks whose values are 2^16 to 2^30 times the others', and whose keys the queries all but pass by."""
+    from nexttransformer_b200.ops.paged import paged_attention
+    H = Hk = 3
+    D, page = 64, 32
+    k, v, ks, vs, table = make_far_apart([keys] * 2, Hk, D, page, seed=keys)
+    q = (torch.randn(2, 1, H, D, device=DEV) * 0.5).to(dtype)
+    blocks = -(-keys // 16)
+    for b in range(2):
+        for j in {0, 1, blocks // 3, blocks // 2, max(0, blocks - 3)} - {blocks - 1}:
+            at, half = table[b, j * 16 // page].long(), j * 16 % page // 16
+            vs[at, :, half] *= 2.0 ** larger
+            # scores of about -80: against the query's signs
+            ks[at, :, half] = 1.0
+            k[at, :, half * 16:half * 16 + 16] = (q[b, 0].float().sign() * -28.0)[:, None].expand(Hk, 16, D).to(F8)
+    if dtype == torch.bfloat16:
+        vs[table[:, -1].long()] *= 2.0 ** -20          # and a last one far below
+    start = torch.full((2,), keys - 1, device=DEV, dtype=torch.int32)
+    got = paged_attention(q, k, v, table, start, window=window, k_scale=ks, v_scale=vs)
+    check_keys(got, q, stands_for(k, ks), stands_for(v, vs), table, [keys - 1] * 2, window)
