@@ -155,10 +155,16 @@ class MoEFFN(nn.Module):
     @torch.no_grad()
     def serve(self, dtype):
         """Lay the weights out in ``dtype`` for ``step``, once before decoding.  A bf16 layer all of whose weights the kernel state keeps
-        uses those, and follows updates as ``forward`` does; otherwise all are copies, to be laid out again after a change."""
+        uses those, and follows updates as ``forward`` does; otherwise all are copies, to be laid out again after a change.  A layer on CUDA
+        that ``ops.moe.moe_tokens`` does not take (``tokens_supported``) is left to ``forward``."""
+        from nexttransformer_b200.ops.moe import tokens_supported
         if self.ep_size > 1:
             raise ValueError("experts of other ranks are not served here")
         experts, router = self.local_experts(), self.router.weight.detach()
+        self._served = None
+        if router.is_cuda and not tokens_supported(dtype, router.shape[1], experts[0].c_fc.weight.shape[0], self.num_experts, self.top_k,
+                                                   0 if self.shared is None else self.shared.c_fc.weight.shape[0]):
+            return
         shared = () if self.shared is None else (self.shared.c_fc, self.shared.c_proj)
         if (self._w_fc is not None and dtype == torch.bfloat16 and router.dtype == torch.float32 and router.is_contiguous()
                 and all(getattr(lin, "_w", None) is not None for lin in shared)):

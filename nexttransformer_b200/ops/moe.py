@@ -165,6 +165,12 @@ def grouped_experts_state(x, choice, w, moe, pl=None):
 TOKENS_MOST = 64
 
 
+def tokens_supported(dtype, d, F, E, top_k, Fs=0):
+    """Whether ``moe_tokens`` takes a layer on CUDA: its type, width, experts' width, experts, choices, the shared expert's width (0: none)."""
+    return (dtype in (torch.bfloat16, torch.float16) and d % 8 == 0 and 8 <= d <= 8192 and F % 8 == 0 and 8 <= F <= 65536
+            and E <= 512 and top_k <= 16 and Fs % 8 == 0 and Fs <= 1048576)
+
+
 def moe_tokens(x, router, w_fc, w_proj, top_k, *, bias=None, shared_fc=None, shared_proj=None):
     """The whole layer for ``x [T, d]``, up to 64 tokens (bf16 or fp16; on the CPU any float type and any T): ``[T, d]``.
 

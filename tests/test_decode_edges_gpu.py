@@ -225,3 +225,22 @@ def test_attention_in_8_bits_beside_blocks_of_larger_values(keys, larger, window
     start = torch.full((2,), keys - 1, device=DEV, dtype=torch.int32)
     got = paged_attention(q, k, v, table, start, window=window, k_scale=ks, v_scale=vs)
     check_keys(got, q, stands_for(k, ks), stands_for(v, vs), table, [keys - 1] * 2, window)
+
+
+# ------------------------------------------------------------------------------------------ the layer
+@pytest.mark.parametrize("dtype,d,F,E,k,shared", [
+    (torch.bfloat16, 64, 60, 8, 2, 0), (torch.bfloat16, 60, 64, 8, 2, 1), (torch.float16, 64, 40, 20, 17, 1), (torch.bfloat16, 64, 8, 520, 2, 0),
+    (torch.bfloat16, 8200, 8, 4, 2, 0), (torch.float32, 64, 32, 8, 2, 1)])
+def test_layers_that_the_kernel_does_not_take_decode_through_forward(dtype, d, F, E, k, shared):
+    from nexttransformer_b200.models.moe import MoEFFN
+    torch.manual_seed(F)
+    layer = MoEFFN(d, E, k, F, shared=shared).eval().to(DEV)
+    with torch.no_grad():
+        for p in layer.parameters():
+            p.normal_(0, 0.1)
+        x = torch.randn(2, 3, d, device=DEV).to(dtype)
+        assert torch.isfinite(layer(x)).all()
+        layer.serve(dtype)
+        assert layer.step(x).shape == x.shape
+        layer.forward = lambda x: x + 1                # (its own sums are atomics, in any order)
+        assert torch.equal(layer.step(x), x + 1)
