@@ -185,6 +185,8 @@ class MoEFFN(nn.Module):
         s = self._served
         if s is None or rows.shape[0] > TOKENS_MOST or s["w_fc"].dtype != x.dtype or s["w_fc"].device != x.device:
             return self(x)
+        if rows.is_cuda and (not rows.is_contiguous() or rows.data_ptr() % 16):  # a part of wider rows
+            rows = rows.clone(memory_format=torch.contiguous_format)
         return moe_tokens(rows, s["router"], s["w_fc"], s["w_proj"], self.top_k, bias=s["bias"], shared_fc=s["shared_fc"],
                           shared_proj=s["shared_proj"]).reshape_as(x)
 

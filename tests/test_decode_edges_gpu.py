@@ -244,3 +244,17 @@ def test_layers_that_the_kernel_does_not_take_decode_through_forward(dtype, d, F
         assert layer.step(x).shape == x.shape
         layer.forward = lambda x: x + 1                # (its own sums are atomics, in any order)
         assert torch.equal(layer.step(x), x + 1)
+
+
+def test_a_step_of_rows_that_are_a_part_of_wider_ones():
+    from nexttransformer_b200.models.moe import MoEFFN
+    torch.manual_seed(1)
+    layer = MoEFFN(64, 8, 2, 32, shared=1).eval().to(DEV)
+    with torch.no_grad():
+        for p in layer.parameters():
+            p.normal_(0, 0.1)
+        layer.serve(torch.bfloat16)
+        wide = torch.randn(5, 71, device=DEV).bfloat16()
+        for rows in (5, 1):
+            x = wide[:rows, 3:67]
+            assert x.data_ptr() % 16 and torch.equal(layer.step(x), layer.step(x.clone(memory_format=torch.contiguous_format)))
