@@ -179,11 +179,13 @@ class MoEFFN(nn.Module):
 
     def step(self, x):
         """``forward`` without gradients and load statistics for a few tokens: ``ops.moe.moe_tokens`` on the weights that ``serve``
-        laid out.  More tokens than that takes, other types than they have, and a layer that was not laid out go through ``forward``."""
+        laid out.  More tokens than that takes, other types than they have, a layer with forward hooks and one that was not laid out go
+        through ``forward``."""
         from nexttransformer_b200.ops.moe import TOKENS_MOST, moe_tokens
         rows = x.reshape(-1, x.shape[-1])
         s = self._served
-        if s is None or rows.shape[0] > TOKENS_MOST or s["w_fc"].dtype != x.dtype or s["w_fc"].device != x.device:
+        if (s is None or rows.shape[0] > TOKENS_MOST or s["w_fc"].dtype != x.dtype or s["w_fc"].device != x.device
+                or self._forward_hooks or self._forward_pre_hooks):
             return self(x)
         if rows.is_cuda and (not rows.is_contiguous() or rows.data_ptr() % 16):  # a part of wider rows
             rows = rows.clone(memory_format=torch.contiguous_format)

@@ -11,3 +11,19 @@ from nexttransformer_b200.ops.moe import tokens_supported
     (dict(E=32, top_k=17), False), (dict(Fs=20), False)])
 def test_what_the_experts_of_a_few_tokens_take(change, taken):
     assert tokens_supported(**dict(dict(dtype=torch.bfloat16, d=64, F=32, E=8, top_k=2), **change)) is taken
+
+
+def test_a_step_calls_the_forward_hooks_of_a_layer():
+    from nexttransformer_b200.models.moe import MoEFFN
+    torch.manual_seed(2)
+    layer, x, seen = MoEFFN(32, 8, 3, 24, shared=1).eval(), torch.randn(5, 32), []
+    with torch.no_grad():
+        layer.serve(torch.float32)
+        plain = layer.step(x)
+        for register, value in ((layer.register_forward_hook, lambda m, a, out: seen.append(out)),
+                                (layer.register_forward_pre_hook, lambda m, a: seen.append(a[0]))):
+            hook = register(value)
+            out = layer.step(x)
+            assert len(seen) == 1 and seen.pop() is (out if register == layer.register_forward_hook else x)
+            hook.remove()
+        assert torch.equal(layer.step(x), plain) and not seen
