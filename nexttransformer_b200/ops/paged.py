@@ -11,7 +11,8 @@ Pages may also be held in 8 bits (``float8_e4m3fn``) beside bf16 or fp16 queries
 ``paged_append`` chooses it: the smallest power of two (2^-100 to 2^120) whose 448-fold reaches the largest number that the
 block's tokens had so far; a call that begins a block chooses anew, one that continues it may raise the scale, and then
 the block's earlier codes are written again.  So a block of 16 tokens takes tokens of one row only in a call, and no other call
-at the same time.  What is not finite becomes NaN and does not count for the scale.
+at the same time.  What is not finite becomes NaN and does not count for the scale.  Blocks may share a scale in memory where it is only
+read, by ``paged_attention``.
 
 * ``paged_append``    rotates and QK-normalises new queries and keys, adds the gated value embedding, writes
   keys and values into the pages and returns the queries;
@@ -158,8 +159,6 @@ def _append_plain(q, k, v, k_pages, v_pages, table, start, count, cos, sin, qk_s
 
 def _attention_plain(q, k_pages, v_pages, table, start, count, window, scale, k_scale, v_scale):
     starts, counts = _check_plain(q, k_pages, v_pages, table, start, count, k_scale, v_scale)
-    if any(n > 1 and s.stride(i) == 0 for s in (k_scale, v_scale) if s is not None for i, n in enumerate(s.shape)):
-        raise RuntimeError("blocks may not share a scale in memory")
     B, t, H, D = q.shape
     Hk = k_pages.shape[1]
     scale = D ** -0.5 if scale is None else scale

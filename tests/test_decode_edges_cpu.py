@@ -3,6 +3,7 @@ import pytest
 import torch
 
 from nexttransformer_b200.ops.moe import tokens_supported
+from nexttransformer_b200.ops.paged import paged_attention
 
 
 @pytest.mark.parametrize("change,taken", [
@@ -27,3 +28,12 @@ def test_a_step_calls_the_forward_hooks_of_a_layer():
             assert len(seen) == 1 and seen.pop() is (out if register == layer.register_forward_hook else x)
             hook.remove()
         assert torch.equal(layer.step(x), plain) and not seen
+
+
+def test_attention_in_8_bits_reads_scales_that_share_memory():
+    torch.manual_seed(4)
+    k, v = (torch.randn(3, 2, 32, 16).mul(60).to(torch.float8_e4m3fn) for _ in "kv")
+    q, table, start = torch.randn(1, 1, 4, 16), torch.tensor([[2, 0]], dtype=torch.int32), torch.tensor([50], dtype=torch.int32)
+    one, heads = torch.full((1, 1, 1), 2.0 ** -5).expand(3, 2, 2), torch.tensor([2.0 ** -6, 2.0 ** -4])[None, :, None].expand(3, 2, 2)
+    got = paged_attention(q, k, v, table, start, k_scale=one, v_scale=heads)
+    assert torch.equal(got, paged_attention(q, k, v, table, start, k_scale=one.contiguous(), v_scale=heads.contiguous()))

@@ -227,6 +227,16 @@ def test_attention_in_8_bits_beside_blocks_of_larger_values(keys, larger, window
     check_keys(got, q, stands_for(k, ks), stands_for(v, vs), table, [keys - 1] * 2, window)
 
 
+def test_attention_in_8_bits_reads_scales_that_share_memory():
+    from nexttransformer_b200.ops.paged import paged_attention
+    k, v, _, _, table = make_far_apart([70], 2, 64, 32, seed=1)
+    shape = (*k.shape[:2], 2)
+    one, heads = torch.full((1, 1, 1), 2.0 ** -7, device=DEV).expand(shape), torch.tensor([2.0 ** -8, 2.0 ** -6], device=DEV)[None, :, None].expand(shape)
+    q, start = torch.randn(1, 1, 4, 64, device=DEV).bfloat16(), torch.tensor([69], device=DEV, dtype=torch.int32)
+    got = paged_attention(q, k, v, table, start, k_scale=one, v_scale=heads)
+    assert torch.equal(got, paged_attention(q, k, v, table, start, k_scale=one.contiguous(), v_scale=heads.contiguous()))
+
+
 # ------------------------------------------------------------------------------------------ the layer
 @pytest.mark.parametrize("dtype,d,F,E,k,shared", [
     (torch.bfloat16, 64, 60, 8, 2, 0), (torch.bfloat16, 60, 64, 8, 2, 1), (torch.float16, 64, 40, 20, 17, 1), (torch.bfloat16, 64, 8, 520, 2, 0),
