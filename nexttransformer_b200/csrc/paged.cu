@@ -1423,7 +1423,10 @@ static int launch_append8(const PagedAppendArgs& a, cudaStream_t s) {
     append8_one_kernel<T, D><<<static_cast<unsigned>((items + PER_CTA - 1) / PER_CTA), 256, 0, s>>>(a);
     return 0;
   }
-  return static_cast<int64_t>(a.B) * a.t * a.H >= 32768 ? launch_append8<T, D, 3, 2>(a, s) : launch_append8<T, D, 1, 1>(a, s);
+  // Many heads of tokens keep the SMs busy with three query heads a group of lanes and two tokens a thread, which take fewer instructions; few
+  // are done sooner by twice the threads.  One head and one token / three and two, us: 10 / 5 heads of 128, one row of 512 tokens
+  // 3.0 / 3.4, of 1024 3.9 / 3.7, 4 of 700 7.8 / 6.9, 8 of 2048 42 / 35; 16 / 1 of 128, one row of 1024 3.4 / 3.6; 12 / 12 of 64, 192 of 4 9.1 / 7.6.
+  return static_cast<int64_t>(a.B) * a.t * a.H >= 10240 ? launch_append8<T, D, 3, 2>(a, s) : launch_append8<T, D, 1, 1>(a, s);
 }
 
 struct Plan {

@@ -4,6 +4,7 @@ import math
 import pytest
 import torch
 
+import tests.test_decode_ops_gpu as ops
 from tests.test_decode_ops_gpu import F8, both, check_experts, experts, make_experts, stands_for
 from tests.test_serving_gpu import U
 
@@ -235,6 +236,38 @@ def test_attention_in_8_bits_reads_scales_that_share_memory():
     q, start = torch.randn(1, 1, 4, 64, device=DEV).bfloat16(), torch.tensor([69], device=DEV, dtype=torch.int32)
     got = paged_attention(q, k, v, table, start, k_scale=one, v_scale=heads)
     assert torch.equal(got, paged_attention(q, k, v, table, start, k_scale=one.contiguous(), v_scale=heads.contiguous()))
+
+
+# ------------------------------------------------------------------------------------------ append in 8 bits
+@pytest.mark.parametrize("dtype,D,H,Hk,page,t,norm,ve,rows", [
+    (torch.float16, 64, 10, 2, 16, 512, True, True, [(0, 512), (9, 300)]),                  # 10240 heads of tokens
+    (torch.bfloat16, 64, 10, 5, 64, 511, False, True, [(7, 511), (0, 16)]),                 # just below
+    (torch.bfloat16, 128, 1, 1, 48, 700, True, False, [(b, 700 - 40 * b) for b in range(16)]),
+    (torch.float16, 128, 16, 4, 32, 40, True, True, [(b * 5 % 37, b % 41) for b in range(20)])])
+def test_append_in_8_bits_of_many_and_few_heads(dtype, D, H, Hk, page, t, norm, ve, rows):
+    ops.test_append_in_8_bits(dtype, D, H, Hk, page, t, norm, ve, rows)
+
+
+@pytest.mark.parametrize("H,Hk,D,dtype", [(10, 5, 128, torch.bfloat16), (12, 12, 64, torch.float16), (16, 1, 128, torch.bfloat16)])
+def test_append_in_8_bits_of_a_batch_and_of_its_rows(H, Hk, D, dtype):
+    """Rows of a large call and of small ones are written alike, to the bit."""
+    from nexttransformer_b200.ops.paged import paged_append
+    torch.manual_seed(H)
+    B, t, page = 6, 400, 32
+    x = torch.randn(B, t, H + 2 * Hk, D, device=DEV).to(dtype)
+    table = torch.randperm(B * 16, device=DEV).int().view(B, 16)
+    start = torch.tensor([0, 5, 16, 31, 100, 111], device=DEV, dtype=torch.int32)
+    count = torch.tensor([400, 1, 33, 400, 399, 16], device=DEV, dtype=torch.int32)
+    angle = torch.outer(torch.arange(512, device=DEV), 1e4 ** (-torch.arange(0, D, 2, device=DEV) / D))
+    cos, sin = angle.cos().to(dtype), angle.sin().to(dtype)
+    held, out = [], []
+    for parts in ([slice(0, B)], [slice(b, b + 1) for b in range(B)]):
+        k, v = (torch.zeros(B * 16, Hk, page, D, device=DEV).to(F8) for _ in "kv")
+        ks, vs = (torch.zeros(B * 16, Hk, 2, device=DEV) for _ in "kv")
+        out.append(torch.cat([paged_append(x[p, :, :H], x[p, :, H:H + Hk], x[p, :, H + Hk:], k, v, table[p], start[p], count[p], cos=cos, sin=sin,
+                                           qk_scale=1.2, k_scale=ks, v_scale=vs) for p in parts]))
+        held.append((k.view(torch.uint8), v.view(torch.uint8), ks, vs))
+    assert torch.equal(*out) and all(torch.equal(a, b) for a, b in zip(*held))
 
 
 # ------------------------------------------------------------------------------------------ the layer
