@@ -902,14 +902,14 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
           }
         } else {
 #pragma unroll
-        for (int d = 0; d < D / 16; ++d) {
-          uint32_t vf[4];
-          ldsm4t(vf, base + vat[d & 3] + (d >> 2) * 128);
+          for (int d = 0; d < D / 16; ++d) {
+            uint32_t vf[4];
+            ldsm4t(vf, base + vat[d & 3] + (d >> 2) * 128);
 #pragma unroll
-          for (int nq = 0; nq < NQ; ++nq) Num<M>::mma(o[nq][d], vf, pf[nq][0], pf[nq][1]);
+            for (int nq = 0; nq < NQ; ++nq) Num<M>::mma(o[nq][d], vf, pf[nq][0], pf[nq][1]);
 #pragma unroll
-          for (int nq = 0; nq < NQ; ++nq) Num<M>::mma(o[nq][d], vf, pl[nq][0], pl[nq][1]);
-        }
+            for (int nq = 0; nq < NQ; ++nq) Num<M>::mma(o[nq][d], vf, pl[nq][0], pl[nq][1]);
+          }
         }
       }
       if (F8)
@@ -1089,10 +1089,6 @@ NT_DEVICE uint32_t to_e4m3(const float (&x)[4]) {
   asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(x[1]), "f"(x[0]));
   asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(x[3]), "f"(x[2]));
   return static_cast<uint32_t>(lo) | (static_cast<uint32_t>(hi) << 16);
-}
-NT_DEVICE void from_e4m3(uint32_t v, float (&x)[4]) {
-  const float2 a = Num<__half>::unpack(widen_low(v)), b = Num<__half>::unpack(widen_high(v));
-  x[0] = a.x; x[1] = a.y; x[2] = b.x; x[3] = b.y;
 }
 // The smallest power of two, 2^-100 to 2^120, whose 448-fold (1.75 2^8) reaches top >= 0.
 NT_DEVICE float block_scale(float top) {
