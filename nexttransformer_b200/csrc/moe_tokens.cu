@@ -16,7 +16,7 @@
 //
 // 12 tokens, d 2048, 64 experts of 1024, 8 a token and a shared one: 91 to 93 us for 438 MB (68 at 6.46 TB/s): fc and proj stream at about 5 TB/s once
 // they run, the rest is three launches' ways to their first tile.  One token: 29 us for 76 MB (11.8), those ways alone.
-// 64 tokens, 256 experts of 320: 100 us for 368 MB (57), where proj's pieces are five stages long and a third of its 190 instructions a
+// 64 tokens, 256 experts of 320: 100 us for 368 MB (57), where proj's pieces are five stages long and a third of its 182 instructions a
 // stage begin and end them (19.7 million instructions and 113 us with tokens found in masks, a third walk through the pieces and one sum).
 // Tried and not kept: stages of 128 columns (12 tokens 97 -> 128 us), fc with 16 rows at three CTAs an SM (93 -> 106), L2 prefetches of 256 bytes
 // (1 %), x kept out of shared memory in route (28.7 -> 29.9), weights fetched into L2 while route runs (0 to 2 %) or while fc ends (64 tokens: +10 %),

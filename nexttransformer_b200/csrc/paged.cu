@@ -1082,8 +1082,8 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
 //
 // A block of one KV head, its keys or its values, is written by one group of lanes or warps, so that nobody else writes
 // its scale: all of its new tokens are in registers before the scale is known, and are read once.  8 prompts of up to 2048 tokens, 10 + 5
-// heads of 128: 31.1 us for 104 MB (16.1 at the copy rate), by instructions: 0.55 of the issue slots are used, at 24 warps
-// an SM.  One token of a row by the same blocks took 5.2 us, and 11.7 for 192 rows; by groups of lanes they take 2.9 and 3.4.
+// heads of 128: 31.1 us for 104 MB (16.1 at the copy rate): 80 registers a thread leave 24 warps an SM, which wait for their tokens longest
+// (long scoreboard 2.3 cycles an issue, 0.54 of the slots used).  One token of a row by the same blocks took 5.2 us, and 11.7 for 192 rows; by groups of lanes they take 2.9 and 3.4.
 NT_DEVICE uint32_t to_e4m3(const float (&x)[4]) {
   uint16_t lo, hi;
   asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(x[1]), "f"(x[0]));

@@ -15,7 +15,7 @@
 // more than 1024 is split by the numbers' bits, and equal logits by their indices.
 //
 // Bound by latency and by 64-bit arithmetic: 1 x 32768, top-k and top-p: 14 us, of which (clock stamps) loads take 0.5, the maximum 1.3, the
-// histogram 1.1, its crossing and the list 3.4, the gathering 1.8, the two borders 3.1, the draw 2.4.  224 x 65536 with a setting for each row: 80 us
+// histogram 1.1, its crossing and the list 3.4, the gathering 1.8, the two borders 3.1, the draw 2.4.  224 x 65536 with a setting for each row: 80 to 83 us
 // for 59 MB (9 at the copy rate): two CTAs an SM, so three to four rounds, each CTA 17 us (top-k) to 40 (top-p alone), with 8 or 9
 // for each pass that takes the exp of every logit in 64 bits.
 // Tried and not kept: a sort of the kept ones (5 us and more), every CTA reading all bins' masses of all (15 us instead of 4).

@@ -19,7 +19,7 @@ struct SampleArgs {
   float* logprobs = nullptr;     // [B]
   int B = 0, V = 0, type = 0, sms = 0;
 };
-// The largest vocabulary that a row's CTAs hold on chip.
+// The largest vocabulary (up to 131072 logits a row are held on chip, of longer rows each pass reads them again).
 int nt_sample_most();
 // 0, or -1 for an unsupported shape.
 int nt_sample_logits(const SampleArgs& a, cudaStream_t s);

@@ -1,7 +1,8 @@
 """A token for each row of next-token logits: temperature, top-k, top-p, min-p, drawn with numbers that the caller gives.
 
-``sample_logits`` reads the logits once (``csrc/sampling.cu``; CPU tensors run the plain form below).  It has no
-backward and draws no random numbers of its own, so a call's result depends on its arguments alone.
+``sample_logits`` is one launch (``csrc/sampling.cu``; CPU tensors run the plain form below), which reads rows of up to 131072 logits once and
+longer ones again in each pass.  It has no backward and draws no random numbers of its own, so a call's result depends on its
+arguments alone.
 """
 import torch
 
@@ -22,8 +23,8 @@ def sample_logits(logits, uniform, *, temperature=1.0, top_k=None, top_p=None, m
 
     and always the first.  The token is the smallest index up to which more than ``uniform`` of the kept mass lies, its
     logprob the log of its share of that mass.  ``temperature``, ``top_p`` and ``min_p`` are numbers or fp32 ``[B]``, ``top_k`` is a
-    number or int32 ``[B]``; None leaves a part out, and so does a NaN in it.  A temperature of 0 or less takes the first
-    token.  A ``uniform`` outside [0, 1) counts as the nearest number inside, NaN as 0.
+    number or int32 ``[B]``; None leaves a part out (a temperature is 1 then), and so does a NaN in ``top_p`` or ``min_p``.  A
+    temperature of 0 or less, or a NaN, takes the first token.  A ``uniform`` outside [0, 1) counts as the nearest number inside, NaN as 0.
 
     Logits of -inf are never drawn; where the largest are inf, they share the choice.  A row without any permitted token
     gives token -1 (logprob -inf), a row with a NaN -2 (logprob NaN).
