@@ -301,3 +301,23 @@ def test_a_step_of_rows_that_are_a_part_of_wider_ones():
         for rows in (5, 1):
             x = wide[:rows, 3:67]
             assert x.data_ptr() % 16 and torch.equal(layer.step(x), layer.step(x.clone(memory_format=torch.contiguous_format)))
+
+
+# ------------------------------------------------------------------------------------------ the engine
+def test_generation_at_low_temperatures_and_with_large_biases():
+    """Answers of a temperature that leaves the largest logit alone are the greedy ones, and a bias of 1e18 settles the choice."""
+    from dataclasses import replace
+    from nexttransformer_b200.inference import generate_batch
+    from nexttransformer_b200.models import build_model
+    from nexttransformer_b200.models.config import debug_config
+    c = replace(debug_config("dense"), width=256, heads=4, kv_heads=2)
+    m = build_model(c, DEV, seed=1).eval()
+    with torch.no_grad():
+        m.lm_head.weight.normal_(0, 0.3)
+    prompts = [[1, 2, 3], [4], list(range(20))]
+    greedy = generate_batch(m, prompts, 8, temperature=0.0)
+    for T in (1e-15, 1e-18, 1e-20):
+        assert generate_batch(m, prompts, 8, temperature=T, top_p=0.9) == greedy
+        assert generate_batch(m, prompts, 8, temperature=[T] * 3, top_k=[0, 3, 50], min_p=0.1) == greedy
+    for T in (0.7, 1.0):
+        assert generate_batch(m, prompts, 4, temperature=T, top_p=0.9, bias={9: 1e18}) == [[9] * 4] * 3
