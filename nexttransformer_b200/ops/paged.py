@@ -59,6 +59,9 @@ def paged_attention(q, k_pages, v_pages, table, start, count=None, *, window=-1,
     which does not remove a NaN.  What no token sees (behind the row's tokens, before every window) may hold anything.
     A query with a NaN gives NaN, and so does one with a score of inf; where every score is -inf the kernel gives zeros, as
     for a token without keys (the plain form NaN).
+
+    Sums are fp32.  Over pages in 8 bits a probability is one fp16 number beside bf16 queries (2^-11 of it, below the output's rounding), two beside
+    fp16 ones.
     """
     if q.is_cuda:
         return ext().paged_attention(q, k_pages, v_pages, table, start, count, window, scale, k_scale, v_scale)

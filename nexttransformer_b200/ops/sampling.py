@@ -22,7 +22,8 @@ def sample_logits(logits, uniform, *, temperature=1.0, top_k=None, top_p=None, m
     * of these, the tokens with ``w >= min_p`` (all, where it is 0 or less; from 1 on those with the largest logit),
 
     and always the first.  The token is the smallest index up to which more than ``uniform`` of the kept mass lies, its
-    logprob the log of its share of that mass.  ``temperature``, ``top_p`` and ``min_p`` are numbers or fp32 ``[B]``, ``top_k`` is a
+    logprob the log of its share of that mass.  Masses are exact sums of weights held as whole multiples of 2^-50 of the largest (2^-42 with
+    524288 tokens): what lies closer to a border than they do may fall to its other side.  ``temperature``, ``top_p`` and ``min_p`` are numbers or fp32 ``[B]``, ``top_k`` is a
     number or int32 ``[B]``; None leaves a part out (a temperature is 1 then), and so does a NaN in ``top_p`` or ``min_p``.  A
     temperature of 0 or less, or a NaN, takes the first token.  A ``uniform`` outside [0, 1) counts as the nearest number inside, NaN as 0.
 
